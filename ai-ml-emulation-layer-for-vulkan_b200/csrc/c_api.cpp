@@ -11,6 +11,7 @@
 #include "kernels/device_common.cuh"
 #include "kernels/gemm_i8_tcgen05.hpp"
 #include "kernels/kernels.hpp"
+#include "kernels/serving.hpp"
 #include "session.hpp"
 
 using namespace mlel;
@@ -1024,6 +1025,58 @@ int mlel_cuda_conv2d_rescale(const mlel_tensor *input, const mlel_tensor *weight
         return runSingle(op, {input, weights, biases, output, multiplier, shift},
                          static_cast<cudaStream_t>(cuda_stream));
     });
+}
+
+/* ---- 8-bit decoder layers ---- */
+
+int mlel_cuda_quantize_rows(const mlel_tensor *input, const mlel_tensor *output, const mlel_tensor *scales, void *cuda_stream) {
+    return guarded([&] { return quantizeRows(input, output, scales, static_cast<cudaStream_t>(cuda_stream)); });
+}
+
+int mlel_cuda_matmul_scaled(const mlel_tensor *a, const mlel_tensor *a_scales, const mlel_tensor *b, const mlel_tensor *b_scales,
+                            const mlel_tensor *biases, const mlel_tensor *output, void *cuda_stream) {
+    return guarded(
+        [&] { return matmulScaled(a, a_scales, b, b_scales, biases, output, static_cast<cudaStream_t>(cuda_stream)); });
+}
+
+int mlel_cuda_paged_append(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *keys,
+                           const mlel_tensor *values, const mlel_tensor *cosines, const mlel_tensor *sines,
+                           const mlel_tensor *queries, const mlel_tensor *rotated_queries, int interleaved, void *cuda_stream) {
+    return guarded([&] {
+        return pagedAppend(cache, batch, keys, values, cosines, sines, queries, rotated_queries, interleaved,
+                           static_cast<cudaStream_t>(cuda_stream));
+    });
+}
+
+int mlel_cuda_paged_attention(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries,
+                              const mlel_tensor *output, float scale, int causal, int32_t window, float softcap, void *workspace,
+                              uint64_t workspace_bytes, void *cuda_stream) {
+    return guarded([&] {
+        return pagedAttention(cache, batch, queries, output, scale, causal, window, softcap, workspace, workspace_bytes,
+                              static_cast<cudaStream_t>(cuda_stream));
+    });
+}
+
+int mlel_paged_attention_workspace(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries,
+                                   uint64_t *bytes) {
+    return guarded([&] {
+        if (bytes == nullptr) {
+            throw std::runtime_error("mlel_paged_attention_workspace: bytes must not be null");
+        }
+        *bytes = pagedAttentionWorkspace(cache, batch, queries);
+        return MLEL_SUCCESS;
+    });
+}
+
+int mlel_paged_error(void) {
+    int code = 0;
+    guarded([&] {
+        cudaDeviceSynchronize();
+        const int append = takePagedErrorAppend(), attention = takePagedErrorAttention();
+        code = append != 0 ? append : attention;
+        return MLEL_SUCCESS;
+    });
+    return code;
 }
 
 } // extern "C"

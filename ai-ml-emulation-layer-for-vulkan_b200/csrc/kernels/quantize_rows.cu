@@ -1,0 +1,165 @@
+// Rows in 8 bits with a scale found at run time: scale = max |x| / 127, q = x / scale to the nearest whole number, ties to
+// the even one, decided as exact arithmetic would (see roundedQuotient).
+//
+// What bounds it: memory.  A row is read once: its 16-byte vectors stay in registers between the maximum and the
+// rounding, four to a thread, and as many threads share a row as that takes (32 to 1024; longer rows are read again).
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "../graph_pipeline.hpp"
+#include "launch_overlapped.cuh"
+#include "serving.hpp"
+#include "serving_device.cuh"
+
+namespace mlel {
+namespace {
+
+constexpr int kHeld = 4; // vectors of a row that a thread keeps
+
+struct QuantizeParams {
+    const char *in;
+    int8_t *out;
+    float *scales;
+    int64_t inStride, outStride; // bytes between rows
+    int32_t rows, length;
+};
+
+// The eight elements from `first` on; those behind the end of the row are zeros.
+template <class T, bool WIDE> __device__ __forceinline__ void loadEight(const T *row, int first, int length, float (&x)[8]) {
+    if (WIDE && first + 8 <= length) {
+        loadWide(row + first, x);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[j] = first + j < length ? toFloat(row[first + j]) : 0.f;
+        }
+    }
+}
+
+template <class T, int TEAM, bool WIDE>
+__global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) quantizeRowsKernel(const QuantizeParams p) {
+    constexpr int kTeams = TEAM < 256 ? 256 / TEAM : 1;
+    __shared__ uint32_t partial[32];
+    dependencySync();
+    const int team = int(threadIdx.x) / TEAM, at = int(threadIdx.x) % TEAM;
+    const int64_t rowIndex = int64_t(blockIdx.x) * kTeams + team;
+    const bool live = rowIndex < p.rows;
+    const T *row = reinterpret_cast<const T *>(p.in + (live ? rowIndex : 0) * p.inStride);
+    const int length = live ? p.length : 0;
+    float x[kHeld][8];
+    uint32_t most = 0; // magnitudes as bits: an infinity is above every number and a NaN above that
+#pragma unroll
+    for (int v = 0; v < kHeld; ++v) {
+        loadEight<T, WIDE>(row, (v * TEAM + at) * 8, length, x[v]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            most = max(most, __float_as_uint(x[v][j]) & 0x7fffffffu);
+        }
+    }
+    for (int first = (kHeld * TEAM + at) * 8; first < length; first += TEAM * 8) {
+        float y[8];
+        loadEight<T, WIDE>(row, first, length, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            most = max(most, __float_as_uint(y[j]) & 0x7fffffffu);
+        }
+    }
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (TEAM > 32) {
+        const int warp = int(threadIdx.x) >> 5, firstWarp = team * (TEAM / 32);
+        if ((threadIdx.x & 31) == 0) {
+            partial[warp] = most;
+        }
+        __syncthreads();
+        most = 0;
+#pragma unroll
+        for (int w = 0; w < TEAM / 32; ++w) {
+            most = max(most, partial[firstWarp + w]);
+        }
+    }
+    if (!live) {
+        return;
+    }
+    const RowScale scale = rowScale(most);
+    if (at == 0) {
+        p.scales[rowIndex] = scale.value;
+    }
+    int8_t *out = p.out + rowIndex * p.outStride;
+    const auto store = [&](int first, const float (&y)[8]) {
+        if (first >= length) {
+            return;
+        }
+        const uint2 packed = quantizeEight(y, scale);
+        if (WIDE && first + 8 <= length) {
+            *reinterpret_cast<uint2 *>(out + first) = packed;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (first + j < length) {
+                    out[first + j] = int8_t((j < 4 ? packed.x >> (8 * j) : packed.y >> (8 * (j - 4))) & 0xffu);
+                }
+            }
+        }
+    };
+#pragma unroll
+    for (int v = 0; v < kHeld; ++v) {
+        store((v * TEAM + at) * 8, x[v]);
+    }
+    for (int first = (kHeld * TEAM + at) * 8; first < length; first += TEAM * 8) {
+        float y[8];
+        loadEight<T, WIDE>(row, first, length, y);
+        store(first, y);
+    }
+}
+
+template <class T, int TEAM> cudaError_t launchTeam(const QuantizeParams &p, bool wide, cudaStream_t s) {
+    constexpr int kTeams = TEAM < 256 ? 256 / TEAM : 1;
+    const dim3 grid(unsigned((int64_t(p.rows) + kTeams - 1) / kTeams));
+    constexpr unsigned threads = TEAM < 256 ? 256 : TEAM;
+    return wide ? launchOverlapped(quantizeRowsKernel<T, TEAM, true>, grid, threads, 0, s, p)
+                : launchOverlapped(quantizeRowsKernel<T, TEAM, false>, grid, threads, 0, s, p);
+}
+
+template <class T> cudaError_t launchType(const QuantizeParams &p, bool wide, cudaStream_t s) {
+    const int vectors = (p.length + 7) / 8;
+    if (vectors <= 32 * kHeld) {
+        return launchTeam<T, 32>(p, wide, s);
+    }
+    if (vectors <= 128 * kHeld) {
+        return launchTeam<T, 128>(p, wide, s);
+    }
+    return vectors <= 256 * kHeld ? launchTeam<T, 256>(p, wide, s) : launchTeam<T, 1024>(p, wide, s);
+}
+
+} // namespace
+
+int quantizeRows(const mlel_tensor *input, const mlel_tensor *output, const mlel_tensor *scales, cudaStream_t s) {
+    const std::string call = "mlel_cuda_quantize_rows";
+    const Operand in = operandOf(call, "input", input, 2), out = writtenOperandOf(call, "output", output, 2),
+                  sc = writtenOperandOf(call, "scales", scales, 1);
+    if (!isFloat(in.dtype)) {
+        throw UnsupportedError(call + ": input has to be f32, f16 or bf16");
+    }
+    wantType(call, "output", out, MLEL_I8, "int8");
+    wantType(call, "scales", sc, MLEL_F32, "f32");
+    if (out.dims[0] != in.dims[0] || out.dims[1] != in.dims[1] || sc.dims[0] != in.dims[0]) {
+        refuse(call, "the shapes of input, output and scales do not fit together");
+    }
+    if (in.dims[0] == 0) {
+        return MLEL_SUCCESS;
+    }
+    if (in.dims[1] == 0) {
+        refuse(call, "rows without elements have no scale");
+    }
+    wantCurrentDevice(call, "output", out.ptr);
+    const QuantizeParams p{in.ptr, reinterpret_cast<int8_t *>(out.ptr), reinterpret_cast<float *>(sc.ptr), in.strides[0], out.strides[0],
+                           int32_t(in.dims[0]), int32_t(in.dims[1])};
+    const bool wide = aligned(in.ptr, 16) && (in.strides[0] % 16 == 0 || p.rows == 1) && aligned(out.ptr, 8) &&
+                      (out.strides[0] % 8 == 0 || p.rows == 1);
+    return launchStatus(call.c_str(), in.dtype == MLEL_F32   ? launchType<float>(p, wide, s)
+                                      : in.dtype == MLEL_F16 ? launchType<__half>(p, wide, s)
+                                                             : launchType<__nv_bfloat16>(p, wide, s));
+}
+
+} // namespace mlel

@@ -1,0 +1,205 @@
+"""The operators of an 8-bit decoder layer on torch tensors: ``quantize_rows``, ``matmul_scaled``, ``QuantizedLinear`` and the
+paged int8 cache (``PagedCache``, ``PagedBatch``) with its attention.
+
+Thin calls of the direct entry points in include/mlel_b200.h (``mlel_cuda_quantize_rows`` and the following), which say what
+each computes.  Work is enqueued on torch's current stream of the tensors' device; nothing waits.  Every call may be captured
+into a CUDA graph.  What the library refuses raises ``MlelError``.
+"""
+from __future__ import annotations
+
+import ctypes
+import struct
+
+import torch
+
+from . import BF16, F16, F32, I8, I32, check, lib
+from .runtime import _current_stream
+
+_DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8, torch.int32: I32}
+_TENSOR = struct.Struct("=Qii6q6q")  # mlel_tensor: address, type, rank, sizes, strides in bytes
+_SIX = (0,) * 6
+
+_entry = {}
+
+
+def _call(name: str, argtypes):
+    """An entry point with its argument types set, in a function object of this module's own."""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = lib()[name]
+        fn.argtypes, fn.restype = argtypes, ctypes.c_int
+        _entry[name] = fn
+    return fn
+
+
+_P, _V, _I, _F, _U64 = ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_uint64
+
+
+def _pack(t: torch.Tensor) -> bytes:
+    """``t`` as an mlel_tensor."""
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"tensors of {t.dtype} are not taken")
+    shape, rank = t.shape, t.dim()
+    if rank > 6:
+        raise ValueError("tensors of more than 6 axes are not taken")
+    if t.is_contiguous():
+        return _TENSOR.pack(t.data_ptr(), code, rank, *shape, *_SIX[rank:], *_SIX)
+    size = t.element_size()
+    strides = [size * n for n in t.stride()]
+    if strides[0] == 0:  # a stride of 0 there stands for a packed tensor
+        if shape[0] > 1:
+            raise ValueError("a tensor that repeats along its first axis is not taken")
+        strides[0] = size * max(1, t.numel())
+    return _TENSOR.pack(t.data_ptr(), code, rank, *shape, *_SIX[rank:], *strides, *_SIX[rank:])
+
+
+def _device(*tensors) -> int:
+    """The one CUDA device of all tensors (None among them are passed over)."""
+    device = tensors[0].device
+    if device.type != "cuda":
+        raise ValueError("tensors have to be on a CUDA device: there is no CPU implementation to fall back to")
+    for t in tensors[1:]:
+        if t is not None and t.device != device:
+            raise ValueError("tensors of one call have to be on one device")
+    return device.index
+
+
+class _on:
+    """Makes ``index`` the current device for the calls inside."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, index: int):
+        self.index = index
+
+    def __enter__(self):
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return _current_stream(self.index)
+
+    def __exit__(self, *_):
+        if self.before != self.index:
+            torch.cuda.set_device(self.before)
+
+
+def quantize_rows(x: torch.Tensor, out: torch.Tensor | None = None, scales: torch.Tensor | None = None):
+    """``(q, scales)``: the rows of ``x`` [..., K] (f32, f16 or bf16) in 8 bits with an f32 scale for each: ``scales = max|x| / 127``,
+    ``q = round(x / scales)``.  ``out`` and ``scales`` are written where they are given ([M, K] int8 and [M], for M rows in all)."""
+    if x.dim() < 1:
+        raise ValueError("x needs an axis")
+    rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    index = _device(x, out, scales)
+    q = torch.empty(rows.shape, dtype=torch.int8, device=x.device) if out is None else out
+    s = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device) if scales is None else scales
+    with _on(index) as stream:
+        check(_call("mlel_cuda_quantize_rows", (_P, _P, _P, _V))(_pack(rows), _pack(q), _pack(s), stream))
+    return (q if out is not None else q.view(x.shape)), (s if scales is not None else s.view(x.shape[:-1]))
+
+
+def matmul_scaled(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch.Tensor | None = None,
+                  out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``(a @ b.T) * a_scales[:, None] * b_scales + bias`` for int8 ``a`` [M, K] (tokens) and ``b`` [N, K] (weights, a row per
+    output channel), scales and bias in f32: the sums are exact, the result is rounded once to ``dtype`` (or ``out``'s type)."""
+    index = _device(a, a_scales, b, b_scales, bias, out)
+    if out is None:
+        out = torch.empty(a.shape[0], b.shape[0], dtype=dtype, device=a.device)
+    with _on(index) as stream:
+        check(_call("mlel_cuda_matmul_scaled", (_P,) * 6 + (_V,))(_pack(a), _pack(a_scales), _pack(b), _pack(b_scales),
+                                                               None if bias is None else _pack(bias), _pack(out), stream))
+    return out
+
+
+class QuantizedLinear:
+    """A projection in 8 bits: ``linear(x)`` quantises the rows of ``x`` [..., K] and multiplies them with int8 ``weight`` [N, K],
+    one f32 scale per output channel, optional f32 bias; the result has ``x``'s type.  The weights are laid out once: rows on
+    16-byte boundaries (copied only where they are not there already)."""
+
+    def __init__(self, weight: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None):
+        _device(weight, scales, bias)
+        n, k = weight.shape
+        self.padded = (k + 15) // 16 * 16
+        if weight.stride(1) != 1 or weight.stride(0) % 16 != 0 or weight.data_ptr() % 16 != 0:
+            rows = torch.zeros(n, self.padded, dtype=torch.int8, device=weight.device)
+            rows[:, :k] = weight
+            weight = rows[:, :k]
+        self.weight, self.scales, self.bias = weight, scales.contiguous(), None if bias is None else bias.contiguous()
+        self.in_features, self.out_features = k, n
+
+    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"x has {x.shape[-1]} features, not {self.in_features}")
+        rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        q = torch.empty(rows.shape[0], self.padded, dtype=torch.int8, device=x.device)[:, :self.in_features]
+        s = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device)
+        quantize_rows(rows, q, s)
+        y = matmul_scaled(q, s, self.weight, self.scales, self.bias, dtype=x.dtype)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], self.out_features)
+
+
+class PagedBatch:
+    """The sequences of one call: new tokens of sequence b are rows ``starts[b]`` to ``starts[b + 1] - 1`` of the token axis and the last
+    of its ``lengths[b]`` tokens; token t lies in page ``page_table[b, t // page]``.  All int32 on the device; ``max_new`` and
+    ``max_length`` are bounds that the host knows."""
+
+    def __init__(self, starts: torch.Tensor, lengths: torch.Tensor, page_table: torch.Tensor, max_new: int, max_length: int):
+        self.device = _device(starts, lengths, page_table)
+        self.starts, self.lengths, self.page_table = starts, lengths, page_table
+        self.max_new, self.max_length = int(max_new), int(max_length)
+        self._packed = (_pack(starts) + _pack(lengths) + _pack(page_table) + struct.pack("=ii", self.max_new, self.max_length))
+
+
+class PagedCache:
+    """Keys and values of a layer, int8 with a scale for each page and head.  ``data`` [2, pages, heads, page, head_dim] and
+    ``scales`` f32 [2, pages, heads]: keys first, then values."""
+
+    def __init__(self, data: torch.Tensor, scales: torch.Tensor):
+        if data.dim() != 5 or data.shape[0] != 2 or scales.shape != data.shape[:3]:
+            raise ValueError("data has to be [2, pages, heads, page, head_dim] and scales [2, pages, heads]")
+        self.device = _device(data, scales)
+        self.data, self.scales = data, scales
+        self._packed = _pack(data[0]) + _pack(data[1]) + _pack(scales[0]) + _pack(scales[1])
+
+    @classmethod
+    def empty(cls, pages: int, heads: int, page: int, head_dim: int, device="cuda") -> "PagedCache":
+        return cls(torch.zeros(2, pages, heads, page, head_dim, dtype=torch.int8, device=device),
+                   torch.zeros(2, pages, heads, dtype=torch.float32, device=device))
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor | None, sin: torch.Tensor | None, batch: PagedBatch,
+               q: torch.Tensor | None = None, q_out: torch.Tensor | None = None, interleaved: bool = False):
+        """Writes new keys and values [tokens, heads, head_dim] into the cache, the keys rotated by their positions; ``cos`` and ``sin``
+        are [positions, rotated / 2], or None for no rotation.  Returns the rotated queries where ``q`` is given (``q_out``, which may
+        be ``q`` itself, or a new tensor, in which rows of no sequence are undefined)."""
+        index = _device(self.data, k, v, cos, sin, q, q_out, batch.starts)
+        if q is not None and q_out is None:
+            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        with _on(index) as stream:
+            check(_call("mlel_cuda_paged_append", (_P,) * 8 + (_I, _V))(
+                self._packed, batch._packed, _pack(k), _pack(v), None if cos is None else _pack(cos), None if sin is None else _pack(sin),
+                None if q is None else _pack(q), None if q_out is None else _pack(q_out), int(interleaved), stream))
+        return q_out
+
+    def attend(self, q: torch.Tensor, batch: PagedBatch, out: torch.Tensor | None = None, scale: float | None = None, causal: bool = True,
+               window: int = 0, softcap: float = 0.0) -> torch.Tensor:
+        """Attention of the new tokens' queries [tokens, query_heads, head_dim] over the cache, which holds the new tokens already.
+        ``scale`` defaults to head_dim ** -0.5; rows of no sequence are left as they are in ``out``, undefined in a new tensor."""
+        index = _device(self.data, q, out, batch.starts)
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        packed_q = _pack(q)
+        need = ctypes.c_uint64()
+        check(_call("mlel_paged_attention_workspace", (_P, _P, _P, _V))(self._packed, batch._packed, packed_q, ctypes.addressof(need)))
+        space = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+        with _on(index) as stream:
+            check(_call("mlel_cuda_paged_attention", (_P, _P, _P, _P, _F, _I, _I, _F, _V, _U64, _V))(
+                self._packed, batch._packed, packed_q, _pack(out), q.shape[-1] ** -0.5 if scale is None else scale, int(causal),
+                int(window), float(softcap), space.data_ptr() if space is not None else None, need.value, stream))
+        return out
+
+
+def paged_error(device: int | None = None) -> int:
+    """0, or what the cache's kernels left out on the device since the last call: 1 a sequence whose numbers contradict the batch's
+    bounds, 2 a page outside the cache.  Waits for the device and clears the record."""
+    with _on(torch.cuda.current_device() if device is None else device):
+        return lib().mlel_paged_error()

@@ -425,6 +425,83 @@ int mlel_cuda_conv2d_static_scratch(const mlel_tensor *input, const mlel_tensor 
                                     const int32_t dilation[2], int32_t input_zp, int32_t weight_zp,
                                     void *cuda_stream);
 
+/* ---- 8-bit decoder layers (no counterpart in the reference, whose RESCALE has constant scales and which keeps nothing
+ * between dispatches) ----
+ * For programs that serve a language model next to the integer graphs above: activations quantised per token at run time,
+ * their products with int8 weights, and a paged int8 cache of keys and values with the attention that reads it.
+ *
+ * Operands are device tensors on the current device; work is enqueued on `cuda_stream`, nothing is allocated or waited for, and
+ * every call may be captured into a CUDA graph.  The elements of a tensor's last axis lie side by side; the other axes may
+ * have any positive stride where nothing else is said, and outputs must not overlap themselves or an input.  A refused
+ * call (MLEL_ERROR_UNKNOWN, or MLEL_ERROR_FEATURE_NOT_PRESENT for a type or size that is not built) has enqueued nothing. */
+
+/* Rows in 8 bits: scales[m] = max_k |input[m][k]| / 127 and output[m][k] = input[m][k] / scales[m] to the nearest whole number
+ * (ties to the even one).  input [M, K] f32, f16 or bf16; output [M, K] int8; scales [M] f32.  A row of zeros has scale 0.  A row
+ * that holds an infinity or a NaN has that as its scale and zeros as output: what is computed from it is NaN. */
+int mlel_cuda_quantize_rows(const mlel_tensor *input, const mlel_tensor *output, const mlel_tensor *scales, void *cuda_stream);
+
+/* Product in 8-bit integers with a scale for each token and channel:
+ *   output[m][n] = (sum_k a[m][k] * b[n][k]) * a_scales[m] * b_scales[n] + biases[n]
+ * The sum is exact (K at most 131071); the rest is computed in f32 and rounded once to the output's type.  a [M, K] int8 (tokens),
+ * b [N, K] int8 (weights, a row per output channel), a_scales [M], b_scales [N], biases [N] or NULL, all packed f32; output
+ * [M, N] f32, f16 or bf16.  Rows of a and b that start on 16-byte boundaries go the fast way. */
+int mlel_cuda_matmul_scaled(const mlel_tensor *a, const mlel_tensor *a_scales, const mlel_tensor *b, const mlel_tensor *b_scales,
+                            const mlel_tensor *biases, const mlel_tensor *output, void *cuda_stream);
+
+/* Keys and values of a decoder layer in pages of `page` tokens (a multiple of 16, at most 256), 8 bits each, with one scale for
+ * each page and head: the value is the int8 element times the scale.  head_dim is a multiple of 16, at most 256. */
+typedef struct mlel_paged_cache {
+    mlel_tensor keys, values;             /* int8 [pages, heads, page, head_dim], packed, on 16-byte boundaries */
+    mlel_tensor key_scales, value_scales; /* f32 [pages, heads], packed */
+} mlel_paged_cache;
+
+/* Sequences of one call and where their tokens lie.  The new tokens of all sequences stand one after another in the token
+ * axis; those of sequence b are rows starts[b] .. starts[b + 1] - 1 (none at all is allowed).  lengths[b] counts the
+ * tokens of the sequence with the new ones, which are its last.  Token t of sequence b is row t % page of page
+ * page_table[b][t / page]; entries past the last token are not read.  Rows of the token axis outside starts[0] ..
+ * starts[sequences] are neither read nor written.  max_new and max_length bound the new tokens and the lengths of any
+ * sequence of the call; closer bounds make better launches.
+ * starts, lengths and page_table are read on the device.  A sequence whose numbers contradict these bounds or the shapes is left
+ * out as a whole (its rows are not written), a page outside the cache by itself (nothing is written there, and its tokens are not
+ * attended to); mlel_paged_error() tells of both. */
+typedef struct mlel_paged_batch {
+    mlel_tensor starts;     /* i32 [sequences + 1], packed */
+    mlel_tensor lengths;    /* i32 [sequences], packed */
+    mlel_tensor page_table; /* i32 [sequences, at least max_length / page rounded up] */
+    int32_t max_new, max_length;
+} mlel_paged_batch;
+
+/* Writes the new tokens' keys and values into the cache, the keys rotated by their positions, and rotates the queries.
+ * keys, values [tokens, heads, head_dim] f16 or bf16; cosines, sines [positions, rotated / 2] f32, positions at least
+ * max_length, rotated an even number up to head_dim: the element pairs (i, i + rotated / 2), or (2 i, 2 i + 1) with `interleaved`, of
+ * a head's first `rotated` elements become (x cos - y sin, y cos + x sin) of row `position`; the other elements stay.
+ * queries, rotated_queries [tokens, query_heads, head_dim] of the keys' type, both NULL where there is nothing to rotate; they may
+ * be the same tensor.  cosines and sines NULL: no rotation.
+ * A page's scale is max |element| / 127 over what is in it.  Where new tokens join older ones in a page and have larger
+ * elements, its older integers are rescaled once, to the nearest whole numbers.  A page whose first row is new starts afresh.
+ * New tokens with an infinity or a NaN make the page's scale that, and with it all that reads the page NaN.
+ * A page that receives tokens belongs to one sequence; pages that are only read may be shared. */
+int mlel_cuda_paged_append(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *keys,
+                           const mlel_tensor *values, const mlel_tensor *cosines, const mlel_tensor *sines,
+                           const mlel_tensor *queries, const mlel_tensor *rotated_queries, int interleaved, void *cuda_stream);
+
+/* Attention of the new tokens over the cache, which holds them already:
+ *   s_j = scale * q . k_j;  with softcap > 0: s_j = softcap * tanh(s_j / softcap);  output = sum_j softmax(s)_j v_j
+ * over the tokens j of the query's own sequence: all of them, or with `causal` those up to the query's own position p; with
+ * window > 0 only j > p - window.  queries, output [tokens, query_heads, head_dim], both f16 or both bf16; query_heads a multiple of
+ * the cache's heads, query head h reads cache head h / (query_heads / heads).  The products run in f16 with f32 sums; the softmax
+ * is in f32.  `workspace`: mlel_paged_attention_workspace() bytes of device memory on a 16-byte boundary that nothing else uses
+ * until the call's work is done (its contents do not matter before or after). */
+int mlel_cuda_paged_attention(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries,
+                              const mlel_tensor *output, float scale, int causal, int32_t window, float softcap, void *workspace,
+                              uint64_t workspace_bytes, void *cuda_stream);
+/* Bytes of workspace that a call with these operands wants (0: none); no device is needed. */
+int mlel_paged_attention_workspace(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries,
+                                   uint64_t *bytes);
+/* What the kernels of the paged cache left out on the current device since the last call: 0 nothing, 1 a sequence whose starts or
+ * lengths contradict the bounds or shapes, 2 a page outside the cache.  Synchronises the device and clears the record. */
+int mlel_paged_error(void);
+
 #ifdef __cplusplus
 }
 #endif

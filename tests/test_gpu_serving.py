@@ -1,0 +1,524 @@
+"""The 8-bit decoder layer's operators against their definitions in 64 bits (tests/serving_ref.py)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from tests import serving_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture()
+def serving(mlel):
+    from mlel_b200 import serving
+    assert serving.paged_error() == 0
+    yield serving
+    assert serving.paged_error() == 0
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def sentinel(*shape, dtype=torch.int8):
+    return torch.full(shape, 77, dtype=dtype, device="cuda")
+
+
+# ---------------------------------------------------------------- rows in 8 bits
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m, k", [(1, 1), (1, 7), (3, 8), (5, 257), (9, 1024), (2, 1025), (33, 2560), (4, 4096), (3, 4100), (2, 8192),
+                                  (2, 8200), (1, 33000), (1000, 64)])
+def test_quantize_rows(serving, dtype, m, k):
+    x = (randn(gen(m * 10007 + k), m, k) * 3).to(DTYPES[dtype])
+    x[m // 2, k // 2] = 300
+    q, s = serving.quantize_rows(x)
+    want_q, want_s = ref.quantize_rows(x)
+    assert np.array_equal(s.cpu().numpy(), want_s)
+    assert np.array_equal(q.cpu().numpy(), want_q)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantize_rows_ties_and_extremes(serving, dtype):
+    t = DTYPES[dtype]
+    x = torch.zeros(9, 64, dtype=t, device="cuda")
+    x[0] = torch.arange(64, device="cuda").to(t) - 31.5
+    x[0, 0] = 127  # scale 1: every other element lies in the middle between two integers
+    x[1] = (torch.arange(64, device="cuda") * 3 - 94.5).to(t)
+    x[1, 0] = -381  # scale 3, whose inverse is rounded
+    x[3] = torch.finfo(t).smallest_normal * torch.finfo(t).eps  # the smallest magnitude there is
+    x[4] = torch.finfo(t).max
+    x[4, ::2] = -torch.finfo(t).max
+    x[5, 5] = float("nan")
+    x[6, 6] = float("-inf")
+    x[6, 7] = 3
+    x[7, 3] = -0.0
+    x[8] = 1e-4
+    q, s = serving.quantize_rows(x)
+    want_q, want_s = ref.quantize_rows(x)
+    assert np.array_equal(s.cpu().numpy(), want_s, equal_nan=True)
+    assert np.array_equal(q.cpu().numpy(), want_q)
+    assert torch.isnan((q.float() * s[:, None])[5]).all() and torch.isnan((q.float() * s[:, None])[6]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("offset, stride", [(0, 200), (1, 173), (8, 184), (3, 170)])
+def test_quantize_rows_strided(serving, dtype, offset, stride):
+    """Rows at any address on both sides; what lies between the output's rows stays."""
+    m, k = 7, 170
+    base = (randn(gen(offset + stride), m * stride + offset) * 2).to(DTYPES[dtype])
+    x = base[offset:].as_strided((m, k), (stride, 1))
+    store, scales = sentinel(m * stride + offset), torch.full((2 * m,), -1.0, device="cuda")
+    q = store[offset:].as_strided((m, k), (stride, 1))
+    serving.quantize_rows(x, q, scales[:m])
+    want_q, want_s = ref.quantize_rows(x)
+    assert np.array_equal(q.cpu().numpy(), want_q) and np.array_equal(scales[:m].cpu().numpy(), want_s)
+    untouched = torch.ones_like(store, dtype=torch.bool)
+    untouched[offset:].as_strided((m, k), (stride, 1))[:] = False
+    assert (store[untouched] == 77).all() and (scales[m:] == -1).all()
+
+
+# ---------------------------------------------------------------- scaled products
+
+def product_operands(seed, m, n, k, bias, extreme=False):
+    g = gen(seed)
+    def ints(r):
+        if extreme:
+            return torch.where(torch.rand(r, k, generator=g, device="cuda") < 0.5, -128, -127).to(torch.int8)
+        return torch.randint(-128, 128, (r, k), generator=g, device="cuda", dtype=torch.int8)
+    return (ints(m), torch.rand(m, generator=g, device="cuda") * 0.01, ints(n), torch.rand(n, generator=g, device="cuda") * 0.01,
+            randn(g, n) if bias else None)
+
+
+def check_product(serving, operands, dtype, out=None, tag=""):
+    y = serving.matmul_scaled(*operands, out=out, dtype=dtype)
+    want, off = ref.matmul_scaled(*operands)
+    bound = off + ref.half_step(dtype) * (np.abs(want) + off) + ref.smallest_half_step(dtype)
+    wrong = np.abs(ref.f64(y) - want) > bound
+    assert not wrong.any(), (tag, int(wrong.sum()), np.argwhere(wrong)[:4].tolist(), np.argwhere(wrong)[-1].tolist())
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 1, 1), (1, 16, 16), (2, 130, 48), (3, 128, 128), (8, 257, 144), (16, 384, 2048), (17, 96, 300),
+                                     (33, 1000, 512), (64, 256, 4096), (65, 129, 127), (100, 515, 1040), (128, 256, 256), (129, 257, 129),
+                                     (256, 512, 128), (300, 77, 640), (511, 384, 96), (700, 1100, 272), (2000, 264, 160), (40, 8192, 1040)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_matmul_scaled(serving, dtype, m, n, k):
+    check_product(serving, product_operands(m + n + k, m, n, k, (m + n) % 2 == 0), DTYPES[dtype])
+
+
+@pytest.mark.parametrize("m", [1, 5, 32, 63, 200, 300])
+def test_matmul_scaled_longest_sums(serving, m):
+    """Sums that fill 32-bit integers (131071 * 128 * 128 is 2^31 - 16384)."""
+    check_product(serving, product_operands(m, m, 130, 131071 // 16 * 16, True, extreme=True), torch.float32)
+
+
+@pytest.mark.parametrize("m, n, k", [(1, 50, 33), (5, 300, 257), (70, 130, 1001), (300, 520, 77), (20, 64, 20000)])
+@pytest.mark.parametrize("a_off, b_off, out_off", [(0, 0, 0), (1, 0, 0), (0, 3, 0), (16, 32, 1), (5, 7, 3)])
+def test_matmul_scaled_strided(serving, m, n, k, a_off, b_off, out_off):
+    """Rows at any address; what lies between the output's rows stays."""
+    a, sa, b, sb, bias = product_operands(m * 31 + n, m, n, k, True)
+    def place(t, offset):
+        stride = (t.shape[1] + 15) // 16 * 16 + (offset % 16)
+        store = sentinel(t.shape[0] * stride + offset)
+        view = store[offset:].as_strided(t.shape, (stride, 1))
+        view.copy_(t)
+        return view
+    store = torch.full((m * (n + 8) + out_off,), 77.0, device="cuda", dtype=torch.bfloat16)
+    out = store[out_off:].as_strided((m, n), (n + 5 if out_off else (n + 7) // 8 * 8, 1))
+    check_product(serving, (place(a, a_off), sa, place(b, b_off), sb, bias), torch.bfloat16, out)
+    mask = torch.ones_like(store, dtype=torch.bool)
+    mask[out_off:].as_strided(out.shape, out.stride())[:] = False
+    assert (store[mask] == 77).all()
+
+
+def test_matmul_scaled_scales_that_are_not_finite(serving):
+    a, sa, b, sb, _ = product_operands(5, 40, 150, 64, False)
+    sa[3], sa[7], sb[100] = float("nan"), float("inf"), float("inf")
+    y = serving.matmul_scaled(a, sa, b, sb, dtype=torch.float32).double()
+    p = a.double() @ b.double().t()
+    want = p * sa.double()[:, None] * sb.double()[None, :]
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+
+
+@pytest.mark.parametrize("shape", [(1, 100), (3, 100), (2, 3, 128), (130, 333), (4, 2064)])
+def test_quantized_linear(serving, shape):
+    g = gen(sum(shape))
+    x, n, k = randn(g, *shape).to(torch.float16), 75, shape[-1]
+    w = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    ws, bias = torch.rand(n, generator=g, device="cuda") * 0.01, randn(g, n)
+    y = serving.QuantizedLinear(w, ws, bias)(x)
+    assert y.shape == (*shape[:-1], n) and y.dtype == x.dtype
+    q, s = ref.quantize_rows(x.reshape(-1, k))
+    want, off = ref.matmul_scaled(torch.from_numpy(q), torch.from_numpy(s), w, ws, bias)
+    bound = off + ref.half_step(x.dtype) * (np.abs(want) + off) + ref.smallest_half_step(x.dtype)
+    assert (np.abs(ref.f64(y).reshape(-1, n) - want) <= bound).all()
+
+
+# ---------------------------------------------------------------- the paged cache
+
+class Paged:
+    """A cache with random contents and a batch over it, the sequences given as (new tokens, length)."""
+
+    def __init__(self, serving, seed, sequences, heads, page, d, skip=0, behind=0, wild=True):
+        g = gen(seed)
+        fresh = [n for n, _ in sequences]
+        self.starts = [skip + sum(fresh[:i]) for i in range(len(fresh) + 1)]
+        self.lengths = [l for _, l in sequences]
+        self.tokens = self.starts[-1] + behind
+        needed = [-(-l // page) for l in self.lengths]
+        pages = sum(needed) + 2
+        order = torch.randperm(pages, generator=torch.Generator().manual_seed(seed)).tolist()
+        self.table, at = [], 0
+        for n in needed:
+            # entries that no token needs are not read
+            self.table.append(order[at:at + n] + [-5, 1 << 30, 0][:max(needed) + 1 - n] + [-1] * max(0, max(needed) - 2 - n))
+            at += n
+        width = max(len(r) for r in self.table) if self.table else 1
+        self.table = [r + [-7] * (width - len(r)) for r in self.table]
+        self.data = torch.randint(-127, 128, (2, pages, heads, page, d), generator=g, device="cuda", dtype=torch.int8)
+        self.scales = (0.3 + torch.rand(2, pages, heads, generator=g, device="cuda")) / 60
+        if wild:  # scales of pages may differ by orders of magnitude
+            self.scales *= 10.0 ** torch.randint(-2, 2, self.scales.shape, generator=g, device="cuda")
+        self.spare = order[at:]
+        self.scales[:, self.spare] = float("nan")  # pages of nobody
+        self.cache = serving.PagedCache(self.data, self.scales)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        table = torch.tensor(self.table, **i32).reshape(len(sequences), width)
+        self.batch = serving.PagedBatch(torch.tensor(self.starts, **i32), torch.tensor(self.lengths, **i32), table, max(fresh, default=0),
+                                        max(self.lengths, default=0))
+        self.g, self.heads, self.page, self.d = g, heads, page, d
+
+    def arrays(self):
+        return self.data.cpu().numpy(), self.scales.cpu().numpy(), self.starts, self.lengths, self.table
+
+
+MIXED = [(1, 1), (0, 0), (3, 3), (1, 16), (1, 17), (0, 40), (20, 49), (1, 100), (16, 16), (70, 150)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("page, d, rot, interleaved", [(16, 64, 64, False), (16, 128, 64, True), (48, 80, 80, False), (64, 256, 128, False),
+                                                       (256, 16, 16, True), (32, 96, 0, False)])
+def test_append(serving, dtype, page, d, rot, interleaved):
+    t, heads, hq = DTYPES[dtype], 3, 6
+    p = Paged(serving, page + d, MIXED, heads, page, d, skip=2, behind=3, wild=False)
+    wide = randn(p.g, p.tokens, (hq + 2 * heads) * d + 8).to(t)  # one projection's output holds all three
+    q, k, v = (wide[:, 8 + a * d:8 + b * d].unflatten(1, (-1, d)) for a, b in [(0, hq), (hq, hq + heads), (hq + heads, hq + 2 * heads)])
+    k[2:][::7] *= 30  # some tokens make their page's scale grow
+    v[2:][::5] *= 0.01
+    angle = torch.arange(200, device="cuda")[:, None] * torch.rand(rot // 2, generator=p.g, device="cuda")
+    cos, sin = (angle.cos(), angle.sin()) if rot else (None, None)
+    before = p.arrays()
+    kept = q.clone()
+    out = torch.full((p.tokens, hq, d), 77.0, dtype=t, device="cuda")
+    got = p.cache.append(k, v, cos, sin, p.batch, q=q, q_out=out, interleaved=interleaved)
+    assert got is out
+    c, s = (None, None) if not rot else (ref.f64(cos), ref.f64(sin))
+    want, want_scales = ref.append(*before, ref.f64(k), ref.f64(v), c, s, interleaved)
+    assert np.array_equal(p.scales.cpu().numpy(), want_scales, equal_nan=True)
+    assert np.array_equal(p.data.cpu().numpy(), want)
+    x, inside = ref.f64(kept), slice(p.starts[0], p.starts[-1])
+    y, off = x.copy(), np.zeros_like(x)
+    for b, length in enumerate(p.lengths):
+        for i in range(p.starts[b], p.starts[b + 1]):
+            if rot:
+                position = length - p.starts[b + 1] + i
+                y[i] = ref.rotate(x[i], c[position], s[position], interleaved)
+                off[i] = 2.0 ** -23 * np.abs(x[i]).max()  # a product and a fused sum of two terms
+    bound = off + ref.half_step(t) * (np.abs(y) + off) + ref.smallest_half_step(t)
+    assert (np.abs(ref.f64(out) - y) <= bound)[inside].all()
+    assert (out[:p.starts[0]] == 77).all() and (out[p.starts[-1]:] == 77).all()
+    # in place, and again: the same integers, since nothing grows any more
+    p.cache.append(k, v, cos, sin, p.batch, q=q, q_out=q, interleaved=interleaved)
+    assert torch.equal(q[inside], out[inside]) and torch.equal(q[:2], kept[:2])
+    assert np.array_equal(p.data.cpu().numpy(), want)
+
+
+def test_append_what_is_not_finite(serving):
+    """An infinity or a NaN makes the scale of its page and head that; other heads and pages do not notice."""
+    p = Paged(serving, 5, [(20, 24), (4, 9)], 2, 16, 32, wild=False)
+    k, v = randn(p.g, p.tokens, 2, 32).half(), randn(p.g, p.tokens, 2, 32).half()
+    k[3, 0, 5], v[15, 1, 0] = float("nan"), float("-inf")
+    before = p.arrays()
+    p.cache.append(k, v, None, None, p.batch)
+    want, want_scales = ref.append(*before, ref.f64(k), ref.f64(v), None, None, False)
+    got = p.scales.cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want_scales)) and np.array_equal(np.isinf(got), np.isinf(want_scales))
+    fine = np.isfinite(want_scales)
+    assert np.array_equal(got[fine], want_scales[fine])
+    assert np.array_equal(p.data.cpu().numpy()[fine], want[fine])
+
+
+def test_append_zeros_and_growth_by_a_little(serving):
+    """Zeros alone give a scale of 0; a scale that grows by one unit in its last place leaves the integers."""
+    p = Paged(serving, 6, [(1, 5)], 1, 16, 16, wild=False)
+    slot = p.table[0][0]
+    p.scales[:, slot] = 0
+    zero = torch.zeros(1, 1, 16, dtype=torch.float16, device="cuda")
+    p.cache.append(zero, zero, None, None, p.batch)
+    assert (p.scales[:, slot] == 0).all() and (p.data[:, slot, 0, 4] == 0).all()
+    one = torch.ones(1, 1, 16, dtype=torch.float16, device="cuda")
+    now = np.float32(1 / 127)
+    p.scales[:, slot] = float(np.nextafter(now, np.float32(0)))
+    before = p.data.clone()
+    p.cache.append(one, one, None, None, p.batch)
+    assert (p.scales[:, slot] == float(now)).all()
+    assert torch.equal(p.data[:, slot, 0, :4], before[:, slot, 0, :4]) and (p.data[:, slot, 0, 4] == 127).all()
+
+
+def check_attention(serving, p, q, out, dtype, **how):
+    got = p.cache.attend(q, p.batch, out=out, **how)
+    assert got is out
+    want, bound = ref.attend(*p.arrays(), ref.f64(q), how.get("scale") or p.d ** -0.5, how.get("causal", True), how.get("window", 0),
+                             how.get("softcap", 0.0), dtype)
+    got = ref.f64(out)
+    left = np.isnan(want)
+    assert (got[left] == 77).all()
+    wrong = ~(np.abs(got - want) <= bound) & ~left
+    assert not wrong.any(), (int(wrong.sum()), np.argwhere(wrong)[:4].tolist(), np.argwhere(wrong)[-1].tolist(),
+                             float(np.nanmax(np.where(wrong, np.abs(got - want) / np.maximum(bound, 1e-30), 0))))
+
+
+def query(p, heads, t, loud=1.0):
+    """Queries as part of a projection's output, and where the answer goes: rows apart, heads apart."""
+    q = (randn(p.g, p.tokens, heads, p.d + 8) * loud).to(t)[..., :p.d]
+    store = torch.full((p.tokens, heads + 1, p.d + 16), 77.0, dtype=t, device="cuda")
+    return q, store[:, 1:, 8:8 + p.d]
+
+
+DECODE = [(1, 1), (1, 2), (0, 30), (1, 16), (1, 17), (1, 63), (1, 64), (1, 65), (1, 200), (0, 0), (1, 1000)]
+FEW = [(2, 2), (3, 70), (0, 9), (5, 5), (1, 300), (4, 129)]
+CHUNKS = [(40, 40), (1, 70), (130, 200), (17, 400), (0, 3), (64, 64), (129, 129)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads, group", [(2, 1), (2, 4), (1, 5), (1, 16), (1, 20), (2, 40)])
+@pytest.mark.parametrize("page, d", [(16, 64), (64, 128), (48, 80), (32, 256), (256, 16), (16, 96)])
+def test_attention_single_tokens(serving, dtype, heads, group, page, d):
+    t = DTYPES[dtype]
+    p = Paged(serving, heads * group + page + d, DECODE, heads, page, d, skip=1, behind=2)
+    check_attention(serving, p, *query(p, heads * group, t, 2.0), t)
+
+
+@pytest.mark.parametrize("sequences", [FEW, CHUNKS], ids=["few", "chunks"])
+@pytest.mark.parametrize("how", [{}, {"causal": False}, {"window": 1}, {"window": 37}, {"softcap": 3.0}, {"scale": -0.3},
+                                 {"window": 100, "causal": False, "softcap": 20.0}], ids=str)
+@pytest.mark.parametrize("group, page, d", [(4, 16, 128), (3, 32, 64), (1, 64, 256), (8, 48, 80)])
+def test_attention_masks(serving, sequences, how, group, page, d):
+    t = torch.float16 if group % 2 else torch.bfloat16
+    p = Paged(serving, group + page + d, sequences, 2, page, d, skip=1, behind=1)
+    check_attention(serving, p, *query(p, 2 * group, t, 2.0), t, **how)
+
+
+@pytest.mark.parametrize("fresh, length, heads, group, d, page", [(300, 300, 1, 4, 128, 64), (257, 1000, 2, 1, 64, 16), (150, 150, 1, 8, 256, 128),
+                                                                  (1, 9000, 1, 8, 128, 16), (2, 5000, 2, 3, 64, 64)])
+def test_attention_long(serving, fresh, length, heads, group, d, page):
+    p = Paged(serving, fresh + length, [(fresh, length)], heads, page, d)
+    check_attention(serving, p, *query(p, heads * group, torch.bfloat16), torch.bfloat16)
+
+
+@pytest.mark.parametrize("sequences", [[(1, 300)], [(100, 300)]], ids=["one", "chunk"])
+def test_attention_one_key_has_all(serving, sequences):
+    """A score that drowns all others: the answer is that token's value; and thousands of others share what is left."""
+    p = Paged(serving, 77, sequences, 1, 16, 64, wild=False)
+    q, out = query(p, 2, torch.float16)
+    q[:] = 0
+    q[..., 0] = 100
+    p.data[0] = 0
+    p.data[0, p.table[0][3], 0, 5, 0] = 127
+    p.scales[0] = 1 / 127
+    check_attention(serving, p, q, out, torch.float16, causal=False, scale=1.0)
+
+
+def test_attention_what_is_not_finite_stays_with_its_rows(serving):
+    """A page without finite scales, and NaN queries: rows that the mask keeps from them are as they were."""
+    sequences = [(100, 160), (1, 200), (4, 64)]
+    p = Paged(serving, 3, sequences, 1, 16, 64, wild=False)
+    q, out = query(p, 4, torch.bfloat16)
+    other = torch.full_like(out, 77.0)
+    p.cache.attend(q, p.batch, out=out)
+    bad_at = 112  # the first row of a page of sequence 0
+    p.scales[:, p.table[0][bad_at // 16]] = float("nan")
+    q[70, 2] = float("nan")
+    p.cache.attend(q, p.batch, out=other)
+    for row in range(p.tokens):
+        position = 60 + row
+        touched = row < 100 and position >= bad_at
+        for h in range(4):
+            if touched or (row == 70 and h == 2):
+                assert torch.isnan(other[row, h]).all(), (row, h)
+            else:
+                assert torch.equal(other[row, h], out[row, h]), (row, h)
+    # a window of 20: row r attends to tokens 60 + r - 19 .. 60 + r, behind the page (112 .. 127) from r = 87 on
+    clean = torch.full_like(out, 77.0)
+    p.cache.attend(q, p.batch, out=clean, window=20)
+    assert torch.isfinite(clean[87:100]).all() and torch.isnan(clean[60:68]).all()
+
+
+@pytest.mark.parametrize("fresh", [1, 3, 150])
+def test_bad_numbers_are_left_out_and_told_of(serving, fresh):
+    """Sequences and pages that contradict the shapes: nothing is read or written there, the others are served."""
+    p = Paged(serving, 9, [(fresh, 170), (fresh, 180), (fresh, 190)], 2, 16, 64, wild=False)
+    q, out = query(p, 4, torch.float16)
+    check_attention(serving, p, q, out, torch.float16)
+    good = out.clone()
+    rows = [slice(p.starts[b], p.starts[b + 1]) for b in range(3)]
+    for field, index, value in [("lengths", 1, 200), ("lengths", 1, fresh - 1), ("lengths", 1, -4), ("starts", 3, p.tokens + 1)]:
+        keep = getattr(p.batch, field)[index].clone()
+        getattr(p.batch, field)[index] = value
+        out.fill_(77.0)
+        p.cache.attend(q, p.batch, out=out)
+        assert serving.paged_error() == 1
+        bad = 1 if field == "lengths" else 2
+        for b in range(3):
+            assert torch.equal(out[rows[b]], good[rows[b]] if b != bad else torch.full_like(out[rows[b]], 77.0)), (field, value, b)
+        data, scales = p.data.clone(), p.scales.clone()
+        k = randn(p.g, p.tokens, 2, 64).half()
+        p.cache.append(k, k, None, None, p.batch, q=q)
+        assert serving.paged_error() == 1
+        mine = [s for s in p.table[bad] if 0 <= s < p.data.shape[1]]
+        assert torch.equal(p.data[:, mine], data[:, mine])
+        p.data.copy_(data)
+        p.scales.copy_(scales)
+        getattr(p.batch, field)[index] = keep
+    # a page outside the cache: its tokens are not attended to
+    for value in (-1, p.data.shape[1], 1 << 30):
+        page = 2
+        keep = p.batch.page_table[1, page].clone()
+        p.batch.page_table[1, page] = value
+        out.fill_(77.0)
+        p.cache.attend(q, p.batch, out=out)
+        assert serving.paged_error() == 2
+        assert torch.equal(out[rows[0]], good[rows[0]]) and torch.equal(out[rows[2]], good[rows[2]])
+        p.batch.page_table[1, page] = keep
+        # the same tokens made negligible: keys that give scores far below all others are as good as none
+    last = (p.lengths[0] - 1) // 16
+    keep = p.batch.page_table[0, last].clone()
+    p.batch.page_table[0, last] = -3
+    data = p.data.clone()
+    k = randn(p.g, p.tokens, 2, 64).half()
+    p.cache.append(k, k, None, None, p.batch)
+    assert serving.paged_error() == 2
+    assert torch.equal(p.data[:, p.table[0][last]], data[:, p.table[0][last]])
+    p.batch.page_table[0, last] = keep
+
+
+# ---------------------------------------------------------------- together, and around them
+
+def test_layer_by_layer_decoding(serving):
+    """A prompt, then tokens one by one, against the same tokens in one go: projections, cache and attention as a program uses
+    them.  The integers of a page depend on the order of its tokens (its scale grows), so the two agree within the cache's steps."""
+    g = gen(1)
+    heads, hq, d, page, total = 2, 8, 64, 16, 75
+    x = randn(g, total, 512).half()
+    w = torch.randint(-127, 128, ((hq + 2 * heads) * d, 512), generator=g, device="cuda", dtype=torch.int8)
+    linear = serving.QuantizedLinear(w, torch.full((w.shape[0],), 0.0006, device="cuda"))
+    angle = torch.arange(total, device="cuda")[:, None] * 10000.0 ** (-torch.arange(d // 2, device="cuda") / (d // 2))
+    cos, sin = angle.cos().float(), angle.sin().float()
+    table = torch.tensor([[3, 0, 4, 1, 5]], dtype=torch.int32, device="cuda")
+
+    def step(cache, lo, hi):
+        y = linear(x[lo:hi])
+        q, k, v = (y[:, a * d:b * d].unflatten(1, (-1, d)) for a, b in ((0, hq), (hq, hq + heads), (hq + heads, hq + 2 * heads)))
+        batch = serving.PagedBatch(torch.tensor([0, hi - lo], dtype=torch.int32, device="cuda"),
+                                   torch.tensor([hi], dtype=torch.int32, device="cuda"), table, hi - lo, total)
+        q = cache.append(k, v, cos, sin, batch, q=q)
+        return q, v, cache.attend(q, batch)
+
+    whole, piece = serving.PagedCache.empty(6, heads, page, d), serving.PagedCache.empty(6, heads, page, d)
+    q, v, want = step(whole, 0, total)
+    parts = [step(piece, lo, hi)[2] for lo, hi in [(0, 40), (40, 41), (41, 43)] + [(i, i + 1) for i in range(43, total)]]
+    got = torch.cat(parts)
+    # integers of 1 / 127 of a page's largest element; rescaled ones are off by up to a step per growth
+    assert (got.float() - want.float()).abs().max() < 0.1 * v.abs().max()
+    assert torch.nn.functional.cosine_similarity(got.float().flatten(), want.float().flatten(), dim=0) > 0.999
+
+
+def test_capture_replay_and_other_streams(serving):
+    """Each call captured into a graph and replayed on new contents gives what the call itself gives, from a stream of its own."""
+    p = Paged(serving, 21, [(1, 130), (1, 700), (1, 20)], 2, 16, 64, wild=False)
+    g, hq = p.g, 8
+    linear = serving.QuantizedLinear(torch.randint(-127, 128, ((hq + 4) * 64, 256), generator=g, device="cuda", dtype=torch.int8),
+                                     torch.full(((hq + 4) * 64,), 0.001, device="cuda"))
+    x = randn(g, 3, 256).half()
+    angle = torch.rand(700, 32, generator=g, device="cuda")
+    cos, sin = angle.cos(), angle.sin()
+
+    def layer():
+        y = linear(x)
+        q, k, v = y[:, :hq * 64].unflatten(1, (-1, 64)), y[:, hq * 64:(hq + 2) * 64].unflatten(1, (-1, 64)), y[:, (hq + 2) * 64:].unflatten(1, (-1, 64))
+        return p.cache.attend(p.cache.append(k, v, cos, sin, p.batch, q=q), p.batch)
+
+    first = (p.data.clone(), p.scales.clone())
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        layer()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            held = layer()
+    torch.cuda.synchronize()
+    for seed in (1, 2):
+        x.copy_(randn(gen(seed), 3, 256).half())
+        p.data.copy_(first[0]), p.scales.copy_(first[1])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = held.clone()
+        p.data.copy_(first[0]), p.scales.copy_(first[1])
+        assert torch.equal(layer(), replayed)
+
+
+def test_two_streams_at_once(serving):
+    """Calls that run beside one another share nothing: the same results as one after another."""
+    jobs = []
+    for seed, sequences in enumerate(([(1, 900)] * 4, [(60, 600)], [(1, 3000)], [(3, 500)] * 3)):
+        p = Paged(serving, seed, sequences, 2, 16, 128)
+        jobs.append((p, query(p, 8, torch.float16)[0]))
+    want = [p.cache.attend(q, p.batch) for p, q in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = []
+    for _ in range(5):
+        for s, (p, q) in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(p.cache.attend(q, p.batch))
+    torch.cuda.synchronize()
+    for i, y in enumerate(got):
+        assert torch.equal(y, want[i % len(jobs)]), i
+
+
+def test_operands_are_where_they_are_said_to_be(mlel, serving):
+    """Host memory under a device tensor's name is refused before anything runs."""
+    x = torch.zeros(4, 64)
+    T, lib = mlel.device_tensor, mlel.lib()
+    rc = lib.mlel_cuda_quantize_rows(ctypes.byref(T(x.data_ptr(), mlel.F32, (4, 64))), ctypes.byref(T(x.data_ptr(), mlel.I8, (4, 64))),
+                                     ctypes.byref(T(x.data_ptr(), mlel.F32, (4,))), None)
+    assert rc == -13 and b"current device" in ctypes.c_char_p(lib.mlel_last_error()).value
+
+
+def test_offsets_beyond_32_bits(serving):
+    """A cache of over 4 GB: pages at both of its ends."""
+    heads, page, d = 8, 256, 256
+    pages = (1 << 32) // (heads * page * d) + 3
+    data = torch.zeros(2, pages, heads, page, d, dtype=torch.int8, device="cuda")
+    cache = serving.PagedCache(data, torch.zeros(2, pages, heads, device="cuda"))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for fresh in (1, 200):
+        batch = serving.PagedBatch(torch.tensor([0, fresh, 2 * fresh], **i32), torch.tensor([fresh, fresh], **i32),
+                                   torch.tensor([[0], [pages - 1]], **i32), fresh, fresh)
+        k, v, q = (randn(gen(fresh + i), 2 * fresh, heads, d).half() for i in range(3))
+        k[fresh:], v[fresh:], q[fresh:] = k[:fresh], v[:fresh], q[:fresh]
+        cache.append(k, v, None, None, batch)
+        y = cache.attend(q, batch)
+        assert torch.equal(data[:, 0], data[:, -1]) and (data[:, 0, :, :fresh] != 0).any()
+        assert torch.equal(y[:fresh], y[fresh:]) and y.abs().max() > 0
