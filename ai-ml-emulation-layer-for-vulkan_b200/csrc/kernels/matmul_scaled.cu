@@ -27,7 +27,8 @@ __device__ __forceinline__ uint32_t wordAt(const int8_t *row, int k, int length)
     return w;
 }
 
-template <class T> __global__ void __launch_bounds__(256) matmulScaledAnyRows(const ScaledProblem p) {
+template <class T>
+__global__ void __launch_bounds__(256) matmulScaledAnyRows(const ScaledProblem p) {
     __shared__ uint32_t tileA[kTile][kSlice + 1], tileB[kTile][kSlice + 1];
     dependencySync();
     const int m0 = int(blockIdx.y) * kTile, n0 = int(blockIdx.x) * kTile;

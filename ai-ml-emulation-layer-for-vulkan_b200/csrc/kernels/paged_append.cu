@@ -184,7 +184,8 @@ template <class T> __device__ __forceinline__ void rotateQueries(const AppendPar
     }
 }
 
-template <class T> __global__ void __launch_bounds__(2 * kSideThreads) pagedAppendKernel(const AppendParams p) {
+template <class T>
+__global__ void __launch_bounds__(2 * kSideThreads) pagedAppendKernel(const AppendParams p) {
     __shared__ unsigned long long partial[2 * kSideThreads / 32];
     dependencySync();
     if (int64_t(blockIdx.x) < p.unitBlocks) {

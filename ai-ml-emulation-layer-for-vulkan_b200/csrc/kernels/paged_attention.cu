@@ -26,7 +26,8 @@ struct AttendParams {
     int32_t causal, window, queryHeads, group;
 };
 
-template <class T> __global__ void __launch_bounds__(256) pagedAttentionSimple(const AttendParams p) {
+template <class T>
+__global__ void __launch_bounds__(256) pagedAttentionSimple(const AttendParams p) {
     dependencySync();
     const int index = int(blockIdx.x), lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
     const Sequence q = sequenceOf(p.batch, index);
