@@ -976,15 +976,16 @@ int waitTimeoutSelfTest(cudaStream_t s, int *codeOut) {
 }
 
 int tcgen05ErrorFlag() {
-    const int v = tc::readErrorWord();
-    if (v != 0) {
-        return v;
+    const int u = tc::readErrorWord();
+    if (u != 0) {
+        return u;
     }
     const int w = ocMajorErrorWord();
     const int x = w != 0 ? w : pairErrorWord();
     const int y = x != 0 ? x : attentionErrorWord();
     const int z = y != 0 ? y : smallErrorWord();
-    return z != 0 ? z : windowErrorWord();
+    const int v = z != 0 ? z : windowErrorWord();
+    return v != 0 ? v : servingErrorWord();
 }
 
 } // namespace mlel

@@ -169,6 +169,7 @@ struct UnitWindow {
 };
 int gemmI8UnitsLaunch(const GemmI8Problem &q, const UnitWindow &u, cudaStream_t stream);
 int windowErrorWord();
+int servingErrorWord(); // the kernels of the 8-bit decoder layer (serving.hpp)
 
 // Kernel-selection knobs of the tensor-core launchers (mlel_set_tuning): 0 = the library's own choice.
 struct TensorCoreTuning {

@@ -1,0 +1,40 @@
+// Attention over the paged int8 cache as its kernels take it (paged_attention.cu chooses among them).
+#pragma once
+
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "gemm_i8_tcgen05.hpp"
+#include "paged_cache.cuh"
+
+namespace mlel {
+
+struct AttendParams {
+    PagedCache cache;
+    PagedBatch batch;
+    const char *queries;
+    char *out;
+    int64_t queryStride[2], outStride[2]; // bytes: token, head
+    float scale, softcap;                 // softcap 0: none
+    int32_t causal, window, queryHeads, group;
+    int32_t halves;      // queries and output are f16 (else bf16)
+    int32_t wideQueries; // every head of the queries starts on a 16-byte boundary; the same for the output
+    int32_t wideOut;
+    float *partials; // split calls: see paged_attention_few.cu
+    FastDiv pageDiv;
+};
+
+// paged_attention_few.cu: few rows per cache head (single tokens, or a handful), keys split over the whole device
+struct FewPlan {
+    int rows;    // rows of a tile: 16 or 32
+    int blocks;  // that share the keys
+    bool joins;  // keys of one tile may lie with several blocks: a second kernel joins their results
+    uint64_t workspace;
+};
+FewPlan pagedAttentionFewPlan(const AttendParams &p);
+int pagedAttentionFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s);
+int takePagedErrorFew();
+int fewAttentionErrorWord();
+
+} // namespace mlel
