@@ -117,6 +117,16 @@ int matmulScaled(const mlel_tensor *a, const mlel_tensor *aScales, const mlel_te
     p.biases = reinterpret_cast<const float *>(bias.ptr), p.out = out.ptr;
     p.aStride = oa.strides[0], p.bStride = ob.strides[0], p.outStride = out.strides[0];
     p.M = int32_t(M), p.N = int32_t(N), p.K = int32_t(K);
+    if (M == 1) { // strides of an axis that is not walked
+        p.aStride = (K + 15) / 16 * 16, p.outStride = (N * elemSize(out.dtype) + 15) / 16 * 16;
+    }
+    if (N == 1) {
+        p.bStride = (K + 15) / 16 * 16;
+    }
+    if (aligned(p.a, 16) && p.aStride % 16 == 0 && aligned(p.b, 16) && p.bStride % 16 == 0) {
+        int rc = MLEL_SUCCESS;
+        return matmulScaledOnPairs(p, out.dtype, s, &rc) ? rc : matmulScaledOnTiles(p, out.dtype, s);
+    }
     return launchStatus(call.c_str(), out.dtype == MLEL_F32   ? launchAnyRows<float>(p, s)
                                       : out.dtype == MLEL_F16 ? launchAnyRows<__half>(p, s)
                                                               : launchAnyRows<__nv_bfloat16>(p, s));

@@ -3,6 +3,7 @@
 
 #include <cmath>
 
+#include "matmul_scaled.hpp"
 #include "paged_attention.hpp"
 
 namespace mlel {
@@ -31,7 +32,7 @@ AttendParams paramsOf(const std::string &call, const mlel_paged_cache *cache, co
 
 uint64_t pagedAttentionWorkspace(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries) {
     const AttendParams p = paramsOf("mlel_paged_attention_workspace", cache, batch, queries);
-    return p.batch.tokens == 0 || p.batch.sequences == 0 ? 0 : pagedAttentionFewPlan(p).workspace;
+    return p.batch.tokens == 0 || p.batch.sequences == 0 || pagedAttentionManyApplies(p) ? 0 : pagedAttentionFewPlan(p).workspace;
 }
 
 int pagedAttention(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries,
@@ -56,6 +57,9 @@ int pagedAttention(const mlel_paged_cache *cache, const mlel_paged_batch *batch,
         return MLEL_SUCCESS;
     }
     wantCurrentDevice(call, "output", p.out);
+    if (pagedAttentionManyApplies(p)) {
+        return pagedAttentionMany(p, s);
+    }
     const FewPlan plan = pagedAttentionFewPlan(p);
     if (plan.workspace > 0 && (workspace == nullptr || workspaceBytes < plan.workspace || !aligned(workspace, 16))) {
         refuse(call, "the workspace is null, off a 16-byte boundary or smaller than mlel_paged_attention_workspace() says");
@@ -64,7 +68,17 @@ int pagedAttention(const mlel_paged_cache *cache, const mlel_paged_batch *batch,
     return pagedAttentionFew(p, plan, s);
 }
 
-int takePagedErrorAttention() { return takePagedErrorFew(); }
-int servingErrorWord() { return fewAttentionErrorWord(); }
+int takePagedErrorAttention() {
+    const int few = takePagedErrorFew(), many = takePagedErrorMany();
+    return few != 0 ? few : many;
+}
+int servingErrorWord() {
+    for (const auto word : {fewAttentionErrorWord, manyAttentionErrorWord, scaledTilesErrorWord, scaledPairErrorWord}) {
+        if (const int code = word()) {
+            return code;
+        }
+    }
+    return 0;
+}
 
 } // namespace mlel

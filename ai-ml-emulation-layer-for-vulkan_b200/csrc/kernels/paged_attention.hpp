@@ -37,4 +37,10 @@ int pagedAttentionFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s
 int takePagedErrorFew();
 int fewAttentionErrorWord();
 
+// paged_attention_many.cu: many rows per cache head (prompts)
+bool pagedAttentionManyApplies(const AttendParams &p);
+int pagedAttentionMany(const AttendParams &p, cudaStream_t s);
+int takePagedErrorMany();
+int manyAttentionErrorWord();
+
 } // namespace mlel

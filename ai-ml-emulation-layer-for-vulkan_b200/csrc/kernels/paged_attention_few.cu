@@ -34,6 +34,7 @@
 
 #include "paged_attention.hpp"
 #include "paged_attention_device.cuh"
+#include "paged_attention_map.hpp"
 #include "serving_device.cuh"
 #include "tcgen05_common.cuh"
 
@@ -582,34 +583,13 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
     }
 }
 
-// Rows of `headDim` bytes of one half of the cache, in boxes of 16 rows, swizzled as panelAddr reads them.
-bool makeCacheMap(CUtensorMap *map, const void *base, const PagedCache &c, int panel, int rowsOfBox) {
-    EncodeTiledFn fn = encodeTiled();
-    if (fn == nullptr) {
-        setLastError("cuTensorMapEncodeTiled is not available from the driver");
-        return false;
-    }
-    const cuuint64_t rows = cuuint64_t(c.pages) * c.heads * c.page;
-    const cuuint64_t dims[3] = {cuuint64_t(c.headDim), rows, 1}, strides[2] = {cuuint64_t(c.headDim), rows * c.headDim};
-    const cuuint32_t box[3] = {cuuint32_t(panel), cuuint32_t(rowsOfBox), 1}, elemStrides[3] = {1, 1, 1};
-    const MapKey key{{6, reinterpret_cast<uint64_t>(base), dims[0], rows, uint64_t(panel), uint64_t(rowsOfBox)}};
-    return rememberedMap(map, key, [&](CUtensorMap *m) {
-        const CUresult rc = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(base), dims, strides, box, elemStrides,
-                               CU_TENSOR_MAP_INTERLEAVE_NONE, panel == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
-                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-        if (rc != CUDA_SUCCESS) {
-            setLastError("cuTensorMapEncodeTiled failed with code " + std::to_string(int(rc)));
-        }
-        return rc == CUDA_SUCCESS;
-    });
-}
-
 int paddedHead(int headDim) { return headDim <= 64 ? 64 : headDim <= 128 ? 128 : 256; }
 
 template <int DP, int MT, bool HALF> int launchFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
     using Shape = FewShape<DP>;
     CUtensorMap k, v;
-    if (!makeCacheMap(&k, p.cache.keys, p.cache, Shape::kPanel, kGroup) || !makeCacheMap(&v, p.cache.values, p.cache, Shape::kPanel, kGroup)) {
+    if (!makeCacheMap(&k, p.cache.keys, p.cache, Shape::kPanel, kGroup, true) ||
+        !makeCacheMap(&v, p.cache.values, p.cache, Shape::kPanel, kGroup, true)) {
         return MLEL_ERROR_DEVICE;
     }
     constexpr size_t smemBytes = Shape::kRing + 1024;

@@ -1,0 +1,613 @@
+// Attention over a paged int8 cache for many rows per cache head: prompts and chunks of them, on tcgen05.
+//
+//   o = sum_j softmax(s)_j v_j,  s_j = scale * q . k_j (capped or not), over the tokens that the masks leave
+//
+// A block takes 256 rows of one sequence and cache head (a row is one token's query head; the heads that share a cache head are
+// neighbouring rows) as two tiles of 128, and walks the keys they see in tiles of 128:
+//   one warp      copies: 16 keys or values at a time (pages hold a multiple of 16), integers into staging buffers
+//   four warps    integers -> f16 (exact), in the 128-byte swizzled layout that both products read: keys are rows of a
+//                 K-major operand, values rows of an MN-major one, the same bytes either way
+//   one warp      products: S = Q K^T into tensor memory, O += P V with P read from tensor memory
+//   two x four    softmax, a lane a row: S out of tensor memory, weights as f16 back over it
+// The tiles take turns: while one's products run the other's softmax does.
+//
+// What bounds it: per 256 x 128 scores the products take 2048 cycles at 128 elements a head, and 32768 exponentials the
+// same at 16 a cycle; everything else (a multiply-add, half a maximum, half a sum, half a conversion per score, and the
+// keys' and values' conversion) shares the four schedulers with them.
+//
+// Softmax in one pass where it can: scores are weighed with the maximum known from the tiles before, and only if one exceeds
+// it by more than 2^8, or at a row's first tile, at masked ones and where the values' reference grows, the maximum is taken first
+// and sums and result are rescaled.  The scale of 16 values is part of the exponent: w = 2^(s - m + log2(scale / r) + 7), r a
+// running power of two, and the sum over the weights of 16 keys is divided by it again.  So a weight is at most 2^15, f16's steps
+// end 2^-31 below the largest, and values whose scale is below 2^-60 of r count as nothing.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "paged_attention.hpp"
+#include "paged_attention_device.cuh"
+#include "paged_attention_map.hpp"
+#include "serving_device.cuh"
+#include "tcgen05_common.cuh"
+
+namespace mlel {
+namespace {
+
+using namespace tc;
+
+constexpr int kRows = 128, kKeys = 128, kGroup = 16, kGroups = kKeys / kGroup;
+constexpr int kSoftmaxWarps = 8, kConvertWarps = 4, kCopyWarp = 12, kProductWarp = 13, kThreads14 = 14 * 32;
+constexpr int kParamRing = 8, kStaging = 2, kSlots = 4; // slots: keys, values, keys, values
+constexpr float kGrowth = 8.f;                          // in powers of two
+constexpr float kWeightBits = 7.f;
+
+template <int DP> struct ManyShape {
+    static constexpr int kQueryBytes = kRows * DP * 2;   // of one tile: panels of 64 elements
+    static constexpr int kSlotBytes = kKeys * DP * 2;
+    static constexpr int kStagingBytes = kKeys * DP;
+    static constexpr size_t kSmem = 2 * size_t(kQueryBytes) + kSlots * size_t(kSlotBytes) + kStaging * size_t(kStagingBytes) + 1024;
+    // tensor-memory columns of the two tiles
+    static constexpr __device__ uint32_t scores(int which) { return uint32_t(128 * which); }
+    static constexpr __device__ uint32_t result(int which) { return uint32_t(256 + DP * which); }
+};
+
+// What the softmax needs to know of a tile of keys.
+struct TileParams {
+    float keyScale[kGroups]; // 0 where there is nothing
+    float shift[kGroups];    // log2(value scale) - reference + kWeightBits
+    float perWeight[kGroups]; // 2^-shift
+    int reference;           // a power of two
+    uint32_t there;          // groups that exist
+};
+
+struct ManyBarriers {
+    uint64_t queries, params[kParamRing], stagingFull[kStaging], stagingEmpty[kStaging], full[kSlots], empty[kSlots];
+    uint64_t scores[2], weights[2], result[2];
+    uint32_t tmemBase;
+};
+
+// kind::f16: f32 results, f16 operands, M = 128
+constexpr uint32_t instrF16(int n, bool bMnMajor) {
+    return (1u << 4) | (uint32_t(bMnMajor) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+__device__ __forceinline__ void mmaShared(uint32_t d, DescWords a, DescWords b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, l;\n\t.reg .b64 a, b;\n\t"
+                 "elect.sync _|l, 0xffffffff;\n\t"
+                 "setp.ne.b32 p, %6, 0;\n\t"
+                 "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+                 "r"(a.low), "r"(a.high), "r"(b.low), "r"(b.high), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void mmaTensor(uint32_t d, uint32_t a, DescWords b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, l;\n\t.reg .b64 b;\n\t"
+                 "elect.sync _|l, 0xffffffff;\n\t"
+                 "setp.ne.b32 p, %5, 0;\n\t"
+                 "mov.b64 b, {%2, %3};\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+                 "r"(a), "r"(b.low), "r"(b.high), "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+__device__ __forceinline__ void tmemStore32(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+                 "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+                 "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+                 "r"(r[31])
+                 : "memory");
+}
+__device__ __forceinline__ void tmemStore16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                 "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int DP, bool HALF, bool CAP>
+__global__ void __launch_bounds__(kThreads14, 1)
+pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p,
+                         const FastDiv heads, const int levels) {
+    using Shape = ManyShape<DP>;
+    using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
+    extern __shared__ uint8_t rawSmem[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rawSmem) + 1023) & ~uintptr_t(1023));
+    uint8_t *queries = smem, *slots = smem + 2 * Shape::kQueryBytes, *staging = slots + kSlots * Shape::kSlotBytes;
+    __shared__ ManyBarriers bars;
+    __shared__ TileParams params[kParamRing];
+    const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
+    dependencySync();
+
+    // blocks: the tiles that see the most keys first
+    const uint32_t overHeads = fastDiv(blockIdx.x, heads);
+    const int head = int(blockIdx.x - overHeads * heads.d), level = int(overHeads / uint32_t(p.batch.sequences)),
+              index = int(overHeads - uint32_t(level) * uint32_t(p.batch.sequences));
+    const Sequence q = sequenceOf(p.batch, index);
+    if (!q.sound && level == 0 && head == 0 && threadIdx.x == 0) {
+        atomicCAS(&g_pagedError, 0, kBadSequence);
+    }
+    const int allRows = q.sound ? q.fresh * p.group : 0, firstRow = (levels - 1 - level) * 2 * kRows;
+    if (firstRow >= allRows) {
+        return;
+    }
+    const int rows = min(2 * kRows, allRows - firstRow), old = q.length - q.fresh;
+    const int firstToken = firstRow / p.group, lastToken = (firstRow + rows - 1) / p.group;
+    const int keyLo = (p.window > 0 ? max(0, old + firstToken - p.window + 1) : 0) / kGroup * kGroup;
+    const int keyHi = p.causal ? old + lastToken + 1 : q.length;
+    const int tiles = (keyHi - keyLo + kKeys - 1) / kKeys;
+    const int32_t *table = p.batch.table + index * p.batch.tableStride;
+
+    if (threadIdx.x == 0) {
+        mbarInit(&bars.queries, kSoftmaxWarps);
+        for (int i = 0; i < kParamRing; ++i) {
+            mbarInit(&bars.params[i], 1u);
+        }
+        for (int i = 0; i < kStaging; ++i) {
+            mbarInit(&bars.stagingFull[i], 1u);
+            mbarInit(&bars.stagingEmpty[i], kConvertWarps);
+        }
+        for (int i = 0; i < kSlots; ++i) {
+            mbarInit(&bars.full[i], kConvertWarps);
+            mbarInit(&bars.empty[i], 1u);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbarInit(&bars.scores[i], 1u);
+            mbarInit(&bars.weights[i], 4u);
+            mbarInit(&bars.result[i], 1u);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kProductWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smemAddr(&bars.tmemBase)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = bars.tmemBase;
+
+    if (warp == kCopyWarp) {
+        // ---------------- copies, and what the softmax needs to know of their pages ----------------
+        const int groups = (keyHi - keyLo + kGroup - 1) / kGroup;
+        const auto slotOf = [&](int tile) { // lane 0 .. 7: the page of a group of the tile; -1: there is none
+            const int n = tile * kGroups + lane;
+            int slot = -1;
+            if (lane < kGroups && n < groups) {
+                slot = table[fastDiv(uint32_t(keyLo + n * kGroup), p.pageDiv)];
+                if (uint32_t(slot) >= uint32_t(p.cache.pages)) {
+                    atomicCAS(&g_pagedError, 0, kBadPage);
+                    slot = -1;
+                }
+            }
+            return slot;
+        };
+        const auto scaleOf = [&](const float *scales, int slot) { return slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : 0.f; };
+        int slot = slotOf(0), nextSlot = slotOf(1), reference = -126;
+        float keyScale = scaleOf(p.cache.keyScales, slot), valueScale = scaleOf(p.cache.valueScales, slot);
+        bool ok = true;
+        uint32_t unit = 0; // keys and values of the tiles in turn
+        for (int tile = 0; tile < tiles && ok; ++tile) {
+            const int nextNextSlot = slotOf(tile + 2);
+            const float nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
+            // parameters of the tile: the ring is longer than the softmax can be behind (see kSlots and kStaging)
+            TileParams &to = params[tile % kParamRing];
+            const float magnitude = fabsf(valueScale);
+            int exponent = magnitude > 0.f && magnitude < INFINITY ? int(__float_as_uint(powerAbove(magnitude)) >> 23) - 127 : -126;
+            exponent = __reduce_max_sync(0xffffffffu, exponent);
+            reference = max(reference, exponent);
+            if (lane < kGroups) {
+                // (a scale that is not finite gives a shift and weights that are not)
+                const float shift = magnitude < 1.f * INFINITY ? fmaxf(log2f(magnitude) - float(reference), -60.f) + kWeightBits
+                                                               : magnitude - magnitude;
+                to.keyScale[lane] = keyScale, to.shift[lane] = valueScale < 0.f ? __int_as_float(0x7fc00000) : shift;
+                to.perWeight[lane] = exp2f(-shift);
+            }
+            const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
+            if (lane == 0) {
+                to.reference = reference, to.there = there;
+            }
+            __syncwarp();
+            if (lane == 0) {
+                mbarArrive(&bars.params[tile % kParamRing]);
+            }
+            const int n = tile * kGroups + lane, key = keyLo + n * kGroup;
+            const int row = (max(slot, 0) * p.cache.heads + head) * p.cache.page + key - int(fastDiv(uint32_t(key), p.pageDiv)) * p.cache.page;
+            const int count = min(kGroups, groups - tile * kGroups);
+#pragma unroll
+            for (int side = 0; side < 2; ++side, ++unit) {
+                const uint32_t buffer = unit % kStaging;
+                ok = ok && mbarWaitWarp(&bars.stagingEmpty[buffer], ((unit / kStaging) & 1u) ^ 1u, 91);
+                if (!ok) {
+                    break;
+                }
+                if (lane == 0) {
+                    mbarArriveExpectTx(&bars.stagingFull[buffer], uint32_t(count * kGroup * DP));
+                }
+                __syncwarp();
+                if (lane < count) {
+                    tmaLoad3d(side == 0 ? &mapK : &mapV, staging + buffer * Shape::kStagingBytes + lane * kGroup * DP, &bars.stagingFull[buffer],
+                              0, row, 0);
+                }
+            }
+            slot = nextSlot, keyScale = nextKeyScale, valueScale = nextValueScale;
+            nextSlot = nextNextSlot;
+        }
+        __syncwarp();
+    } else if (warp == kProductWarp) {
+        // ---------------- products (the whole warp: see ummaBlockPeek) ----------------
+        constexpr uint32_t kScoreDesc = instrF16(kKeys, false), kResultDesc = instrF16(DP, true);
+        constexpr uint32_t kPanel = kRows * 128; // bytes: 64 elements of 128 rows
+        const uint32_t queryAddr = smemAddr(queries), slotAddr = smemAddr(slots);
+        bool failed = !mbarWait(&bars.queries, 0u, 92);
+        const auto scoreProduct = [&](int tile, int which) {
+            const uint32_t slot = uint32_t(2 * tile) % kSlots;
+            if (which == 0) {
+                failed = failed || !mbarWait(&bars.full[slot], (uint32_t(2 * tile) / kSlots) & 1u, 93);
+            }
+            __syncwarp();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                const uint32_t at = uint32_t(k / 4) * kPanel + uint32_t(k % 4) * 32u;
+                mmaShared(tmem + Shape::scores(which), descWords(smemDesc(queryAddr + uint32_t(which * Shape::kQueryBytes) + at, 16, 1024)),
+                          descWords(smemDesc(slotAddr + slot * uint32_t(Shape::kSlotBytes) + at, 16, 1024)), kScoreDesc, k != 0 ? 1u : 0u);
+            }
+            ummaCommit(&bars.scores[which]);
+            if (which == 1) {
+                ummaCommit(&bars.empty[slot]);
+            }
+        };
+        const auto resultProduct = [&](int tile, int which) {
+            const uint32_t unit = uint32_t(2 * tile + 1), slot = unit % kSlots;
+            if (which == 0) {
+                failed = failed || !mbarWait(&bars.full[slot], (unit / kSlots) & 1u, 94);
+            }
+            failed = failed || !mbarWait(&bars.weights[which], uint32_t(tile) & 1u, 95);
+            __syncwarp();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k) {
+                mmaTensor(tmem + Shape::result(which), tmem + Shape::scores(which) + uint32_t(k * 8),
+                          descWords(smemDesc(slotAddr + slot * uint32_t(Shape::kSlotBytes) + uint32_t(k) * 2048u, kPanel, 1024)), kResultDesc,
+                          tile != 0 || k != 0 ? 1u : 0u);
+            }
+            if (tile == tiles - 1) {
+                ummaCommit(&bars.result[which]);
+            }
+            if (which == 1) {
+                ummaCommit(&bars.empty[slot]);
+            }
+        };
+        scoreProduct(0, 0);
+        scoreProduct(0, 1);
+        for (int tile = 0; tile < tiles; ++tile) {
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                resultProduct(tile, which);
+                if (tile + 1 < tiles) {
+                    scoreProduct(tile + 1, which);
+                }
+            }
+        }
+    } else if (warp >= kSoftmaxWarps) {
+        // ---------------- integers -> f16 ----------------
+        constexpr int kLanes = DP / 16, kRowsAtOnce = kConvertWarps * 32 / kLanes; // lanes of a key
+        const int thread = int(threadIdx.x) - kSoftmaxWarps * 32, part = thread % kLanes, row0 = thread / kLanes;
+        for (uint32_t unit = 0; unit < uint32_t(2 * tiles); ++unit) {
+            const uint32_t buffer = unit % kStaging, slot = unit % kSlots;
+            if (!mbarWaitWarp(&bars.stagingFull[buffer], (unit / kStaging) & 1u, 96) ||
+                !mbarWaitWarp(&bars.empty[slot], ((unit / kSlots) & 1u) ^ 1u, 97)) {
+                break;
+            }
+            const uint32_t from = smemAddr(staging) + buffer * uint32_t(Shape::kStagingBytes);
+            // element chunk `part` (16 of them) fills chunks 2 part and 2 part + 1 of 8 elements; the upper half of the lanes
+            // takes its two in the other order, so that panels of the same banks are not written at once
+            const uint32_t to = smemAddr(slots) + slot * uint32_t(Shape::kSlotBytes) + uint32_t(part / 4) * (kKeys * 128u);
+            const int swap = part >> 2;
+#pragma unroll 4
+            for (int row = row0; row < kKeys; row += kRowsAtOnce) {
+                const uint4 v = ldsVector(from + uint32_t(row * DP + part * 16));
+                uint4 a, b;
+                bytesToHalves(v.x, a.x, a.y);
+                bytesToHalves(v.y, a.z, a.w);
+                bytesToHalves(v.z, b.x, b.y);
+                bytesToHalves(v.w, b.z, b.w);
+                const int chunk = 2 * (part & 3);
+                const uint32_t line = to + uint32_t(row * 128), at0 = line + uint32_t((chunk ^ (row & 7)) << 4),
+                               at1 = line + uint32_t(((chunk + 1) ^ (row & 7)) << 4);
+                const uint4 x = swap ? b : a, y = swap ? a : b;
+                const uint32_t atX = swap ? at1 : at0, atY = swap ? at0 : at1;
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(atX), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(atY), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbarArrive(&bars.full[slot]);
+                mbarArrive(&bars.stagingEmpty[buffer]);
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---------------- softmax: a lane a row ----------------
+        const int which = warp >> 2, quarter = warp & 3, tileRow = quarter * 32 + lane, row = firstRow + which * kRows + tileRow;
+        const bool live = which * kRows + tileRow < rows;
+        const int token = live ? row / p.group : lastToken, queryHead = head * p.group + (live ? row - token * p.group : 0);
+        float rowScale;
+        {
+            const T *from = reinterpret_cast<const T *>(p.queries + int64_t(q.first + token) * p.queryStride[0] + queryHead * p.queryStride[1]);
+            const int length = live ? p.cache.headDim : 0;
+            float most = 0.f, inverse = 1.f, unit = 1.f;
+            if (!HALF) {
+#pragma unroll 1
+                for (int d = 0; d < length; d += 16) {
+                    uint32_t w[8];
+                    loadQuerySixteen(from, d, length, p.wideQueries != 0, w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 f = unpackTwo(w[j], T());
+                        most = maxBits(most, maxBits(f.x, f.y));
+                    }
+                }
+                unit = halfUnit(most);
+                inverse = 1.f / unit;
+            }
+            rowScale = unit * fabsf(p.scale) * (CAP ? 1.f : kLog2e);
+            const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u; // keeps the order of scores that of the products
+            const uint32_t line = smemAddr(queries) + uint32_t(which * Shape::kQueryBytes + tileRow * 128);
+#pragma unroll 2
+            for (int d = 0; d < DP; d += 16) {
+                uint32_t w[8];
+                loadQuerySixteen(from, d, length, p.wideQueries != 0, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (!HALF) {
+                        const float2 f = unpackTwo(w[j], T());
+                        w[j] = packTwo(f.x * inverse, f.y * inverse, __half());
+                    }
+                    w[j] ^= sign;
+                }
+                const uint32_t panel = line + uint32_t(d / 64) * (kRows * 128u);
+                const int chunk = (d % 64) / 8;
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(panel + uint32_t((chunk ^ (tileRow & 7)) << 4)), "r"(w[0]),
+                             "r"(w[1]), "r"(w[2]), "r"(w[3])
+                             : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(panel + uint32_t(((chunk + 1) ^ (tileRow & 7)) << 4)), "r"(w[4]),
+                             "r"(w[5]), "r"(w[6]), "r"(w[7])
+                             : "memory");
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbarArrive(&bars.queries);
+            }
+        }
+        const int position = old + token;
+        const int rowHi = !live ? 0 : p.causal ? position + 1 : q.length, rowLo = p.window > 0 ? max(0, position - p.window + 1) : 0;
+        // keys that every row of this tile sees
+        const int tileFirst = firstRow + which * kRows, tileLast = min(tileFirst + kRows, firstRow + rows) - 1;
+        const int openHi = tileFirst > tileLast ? 0x7fffffff : p.causal ? old + tileFirst / p.group + 1 : q.length;
+        const int openLo = p.window > 0 && tileFirst <= tileLast ? max(0, old + tileLast / p.group - p.window + 1) : 0;
+        const uint32_t scoresAt = tmem + Shape::scores(which) + (uint32_t(quarter * 32) << 16),
+                       resultAt = tmem + Shape::result(which) + (uint32_t(quarter * 32) << 16);
+
+        float most = -INFINITY, sum = 0.f;
+        int reference = -126;
+        bool ok = true;
+        const auto scoreOf = [&](uint32_t s, float factor) { // in powers of two
+            const float x = __uint_as_float(s) * factor;
+            return CAP ? softCapped(x, p.softcap) * kLog2e : x;
+        };
+        for (int tile = 0; tile < tiles && ok; ++tile) {
+            ok = mbarWaitWarp(&bars.params[tile % kParamRing], uint32_t(tile / kParamRing) & 1u, 98) &&
+                 mbarWaitWarp(&bars.scores[which], uint32_t(tile) & 1u, 99);
+            if (!ok) {
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const TileParams &tp = params[tile % kParamRing];
+            const int key0 = keyLo + tile * kKeys;
+            const bool masked = key0 + kKeys > openHi || key0 < openLo || tp.there != (1u << kGroups) - 1u;
+            uint32_t weights[kKeys / 2];
+            bool again = tile == 0 || masked || tp.reference != reference;
+            float added = 0.f;
+            if (!again) {
+                bool grows = false;
+                const float base = most == -INFINITY ? 0.f : most;
+#pragma unroll
+                for (int g = 0; g < kGroups; g += 2) {
+                    uint32_t s0[16], s1[16];
+                    tmemLoad16(scoresAt + uint32_t(g * 16), s0);
+                    tmemLoad16(scoresAt + uint32_t(g * 16 + 16), s1);
+                    tmemWait16(s0);
+                    tmemWait16(s1);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float factor = rowScale * tp.keyScale[g + h], shift = tp.shift[g + h] - base;
+                        float top = -INFINITY, part = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            const uint32_t a = h == 0 ? s0[j] : s1[j], b = h == 0 ? s0[j + 1] : s1[j + 1];
+                            float w0, w1;
+                            if (CAP) {
+                                const float x = scoreOf(a, factor), y = scoreOf(b, factor);
+                                top = fmaxf(top, fmaxf(x, y));
+                                w0 = exp2Fast(x + shift), w1 = exp2Fast(y + shift);
+                            } else {
+                                top = fmaxf(top, fmaxf(__uint_as_float(a), __uint_as_float(b)));
+                                w0 = exp2Fast(fmaf(__uint_as_float(a), factor, shift)), w1 = exp2Fast(fmaf(__uint_as_float(b), factor, shift));
+                            }
+                            part += w0 + w1;
+                            weights[(g + h) * 8 + j / 2] = packTwo(w0, w1, __half());
+                        }
+                        added = fmaf(part, tp.perWeight[g + h], added);
+                        // (a row that has seen nothing yet takes the long way, too)
+                        grows = grows || (CAP ? top : top * factor) > most + kGrowth;
+                    }
+                }
+                again = __any_sync(0xffffffffu, grows) != 0;
+            }
+            if (__any_sync(0xffffffffu, again)) {
+                // the maximum first, then sums and result in its units
+                const auto seen = [&](int key, int g) { return ((tp.there >> g) & 1u) != 0u && key < rowHi && key >= rowLo; };
+                float top = most;
+#pragma unroll 1
+                for (int g = 0; g < kGroups; ++g) {
+                    uint32_t s[16];
+                    tmemLoad16(scoresAt + uint32_t(g * 16), s);
+                    tmemWait16(s);
+                    const float factor = rowScale * tp.keyScale[g];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        top = !masked || seen(key0 + g * 16 + j, g) ? fmaxf(top, scoreOf(s[j], factor)) : top;
+                    }
+                }
+                const float keep = top == -INFINITY ? 1.f : exp2Fast(most - top);
+                const float factorO = keep * exp2f(float(reference - tp.reference));
+                sum *= keep;
+                if (tile > 0 && __any_sync(0xffffffffu, factorO != 1.f)) {
+#pragma unroll 1
+                    for (int d = 0; d < DP; d += 16) {
+                        uint32_t o[16];
+                        tmemLoad16(resultAt + uint32_t(d), o);
+                        tmemWait16(o);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            o[j] = __float_as_uint(__uint_as_float(o[j]) * factorO);
+                        }
+                        tmemStore16(resultAt + uint32_t(d), o);
+                    }
+                    tmemStoreWait();
+                }
+                most = top, reference = tp.reference;
+                const float base = most == -INFINITY ? 0.f : most;
+                added = 0.f;
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+                    uint32_t s[16];
+                    tmemLoad16(scoresAt + uint32_t(g * 16), s);
+                    tmemWait16(s);
+                    const float factor = rowScale * tp.keyScale[g], shift = tp.shift[g] - base;
+                    float part = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        float w0 = exp2Fast(scoreOf(s[j], factor) + shift), w1 = exp2Fast(scoreOf(s[j + 1], factor) + shift);
+                        if (masked) { // what the mask hides stays out, whatever its page's scales are
+                            w0 = seen(key0 + g * 16 + j, g) ? w0 : 0.f;
+                            w1 = seen(key0 + g * 16 + j + 1, g) ? w1 : 0.f;
+                        }
+                        part += w0 + w1;
+                        weights[g * 8 + j / 2] = packTwo(w0, w1, __half());
+                    }
+                    added = part == 0.f ? added : fmaf(part, tp.perWeight[g], added);
+                }
+            }
+            sum += added;
+            tmemStore32(scoresAt, weights);
+            tmemStore32(scoresAt + 32u, weights + 32);
+            tmemStoreWait();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbarArrive(&bars.weights[which]);
+            }
+        }
+        // ---- the rows, by way of the queries' memory, which no product reads any more ----
+        if (ok && mbarWaitWarp(&bars.result[which], 0u, 90)) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const float f = sum == 0.f ? 0.f : exp2f(float(reference) - kWeightBits) / sum;
+            uint8_t *mine = queries + which * Shape::kQueryBytes + quarter * (32 * DP * 2);
+#pragma unroll 1
+            for (int d = 0; d < DP; d += 16) {
+                uint32_t o[16];
+                tmemLoad16(resultAt + uint32_t(d), o);
+                tmemWait16(o);
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float x = sum == 0.f ? 0.f : __uint_as_float(o[2 * j]) * f, y = sum == 0.f ? 0.f : __uint_as_float(o[2 * j + 1]) * f;
+                    w[j] = packTwo(x, y, T());
+                }
+                // 16-byte chunks of a row, each lane's turned by its number
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int chunk = d / 8 + half;
+                    *reinterpret_cast<uint4 *>(mine + lane * (DP * 2) + ((chunk ^ (lane & 7)) << 4)) = {w[4 * half], w[4 * half + 1],
+                                                                                                       w[4 * half + 2], w[4 * half + 3]};
+                }
+            }
+            __syncwarp();
+            constexpr int kChunks = DP / 8, kLinesAtOnce = 32 / kChunks; // lanes of a row
+            const int chunk = lane % kChunks;
+#pragma unroll 1
+            for (int r = lane / kChunks; r < 32; r += kLinesAtOnce) {
+                const int outRow = firstRow + which * kRows + quarter * 32 + r;
+                if (which * kRows + quarter * 32 + r < rows && chunk * 8 < p.cache.headDim) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * (DP * 2) + ((chunk ^ (r & 7)) << 4));
+                    const int outToken = outRow / p.group, outHead = head * p.group + outRow - outToken * p.group;
+                    char *to = p.out + int64_t(q.first + outToken) * p.outStride[0] + outHead * p.outStride[1] + chunk * 16;
+                    if (p.wideOut) {
+                        *reinterpret_cast<uint4 *>(to) = v;
+                    } else {
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            reinterpret_cast<uint16_t *>(to)[2 * j] = uint16_t(w[j]), reinterpret_cast<uint16_t *>(to)[2 * j + 1] = uint16_t(w[j] >> 16);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (warp == kProductWarp) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+template <int DP, bool HALF, bool CAP> int launchMany(const AttendParams &p, cudaStream_t s) {
+    using Shape = ManyShape<DP>;
+    static_assert(Shape::kSmem + sizeof(ManyBarriers) + kParamRing * sizeof(TileParams) <= 232448, "shared memory per block");
+    CUtensorMap k, v;
+    if (!makeCacheMap(&k, p.cache.keys, p.cache, DP, kGroup, false) || !makeCacheMap(&v, p.cache.values, p.cache, DP, kGroup, false)) {
+        return MLEL_ERROR_DEVICE;
+    }
+    const auto kernel = pagedAttentionManyKernel<DP, HALF, CAP>;
+    if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), Shape::kSmem)) {
+        return MLEL_ERROR_DEVICE;
+    }
+    const int64_t levels = (int64_t(p.batch.maxNew) * p.group + 2 * kRows - 1) / (2 * kRows), blocks = levels * p.cache.heads * p.batch.sequences;
+    if (blocks > 0x7fffffff) {
+        refuse("mlel_cuda_paged_attention", "too many tokens and sequences for one call");
+    }
+    return launchStatus("mlel_cuda_paged_attention", launchOverlapped(kernel, dim3(unsigned(blocks)), kThreads14, Shape::kSmem, s, k, v, p,
+                                                                      makeFastDiv(p.cache.heads), int(levels)));
+}
+
+template <int DP> int launchManyType(const AttendParams &p, cudaStream_t s) {
+    if (p.softcap > 0.f) {
+        return p.halves ? launchMany<DP, true, true>(p, s) : launchMany<DP, false, true>(p, s);
+    }
+    return p.halves ? launchMany<DP, true, false>(p, s) : launchMany<DP, false, false>(p, s);
+}
+
+} // namespace
+
+bool pagedAttentionManyApplies(const AttendParams &p) {
+    return p.cache.headDim <= 128 && int64_t(p.batch.maxNew) * p.group > 64;
+}
+int pagedAttentionMany(const AttendParams &p, cudaStream_t s) {
+    return p.cache.headDim <= 64 ? launchManyType<64>(p, s) : launchManyType<128>(p, s);
+}
+
+int takePagedErrorMany() { return takePagedError(); }
+int manyAttentionErrorWord() { return tc::readErrorWord(); }
+
+} // namespace mlel

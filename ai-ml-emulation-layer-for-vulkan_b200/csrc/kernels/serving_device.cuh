@@ -49,6 +49,13 @@ __device__ __forceinline__ void loadWide(const float *from, float (&x)[8]) {
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
 }
 
+__device__ __forceinline__ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Four elements from `at` on; zeros from `length` on.
+__device__ __forceinline__ float4 fourOf(const float *from, int at, int length) {
+    return {at < length ? from[at] : 0.f, at + 1 < length ? from[at + 1] : 0.f, at + 2 < length ? from[at + 2] : 0.f,
+            at + 3 < length ? from[at + 3] : 0.f};
+}
+
 // A row's scale, from the bits of its largest magnitude.
 struct RowScale {
     float value;   // what is stored

@@ -116,10 +116,10 @@ def attend(data, scales, starts, lengths, table, q, scale, causal, window, softc
                 out[first + i, h] = o
                 # weights: twice the scores' error (numerator and sum), f16's half step, the exponential's and the sums' roundings
                 error = most * (2 * off + 2.0 ** -11 + 2.0 ** -20 + (hi - lo) * 2.0 ** -23)
-                # f16 has steps of 2^-24 at its lower end.  Weights are held as p * scale / r * 2^14, r at most twice the largest
-                # scale in use, so half a step is 2^-25 * 2^-14 * 2 * scale = 2^-38 * scale for each integer, and sums of p
-                # are at least 1
+                # f16 has steps of 2^-24 at its lower end.  Weights are held as p * scale / r * 2^n, r at most twice the largest
+                # scale of the sequence's pages (rows of one call are weighed together, whatever the mask leaves to each), and n at least 7 (more would leave no room for a maximum that grows by up to 2^8 before it is
+                # taken up), so half a step is 2^-25 * 2^-7 * 2 * scale = 2^-31 * scale for each integer; sums of p are at least 1
                 integers = np.abs(data[1, slot[lo:hi], h // group, row[lo:hi]].astype(np.float64)).sum(axis=0)
-                error += 2.0 ** -38 * np.abs(scales[1, slot[lo:hi], h // group]).max() * integers
+                error += 2.0 ** -31 * np.abs(scales[1, slot, h // group]).max() * integers
                 bound[first + i, h] = error + half_step(dtype) * (np.abs(o) + error) + smallest_half_step(dtype)
     return out, bound

@@ -116,6 +116,16 @@ def test_matmul_scaled(serving, dtype, m, n, k):
     check_product(serving, product_operands(m + n + k, m, n, k, (m + n) % 2 == 0), DTYPES[dtype])
 
 
+@pytest.mark.parametrize("m, n, k", [(300, 5000, 272), (1500, 4080, 400), (700, 9500, 128), (2049, 2568, 96)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_matmul_scaled_many_tiles(serving, dtype, m, n, k):
+    """Enough tiles of 256 tokens for every pair of SMs, over channels that end inside one; an output of wider rows."""
+    t = DTYPES[dtype]
+    store = torch.full((m, n + 24), 77.0, device="cuda", dtype=t)
+    check_product(serving, product_operands(m + n + k, m, n, k, True), t, out=store[:, :n])
+    assert (store[:, n:] == 77).all()
+
+
 @pytest.mark.parametrize("m", [1, 5, 32, 63, 200, 300])
 def test_matmul_scaled_longest_sums(serving, m):
     """Sums that fill 32-bit integers (131071 * 128 * 128 is 2^31 - 16384)."""
