@@ -1039,6 +1039,13 @@ int mlel_cuda_matmul_scaled(const mlel_tensor *a, const mlel_tensor *a_scales, c
         [&] { return matmulScaled(a, a_scales, b, b_scales, biases, output, static_cast<cudaStream_t>(cuda_stream)); });
 }
 
+int mlel_cuda_quantized_linear(const mlel_tensor *input, const mlel_tensor *b, const mlel_tensor *b_scales, const mlel_tensor *biases,
+                               const mlel_tensor *output, void *workspace, uint64_t workspace_bytes, void *cuda_stream) {
+    return guarded([&] {
+        return quantizedLinear(input, b, b_scales, biases, output, workspace, workspace_bytes, static_cast<cudaStream_t>(cuda_stream));
+    });
+}
+
 int mlel_cuda_paged_append(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *keys,
                            const mlel_tensor *values, const mlel_tensor *cosines, const mlel_tensor *sines,
                            const mlel_tensor *queries, const mlel_tensor *rotated_queries, int interleaved, void *cuda_stream) {

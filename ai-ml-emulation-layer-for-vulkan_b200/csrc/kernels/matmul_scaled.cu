@@ -77,11 +77,9 @@ template <class T> cudaError_t launchAnyRows(const ScaledProblem &p, cudaStream_
                             0, s, p);
 }
 
-} // namespace
-
-int matmulScaled(const mlel_tensor *a, const mlel_tensor *aScales, const mlel_tensor *b, const mlel_tensor *bScales,
-                 const mlel_tensor *biases, const mlel_tensor *output, cudaStream_t s) {
-    const std::string call = "mlel_cuda_matmul_scaled";
+// The operands of a product, checked; where there is work, on the current device.
+ScaledProblem scaledProblemOf(const std::string &call, const mlel_tensor *a, const mlel_tensor *aScales, const mlel_tensor *b,
+                              const mlel_tensor *bScales, const mlel_tensor *biases, const mlel_tensor *output) {
     const Operand oa = operandOf(call, "a", a, 2), sa = operandOf(call, "a_scales", aScales, 1), ob = operandOf(call, "b", b, 2),
                   sb = operandOf(call, "b_scales", bScales, 1), out = writtenOperandOf(call, "output", output, 2);
     Operand bias{};
@@ -104,32 +102,64 @@ int matmulScaled(const mlel_tensor *a, const mlel_tensor *aScales, const mlel_te
     if (K < 1 || K > 131071) {
         refuse(call, "K has to be 1 to 131071: longer sums of products do not fit 32-bit integers");
     }
-    if (M == 0 || N == 0) {
-        return MLEL_SUCCESS;
-    }
     if (M > 65535 * int64_t(kTile)) {
         refuse(call, "more than 4194240 tokens");
     }
-    wantCurrentDevice(call, "output", out.ptr);
+    if (M > 0 && N > 0) {
+        wantCurrentDevice(call, "output", out.ptr);
+    }
     ScaledProblem p{};
     p.a = reinterpret_cast<const int8_t *>(oa.ptr), p.b = reinterpret_cast<const int8_t *>(ob.ptr);
     p.aScales = reinterpret_cast<const float *>(sa.ptr), p.bScales = reinterpret_cast<const float *>(sb.ptr);
     p.biases = reinterpret_cast<const float *>(bias.ptr), p.out = out.ptr;
     p.aStride = oa.strides[0], p.bStride = ob.strides[0], p.outStride = out.strides[0];
     p.M = int32_t(M), p.N = int32_t(N), p.K = int32_t(K);
-    if (M == 1) { // strides of an axis that is not walked
+    // strides of an axis that is not walked: any would do
+    if (M == 1) {
         p.aStride = (K + 15) / 16 * 16, p.outStride = (N * elemSize(out.dtype) + 15) / 16 * 16;
     }
     if (N == 1) {
         p.bStride = (K + 15) / 16 * 16;
     }
+    return p;
+}
+
+int launchScaled(const std::string &call, const ScaledProblem &p, int32_t dtype, cudaStream_t s) {
     if (aligned(p.a, 16) && p.aStride % 16 == 0 && aligned(p.b, 16) && p.bStride % 16 == 0) {
         int rc = MLEL_SUCCESS;
-        return matmulScaledOnPairs(p, out.dtype, s, &rc) ? rc : matmulScaledOnTiles(p, out.dtype, s);
+        return matmulScaledOnPairs(p, dtype, s, &rc) ? rc : matmulScaledOnTiles(p, dtype, s);
     }
-    return launchStatus(call.c_str(), out.dtype == MLEL_F32   ? launchAnyRows<float>(p, s)
-                                      : out.dtype == MLEL_F16 ? launchAnyRows<__half>(p, s)
-                                                              : launchAnyRows<__nv_bfloat16>(p, s));
+    return launchStatus(call.c_str(), dtype == MLEL_F32   ? launchAnyRows<float>(p, s)
+                                      : dtype == MLEL_F16 ? launchAnyRows<__half>(p, s)
+                                                          : launchAnyRows<__nv_bfloat16>(p, s));
+}
+
+} // namespace
+
+int matmulScaled(const mlel_tensor *a, const mlel_tensor *aScales, const mlel_tensor *b, const mlel_tensor *bScales,
+                 const mlel_tensor *biases, const mlel_tensor *output, cudaStream_t s) {
+    const std::string call = "mlel_cuda_matmul_scaled";
+    const ScaledProblem p = scaledProblemOf(call, a, aScales, b, bScales, biases, output);
+    return p.M == 0 || p.N == 0 ? int(MLEL_SUCCESS) : launchScaled(call, p, output->desc.dtype, s);
+}
+
+int quantizedLinear(const mlel_tensor *input, const mlel_tensor *b, const mlel_tensor *bScales, const mlel_tensor *biases,
+                    const mlel_tensor *output, void *workspace, uint64_t workspaceBytes, cudaStream_t s) {
+    const std::string call = "mlel_cuda_quantized_linear";
+    const Operand x = operandOf(call, "input", input, 2);
+    const int64_t M = x.dims[0], K = x.dims[1], padded = (K + 15) / 16 * 16;
+    if (M > 0 && (workspace == nullptr || !aligned(workspace, 16) || workspaceBytes < uint64_t(M * padded + 4 * M))) {
+        refuse(call, "the workspace is null, off a 16-byte boundary or smaller than the quantised rows and their scales");
+    }
+    mlel_tensor q{}, scales{};
+    q.data = workspace, scales.data = M > 0 ? static_cast<char *>(workspace) + M * padded : nullptr;
+    q.desc.dtype = MLEL_I8, q.desc.rank = 2;
+    q.desc.dims[0] = M, q.desc.dims[1] = K, q.desc.strides[0] = padded, q.desc.strides[1] = 1;
+    scales.desc.dtype = MLEL_F32, scales.desc.rank = 1, scales.desc.dims[0] = M;
+    // the product's operands are in order before anything is enqueued
+    const ScaledProblem p = scaledProblemOf(call, &q, &scales, b, bScales, biases, output);
+    const int rc = quantizeRows(input, &q, &scales, s);
+    return rc != MLEL_SUCCESS || p.M == 0 || p.N == 0 ? rc : launchScaled(call, p, output->desc.dtype, s);
 }
 
 } // namespace mlel

@@ -1,5 +1,5 @@
 // Operators of an 8-bit decoder layer behind the direct entry points mlel_cuda_quantize_rows, mlel_cuda_matmul_scaled,
-// mlel_cuda_paged_append and mlel_cuda_paged_attention: their launchers, and the checks of operands that they share.
+// mlel_cuda_quantized_linear, mlel_cuda_paged_append and mlel_cuda_paged_attention: their launchers, and the checks of operands that they share.
 // Launchers return an mlel_status, or throw what the C boundary turns into one.
 #pragma once
 
@@ -16,6 +16,8 @@ namespace mlel {
 int quantizeRows(const mlel_tensor *input, const mlel_tensor *output, const mlel_tensor *scales, cudaStream_t s);
 int matmulScaled(const mlel_tensor *a, const mlel_tensor *aScales, const mlel_tensor *b, const mlel_tensor *bScales,
                  const mlel_tensor *biases, const mlel_tensor *output, cudaStream_t s);
+int quantizedLinear(const mlel_tensor *input, const mlel_tensor *b, const mlel_tensor *bScales, const mlel_tensor *biases,
+                    const mlel_tensor *output, void *workspace, uint64_t workspaceBytes, cudaStream_t s);
 int pagedAppend(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *keys, const mlel_tensor *values,
                 const mlel_tensor *cosines, const mlel_tensor *sines, const mlel_tensor *queries, const mlel_tensor *rotated,
                 int interleaved, cudaStream_t s);

@@ -4,6 +4,9 @@ paged int8 cache (``PagedCache``, ``PagedBatch``) with its attention.
 Thin calls of the direct entry points in include/mlel_b200.h (``mlel_cuda_quantize_rows`` and the following), which say what
 each computes.  Work is enqueued on torch's current stream of the tensors' device; nothing waits.  Every call may be captured
 into a CUDA graph.  What the library refuses raises ``MlelError``.
+
+A decode step's kernels take a few microseconds each, so the way to them is kept short: objects that a program keeps
+(weights, a cache, a batch) hold their descriptions ready, a call describes its own tensors and enters the library once.
 """
 from __future__ import annotations
 
@@ -16,23 +19,32 @@ from . import BF16, F16, F32, I8, I32, check, lib
 from .runtime import _current_stream
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8, torch.int32: I32}
-_TENSOR = struct.Struct("=Qii6q6q")  # mlel_tensor: address, type, rank, sizes, strides in bytes
+_TENSOR = struct.Struct("=Qii6q6q").pack  # mlel_tensor: address, type, rank, sizes, strides in bytes
+_PADDED = [(0,) * (6 - rank) for rank in range(7)]
 _SIX = (0,) * 6
 
-_entry = {}
+_P, _I, _F, _U64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_uint64
+_SIGNATURES = {
+    "mlel_cuda_quantize_rows": (_P,) * 4,
+    "mlel_cuda_matmul_scaled": (_P,) * 7,
+    "mlel_cuda_quantized_linear": (_P,) * 6 + (_U64, _P),
+    "mlel_cuda_paged_append": (_P,) * 8 + (_I, _P),
+    "mlel_cuda_paged_attention": (_P,) * 4 + (_F, _I, _I, _F, _P, _U64, _P),
+    "mlel_paged_attention_workspace": (_P,) * 4,
+}
 
 
-def _call(name: str, argtypes):
-    """An entry point with its argument types set, in a function object of this module's own."""
-    fn = _entry.get(name)
-    if fn is None:
+class _Entries:
+    """The entry points, in function objects of this module's own, made when first used."""
+
+    def __getattr__(self, name):
         fn = lib()[name]
-        fn.argtypes, fn.restype = argtypes, ctypes.c_int
-        _entry[name] = fn
-    return fn
+        fn.argtypes, fn.restype = _SIGNATURES[name], ctypes.c_int
+        setattr(self, name, fn)
+        return fn
 
 
-_P, _V, _I, _F, _U64 = ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_uint64
+_entries = _Entries()
 
 
 def _pack(t: torch.Tensor) -> bytes:
@@ -40,62 +52,58 @@ def _pack(t: torch.Tensor) -> bytes:
     code = _DTYPES.get(t.dtype)
     if code is None:
         raise TypeError(f"tensors of {t.dtype} are not taken")
-    shape, rank = t.shape, t.dim()
+    shape = t.shape
+    rank = len(shape)
     if rank > 6:
         raise ValueError("tensors of more than 6 axes are not taken")
     if t.is_contiguous():
-        return _TENSOR.pack(t.data_ptr(), code, rank, *shape, *_SIX[rank:], *_SIX)
+        return _TENSOR(t.data_ptr(), code, rank, *shape, *_PADDED[rank], *_SIX)
     size = t.element_size()
     strides = [size * n for n in t.stride()]
     if strides[0] == 0:  # a stride of 0 there stands for a packed tensor
         if shape[0] > 1:
             raise ValueError("a tensor that repeats along its first axis is not taken")
         strides[0] = size * max(1, t.numel())
-    return _TENSOR.pack(t.data_ptr(), code, rank, *shape, *_SIX[rank:], *strides, *_SIX[rank:])
+    return _TENSOR(t.data_ptr(), code, rank, *shape, *_PADDED[rank], *strides, *_PADDED[rank])
 
 
-def _device(*tensors) -> int:
+def _device(first: torch.Tensor, *others) -> int:
     """The one CUDA device of all tensors (None among them are passed over)."""
-    device = tensors[0].device
-    if device.type != "cuda":
+    index = first.get_device()
+    if index < 0:
         raise ValueError("tensors have to be on a CUDA device: there is no CPU implementation to fall back to")
-    for t in tensors[1:]:
-        if t is not None and t.device != device:
+    for t in others:
+        if t is not None and t.get_device() != index:
             raise ValueError("tensors of one call have to be on one device")
-    return device.index
+    return index
 
 
-class _on:
-    """Makes ``index`` the current device for the calls inside."""
-
-    __slots__ = ("index", "before")
-
-    def __init__(self, index: int):
-        self.index = index
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-        return _current_stream(self.index)
-
-    def __exit__(self, *_):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
+def _enter(index: int, entry, *arguments) -> None:
+    """``entry(*arguments, stream)`` with ``index`` as the current device and torch's stream of it."""
+    before = torch.cuda.current_device()
+    if before == index:
+        status = entry(*arguments, _current_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = entry(*arguments, _current_stream(index))
+    if status != 0:
+        check(status)
 
 
 def quantize_rows(x: torch.Tensor, out: torch.Tensor | None = None, scales: torch.Tensor | None = None):
     """``(q, scales)``: the rows of ``x`` [..., K] (f32, f16 or bf16) in 8 bits with an f32 scale for each: ``scales = max|x| / 127``,
     ``q = round(x / scales)``.  ``out`` and ``scales`` are written where they are given ([M, K] int8 and [M], for M rows in all)."""
-    if x.dim() < 1:
-        raise ValueError("x needs an axis")
-    rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     index = _device(x, out, scales)
-    q = torch.empty(rows.shape, dtype=torch.int8, device=x.device) if out is None else out
-    s = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device) if scales is None else scales
-    with _on(index) as stream:
-        check(_call("mlel_cuda_quantize_rows", (_P, _P, _P, _V))(_pack(rows), _pack(q), _pack(s), stream))
-    return (q if out is not None else q.view(x.shape)), (s if scales is not None else s.view(x.shape[:-1]))
+    shape = x.shape
+    if len(shape) < 1:
+        raise ValueError("x needs an axis")
+    rows = x if len(shape) == 2 else x.reshape(-1, shape[-1])
+    q = rows.new_empty(rows.shape, dtype=torch.int8) if out is None else out
+    s = rows.new_empty(rows.shape[0], dtype=torch.float32) if scales is None else scales
+    _enter(index, _entries.mlel_cuda_quantize_rows, _pack(rows), _pack(q), _pack(s))
+    if len(shape) != 2:
+        return (q if out is not None else q.view(shape)), (s if scales is not None else s.view(shape[:-1]))
+    return q, s
 
 
 def matmul_scaled(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch.Tensor | None = None,
@@ -104,50 +112,56 @@ def matmul_scaled(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sc
     output channel), scales and bias in f32: the sums are exact, the result is rounded once to ``dtype`` (or ``out``'s type)."""
     index = _device(a, a_scales, b, b_scales, bias, out)
     if out is None:
-        out = torch.empty(a.shape[0], b.shape[0], dtype=dtype, device=a.device)
-    with _on(index) as stream:
-        check(_call("mlel_cuda_matmul_scaled", (_P,) * 6 + (_V,))(_pack(a), _pack(a_scales), _pack(b), _pack(b_scales),
-                                                               None if bias is None else _pack(bias), _pack(out), stream))
+        out = a.new_empty((a.shape[0], b.shape[0]), dtype=dtype)
+    _enter(index, _entries.mlel_cuda_matmul_scaled, _pack(a), _pack(a_scales), _pack(b), _pack(b_scales),
+           None if bias is None else _pack(bias), _pack(out))
     return out
 
 
 class QuantizedLinear:
     """A projection in 8 bits: ``linear(x)`` quantises the rows of ``x`` [..., K] and multiplies them with int8 ``weight`` [N, K],
     one f32 scale per output channel, optional f32 bias; the result has ``x``'s type.  The weights are laid out once: rows on
-    16-byte boundaries (copied only where they are not there already)."""
+    16-byte boundaries (copied only where they are not there already).  Their values may change between calls, their tensors not."""
 
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None):
-        _device(weight, scales, bias)
+        self.device = _device(weight, scales, bias)
         n, k = weight.shape
-        self.padded = (k + 15) // 16 * 16
+        self._padded = (k + 15) // 16 * 16
         if weight.stride(1) != 1 or weight.stride(0) % 16 != 0 or weight.data_ptr() % 16 != 0:
-            rows = torch.zeros(n, self.padded, dtype=torch.int8, device=weight.device)
+            rows = torch.zeros(n, self._padded, dtype=torch.int8, device=weight.device)
             rows[:, :k] = weight
             weight = rows[:, :k]
         self.weight, self.scales, self.bias = weight, scales.contiguous(), None if bias is None else bias.contiguous()
         self.in_features, self.out_features = k, n
+        self._packed = _pack(self.weight), _pack(self.scales), None if bias is None else _pack(self.bias)
 
     def __call__(self, x: torch.Tensor) -> torch.Tensor:
-        if x.shape[-1] != self.in_features:
-            raise ValueError(f"x has {x.shape[-1]} features, not {self.in_features}")
-        rows = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-        q = torch.empty(rows.shape[0], self.padded, dtype=torch.int8, device=x.device)[:, :self.in_features]
-        s = torch.empty(rows.shape[0], dtype=torch.float32, device=x.device)
-        quantize_rows(rows, q, s)
-        y = matmul_scaled(q, s, self.weight, self.scales, self.bias, dtype=x.dtype)
-        return y if x.dim() == 2 else y.view(*x.shape[:-1], self.out_features)
+        shape = x.shape
+        if shape[-1] != self.in_features:
+            raise ValueError(f"x has {shape[-1]} features, not {self.in_features}")
+        if x.get_device() != self.device:
+            raise ValueError("x has to be on the weights' device")
+        rows = x if len(shape) == 2 else x.reshape(-1, shape[-1])
+        m = rows.shape[0]
+        y = x.new_empty((m, self.out_features))
+        need = m * (self._padded + 4)
+        space = x.new_empty(need, dtype=torch.int8)
+        weight, scales, bias = self._packed
+        _enter(self.device, _entries.mlel_cuda_quantized_linear, _pack(rows), weight, scales, bias, _pack(y), space.data_ptr(), need)
+        return y if len(shape) == 2 else y.view(*shape[:-1], self.out_features)
 
 
 class PagedBatch:
     """The sequences of one call: new tokens of sequence b are rows ``starts[b]`` to ``starts[b + 1] - 1`` of the token axis and the last
-    of its ``lengths[b]`` tokens; token t lies in page ``page_table[b, t // page]``.  All int32 on the device; ``max_new`` and
-    ``max_length`` are bounds that the host knows."""
+    of its ``lengths[b]`` tokens; token t lies in page ``page_table[b, t // page]``.  All int32 on the device, read when the kernels
+    run; ``max_new`` and ``max_length`` are bounds that the host knows."""
 
     def __init__(self, starts: torch.Tensor, lengths: torch.Tensor, page_table: torch.Tensor, max_new: int, max_length: int):
         self.device = _device(starts, lengths, page_table)
         self.starts, self.lengths, self.page_table = starts, lengths, page_table
         self.max_new, self.max_length = int(max_new), int(max_length)
-        self._packed = (_pack(starts) + _pack(lengths) + _pack(page_table) + struct.pack("=ii", self.max_new, self.max_length))
+        self._packed = _pack(starts) + _pack(lengths) + _pack(page_table) + struct.pack("=ii", self.max_new, self.max_length)
+        self._space = {}  # bytes of workspace by the sizes that decide them
 
 
 class PagedCache:
@@ -160,6 +174,7 @@ class PagedCache:
         self.device = _device(data, scales)
         self.data, self.scales = data, scales
         self._packed = _pack(data[0]) + _pack(data[1]) + _pack(scales[0]) + _pack(scales[1])
+        self._sizes = tuple(data.shape[2:])
 
     @classmethod
     def empty(cls, pages: int, heads: int, page: int, head_dim: int, device="cuda") -> "PagedCache":
@@ -171,35 +186,39 @@ class PagedCache:
         """Writes new keys and values [tokens, heads, head_dim] into the cache, the keys rotated by their positions; ``cos`` and ``sin``
         are [positions, rotated / 2], or None for no rotation.  Returns the rotated queries where ``q`` is given (``q_out``, which may
         be ``q`` itself, or a new tensor, in which rows of no sequence are undefined)."""
-        index = _device(self.data, k, v, cos, sin, q, q_out, batch.starts)
+        if _device(k, v, cos, sin, q, q_out) != self.device or batch.device != self.device:
+            raise ValueError("tensors have to be on the cache's device")
         if q is not None and q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        with _on(index) as stream:
-            check(_call("mlel_cuda_paged_append", (_P,) * 8 + (_I, _V))(
-                self._packed, batch._packed, _pack(k), _pack(v), None if cos is None else _pack(cos), None if sin is None else _pack(sin),
-                None if q is None else _pack(q), None if q_out is None else _pack(q_out), int(interleaved), stream))
+            q_out = q.new_empty(q.shape)
+        _enter(self.device, _entries.mlel_cuda_paged_append, self._packed, batch._packed, _pack(k), _pack(v),
+               None if cos is None else _pack(cos), None if sin is None else _pack(sin), None if q is None else _pack(q),
+               None if q_out is None else _pack(q_out), 1 if interleaved else 0)
         return q_out
 
     def attend(self, q: torch.Tensor, batch: PagedBatch, out: torch.Tensor | None = None, scale: float | None = None, causal: bool = True,
                window: int = 0, softcap: float = 0.0) -> torch.Tensor:
         """Attention of the new tokens' queries [tokens, query_heads, head_dim] over the cache, which holds the new tokens already.
         ``scale`` defaults to head_dim ** -0.5; rows of no sequence are left as they are in ``out``, undefined in a new tensor."""
-        index = _device(self.data, q, out, batch.starts)
+        if _device(q, out) != self.device or batch.device != self.device:
+            raise ValueError("tensors have to be on the cache's device")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        packed_q = _pack(q)
-        need = ctypes.c_uint64()
-        check(_call("mlel_paged_attention_workspace", (_P, _P, _P, _V))(self._packed, batch._packed, packed_q, ctypes.addressof(need)))
-        space = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
-        with _on(index) as stream:
-            check(_call("mlel_cuda_paged_attention", (_P, _P, _P, _P, _F, _I, _I, _F, _V, _U64, _V))(
-                self._packed, batch._packed, packed_q, _pack(out), q.shape[-1] ** -0.5 if scale is None else scale, int(causal),
-                int(window), float(softcap), space.data_ptr() if space is not None else None, need.value, stream))
+            out = q.new_empty(q.shape)
+        packed = _pack(q)
+        sizes = (q.shape, self._sizes)
+        need = batch._space.get(sizes)
+        if need is None:
+            value = ctypes.c_uint64()
+            check(_entries.mlel_paged_attention_workspace(self._packed, batch._packed, packed, ctypes.addressof(value)))
+            need = batch._space[sizes] = value.value
+        space = q.new_empty(need, dtype=torch.int8) if need else None
+        _enter(self.device, _entries.mlel_cuda_paged_attention, self._packed, batch._packed, packed, _pack(out),
+               q.shape[-1] ** -0.5 if scale is None else scale, 1 if causal else 0, window, softcap,
+               None if space is None else space.data_ptr(), need)
         return out
 
 
 def paged_error(device: int | None = None) -> int:
     """0, or what the cache's kernels left out on the device since the last call: 1 a sequence whose numbers contradict the batch's
     bounds, 2 a page outside the cache.  Waits for the device and clears the record."""
-    with _on(torch.cuda.current_device() if device is None else device):
+    with torch.cuda.device(torch.cuda.current_device() if device is None else device):
         return lib().mlel_paged_error()

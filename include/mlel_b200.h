@@ -448,8 +448,14 @@ int mlel_cuda_quantize_rows(const mlel_tensor *input, const mlel_tensor *output,
 int mlel_cuda_matmul_scaled(const mlel_tensor *a, const mlel_tensor *a_scales, const mlel_tensor *b, const mlel_tensor *b_scales,
                             const mlel_tensor *biases, const mlel_tensor *output, void *cuda_stream);
 
+/* Both in one call: output = quantised rows of input [M, K] (f32, f16 or bf16) times b, in the output's type.  `workspace`: at least
+ * M * (K rounded up to 16) + 4 * M bytes of device memory on a 16-byte boundary that nothing else uses until the call's work is
+ * done; the quantised rows and then their scales lie in it afterwards. */
+int mlel_cuda_quantized_linear(const mlel_tensor *input, const mlel_tensor *b, const mlel_tensor *b_scales, const mlel_tensor *biases,
+                               const mlel_tensor *output, void *workspace, uint64_t workspace_bytes, void *cuda_stream);
+
 /* Keys and values of a decoder layer in pages of `page` tokens (a multiple of 16, at most 256), 8 bits each, with one scale for
- * each page and head: the value is the int8 element times the scale.  head_dim is a multiple of 16, at most 256. */
+ * each page and head, which is not negative: the value is the int8 element times the scale.  head_dim is a multiple of 16, at most 256. */
 typedef struct mlel_paged_cache {
     mlel_tensor keys, values;             /* int8 [pages, heads, page, head_dim], packed, on 16-byte boundaries */
     mlel_tensor key_scales, value_scales; /* f32 [pages, heads], packed */
