@@ -24,7 +24,7 @@ AttendParams paramsOf(const std::string &call, const mlel_paged_cache *cache, co
     p.queryHeads = int32_t(q.dims[1]), p.group = p.queryHeads / p.cache.heads;
     p.halves = q.dtype == MLEL_F16;
     p.wideQueries = aligned(q.ptr, 16) && q.strides[0] % 16 == 0 && q.strides[1] % 16 == 0;
-    p.pageDiv = makeFastDiv(p.cache.page);
+    p.pageDiv = makeFastDiv(p.cache.page), p.groupDiv = makeFastDiv(p.group);
     return p;
 }
 

@@ -22,7 +22,7 @@ struct AttendParams {
     int32_t wideQueries; // every head of the queries starts on a 16-byte boundary; the same for the output
     int32_t wideOut;
     float *partials; // split calls: see paged_attention_few.cu
-    FastDiv pageDiv;
+    FastDiv pageDiv, groupDiv;
 };
 
 // paged_attention_few.cu: few rows per cache head (single tokens, or a handful), keys split over the whole device

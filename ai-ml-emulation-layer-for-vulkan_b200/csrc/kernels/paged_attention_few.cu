@@ -58,7 +58,7 @@ template <int DP> struct FewShape {
 // Keys that any row of a sequence sees, in groups of 16, and the tiles that need them.
 struct FewWork {
     Sequence q;
-    int firstGroup, groups, steps, tiles;
+    int firstGroup, groups, steps, tiles, work;
 };
 template <int ROWS> __device__ __forceinline__ FewWork fewWorkOf(const AttendParams &p, int index) {
     FewWork w{};
@@ -69,67 +69,78 @@ template <int ROWS> __device__ __forceinline__ FewWork fewWorkOf(const AttendPar
         w.groups = (w.q.length + kGroup - 1) / kGroup - w.firstGroup;
         w.steps = (w.groups + kWarps - 1) / kWarps;
         w.tiles = (w.q.fresh * p.group + ROWS - 1) / ROWS * p.cache.heads;
+        w.work = w.steps * w.tiles; // (the plan has seen to it that the whole line has fewer than 2^31 steps)
     }
     return w;
 }
 
-struct FewScan {
-    long long sums[kWarps];
-    long long before; // work in front of the sequence found
-    int sequence;
+// The line of `total` steps in pieces: the first `longer` have one step more than the others.
+struct Pieces {
+    int base, longer;
+    __device__ Pieces(int total, int pieces) : base(total / pieces), longer(total - total / pieces * pieces) {}
+    __device__ int start(int c) const { return c * base + min(c, longer); }
+    __device__ int of(int x) const { // the piece that step x lies in
+        const int edge = longer * (base + 1);
+        return x < edge ? x / (base + 1) : longer + (x - edge) / base;
+    }
 };
 
-// All threads: the work of the whole batch; and for position `at` of it (negative: none wanted) the sequence and the work in
-// front of that, in `scan`.
-template <int ROWS> __device__ long long locate(const AttendParams &p, FewScan &scan, long long at, int pieces, bool report) {
+struct FewScan {
+    int sums[kWarps];
+    int total, before, sequence; // steps of all, and in front of the sequence found
+    FewWork work;
+};
+
+// All threads: how many steps the batch has, and the sequence that this block's piece starts in.
+template <int ROWS> __device__ void locate(const AttendParams &p, FewScan &scan, int piece, int pieces, bool report) {
     const int B = p.batch.sequences, each = (B + kWarps * 32 - 1) / (kWarps * 32);
     const int lo = min(B, int(threadIdx.x) * each), hi = min(B, lo + each);
     const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
-    long long own = 0;
+    int own = 0;
+    FewWork w{};
     for (int b = lo; b < hi; ++b) {
-        const FewWork w = fewWorkOf<ROWS>(p, b);
-        own += (long long)w.steps * w.tiles;
+        w = fewWorkOf<ROWS>(p, b);
+        own += w.work;
         if (report && !w.q.sound) {
             atomicCAS(&g_pagedError, 0, kBadSequence);
         }
     }
-    long long upTo = own;
+    int upTo = own;
 #pragma unroll
     for (int step = 1; step < 32; step <<= 1) {
-        const long long other = __shfl_up_sync(0xffffffffu, upTo, step);
+        const int other = __shfl_up_sync(0xffffffffu, upTo, step);
         upTo += lane >= step ? other : 0;
     }
     if (lane == 31) {
         scan.sums[warp] = upTo;
     }
     __syncthreads();
-    long long total = 0;
+    int total = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        upTo += w < warp ? scan.sums[w] : 0;
-        total += scan.sums[w];
+    for (int v = 0; v < kWarps; ++v) {
+        upTo += v < warp ? scan.sums[v] : 0;
+        total += scan.sums[v];
     }
-    if (pieces > 0) {
-        at = total * at / pieces;
-    }
-    long long before = upTo - own;
+    const int at = Pieces(total, pieces).start(piece);
+    int before = upTo - own;
     if (at >= before && at < upTo) {
-        for (int b = lo; b < hi; ++b) {
-            const FewWork w = fewWorkOf<ROWS>(p, b);
-            const long long work = (long long)w.steps * w.tiles;
-            if (at < before + work) {
-                scan.before = before, scan.sequence = b;
-                break;
+        int b = lo;
+        if (each > 1) {
+            for (;; ++b) {
+                w = fewWorkOf<ROWS>(p, b);
+                if (at < before + w.work) {
+                    break;
+                }
+                before += w.work;
             }
-            before += work;
         }
+        scan.before = before, scan.sequence = b, scan.work = w;
+    }
+    if (threadIdx.x == 0) {
+        scan.total = total;
     }
     __syncthreads();
-    return total;
 }
-
-// Where block `piece` of `pieces` starts on a line of `total` steps.
-__device__ __forceinline__ long long pieceStart(long long total, long long piece, int pieces) { return total * piece / pieces; }
 
 // One row of a partial result: maximum, sum, then DP elements.
 template <int DP> __device__ __forceinline__ float *partialRow(const AttendParams &p, int piece, int which, int row, int rows) {
@@ -157,29 +168,27 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     dependencySync();
-    const int pieces = int(gridDim.x);
-    const long long total = locate<ROWS>(p, scan, blockIdx.x, pieces, blockIdx.x == 0); // (its barriers cover mbarInit too)
-    const long long end = pieceStart(total, blockIdx.x + 1, pieces);
-    long long at = pieceStart(total, blockIdx.x, pieces);
+    locate<ROWS>(p, scan, int(blockIdx.x), int(gridDim.x), blockIdx.x == 0); // (its barriers cover mbarInit too)
+    const Pieces pieces(scan.total, int(gridDim.x));
+    const int begin = pieces.start(int(blockIdx.x)), end = pieces.start(int(blockIdx.x) + 1);
+    int at = begin;
     if (at >= end) {
         return;
     }
-    int index = scan.sequence;
-    long long before = scan.before;
-    const long long begin = at;
+    int index = scan.sequence, before = scan.before;
+    FewWork w = scan.work;
     uint8_t *own = ring + warp * (Shape::kStages * Shape::kStageBytes);
     int stage = 0;      // next to be read
     uint32_t phase = 0; // of that stage
     bool broken = false;
 
     while (at < end) {
-        FewWork w = fewWorkOf<ROWS>(p, index);
-        while (at >= before + (long long)w.steps * w.tiles) {
-            before += (long long)w.steps * w.tiles;
+        while (at >= before + w.work) {
+            before += w.work;
             w = fewWorkOf<ROWS>(p, ++index); // (there is one: `at` lies on the line)
         }
-        const int tileIndex = int((at - before) / w.steps), firstStep = int((at - before) - (long long)tileIndex * w.steps);
-        const int lastStep = int(min((long long)w.steps, firstStep + (end - at)));
+        const int tileIndex = (at - before) / w.steps, firstStep = at - before - tileIndex * w.steps;
+        const int lastStep = min(w.steps, firstStep + (end - at));
         const int head = tileIndex % p.cache.heads, firstRow = tileIndex / p.cache.heads * ROWS;
         const int rows = min(ROWS, w.q.fresh * p.group - firstRow), old = w.q.length - w.q.fresh;
         // this warp's groups: every fourth of the piece
@@ -221,10 +230,6 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             ++issued;
             writeStage = writeStage + 1 == Shape::kStages ? 0 : writeStage + 1;
         };
-        for (int n = 0; n < min(count, Shape::kStages) && !broken; ++n) {
-            fill();
-        }
-
         // queries: lane (g, t) holds rows g and g + 8 of each 16, elements 64 seg + 16 t .. + 15
         uint32_t qf[MT][SEGS][4][4];
         float rowScale[MT][2]; // scores in powers of two, up to the key's scale
@@ -235,7 +240,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             for (int r = 0; r < 2; ++r) {
                 const int row = firstRow + 16 * mt + 8 * r + g;
                 const bool live = 16 * mt + 8 * r + g < rows;
-                const int token = live ? row / p.group : 0, queryHead = head * p.group + (live ? row - token * p.group : 0);
+                const int token = live ? int(fastDiv(uint32_t(row), p.groupDiv)) : 0, queryHead = head * p.group + (live ? row - token * p.group : 0);
                 const T *q = reinterpret_cast<const T *>(p.queries + int64_t(w.q.first + token) * p.queryStride[0] +
                                                          queryHead * p.queryStride[1]);
                 const int position = old + token;
@@ -246,6 +251,14 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
 #pragma unroll
                 for (int seg = 0; seg < SEGS; ++seg) {
                     loadQuerySixteen(q, seg * 64 + t * 16, live ? p.cache.headDim : 0, p.wideQueries != 0, words[seg]);
+                }
+                if (mt == 0 && r == 0) { // the first copies go out while the queries are on their way
+                    for (int n = 0; n < min(count, Shape::kStages) && !broken; ++n) {
+                        fill();
+                    }
+                }
+#pragma unroll
+                for (int seg = 0; seg < SEGS; ++seg) {
                     if (!HALF) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
@@ -507,10 +520,10 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
 
 // Joins the pieces of one row of one tile (blockIdx.y: the row).
 template <int DP, int MT, bool HALF>
-__global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const AttendParams p, const int pieces) {
+__global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const AttendParams p, const int count) {
     constexpr int ROWS = 16 * MT;
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
-    __shared__ long long parts[2][kWarps];
+    __shared__ int parts[2][kWarps];
     dependencySync();
     // the tiles of all sequences in a row, those of a sequence without work included: ceil(max_new * group / ROWS) * heads each
     const int perSequence = int(gridDim.x) / p.batch.sequences;
@@ -520,64 +533,42 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
     if (tile >= w.tiles || row >= w.q.fresh * p.group - firstRow || w.steps < 2) { // (the whole block)
         return;
     }
-    // work in front of this sequence: a scan over all, of which those behind count nothing
-    long long before = 0, total = 0;
-    {
-        const int B = p.batch.sequences;
-        long long front = 0, all = 0;
-        for (int b = int(threadIdx.x); b < B; b += kWarps * 32) {
-            const FewWork v = fewWorkOf<ROWS>(p, b);
-            const long long work = (long long)v.steps * v.tiles;
-            all += work;
-            front += b < index ? work : 0;
-        }
-#pragma unroll
-        for (int step = 16; step > 0; step >>= 1) {
-            all += __shfl_xor_sync(0xffffffffu, all, step);
-            front += __shfl_xor_sync(0xffffffffu, front, step);
-        }
-        if ((threadIdx.x & 31) == 0) {
-            parts[0][threadIdx.x >> 5] = all, parts[1][threadIdx.x >> 5] = front;
-        }
-        __syncthreads();
-        for (int v = 0; v < kWarps; ++v) {
-            total += parts[0][v], before += parts[1][v];
-        }
+    // the steps of all sequences, and of those in front of this one
+    int all = 0, front = 0;
+    for (int b = int(threadIdx.x); b < p.batch.sequences; b += kWarps * 32) {
+        const int work = fewWorkOf<ROWS>(p, b).work;
+        all += work;
+        front += b < index ? work : 0;
     }
-    const long long x0 = before + (long long)tile * w.steps, x1 = x0 + w.steps - 1;
-    // the piece that position x lies in: the last one that starts at or before x
-    const auto pieceOf = [&](long long x) {
-        long long c = (x * pieces + pieces - 1) / total;
-        while (c > 0 && pieceStart(total, c, pieces) > x) {
-            --c;
-        }
-        while (c + 1 < pieces && pieceStart(total, c + 1, pieces) <= x) {
-            ++c;
-        }
-        return int(c);
-    };
-    const int c0 = pieceOf(x0), c1 = pieceOf(x1);
+    all = __reduce_add_sync(0xffffffffu, all), front = __reduce_add_sync(0xffffffffu, front);
+    if ((threadIdx.x & 31) == 0) {
+        parts[0][threadIdx.x >> 5] = all, parts[1][threadIdx.x >> 5] = front;
+    }
+    __syncthreads();
+    int total = 0, before = 0;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) {
+        total += parts[0][v], before += parts[1][v];
+    }
+    const Pieces pieces(total, count);
+    const int x0 = before + tile * w.steps, c0 = pieces.of(x0), c1 = pieces.of(x0 + w.steps - 1);
     if (c0 == c1) {
         return; // written by that piece
     }
-    const int first = x0 == pieceStart(total, c0, pieces) ? 0 : 1; // where piece c0 left it: as its first tile, or as its last
+    const int first = x0 == pieces.start(c0) ? 0 : 1; // where piece c0 left it: as its first tile, or as its last
     float top = -INFINITY;
     for (int c = c0; c <= c1; ++c) {
-        if (pieceStart(total, c, pieces) < pieceStart(total, c + 1, pieces)) {
-            top = fmaxf(top, partialRow<DP>(p, c, c == c0 ? first : 0, row, ROWS)[0]);
-        }
+        top = fmaxf(top, partialRow<DP>(p, c, c == c0 ? first : 0, row, ROWS)[0]);
     }
     for (int d = int(threadIdx.x) * 4; d < DP; d += kWarps * 32 * 4) {
         float4 y = {};
         float sum = 0.f;
         for (int c = c0; c <= c1; ++c) {
-            if (pieceStart(total, c, pieces) < pieceStart(total, c + 1, pieces)) {
-                const float *from = partialRow<DP>(p, c, c == c0 ? first : 0, row, ROWS);
-                const float factor = top == -INFINITY ? 1.f : exp2Fast(from[0] - top);
-                const float4 a = *reinterpret_cast<const float4 *>(from + 4 + d);
-                y.x += a.x * factor, y.y += a.y * factor, y.z += a.z * factor, y.w += a.w * factor;
-                sum += from[1] * factor;
-            }
+            const float *from = partialRow<DP>(p, c, c == c0 ? first : 0, row, ROWS);
+            const float factor = top == -INFINITY ? 1.f : exp2Fast(from[0] - top);
+            const float4 a = *reinterpret_cast<const float4 *>(from + 4 + d);
+            y.x += a.x * factor, y.y += a.y * factor, y.z += a.z * factor, y.w += a.w * factor;
+            sum += from[1] * factor;
         }
         writeOut<T>(p, w.q.first, firstRow + row, head, d, y, sum);
     }
@@ -621,6 +612,9 @@ FewPlan pagedAttentionFewPlan(const AttendParams &p) {
     const int64_t steps = (int64_t(p.batch.maxLength) + kGroup * kWarps - 1) / (kGroup * kWarps);
     const int64_t work = steps * ((rows + plan.rows - 1) / plan.rows) * p.cache.heads * p.batch.sequences;
     const int resident = dp == 256 || plan.rows == 32 ? 2 : 3;
+    if (work > 0x7fffffff) {
+        refuse("mlel_cuda_paged_attention", "sequences, tokens and lengths give too much work for one call");
+    }
     plan.blocks = int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(resident) * smCount())));
     plan.joins = steps > 1 && plan.blocks > 1;
     plan.workspace = plan.joins ? uint64_t(plan.blocks) * 2 * uint64_t(plan.rows) * uint64_t(dp + 4) * 4 : 0;
