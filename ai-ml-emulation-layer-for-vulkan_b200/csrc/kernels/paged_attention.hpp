@@ -27,10 +27,10 @@ struct AttendParams {
 
 // paged_attention_few.cu: few rows per cache head (single tokens, or a handful), keys split over the whole device
 struct FewPlan {
-    int rows;    // rows of a tile: 16 or 32
-    int blocks;  // that share the keys
-    bool joins;  // keys of one tile may lie with several blocks: a second kernel joins their results
-    uint64_t workspace;
+    int rows;           // of a tile: 8, 16 or 32
+    int split;          // blocks of the cluster that shares a tile's keys; 0: all blocks share all keys
+    int blocks;
+    uint64_t workspace; // where parts of a tile may lie with blocks that are no cluster: a second kernel joins them
 };
 FewPlan pagedAttentionFewPlan(const AttendParams &p);
 int pagedAttentionFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s);

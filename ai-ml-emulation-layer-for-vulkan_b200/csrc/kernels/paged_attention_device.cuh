@@ -51,6 +51,22 @@ __device__ __forceinline__ void bytesToHalves(uint32_t word, uint32_t &low, uint
     low = minus1152(__byte_perm(u, 0x64646464u, 0x4140));
     high = minus1152(__byte_perm(u, 0x64646464u, 0x4342));
 }
+// Four signed bytes x as the subnormal halves (x + 128) 2^-24.
+__device__ __forceinline__ void bytesToSubnormals(uint32_t word, uint32_t &low, uint32_t &high) {
+    const uint32_t u = word ^ 0x80808080u;
+    low = __byte_perm(u, 0u, 0x4140), high = __byte_perm(u, 0u, 0x4342);
+}
+// 8 x 8 halves, lane (g, t) holding row g, columns 2 t and 2 t + 1: the same of the transposed matrix.
+__device__ __forceinline__ uint32_t transposeHalves(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float4 loadCluster(uint32_t clusterAddr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(clusterAddr) : "memory");
+    return v;
+}
 // Byte d of `a` and of `b` side by side as f16, d = 0 .. 3.
 __device__ __forceinline__ void transposeToHalves(uint32_t a, uint32_t b, uint32_t (&out)[4]) {
     bytesToHalves(__byte_perm(a, b, 0x5140), out[0], out[1]);

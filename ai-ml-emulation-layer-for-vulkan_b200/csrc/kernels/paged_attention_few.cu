@@ -2,30 +2,37 @@
 //
 //   o = sum_j softmax(s)_j v_j,  s_j = scale * q . k_j (capped or not), over the tokens that the masks leave
 //
-// What bounds it: the bytes of the cache.  Every key and value is read once per tile of 16 or 32 rows (a row is one token's query
-// head; the heads that share a cache head are rows of one tile), so a tile does 2 x 16 multiply-adds per byte and the
-// arithmetic has to stay out of the way of 6.5 TB/s, some 23 bytes per cycle and SM.
+// What bounds it: the bytes of the cache, and close behind them the instructions that turn them into operands.  Every key and
+// value is read once per tile of 8, 16 or 32 rows (a row is one token's query head; the heads that share a cache head are rows of
+// one tile).  At 6.5 TB/s an SM gets some 23 bytes a cycle, 16 keys and values of 128 elements every 180 cycles.
 //
-// Work.  All tiles' keys, in steps of 64, form one line that is cut into as many equal pieces as there are blocks, whatever the
+// Work.  All tiles' keys, in steps of 128, form one line that is cut into as many equal pieces as there are blocks, whatever the
 // lengths of the sequences: a block works through the ends of the tiles that its piece touches.  Tiles that lie in
 // one piece are written straight away; of the others the blocks leave (maximum, sum, unscaled result) in the workspace,
-// and a second kernel joins them.  A block has four warps; three blocks fit an SM, so that one's start and end of a tile run
-// under the others' reads.
+// and a second kernel joins them.  A block has four warps; two to three blocks fit an SM, so that one's start and end of a tile
+// run under the others' reads.  Where the line is short, a cluster of up to eight blocks takes a tile instead, each an equal part of
+// its keys, and joins the parts through distributed shared memory: no search, no workspace and no second kernel.
 //
-// A warp has a ring of its own, 16 keys and values a stage, filled by its own lane 0 with bulk tensor copies (128-byte or 64-byte
-// swizzle), and no barrier with the other warps before the end of a tile.  Pages hold a multiple of 16 tokens, so 16
-// keys lie in one page, with one scale.
+// A warp has a ring of its own, 32 keys and values a stage, filled by its own lanes with bulk tensor copies of 16 rows (128-byte
+// or 64-byte swizzle; pages hold a multiple of 16 tokens, so 16 keys lie in one page, with one scale), and no barrier with
+// the other warps before the end of a tile.
 //
-// Products on m16n8k16 in f16 with f32 sums: an integer of 8 bits is exact in f16, made by placing it (plus 128) in the low
-// mantissa bits of 1024 and subtracting 1152.  Which element of a head is which k of the product is free as long as both
-// operands agree, so a lane takes 16 consecutive bytes of a key; which key is which column is free as long as the weights
-// and the values agree, so a lane's four keys are t, t + 4, t + 8, t + 12 and its values 16 consecutive bytes of each, which
-// four byte transpositions turn into operands.  All these reads are free of bank conflicts.
+// Products on m16n8k16 in f16 with f32 sums, transposed: S^T = K Q^T and O^T = V^T P^T, so that 16 keys (16 elements of the
+// result) are the rows and 8 queries the columns: with at most 8 rows to a tile that is half the products and half the scores
+// per lane of the untransposed form, which pads to 16.  P^T changes from result to operand by a transposition of 8 x 8.
+// Which element of a head is which k of the first product is free as long as both operands agree, so a lane takes 16
+// consecutive bytes of a key; which key is which row is free as long as weights and values agree, so a lane's keys are t,
+// t + 4, t + 8, t + 12 and its values 16 consecutive bytes of each.  All these reads are free of bank conflicts.
+//
+// Integers of 8 bits are exact in f16.  Keys: x + 128 as the low byte of a half is the subnormal number (x + 128) 2^-24, one byte
+// permutation per two; the product's accumulator starts at -128 sum(q) 2^-24 and the scale takes the 2^24.  (Sums are then some four
+// times as large as they need be, and still 2^-22 exact.)  Values: x + 128 in the low bits of 1024, minus 1152: an offset in the
+// result would have to be subtracted from sums that may be a thousand times smaller than it.
 //
 // bf16 queries become f16 after a row-wise power of two that puts the largest at 2^14; elements down to 2^-29 of that stay
 // exact.  Weights are rounded to f16: p * (v scale / reference) * 2^14, the reference a running power of two, so that
 // what is lost lies 2^-38 below the largest.  The result stays in registers in units of that reference; it is
-// rescaled only when a maximum or the reference grows, which one vote per 16 keys finds out.
+// rescaled only when a maximum or the reference grows, which one vote per 32 keys finds out.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -37,6 +44,7 @@
 #include "paged_attention_map.hpp"
 #include "serving_device.cuh"
 #include "tcgen05_common.cuh"
+#include "tcgen05_pair.cuh"
 
 namespace mlel {
 namespace {
@@ -44,15 +52,20 @@ namespace {
 using namespace tc;
 
 constexpr int kWarps = 4;
-constexpr int kGroup = 16; // keys of a stage
+constexpr int kGroup = 16; // keys that share a page and a scale for certain
+constexpr int kStageGroups = 2;
+constexpr int kStepGroups = kWarps * kStageGroups;
 constexpr float kWeightScale = 16384.f;
+constexpr int kClusterSteps = 3; // steps by which a cluster's blocks may outlast the line's
 
 template <int DP> struct FewShape {
-    static constexpr int kStageBytes = 2 * kGroup * DP; // keys and values
-    static constexpr int kPanel = DP < 128 ? DP : 128;  // bytes of a row of a swizzled box
+    static constexpr int kGroupBytes = kGroup * DP; // of keys, or of values
+    static constexpr int kStageBytes = 2 * kStageGroups * kGroupBytes;
+    static constexpr int kPanel = DP < 128 ? DP : 128; // bytes of a row of a swizzled box
     static constexpr int kPanels = DP / kPanel;
-    static constexpr int kStages = DP == 256 ? 3 : DP == 128 ? 4 : 6;
+    static constexpr int kStages = DP == 64 ? 3 : 2;
     static constexpr int kRing = kWarps * kStages * kStageBytes;
+    static constexpr int kPitch = DP + 4; // floats between the rows of results
 };
 
 // Keys that any row of a sequence sees, in groups of 16, and the tiles that need them.
@@ -67,7 +80,7 @@ template <int ROWS> __device__ __forceinline__ FewWork fewWorkOf(const AttendPar
         const int lo = p.window > 0 ? max(0, w.q.length - w.q.fresh - p.window + 1) : 0;
         w.firstGroup = lo / kGroup;
         w.groups = (w.q.length + kGroup - 1) / kGroup - w.firstGroup;
-        w.steps = (w.groups + kWarps - 1) / kWarps;
+        w.steps = (w.groups + kStepGroups - 1) / kStepGroups;
         w.tiles = (w.q.fresh * p.group + ROWS - 1) / ROWS * p.cache.heads;
         w.work = w.steps * w.tiles; // (the plan has seen to it that the whole line has fewer than 2^31 steps)
     }
@@ -147,291 +160,348 @@ template <int DP> __device__ __forceinline__ float *partialRow(const AttendParam
     return p.partials + ((int64_t(piece) * 2 + which) * rows + row) * (DP + 4);
 }
 
-template <int DP, int MT, bool HALF>
-__global__ void __launch_bounds__(kWarps * 32, DP == 256 || MT == 2 ? 2 : 3)
-pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p) {
+template <int DP, int NQ, bool HALF>
+__global__ void __launch_bounds__(kWarps * 32, NQ * DP <= 128 ? 3 : 2)
+pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p,
+                        const int split) { // blocks of the cluster that shares a tile; 0: pieces of the line
     using Shape = FewShape<DP>;
-    constexpr int ROWS = 16 * MT, SEGS = DP / 64, NT = DP / 8;
+    constexpr int ROWS = 8 * NQ, SEGS = DP / 64, MT = DP / 16, STAGES = Shape::kStages;
+    constexpr int AT = NQ * DP <= 128 ? 2 : 1; // groups taken at once: as many as the registers hold
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     extern __shared__ uint8_t rawSmem[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rawSmem) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t full[kWarps][Shape::kStages];
+    __shared__ uint64_t full[kWarps][STAGES];
     __shared__ FewScan scan;
     __shared__ float joinMax[kWarps][ROWS], joinSum[kWarps][ROWS];
     const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5, g = lane >> 2, t = lane & 3;
     if (threadIdx.x == 0) {
         for (int w = 0; w < kWarps; ++w) {
-            for (int s = 0; s < Shape::kStages; ++s) {
+            for (int s = 0; s < STAGES; ++s) {
                 mbarInit(&full[w][s], 1u);
             }
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     dependencySync();
-    locate<ROWS>(p, scan, int(blockIdx.x), int(gridDim.x), blockIdx.x == 0); // (its barriers cover mbarInit too)
-    const Pieces pieces(scan.total, int(gridDim.x));
-    const int begin = pieces.start(int(blockIdx.x)), end = pieces.start(int(blockIdx.x) + 1);
-    int at = begin;
-    if (at >= end) {
-        return;
+    int index, before = 0, begin, end, rank = 0;
+    FewWork w;
+    if (split > 0) {
+        rank = int(clusterCtaRank());
+        const int cluster = int(blockIdx.x) / split, perSequence = int(gridDim.x) / (split * p.batch.sequences);
+        index = cluster / perSequence;
+        w = fewWorkOf<ROWS>(p, index);
+        const int tile = cluster - index * perSequence;
+        if (!w.q.sound && tile == 0 && rank == 0 && threadIdx.x == 0) {
+            atomicCAS(&g_pagedError, 0, kBadSequence);
+        }
+        if (tile >= w.tiles) { // (the whole cluster)
+            return;
+        }
+        begin = tile * w.steps + w.steps * rank / split, end = tile * w.steps + w.steps * (rank + 1) / split;
+        __syncthreads();
+    } else {
+        locate<ROWS>(p, scan, int(blockIdx.x), int(gridDim.x), blockIdx.x == 0); // (its barriers cover mbarInit too)
+        const Pieces pieces(scan.total, int(gridDim.x));
+        begin = pieces.start(int(blockIdx.x)), end = pieces.start(int(blockIdx.x) + 1);
+        if (begin >= end) {
+            return;
+        }
+        index = scan.sequence, before = scan.before, w = scan.work;
     }
-    int index = scan.sequence, before = scan.before;
-    FewWork w = scan.work;
-    uint8_t *own = ring + warp * (Shape::kStages * Shape::kStageBytes);
+    uint8_t *own = ring + warp * (STAGES * Shape::kStageBytes);
     int stage = 0;      // next to be read
     uint32_t phase = 0; // of that stage
     bool broken = false;
 
-    while (at < end) {
-        while (at >= before + w.work) {
+    int at = begin;
+    do { // (a block of a cluster whose part is empty still takes part in joining)
+        while (split == 0 && at >= before + w.work) {
             before += w.work;
             w = fewWorkOf<ROWS>(p, ++index); // (there is one: `at` lies on the line)
         }
-        const int tileIndex = (at - before) / w.steps, firstStep = at - before - tileIndex * w.steps;
-        const int lastStep = min(w.steps, firstStep + (end - at));
+        const int tileIndex = split > 0 ? int(blockIdx.x) / split % (int(gridDim.x) / (split * p.batch.sequences)) : (at - before) / w.steps;
+        const int firstStep = at - before - tileIndex * w.steps, lastStep = min(w.steps, firstStep + (end - at));
         const int head = tileIndex % p.cache.heads, firstRow = tileIndex / p.cache.heads * ROWS;
         const int rows = min(ROWS, w.q.fresh * p.group - firstRow), old = w.q.length - w.q.fresh;
-        // this warp's groups: every fourth of the piece
-        const int firstGroup = w.firstGroup + firstStep * kWarps + warp,
-                  groupEnd = min(w.firstGroup + w.groups, w.firstGroup + lastStep * kWarps);
-        const int count = firstGroup < groupEnd ? (groupEnd - firstGroup + kWarps - 1) / kWarps : 0;
+        // this warp's stages: two groups each, every fourth pair of the piece
+        const int firstGroup = w.firstGroup + firstStep * kStepGroups + warp * kStageGroups,
+                  groupEnd = min(w.firstGroup + w.groups, w.firstGroup + lastStep * kStepGroups);
+        const int count = firstGroup < groupEnd ? (groupEnd - firstGroup + kStepGroups - 1) / kStepGroups : 0;
         const int32_t *table = p.batch.table + index * p.batch.tableStride;
 
-        // The slots and scales of 32 groups at a time, a lane each: scales are fetched a batch, slots two batches ahead.
+        // The pages and scales of 16 stages at a time, a lane a group: scales are fetched a batch, pages two batches ahead.
+        const auto groupOf = [&](int n) { return firstGroup + (n >> 1) * kStepGroups + (n & 1); }; // n: groups of this warp
         const auto slotOf = [&](int n) {
-            const int slot = n < count ? table[fastDiv(uint32_t(firstGroup + n * kWarps) * kGroup, p.pageDiv)] : -1;
-            if (n < count && uint32_t(slot) >= uint32_t(p.cache.pages)) {
-                atomicCAS(&g_pagedError, 0, kBadPage);
+            const int group = groupOf(n);
+            int slot = -1;
+            if (group < groupEnd) {
+                slot = table[fastDiv(uint32_t(group * kGroup), p.pageDiv)];
+                if (uint32_t(slot) >= uint32_t(p.cache.pages)) {
+                    atomicCAS(&g_pagedError, 0, kBadPage);
+                    slot = -1;
+                }
             }
-            return uint32_t(slot) < uint32_t(p.cache.pages) ? slot : -1;
+            return slot;
         };
-        const auto scaleOf = [&](const float *scales, int slot) { return slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : 0.f; };
+        // a key scale of -1 stands for a group that is not there
+        const auto scaleOf = [&](const float *scales, int slot) { return slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : -1.f; };
         int slots = slotOf(lane), nextSlots = slotOf(32 + lane);
         float keyScales = scaleOf(p.cache.keyScales, slots), valueScales = scaleOf(p.cache.valueScales, slots);
         int issued = 0, writeStage = stage, issueSlots = slots;
-        const auto fill = [&] { // the next group into the ring, all lanes together
-            if (issued > 0 && (issued & 31) == 0) {
+        // lanes that issue a copy: keys or values, which of the two groups, which panel
+        const int side = lane & 1, sub = (lane >> 1) & 1, panel = lane >> 2;
+        const auto fill = [&] { // the next stage of the ring, all lanes together
+            if (issued > 0 && (issued & 15) == 0) {
                 issueSlots = nextSlots;
             }
-            const int slot = max(0, __shfl_sync(0xffffffffu, issueSlots, issued & 31));
+            const int slot = max(0, __shfl_sync(0xffffffffu, issueSlots, (2 * issued + sub) & 31));
+            const int group = groupOf(2 * issued + sub), key = group * kGroup;
+            const int row = (slot * p.cache.heads + head) * p.cache.page + key - int(fastDiv(uint32_t(key), p.pageDiv)) * p.cache.page;
+            uint64_t *bar = &full[warp][writeStage];
+            const int groups = min(kStageGroups, groupEnd - groupOf(2 * issued));
             if (lane == 0) {
-                const int key = (firstGroup + issued * kWarps) * kGroup;
-                const int inPage = key - int(fastDiv(uint32_t(key), p.pageDiv)) * p.cache.page;
-                const int row = (slot * p.cache.heads + head) * p.cache.page + inPage;
-                uint64_t *bar = &full[warp][writeStage];
-                uint8_t *to = own + writeStage * Shape::kStageBytes;
-                mbarArriveExpectTx(bar, uint32_t(Shape::kStageBytes));
-#pragma unroll
-                for (int panel = 0; panel < Shape::kPanels; ++panel) {
-                    tmaLoad3d(&mapK, to + panel * (kGroup * Shape::kPanel), bar, panel * 128, row, 0);
-                    tmaLoad3d(&mapV, to + kGroup * DP + panel * (kGroup * Shape::kPanel), bar, panel * 128, row, 0);
-                }
+                mbarArriveExpectTx(bar, uint32_t(groups * 2 * Shape::kGroupBytes));
+            }
+            __syncwarp();
+            if (lane < 4 * Shape::kPanels && sub < groups) {
+                tmaLoad3d(side == 0 ? &mapK : &mapV,
+                          own + writeStage * Shape::kStageBytes + (2 * side + sub) * Shape::kGroupBytes + panel * (kGroup * Shape::kPanel), bar,
+                          panel * 128, row, 0);
             }
             ++issued;
-            writeStage = writeStage + 1 == Shape::kStages ? 0 : writeStage + 1;
+            writeStage = writeStage + 1 == STAGES ? 0 : writeStage + 1;
         };
-        // queries: lane (g, t) holds rows g and g + 8 of each 16, elements 64 seg + 16 t .. + 15
-        uint32_t qf[MT][SEGS][4][4];
-        float rowScale[MT][2]; // scores in powers of two, up to the key's scale
-        int rowLo[MT][2], rowHi[MT][2];
+
+        // queries, the second operand of S^T: lane (g, t) holds row 8 nq + g, elements 64 seg + 16 t .. + 15
+        uint32_t qf[NQ][SEGS][4][2];
+        float rowScale[NQ][2], offset[NQ][2]; // of rows 8 nq + 2 t and + 1, whose scores the lane gets
+        int rowLo[NQ][2], rowHi[NQ][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int nq = 0; nq < NQ; ++nq) {
+            const int row = firstRow + 8 * nq + g;
+            const bool live = 8 * nq + g < rows;
+            const int token = live ? int(fastDiv(uint32_t(row), p.groupDiv)) : 0, queryHead = head * p.group + (live ? row - token * p.group : 0);
+            const T *q = reinterpret_cast<const T *>(p.queries + int64_t(w.q.first + token) * p.queryStride[0] + queryHead * p.queryStride[1]);
+            uint32_t words[SEGS][8]; // two elements each, as they lie in memory
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int row = firstRow + 16 * mt + 8 * r + g;
-                const bool live = 16 * mt + 8 * r + g < rows;
-                const int token = live ? int(fastDiv(uint32_t(row), p.groupDiv)) : 0, queryHead = head * p.group + (live ? row - token * p.group : 0);
-                const T *q = reinterpret_cast<const T *>(p.queries + int64_t(w.q.first + token) * p.queryStride[0] +
-                                                         queryHead * p.queryStride[1]);
-                const int position = old + token;
-                rowHi[mt][r] = !live ? 0 : p.causal ? position + 1 : w.q.length;
-                rowLo[mt][r] = p.window > 0 ? max(0, position - p.window + 1) : 0;
-                uint32_t words[SEGS][8]; // two elements each, as they lie in memory
+            for (int seg = 0; seg < SEGS; ++seg) {
+                loadQuerySixteen(q, seg * 64 + t * 16, live ? p.cache.headDim : 0, p.wideQueries != 0, words[seg]);
+            }
+            if (nq == 0) { // the first copies go out while the queries are on their way
+                for (int n = 0; n < min(count, STAGES) && !broken; ++n) {
+                    fill();
+                }
+            }
+            float unit = 1.f, total = 0.f;
+            if (!HALF) {
                 float most = 0.f;
 #pragma unroll
                 for (int seg = 0; seg < SEGS; ++seg) {
-                    loadQuerySixteen(q, seg * 64 + t * 16, live ? p.cache.headDim : 0, p.wideQueries != 0, words[seg]);
-                }
-                if (mt == 0 && r == 0) { // the first copies go out while the queries are on their way
-                    for (int n = 0; n < min(count, Shape::kStages) && !broken; ++n) {
-                        fill();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 f = unpackTwo(words[seg][j], T());
+                        most = maxBits(most, maxBits(f.x, f.y));
                     }
                 }
-#pragma unroll
-                for (int seg = 0; seg < SEGS; ++seg) {
-                    if (!HALF) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float2 f = unpackTwo(words[seg][j], T());
-                            most = maxBits(most, maxBits(f.x, f.y));
-                        }
-                    }
-                }
-                float unit = 1.f;
-                if (!HALF) {
-                    most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                    most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                    unit = halfUnit(most);
-                    const float inverse = 1.f / unit; // powers of two
-#pragma unroll
-                    for (int seg = 0; seg < SEGS; ++seg) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float2 f = unpackTwo(words[seg][j], T());
-                            words[seg][j] = packTwo(f.x * inverse, f.y * inverse, __half());
-                        }
-                    }
-                }
-                rowScale[mt][r] = unit * p.scale * (p.softcap > 0.f ? 1.f : kLog2e);
+                most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                unit = halfUnit(most);
+                const float inverse = 1.f / unit; // powers of two
 #pragma unroll
                 for (int seg = 0; seg < SEGS; ++seg) {
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        qf[mt][seg][u][r] = words[seg][2 * u], qf[mt][seg][u][2 + r] = words[seg][2 * u + 1];
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 f = unpackTwo(words[seg][j], T());
+                        words[seg][j] = packTwo(f.x * inverse, f.y * inverse, __half());
                     }
                 }
+            }
+#pragma unroll
+            for (int seg = 0; seg < SEGS; ++seg) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    qf[nq][seg][u][0] = words[seg][2 * u], qf[nq][seg][u][1] = words[seg][2 * u + 1];
+                    const float2 a = unpackTwo(words[seg][2 * u], __half()), b = unpackTwo(words[seg][2 * u + 1], __half());
+                    total += (a.x + a.y) + (b.x + b.y);
+                }
+            }
+            total += __shfl_xor_sync(0xffffffffu, total, 1);
+            total += __shfl_xor_sync(0xffffffffu, total, 2);
+            const int position = old + token;
+            const int hi = !live ? 0 : p.causal ? position + 1 : w.q.length, lo = p.window > 0 ? max(0, position - p.window + 1) : 0;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) { // from the lanes that hold rows 2 t and 2 t + 1
+                const int from = (2 * t + x) * 4;
+                rowScale[nq][x] = __shfl_sync(0xffffffffu, unit, from) * 16777216.f * p.scale * (p.softcap > 0.f ? 1.f : kLog2e);
+                offset[nq][x] = __shfl_sync(0xffffffffu, total, from) * (-128.f / 16777216.f);
+                rowLo[nq][x] = __shfl_sync(0xffffffffu, lo, from), rowHi[nq][x] = __shfl_sync(0xffffffffu, hi, from);
             }
         }
         // keys below `openLo` or from `openHi` on are hidden from some row
-        const int lastToken = (firstRow + rows - 1) / p.group, firstToken = firstRow / p.group;
+        const int lastToken = int(fastDiv(uint32_t(firstRow + rows - 1), p.groupDiv)), firstToken = int(fastDiv(uint32_t(firstRow), p.groupDiv));
         const int openHi = p.causal ? old + firstToken + 1 : w.q.length, openLo = p.window > 0 ? max(0, old + lastToken - p.window + 1) : 0;
 
-        float o[MT][NT][4] = {}, most[MT][2], sum[MT][2] = {};
+        float o[NQ][MT][4] = {}, most[NQ][2], sum[NQ][2] = {};
         float reference = 0.f, perReference = 1.f; // unit of `o`, a power of two, and kWeightScale over it
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            most[mt][0] = most[mt][1] = -INFINITY;
+        for (int nq = 0; nq < NQ; ++nq) {
+            most[nq][0] = most[nq][1] = -INFINITY;
         }
         for (int n = 0; n < count; ++n) {
-            if (n > 0 && (n & 31) == 0) {
+            if (n > 0 && (n & 15) == 0) {
                 slots = nextSlots;
                 keyScales = scaleOf(p.cache.keyScales, slots), valueScales = scaleOf(p.cache.valueScales, slots);
-                nextSlots = slotOf(n + 32 + lane);
+                nextSlots = slotOf(2 * n + 32 + lane);
             }
-            const bool there = __shfl_sync(0xffffffffu, slots, n & 31) >= 0;
-            const float keyScale = __shfl_sync(0xffffffffu, keyScales, n & 31), valueScale = __shfl_sync(0xffffffffu, valueScales, n & 31);
-            const int key0 = (firstGroup + n * kWarps) * kGroup;
             if (n < issued) {
                 broken = !mbarWaitWarp(&full[warp][stage], phase, 61) || broken;
             }
-            const uint32_t keys = smemAddr(own + stage * Shape::kStageBytes), values = keys + kGroup * DP;
-            if (there && !broken) {
-                float s[MT][2][4] = {};
+#pragma unroll 1
+            for (int h0 = 0; h0 < kStageGroups && !broken; h0 += AT) {
+                float keyScale[AT], valueScale[AT];
+                bool absent = false;
 #pragma unroll
-                for (int seg = 0; seg < SEGS; ++seg) {
+                for (int h = 0; h < AT; ++h) {
+                    keyScale[h] = __shfl_sync(0xffffffffu, keyScales, (2 * n + h0 + h) & 31);
+                    valueScale[h] = __shfl_sync(0xffffffffu, valueScales, (2 * n + h0 + h) & 31);
+                    absent = absent || keyScale[h] == -1.f;
+                }
+                const int key0 = groupOf(2 * n + h0) * kGroup;
+                const uint32_t keys = smemAddr(own + stage * Shape::kStageBytes) + uint32_t(h0 * Shape::kGroupBytes),
+                               values = keys + kStageGroups * Shape::kGroupBytes;
+                float s[AT][NQ][4]; // [group][..]: keys g and g + 8 in the lanes' order, rows 2 t and 2 t + 1
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const uint4 k = ldsVector(panelAddr<DP>(keys, 8 * j + (g >> 1) + 4 * (g & 1), seg * 4 + t));
-                        const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
+                for (int h = 0; h < AT; ++h) {
+#pragma unroll
+                    for (int nq = 0; nq < NQ; ++nq) {
+                        s[h][nq][0] = s[h][nq][2] = offset[nq][0], s[h][nq][1] = s[h][nq][3] = offset[nq][1];
+                    }
+#pragma unroll
+                    for (int seg = 0; seg < SEGS; ++seg) {
+                        const uint32_t group = keys + uint32_t(h * Shape::kGroupBytes);
+                        const uint4 k0 = ldsVector(panelAddr<DP>(group, (g >> 1) + 4 * (g & 1), seg * 4 + t));
+                        const uint4 k1 = ldsVector(panelAddr<DP>(group, 8 + (g >> 1) + 4 * (g & 1), seg * 4 + t));
+                        const uint32_t low[4] = {k0.x, k0.y, k0.z, k0.w}, high[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
-                            uint32_t b0, b1;
-                            bytesToHalves(kw[u], b0, b1);
+                            uint32_t a[4];
+                            bytesToSubnormals(low[u], a[0], a[2]);
+                            bytesToSubnormals(high[u], a[1], a[3]);
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) {
-                                mmaF16(s[mt][j], qf[mt][seg][u], b0, b1);
+                            for (int nq = 0; nq < NQ; ++nq) {
+                                mmaF16(s[h][nq], a, qf[nq][seg][u][0], qf[nq][seg][u][1]);
                             }
                         }
                     }
                 }
-                const bool masked = key0 + kGroup > openHi || key0 < openLo;
+                const bool masked = key0 + AT * kGroup > openHi || key0 < openLo || absent;
                 bool grows = false;
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
+                for (int h = 0; h < AT; ++h) {
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
+                    for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            float x = s[mt][j][e] * (rowScale[mt][e >> 1] * keyScale);
+                            float x = s[h][nq][e] * (rowScale[nq][e & 1] * keyScale[h]);
                             if (p.softcap > 0.f) {
                                 x = softCapped(x, p.softcap) * kLog2e;
                             }
-                            if (masked) { // column 2 t + (e & 1) is key 8 j + t + 4 (e & 1)
-                                const int key = key0 + 8 * j + t + 4 * (e & 1);
-                                x = key < rowHi[mt][e >> 1] && key >= rowLo[mt][e >> 1] ? x : -INFINITY;
+                            if (masked) { // row g (or g + 8) of the product is key (g >> 1) + 4 (g & 1) (+ 8) of the group
+                                const int key = key0 + h * kGroup + (g >> 1) + 4 * (g & 1) + 8 * (e >> 1);
+                                x = key < rowHi[nq][e & 1] && key >= rowLo[nq][e & 1] && keyScale[h] != -1.f ? x : -INFINITY;
                             }
-                            s[mt][j][e] = x;
-                            grows = grows || x > most[mt][e >> 1];
+                            s[h][nq][e] = x;
+                            grows = grows || x > most[nq][e & 1];
                         }
                     }
                 }
-                // the weights' factor; a scale that is not finite reaches the rows that see it through their weights
-                const float magnitude = fabsf(valueScale);
-                const bool raise = magnitude > reference && magnitude < INFINITY;
+                // the values' unit; a scale that is not finite reaches the rows that see it through their weights
+                float magnitude = 0.f;
+#pragma unroll
+                for (int h = 0; h < AT; ++h) {
+                    magnitude = fmaxf(magnitude, valueScale[h] < INFINITY ? valueScale[h] : 0.f);
+                }
+                const bool raise = magnitude > reference;
                 if (__any_sync(0xffffffffu, grows) || raise) {
                     const float unit = raise ? powerAbove(magnitude) : reference;
                     const float shrink = raise ? (reference > 0.f ? reference / unit : 0.f) : 1.f;
                     reference = unit;
                     perReference = unit > 0.f ? kWeightScale / unit : 1.f;
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
+                    for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-                        for (int r = 0; r < 2; ++r) {
-                            float top = fmaxf(fmaxf(s[mt][0][2 * r], s[mt][0][2 * r + 1]), fmaxf(s[mt][1][2 * r], s[mt][1][2 * r + 1]));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                            top = fmaxf(top, most[mt][r]);
-                            const float keep = top == -INFINITY ? 1.f : exp2Fast(most[mt][r] - top);
-                            most[mt][r] = top;
-                            sum[mt][r] *= keep;
+                        for (int x = 0; x < 2; ++x) {
+                            float top = most[nq][x];
+#pragma unroll
+                            for (int h = 0; h < AT; ++h) {
+                                top = fmaxf(top, fmaxf(s[h][nq][x], s[h][nq][2 + x]));
+                            }
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                            const float keep = top == -INFINITY ? 1.f : exp2Fast(most[nq][x] - top);
+                            most[nq][x] = top;
+                            sum[nq][x] *= keep;
                             const float factor = keep * shrink;
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                o[mt][nt][2 * r] *= factor, o[mt][nt][2 * r + 1] *= factor;
+                            for (int mt = 0; mt < MT; ++mt) {
+                                o[nq][mt][x] *= factor, o[nq][mt][2 + x] *= factor;
                             }
                         }
                     }
                 }
-                const float weightUnit = valueScale * perReference;
-                uint32_t wf[MT][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
+                for (int h = 0; h < AT; ++h) {
+                    const float weightUnit = valueScale[h] * perReference;
+                    uint32_t wf[NQ][2]; // P^T: rows 2 t and 2 t + 1 of the group's keys, rows 8 nq + g
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float shift = most[mt][r] == -INFINITY ? 0.f : most[mt][r];
+                    for (int nq = 0; nq < NQ; ++nq) {
+                        const float shift0 = most[nq][0] == -INFINITY ? 0.f : most[nq][0], shift1 = most[nq][1] == -INFINITY ? 0.f : most[nq][1];
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const float x0 = s[mt][j][2 * r], x1 = s[mt][j][2 * r + 1];
-                            const float p0 = exp2Fast(x0 - shift), p1 = exp2Fast(x1 - shift);
-                            sum[mt][r] += p0 + p1;
+                        for (int half = 0; half < 2; ++half) {
+                            const float x0 = s[h][nq][2 * half], x1 = s[h][nq][2 * half + 1];
+                            const float p0 = exp2Fast(x0 - shift0), p1 = exp2Fast(x1 - shift1);
+                            sum[nq][0] += p0, sum[nq][1] += p1;
                             // what the mask hides stays out, whatever its page's scale is
                             const float w0 = masked && x0 == -INFINITY ? 0.f : p0 * weightUnit;
                             const float w1 = masked && x1 == -INFINITY ? 0.f : p1 * weightUnit;
-                            wf[mt][2 * j + r] = packTwo(w0, w1, __half());
+                            wf[nq][half] = transposeHalves(packTwo(w0, w1, __half()));
                         }
                     }
-                }
-                constexpr int CHUNKS = DP < 128 ? 1 : DP / 128; // 16 (or, below 128, 8) bytes of a value row per lane each
+                    constexpr int CHUNKS = DP < 128 ? 1 : DP / 128, WORDS = DP < 128 ? 2 : 4; // 16 (or, below 128, 8) bytes of a value row per lane each
+                    const uint32_t group = values + uint32_t(h * Shape::kGroupBytes);
 #pragma unroll
-                for (int c = 0; c < CHUNKS; ++c) {
-                    uint32_t v[4][DP < 128 ? 2 : 4];
+                    for (int c = 0; c < CHUNKS; ++c) {
+                        uint32_t v[4][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (DP < 128) {
-                            const uint2 x = ldsPair(panelAddr<DP>(values, t + 4 * i, g >> 1) + 8u * uint32_t(g & 1));
-                            v[i][0] = x.x, v[i][1] = x.y;
-                        } else {
-                            const uint4 x = ldsVector(panelAddr<DP>(values, t + 4 * i, 8 * c + (g >> 1) + 4 * (g & 1)));
-                            v[i][0] = x.x, v[i][1] = x.y, v[i][DP < 128 ? 0 : 2] = x.z, v[i][DP < 128 ? 1 : 3] = x.w;
+                        for (int i = 0; i < 4; ++i) {
+                            if (DP < 128) {
+                                const uint2 x = ldsPair(panelAddr<DP>(group, t + 4 * i, g >> 1) + 8u * uint32_t(g & 1));
+                                v[i][0] = x.x, v[i][1] = x.y;
+                            } else {
+                                const uint4 x = ldsVector(panelAddr<DP>(group, t + 4 * i, 8 * c + (g >> 1) + 4 * (g & 1)));
+                                v[i][0] = x.x, v[i][1] = x.y, v[i][2] = x.z, v[i][3] = x.w;
+                            }
                         }
-                    }
 #pragma unroll
-                    for (int word = 0; word < (DP < 128 ? 2 : 4); ++word) {
-                        uint32_t b0[4], b1[4];
-                        transposeToHalves(v[0][word], v[1][word], b0);
-                        transposeToHalves(v[2][word], v[3][word], b1);
+                        for (int word = 0; word < WORDS; ++word) {
+                            uint32_t low[4], high[4]; // elements 4 word + .. of keys t, t + 4 and of keys t + 8, t + 12
+                            transposeToHalves(v[0][word], v[1][word], low);
+                            transposeToHalves(v[2][word], v[3][word], high);
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) {
+                            for (int d = 0; d < 2; ++d) {
+                                const uint32_t a[4] = {low[2 * d], low[2 * d + 1], high[2 * d], high[2 * d + 1]};
 #pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) {
-                                mmaF16(o[mt][c * 16 + word * 4 + d], wf[mt], b0[d], b1[d]);
+                                for (int nq = 0; nq < NQ; ++nq) {
+                                    mmaF16(o[nq][c * 8 + word * 2 + d], a, wf[nq][0], wf[nq][1]);
+                                }
                             }
                         }
                     }
                 }
             }
             if (n < issued) {
-                stage = stage + 1 == Shape::kStages ? 0 : stage + 1;
+                stage = stage + 1 == STAGES ? 0 : stage + 1;
                 phase ^= stage == 0 ? 1u : 0u;
             }
             __syncwarp(); // the stage has been read
@@ -442,86 +512,111 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
 
         // ---- the four warps' results as one ----
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int nq = 0; nq < NQ; ++nq) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                sum[mt][r] += __shfl_xor_sync(0xffffffffu, sum[mt][r], 1);
-                sum[mt][r] += __shfl_xor_sync(0xffffffffu, sum[mt][r], 2);
-                if (t == 0) {
-                    joinMax[warp][16 * mt + 8 * r + g] = most[mt][r], joinSum[warp][16 * mt + 8 * r + g] = sum[mt][r];
+            for (int x = 0; x < 2; ++x) {
+                sum[nq][x] += __shfl_xor_sync(0xffffffffu, sum[nq][x], 4);
+                sum[nq][x] += __shfl_xor_sync(0xffffffffu, sum[nq][x], 8);
+                sum[nq][x] += __shfl_xor_sync(0xffffffffu, sum[nq][x], 16);
+                if (g == 0) {
+                    joinMax[warp][8 * nq + 2 * t + x] = most[nq][x], joinSum[warp][8 * nq + 2 * t + x] = sum[nq][x];
                 }
             }
         }
         __syncthreads(); // every warp's copies have been read: the ring holds results from here on
-        constexpr int kPitch = DP + 4;
-        float *results = reinterpret_cast<float *>(ring);
-        static_assert(kWarps * 16 * kPitch * 4 <= Shape::kRing, "the results of 16 rows fit the ring");
-        const bool whole = firstStep == 0 && lastStep == w.steps;
+        constexpr int kPitch = Shape::kPitch, PASS = NQ < 2 ? 8 : 16; // rows joined at a time
+        float *results = reinterpret_cast<float *>(ring), *joined = results + kWarps * PASS * kPitch;
+        static_assert((kWarps * PASS + ROWS) * kPitch * 4 <= Shape::kRing, "the results fit the ring");
+        const bool whole = split <= 1 && firstStep == 0 && lastStep == w.steps;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int pass = 0; pass < ROWS / PASS; ++pass) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r) {
-                const int row = 16 * mt + 8 * r + g;
-                if (row < rows) {
-                    float top = -INFINITY;
-                    for (int v = 0; v < kWarps; ++v) {
-                        top = fmaxf(top, joinMax[v][row]);
-                    }
-                    const float factor = (top == -INFINITY ? 1.f : exp2Fast(most[mt][r] - top)) * (reference * (1.f / kWeightScale));
-                    float *to = results + (warp * 16 + 8 * r + g) * kPitch;
-                    // column 2 t + x of tile nt is element elementOf(nt, 2 t + x)
+            for (int sub8 = 0; sub8 < PASS / 8; ++sub8) {
+                const int nq = pass * (PASS / 8) + sub8;
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
+                for (int x = 0; x < 2; ++x) {
+                    const int row = 8 * nq + 2 * t + x;
+                    if (row < rows) {
+                        float top = -INFINITY;
+                        for (int v = 0; v < kWarps; ++v) {
+                            top = fmaxf(top, joinMax[v][row]);
+                        }
+                        const float factor = (top == -INFINITY ? 1.f : exp2Fast(most[nq][x] - top)) * (reference * (1.f / kWeightScale));
+                        float *to = results + (warp * PASS + 8 * sub8 + 2 * t + x) * kPitch;
+                        // tile mt holds elements 2 (mt % 8) and the next of the lane's 16 (or 8) of each chunk
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt += 4) {
+                        for (int mt = 0; mt < MT; mt += 2) {
                             float4 four;
-                            four.x = o[mt][nt][2 * r + x] * factor, four.y = o[mt][nt + 1][2 * r + x] * factor;
-                            four.z = o[mt][nt + 2][2 * r + x] * factor, four.w = o[mt][nt + 3][2 * r + x] * factor;
-                            const int element = DP < 128 ? (2 * t + x) * 8 + nt : (nt >> 4) * 128 + (t + 4 * x) * 16 + (nt & 15);
+                            four.x = o[nq][mt][x] * factor, four.y = o[nq][mt][2 + x] * factor;
+                            four.z = o[nq][mt + 1][x] * factor, four.w = o[nq][mt + 1][2 + x] * factor;
+                            const int element = DP < 128 ? g * 8 + 2 * mt : (mt >> 3) * 128 + ((g >> 1) + 4 * (g & 1)) * 16 + 2 * (mt & 7);
                             *reinterpret_cast<float4 *>(to + element) = four;
                         }
                     }
                 }
             }
             __syncthreads();
-            const int live = min(16, rows - 16 * mt);
+            const int live = min(PASS, rows - PASS * pass);
             for (int i = int(threadIdx.x); i < live * (DP / 4); i += kWarps * 32) {
                 const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
                 float4 y = {};
                 float top = -INFINITY, weights = 0.f;
 #pragma unroll
                 for (int v = 0; v < kWarps; ++v) {
-                    top = fmaxf(top, joinMax[v][16 * mt + row]);
-                    const float4 a = *reinterpret_cast<const float4 *>(results + (v * 16 + row) * kPitch + d);
+                    top = fmaxf(top, joinMax[v][PASS * pass + row]);
+                    const float4 a = *reinterpret_cast<const float4 *>(results + (v * PASS + row) * kPitch + d);
                     y.x += a.x, y.y += a.y, y.z += a.z, y.w += a.w;
                 }
 #pragma unroll
                 for (int v = 0; v < kWarps; ++v) {
-                    const float m = joinMax[v][16 * mt + row];
-                    weights += joinSum[v][16 * mt + row] * (top == -INFINITY ? 1.f : exp2Fast(m - top));
+                    const float m = joinMax[v][PASS * pass + row];
+                    weights += joinSum[v][PASS * pass + row] * (top == -INFINITY ? 1.f : exp2Fast(m - top));
                 }
                 if (whole) {
-                    writeOut<T>(p, w.q.first, firstRow + 16 * mt + row, head, d, y, weights);
+                    writeOut<T>(p, w.q.first, firstRow + PASS * pass + row, head, d, y, weights);
                 } else {
-                    float *to = partialRow<DP>(p, blockIdx.x, at == begin ? 0 : 1, 16 * mt + row, ROWS);
-                    *reinterpret_cast<float4 *>(to + 4 + d) = y;
+                    float *to = split > 0 ? joined + (PASS * pass + row) * kPitch
+                                          : partialRow<DP>(p, blockIdx.x, at == begin ? 0 : 1, PASS * pass + row, ROWS);
+                    *reinterpret_cast<float4 *>(to + 4 + d - (split > 0 ? 4 : 0)) = y;
                     if (d == 0) {
-                        to[0] = top, to[1] = weights;
+                        to[split > 0 ? DP : 0] = top, to[split > 0 ? DP + 1 : 1] = weights;
                     }
                 }
             }
             __syncthreads();
         }
+        if (split > 1) { // the cluster's parts as one: elements in turn
+            clusterSync();
+            const uint32_t from = smemAddr(joined);
+            for (int i = int(threadIdx.x) + rank * (kWarps * 32); i < rows * (DP / 4); i += split * (kWarps * 32)) {
+                const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+                float top = -INFINITY, weights = 0.f;
+                float4 y = {};
+                for (int r = 0; r < split; ++r) {
+                    top = fmaxf(top, loadCluster(mapToCta(from + uint32_t((row * kPitch + DP) * 4), uint32_t(r))).x);
+                }
+                for (int r = 0; r < split; ++r) {
+                    const float4 stats = loadCluster(mapToCta(from + uint32_t((row * kPitch + DP) * 4), uint32_t(r)));
+                    const float4 a = loadCluster(mapToCta(from + uint32_t((row * kPitch + d) * 4), uint32_t(r)));
+                    const float factor = top == -INFINITY ? 1.f : exp2Fast(stats.x - top);
+                    y.x += a.x * factor, y.y += a.y * factor, y.z += a.z * factor, y.w += a.w * factor;
+                    weights += stats.y * factor;
+                }
+                writeOut<T>(p, w.q.first, firstRow + row, head, d, y, weights);
+            }
+            __syncwarp();
+            clusterSync(); // nobody leaves while its part is being read
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); // the ring is filled by copies again
         __syncthreads();
         at += lastStep - firstStep;
-    }
+    } while (split == 0 && at < end);
 }
 
 // Joins the pieces of one row of one tile (blockIdx.y: the row).
-template <int DP, int MT, bool HALF>
+template <int DP, int NQ, bool HALF>
 __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const AttendParams p, const int count) {
-    constexpr int ROWS = 16 * MT;
+    constexpr int ROWS = 8 * NQ;
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     __shared__ int parts[2][kWarps];
     dependencySync();
@@ -576,7 +671,7 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
 
 int paddedHead(int headDim) { return headDim <= 64 ? 64 : headDim <= 128 ? 128 : 256; }
 
-template <int DP, int MT, bool HALF> int launchFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
+template <int DP, int NQ, bool HALF> int launchFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
     using Shape = FewShape<DP>;
     CUtensorMap k, v;
     if (!makeCacheMap(&k, p.cache.keys, p.cache, Shape::kPanel, kGroup, true) ||
@@ -584,21 +679,44 @@ template <int DP, int MT, bool HALF> int launchFew(const AttendParams &p, const 
         return MLEL_ERROR_DEVICE;
     }
     constexpr size_t smemBytes = Shape::kRing + 1024;
-    const auto kernel = pagedAttentionFewKernel<DP, MT, HALF>;
+    const auto kernel = pagedAttentionFewKernel<DP, NQ, HALF>;
     if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), smemBytes)) {
         return MLEL_ERROR_DEVICE;
     }
-    cudaError_t err = launchOverlapped(kernel, dim3(unsigned(plan.blocks)), kWarps * 32, smemBytes, s, k, v, p);
-    if (err == cudaSuccess && plan.joins) {
-        const int64_t rows = int64_t(p.batch.maxNew) * p.group, tiles = (rows + 16 * MT - 1) / (16 * MT) * p.cache.heads;
-        const dim3 grid(unsigned(tiles * p.batch.sequences), unsigned(std::min<int64_t>(rows, 16 * MT)));
-        err = launchOverlapped(pagedAttentionFewJoin<DP, MT, HALF>, grid, kWarps * 32, 0, s, p, plan.blocks);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(plan.blocks));
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smemBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attrs[2]{};
+    int count = 0;
+    if (dependentLaunches()) {
+        attrs[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[count++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (plan.split > 1) {
+        attrs[count].id = cudaLaunchAttributeClusterDimension;
+        attrs[count].val.clusterDim.x = unsigned(plan.split), attrs[count].val.clusterDim.y = 1, attrs[count++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attrs;
+    cfg.numAttrs = unsigned(count);
+    cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, k, v, p, plan.split);
+    if (err == cudaSuccess && plan.workspace > 0) {
+        const int64_t rows = int64_t(p.batch.maxNew) * p.group, tiles = (rows + 8 * NQ - 1) / (8 * NQ) * p.cache.heads;
+        const dim3 grid(unsigned(tiles * p.batch.sequences), unsigned(std::min<int64_t>(rows, 8 * NQ)));
+        err = launchOverlapped(pagedAttentionFewJoin<DP, NQ, HALF>, grid, kWarps * 32, 0, s, p, plan.blocks);
     }
     return launchStatus("mlel_cuda_paged_attention", err);
 }
 
-template <int DP, int MT> int launchFewType(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
-    return p.halves ? launchFew<DP, MT, true>(p, plan, s) : launchFew<DP, MT, false>(p, plan, s);
+template <int DP> int launchFewRows(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
+    if (plan.rows == 8) {
+        return p.halves ? launchFew<DP, 1, true>(p, plan, s) : launchFew<DP, 1, false>(p, plan, s);
+    }
+    if (DP == 256 || plan.rows == 16) {
+        return p.halves ? launchFew<DP, 2, true>(p, plan, s) : launchFew<DP, 2, false>(p, plan, s);
+    }
+    return p.halves ? launchFew<(DP < 256 ? DP : 128), 4, true>(p, plan, s) : launchFew<(DP < 256 ? DP : 128), 4, false>(p, plan, s);
 }
 
 } // namespace
@@ -607,29 +725,31 @@ FewPlan pagedAttentionFewPlan(const AttendParams &p) {
     FewPlan plan{};
     const int dp = paddedHead(p.cache.headDim);
     const int64_t rows = int64_t(p.batch.maxNew) * p.group;
-    plan.rows = rows <= 16 || dp == 256 ? 16 : 32;
-    // the most steps that the batch can have
-    const int64_t steps = (int64_t(p.batch.maxLength) + kGroup * kWarps - 1) / (kGroup * kWarps);
-    const int64_t work = steps * ((rows + plan.rows - 1) / plan.rows) * p.cache.heads * p.batch.sequences;
-    const int resident = dp == 256 || plan.rows == 32 ? 2 : 3;
+    plan.rows = rows <= 8 ? 8 : rows <= 16 || dp == 256 ? 16 : 32;
+    // the most tiles and steps that the batch can have
+    const int64_t steps = (int64_t(p.batch.maxLength) + kGroup * kStepGroups - 1) / (kGroup * kStepGroups);
+    const int64_t tiles = (rows + plan.rows - 1) / plan.rows * p.cache.heads * p.batch.sequences, work = steps * tiles;
     if (work > 0x7fffffff) {
         refuse("mlel_cuda_paged_attention", "sequences, tokens and lengths give too much work for one call");
     }
-    plan.blocks = int(std::max<int64_t>(1, std::min<int64_t>(work, int64_t(resident) * smCount())));
-    plan.joins = steps > 1 && plan.blocks > 1;
-    plan.workspace = plan.joins ? uint64_t(plan.blocks) * 2 * uint64_t(plan.rows) * uint64_t(dp + 4) * 4 : 0;
+    const int64_t resident = int64_t(dp * plan.rows <= 8 * 128 ? 3 : 2) * smCount();
+    int split = 1;
+    while (split < 8 && split < steps && tiles * split * 2 <= resident) {
+        split *= 2;
+    }
+    const int64_t inClusters = (tiles * split + resident - 1) / resident * ((steps + split - 1) / split);
+    if (inClusters <= (work + resident - 1) / resident + kClusterSteps) {
+        plan.split = split, plan.blocks = int(tiles * split);
+        return plan;
+    }
+    plan.blocks = int(std::max<int64_t>(1, std::min<int64_t>(work, resident)));
+    plan.workspace = steps > 1 && plan.blocks > 1 ? uint64_t(plan.blocks) * 2 * uint64_t(plan.rows) * uint64_t(dp + 4) * 4 : 0;
     return plan;
 }
 
 int pagedAttentionFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
     const int dp = paddedHead(p.cache.headDim);
-    if (dp == 256) {
-        return launchFewType<256, 1>(p, plan, s);
-    }
-    if (dp == 128) {
-        return plan.rows == 16 ? launchFewType<128, 1>(p, plan, s) : launchFewType<128, 2>(p, plan, s);
-    }
-    return plan.rows == 16 ? launchFewType<64, 1>(p, plan, s) : launchFewType<64, 2>(p, plan, s);
+    return dp == 256 ? launchFewRows<256>(p, plan, s) : dp == 128 ? launchFewRows<128>(p, plan, s) : launchFewRows<64>(p, plan, s);
 }
 
 int takePagedErrorFew() { return takePagedError(); }

@@ -104,8 +104,10 @@ def attend(data, scales, starts, lengths, table, q, scale, causal, window, softc
                     out[first + i, h] = 0
                     continue
                 s = k[lo:hi] @ x * scale
-                # d + 3 roundings of the sum, the two scales' products and their own, each against the sum of magnitudes
-                off = ((d + 6) * 2.0 ** -24 * abs(scale) * (np.abs(k[lo:hi]) @ np.abs(x))).max()
+                # d + 6 roundings, of the sum, the two scales' products and their own, each against the sum of magnitudes; keys
+                # may be summed as integers plus 128 (up to 255) with 128 times the sum of the query taken off again
+                unsigned = 256 * scales[0, slot[lo:hi], h // group].astype(np.float64)[:, None]
+                off = ((d + 6) * 2.0 ** -24 * abs(scale) * ((np.abs(k[lo:hi]) + unsigned) @ np.abs(x))).max()
                 if softcap > 0:
                     s = softcap * np.tanh(s / softcap)  # its slope is at most 1
                     off += 16 * 2.0 ** -24 * softcap
