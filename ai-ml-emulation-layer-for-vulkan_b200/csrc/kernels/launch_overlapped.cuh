@@ -16,6 +16,11 @@
 // ordinary launches, 5.6-6.4 with these; one image of the ResNet-50 shape 214.4 -> 212.1).  Not for average pools (one image of
 // the MobileNetV2 shape 2 us slower) and not in a chain of short element-wise kernels (the twelve operators of a graph of
 // small ones: 31 us with ordinary launches, 34 with these, 18 on lanes of their own, see Session::capture).
+//
+// A kernel whose blocks fill the SMs lets its successor in late: at the start it would take room that blocks of this kernel
+// still have to find, or itself be spread over the SMs as they happen to be free.  (444 blocks of attention over 32 long
+// sequences and the kernel that joins their results, pass after pass: 138 us with both triggers at the start, 107 with that of
+// the first behind its main loop and none in the second.)
 #pragma once
 
 #include <cuda_runtime.h>

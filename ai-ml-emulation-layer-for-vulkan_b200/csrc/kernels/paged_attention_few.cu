@@ -182,7 +182,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    dependencySync();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     int index, before = 0, begin, end, rank = 0;
     FewWork w;
     if (split > 0) {
@@ -204,7 +204,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         const Pieces pieces(scan.total, int(gridDim.x));
         begin = pieces.start(int(blockIdx.x)), end = pieces.start(int(blockIdx.x) + 1);
         if (begin >= end) {
-            return;
+            return; // (what has ended lets the next kernel in)
         }
         index = scan.sequence, before = scan.before, w = scan.work;
     }
@@ -611,29 +611,29 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         __syncthreads();
         at += lastStep - firstStep;
     } while (split == 0 && at < end);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Joins the pieces of one row of one tile (blockIdx.y: the row).
+// Joins the pieces of one tile: DP / 4 lanes a row.
 template <int DP, int NQ, bool HALF>
 __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const AttendParams p, const int count) {
     constexpr int ROWS = 8 * NQ;
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     __shared__ int parts[2][kWarps];
-    dependencySync();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     // the tiles of all sequences in a row, those of a sequence without work included: ceil(max_new * group / ROWS) * heads each
     const int perSequence = int(gridDim.x) / p.batch.sequences;
     const int index = int(blockIdx.x) / perSequence, tile = int(blockIdx.x) - index * perSequence;
-    const FewWork w = fewWorkOf<ROWS>(p, index);
-    const int row = int(blockIdx.y), head = tile % p.cache.heads, firstRow = tile / p.cache.heads * ROWS;
-    if (tile >= w.tiles || row >= w.q.fresh * p.group - firstRow || w.steps < 2) { // (the whole block)
-        return;
-    }
     // the steps of all sequences, and of those in front of this one
     int all = 0, front = 0;
     for (int b = int(threadIdx.x); b < p.batch.sequences; b += kWarps * 32) {
         const int work = fewWorkOf<ROWS>(p, b).work;
         all += work;
         front += b < index ? work : 0;
+    }
+    const FewWork w = fewWorkOf<ROWS>(p, index);
+    if (tile >= w.tiles || w.steps < 2) { // (the whole block)
+        return;
     }
     all = __reduce_add_sync(0xffffffffu, all), front = __reduce_add_sync(0xffffffffu, front);
     if ((threadIdx.x & 31) == 0) {
@@ -651,19 +651,22 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
         return; // written by that piece
     }
     const int first = x0 == pieces.start(c0) ? 0 : 1; // where piece c0 left it: as its first tile, or as its last
-    float top = -INFINITY;
-    for (int c = c0; c <= c1; ++c) {
-        top = fmaxf(top, partialRow<DP>(p, c, c == c0 ? first : 0, row, ROWS)[0]);
-    }
-    for (int d = int(threadIdx.x) * 4; d < DP; d += kWarps * 32 * 4) {
+    const int head = tile % p.cache.heads, firstRow = tile / p.cache.heads * ROWS, rows = min(ROWS, w.q.fresh * p.group - firstRow);
+    constexpr int kLanes = DP / 4;
+    const int d = int(threadIdx.x) % kLanes * 4;
+    for (int row = int(threadIdx.x) / kLanes; row < rows; row += kWarps * 32 / kLanes) {
+        // one pass with a running maximum, as over keys
+        float top = -INFINITY, sum = 0.f;
         float4 y = {};
-        float sum = 0.f;
         for (int c = c0; c <= c1; ++c) {
             const float *from = partialRow<DP>(p, c, c == c0 ? first : 0, row, ROWS);
-            const float factor = top == -INFINITY ? 1.f : exp2Fast(from[0] - top);
+            const float2 stats = *reinterpret_cast<const float2 *>(from);
             const float4 a = *reinterpret_cast<const float4 *>(from + 4 + d);
-            y.x += a.x * factor, y.y += a.y * factor, y.z += a.z * factor, y.w += a.w * factor;
-            sum += from[1] * factor;
+            const float now = fmaxf(top, stats.x);
+            const float keep = now == -INFINITY ? 1.f : exp2Fast(top - now), factor = now == -INFINITY ? 1.f : exp2Fast(stats.x - now);
+            top = now;
+            sum = sum * keep + stats.y * factor;
+            y.x = y.x * keep + a.x * factor, y.y = y.y * keep + a.y * factor, y.z = y.z * keep + a.z * factor, y.w = y.w * keep + a.w * factor;
         }
         writeOut<T>(p, w.q.first, firstRow + row, head, d, y, sum);
     }
@@ -703,8 +706,7 @@ template <int DP, int NQ, bool HALF> int launchFew(const AttendParams &p, const 
     cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, k, v, p, plan.split);
     if (err == cudaSuccess && plan.workspace > 0) {
         const int64_t rows = int64_t(p.batch.maxNew) * p.group, tiles = (rows + 8 * NQ - 1) / (8 * NQ) * p.cache.heads;
-        const dim3 grid(unsigned(tiles * p.batch.sequences), unsigned(std::min<int64_t>(rows, 8 * NQ)));
-        err = launchOverlapped(pagedAttentionFewJoin<DP, NQ, HALF>, grid, kWarps * 32, 0, s, p, plan.blocks);
+        err = launchOverlapped(pagedAttentionFewJoin<DP, NQ, HALF>, dim3(unsigned(tiles * p.batch.sequences)), kWarps * 32, 0, s, p, plan.blocks);
     }
     return launchStatus("mlel_cuda_paged_attention", err);
 }
