@@ -614,30 +614,36 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Joins the pieces of one tile: DP / 4 lanes a row.
+// Joins the pieces of one row of one tile (blockIdx.y: the row).  First all pieces' maxima and sums, a thread each, then the
+// results, pieces in turn over the warps, so that a row in hundreds of pieces (one long sequence) waits for a few reads only.
+constexpr int kMostPieces = 1024;
+
 template <int DP, int NQ, bool HALF>
 __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const AttendParams p, const int count) {
-    constexpr int ROWS = 8 * NQ;
+    constexpr int ROWS = 8 * NQ, THREADS = kWarps * 32;
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     __shared__ int parts[2][kWarps];
+    __shared__ float factors[kMostPieces], stats[2][kWarps];
+    __shared__ float4 sums[THREADS];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // the tiles of all sequences in a row, those of a sequence without work included: ceil(max_new * group / ROWS) * heads each
-    const int perSequence = int(gridDim.x) / p.batch.sequences;
+    const int perSequence = int(gridDim.x) / p.batch.sequences, lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
     const int index = int(blockIdx.x) / perSequence, tile = int(blockIdx.x) - index * perSequence;
     // the steps of all sequences, and of those in front of this one
     int all = 0, front = 0;
-    for (int b = int(threadIdx.x); b < p.batch.sequences; b += kWarps * 32) {
+    for (int b = int(threadIdx.x); b < p.batch.sequences; b += THREADS) {
         const int work = fewWorkOf<ROWS>(p, b).work;
         all += work;
         front += b < index ? work : 0;
     }
     const FewWork w = fewWorkOf<ROWS>(p, index);
-    if (tile >= w.tiles || w.steps < 2) { // (the whole block)
+    const int row = int(blockIdx.y), head = tile % p.cache.heads, firstRow = tile / p.cache.heads * ROWS;
+    if (tile >= w.tiles || row >= w.q.fresh * p.group - firstRow || w.steps < 2) { // (the whole block)
         return;
     }
     all = __reduce_add_sync(0xffffffffu, all), front = __reduce_add_sync(0xffffffffu, front);
-    if ((threadIdx.x & 31) == 0) {
-        parts[0][threadIdx.x >> 5] = all, parts[1][threadIdx.x >> 5] = front;
+    if (lane == 0) {
+        parts[0][warp] = all, parts[1][warp] = front;
     }
     __syncthreads();
     int total = 0, before = 0;
@@ -646,29 +652,66 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
         total += parts[0][v], before += parts[1][v];
     }
     const Pieces pieces(total, count);
-    const int x0 = before + tile * w.steps, c0 = pieces.of(x0), c1 = pieces.of(x0 + w.steps - 1);
-    if (c0 == c1) {
+    const int x0 = before + tile * w.steps, c0 = pieces.of(x0), n = pieces.of(x0 + w.steps - 1) - c0 + 1;
+    if (n == 1) {
         return; // written by that piece
     }
     const int first = x0 == pieces.start(c0) ? 0 : 1; // where piece c0 left it: as its first tile, or as its last
-    const int head = tile % p.cache.heads, firstRow = tile / p.cache.heads * ROWS, rows = min(ROWS, w.q.fresh * p.group - firstRow);
-    constexpr int kLanes = DP / 4;
-    const int d = int(threadIdx.x) % kLanes * 4;
-    for (int row = int(threadIdx.x) / kLanes; row < rows; row += kWarps * 32 / kLanes) {
-        // one pass with a running maximum, as over keys
-        float top = -INFINITY, sum = 0.f;
-        float4 y = {};
-        for (int c = c0; c <= c1; ++c) {
-            const float *from = partialRow<DP>(p, c, c == c0 ? first : 0, row, ROWS);
-            const float2 stats = *reinterpret_cast<const float2 *>(from);
-            const float4 a = *reinterpret_cast<const float4 *>(from + 4 + d);
-            const float now = fmaxf(top, stats.x);
-            const float keep = now == -INFINITY ? 1.f : exp2Fast(top - now), factor = now == -INFINITY ? 1.f : exp2Fast(stats.x - now);
-            top = now;
-            sum = sum * keep + stats.y * factor;
-            y.x = y.x * keep + a.x * factor, y.y = y.y * keep + a.y * factor, y.z = y.z * keep + a.z * factor, y.w = y.w * keep + a.w * factor;
+    const auto part = [&](int c) { return partialRow<DP>(p, c0 + c, c == 0 ? first : 0, row, ROWS); };
+    float top = -INFINITY;
+    for (int c = int(threadIdx.x); c < n; c += THREADS) {
+        top = fmaxf(top, part(c)[0]);
+    }
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+    }
+    if (lane == 0) {
+        stats[0][warp] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) {
+        top = fmaxf(top, stats[0][v]);
+    }
+    float weights = 0.f;
+    for (int c = int(threadIdx.x); c < n; c += THREADS) {
+        const float2 s = *reinterpret_cast<const float2 *>(part(c));
+        const float factor = top == -INFINITY ? 1.f : exp2Fast(s.x - top);
+        factors[c] = factor;
+        weights += s.y * factor;
+    }
+#pragma unroll
+    for (int step = 16; step > 0; step >>= 1) {
+        weights += __shfl_xor_sync(0xffffffffu, weights, step);
+    }
+    if (lane == 0) {
+        stats[1][warp] = weights;
+    }
+    __syncthreads();
+    weights = 0.f;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) {
+        weights += stats[1][v];
+    }
+    constexpr int kLanes = DP / 4, kTeams = THREADS / kLanes; // threads of a row, rows at once
+    const int team = int(threadIdx.x) / kLanes, d = int(threadIdx.x) % kLanes * 4;
+    float4 y = {};
+#pragma unroll 4
+    for (int c = team; c < n; c += kTeams) {
+        const float4 a = *reinterpret_cast<const float4 *>(part(c) + 4 + d);
+        const float factor = factors[c];
+        y.x += a.x * factor, y.y += a.y * factor, y.z += a.z * factor, y.w += a.w * factor;
+    }
+    sums[threadIdx.x] = y;
+    __syncthreads();
+    if (team == 0) {
+#pragma unroll
+        for (int v = 1; v < kTeams; ++v) {
+            const float4 a = sums[v * kLanes + int(threadIdx.x)];
+            y.x += a.x, y.y += a.y, y.z += a.z, y.w += a.w;
         }
-        writeOut<T>(p, w.q.first, firstRow + row, head, d, y, sum);
+        writeOut<T>(p, w.q.first, firstRow + row, head, d, y, weights);
     }
 }
 
@@ -706,7 +749,8 @@ template <int DP, int NQ, bool HALF> int launchFew(const AttendParams &p, const 
     cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, k, v, p, plan.split);
     if (err == cudaSuccess && plan.workspace > 0) {
         const int64_t rows = int64_t(p.batch.maxNew) * p.group, tiles = (rows + 8 * NQ - 1) / (8 * NQ) * p.cache.heads;
-        err = launchOverlapped(pagedAttentionFewJoin<DP, NQ, HALF>, dim3(unsigned(tiles * p.batch.sequences)), kWarps * 32, 0, s, p, plan.blocks);
+        err = launchOverlapped(pagedAttentionFewJoin<DP, NQ, HALF>,
+                               dim3(unsigned(tiles * p.batch.sequences), unsigned(std::min<int64_t>(rows, 8 * NQ))), kWarps * 32, 0, s, p, plan.blocks);
     }
     return launchStatus("mlel_cuda_paged_attention", err);
 }
@@ -744,7 +788,7 @@ FewPlan pagedAttentionFewPlan(const AttendParams &p) {
         plan.split = split, plan.blocks = int(tiles * split);
         return plan;
     }
-    plan.blocks = int(std::max<int64_t>(1, std::min<int64_t>(work, resident)));
+    plan.blocks = int(std::max<int64_t>(1, std::min<int64_t>({work, resident, kMostPieces})));
     plan.workspace = steps > 1 && plan.blocks > 1 ? uint64_t(plan.blocks) * 2 * uint64_t(plan.rows) * uint64_t(dp + 4) * 4 : 0;
     return plan;
 }
