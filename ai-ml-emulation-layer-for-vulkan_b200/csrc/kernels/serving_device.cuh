@@ -34,15 +34,20 @@ __device__ __forceinline__ float2 unpackTwo(uint32_t w, __nv_bfloat16) {
     return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
 }
 
-// Eight elements at a 16-byte boundary.
-template <class T> __device__ __forceinline__ void loadWide(const T *from, float (&x)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4 *>(from);
+template <class T> __device__ __forceinline__ void unpackEight(const uint4 &v, float (&x)[8], T) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const float2 f = unpackTwo(w[j], T());
         x[2 * j] = f.x, x[2 * j + 1] = f.y;
     }
+}
+template <class T> __device__ __forceinline__ uint4 packEight(const float (&x)[8], T) {
+    return {packTwo(x[0], x[1], T()), packTwo(x[2], x[3], T()), packTwo(x[4], x[5], T()), packTwo(x[6], x[7], T())};
+}
+// Eight elements at a 16-byte boundary.
+template <class T> __device__ __forceinline__ void loadWide(const T *from, float (&x)[8]) {
+    unpackEight(*reinterpret_cast<const uint4 *>(from), x, T());
 }
 __device__ __forceinline__ void loadWide(const float *from, float (&x)[8]) {
     const float4 a = reinterpret_cast<const float4 *>(from)[0], b = reinterpret_cast<const float4 *>(from)[1];

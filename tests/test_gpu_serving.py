@@ -253,6 +253,59 @@ def test_append(serving, dtype, page, d, rot, interleaved):
     assert np.array_equal(p.data.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("d, rot, interleaved, shift", [(64, 24, False, 0), (64, 48, True, 0), (32, 32, False, 1), (48, 20, True, 3), (128, 8, False, 0)])
+def test_append_odd_rotations_and_addresses(serving, dtype, d, rot, interleaved, shift):
+    """Rotated parts that no vector width divides, and rows at any element's address."""
+    t = DTYPES[dtype]
+    p = Paged(serving, d + rot, MIXED, 2, 16, d, wild=False)
+    wide = randn(p.g, p.tokens, 6 * d + shift).to(t)
+    q, k, v = (wide[:, shift + a * d:shift + b * d].unflatten(1, (-1, d)) for a, b in [(0, 2), (2, 4), (4, 6)])
+    angle = torch.arange(200, device="cuda")[:, None] * torch.rand(rot // 2, generator=p.g, device="cuda")
+    before = p.arrays()
+    out = p.cache.append(k, v, angle.cos(), angle.sin(), p.batch, q=q, interleaved=interleaved)
+    c, s = ref.f64(angle.cos()), ref.f64(angle.sin())
+    want, want_scales = ref.append(*before, ref.f64(k), ref.f64(v), c, s, interleaved)
+    assert np.array_equal(p.scales.cpu().numpy(), want_scales, equal_nan=True) and np.array_equal(p.data.cpu().numpy(), want)
+    x = ref.f64(q)
+    for b, length in enumerate(p.lengths):
+        for i in range(p.starts[b], p.starts[b + 1]):
+            position = length - p.starts[b + 1] + i
+            y = ref.rotate(x[i], c[position], s[position], interleaved)
+            off = 2.0 ** -23 * np.abs(x[i]).max()
+            assert (np.abs(ref.f64(out[i]) - y) <= off + ref.half_step(t) * (np.abs(y) + off) + ref.smallest_half_step(t)).all()
+
+
+def test_append_many_tokens(serving):
+    """Blocks of several queries that straddle sequences, some of them empty."""
+    sequences = [(500, 500), (0, 7), (1, 90), (0, 0), (3, 3), (700, 733), (1, 1)]
+    p = Paged(serving, 4, sequences, 1, 32, 16, skip=3, behind=9, wild=False)
+    q, k, v = (randn(p.g, p.tokens, 1, 16).bfloat16() for _ in range(3))
+    angle = torch.arange(800, device="cuda")[:, None] * torch.rand(8, generator=p.g, device="cuda")
+    before = p.arrays()
+    out = torch.full_like(q, 77.0)
+    p.cache.append(k, v, angle.cos(), angle.sin(), p.batch, q=q, q_out=out)
+    want, want_scales = ref.append(*before, ref.f64(k), ref.f64(v), ref.f64(angle.cos()), ref.f64(angle.sin()), False)
+    assert np.array_equal(p.scales.cpu().numpy(), want_scales, equal_nan=True) and np.array_equal(p.data.cpu().numpy(), want)
+    position = torch.cat([torch.arange(l - n, l) for n, l in sequences]).cuda()
+    x, c, s = q[3:-9, 0].double(), angle.cos()[position].double(), angle.sin()[position].double()
+    y = torch.cat((x[:, :8] * c - x[:, 8:] * s, x[:, 8:] * c + x[:, :8] * s), 1)
+    assert ((out[3:-9, 0].double() - y).abs() <= 2.0 ** -8 * (y.abs() + 2.0 ** -20 * x.abs().amax()) + 2.0 ** -22 * x.abs().amax()).all()
+    assert (out[:3] == 77).all() and (out[-9:] == 77).all()
+
+
+@pytest.mark.parametrize("tiny", [1e-40, 3e-39, 1e-37])
+def test_append_the_smallest_magnitudes(serving, tiny):
+    """Scales among the subnormal numbers: quotients are rounded and bounded as elsewhere."""
+    p = Paged(serving, 8, [(5, 9), (1, 40)], 2, 16, 16, wild=False)
+    p.scales[:, [s for t in p.table for s in t if 0 <= s < p.data.shape[1]]] = 0
+    k, v = (randn(p.g, p.tokens, 2, 16) * tiny).bfloat16(), (randn(p.g, p.tokens, 2, 16) * tiny).bfloat16()
+    before = p.arrays()
+    p.cache.append(k, v, None, None, p.batch)
+    want, want_scales = ref.append(*before, ref.f64(k), ref.f64(v), None, None, False)
+    assert np.array_equal(p.scales.cpu().numpy(), want_scales, equal_nan=True) and np.array_equal(p.data.cpu().numpy(), want)
+
+
 def test_append_what_is_not_finite(serving):
     """An infinity or a NaN makes the scale of its page and head that; other heads and pages do not notice."""
     p = Paged(serving, 5, [(20, 24), (4, 9)], 2, 16, 32, wild=False)
