@@ -4,20 +4,22 @@
 //
 // A block takes 256 rows of one sequence and cache head (a row is one token's query head; the heads that share a cache head are
 // neighbouring rows) as two tiles of 128, and walks the keys they see in tiles of 128:
-//   one warp      copies: 16 keys or values at a time (pages hold a multiple of 16), integers into staging buffers
-//   four warps    integers -> f16 (exact), in the 128-byte swizzled layout that both products read: keys are rows of a
-//                 K-major operand, values rows of an MN-major one, the same bytes either way
-//   one warp      products: S = Q K^T into tensor memory, O += P V with P read from tensor memory
-//   two x four    softmax, a lane a row: S out of tensor memory, weights as f16 back over it
-// The tiles take turns: while one's products run the other's softmax does.
+//   one warp       copies: 16 keys or values at a time (pages hold a multiple of 16), integers into staging buffers
+//   two warps      integers -> f16 (exact), in the 128-byte swizzled layout that both products read: keys are rows of a
+//                  K-major operand, values rows of an MN-major one, the same bytes either way
+//   one warp       products: S = Q K^T into tensor memory, O += P V with P read from tensor memory
+//   two x eight    softmax, a lane half a row: S out of tensor memory, weights as f16 back over it
+// The tiles take turns: while one's products run the other's softmax does.  Tensor memory is full (two times S and O), so a tile's
+// next scores wait for its weights to be used up; what counts is how long a tile's softmax takes, hence two warps to a
+// scheduler for it (with one, whose lanes had a row each: 5200 cycles per 128 keys, of which 2700 the softmax).
 //
 // What bounds it: per 256 x 128 scores the products take 2048 cycles at 128 elements a head, and 32768 exponentials the
 // same at 16 a cycle; everything else (a multiply-add, half a maximum, half a sum, half a conversion per score, and the
 // keys' and values' conversion) shares the four schedulers with them.
 //
 // Softmax in one pass where it can: scores are weighed with the maximum known from the tiles before, and only if one exceeds
-// it by more than 2^8, or at a row's first tile, at masked ones and where the values' reference grows, the maximum is taken first
-// and sums and result are rescaled.  The scale of 16 values is part of the exponent: w = 2^(s - m + log2(scale / r) + 7), r a
+// it by more than 2^8, or at a row's first tile and where the values' reference grows, the maximum is taken first and sums
+// and result are rescaled.  The scale of 16 values is part of the exponent: w = 2^(s - m + log2(scale / r) + 7), r a
 // running power of two, and the sum over the weights of 16 keys is divided by it again.  So a weight is at most 2^15, f16's steps
 // end 2^-31 below the largest, and values whose scale is below 2^-60 of r count as nothing.
 #include <cuda_bf16.h>
@@ -38,8 +40,9 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 128, kKeys = 128, kGroup = 16, kGroups = kKeys / kGroup;
-constexpr int kSoftmaxWarps = 8, kConvertWarps = 4, kCopyWarp = 12, kProductWarp = 13, kThreads14 = 14 * 32;
-constexpr int kParamRing = 8, kStaging = 2, kSlots = 4; // slots: keys, values, keys, values
+constexpr int kSoftmaxWarps = 16, kConvertWarps = 2, kCopyWarp = 18, kProductWarp = 19, kManyThreads = 20 * 32;
+constexpr int kTileWarps = kSoftmaxWarps / 2, kHalfGroups = kGroups / 2; // warps of a tile; groups of a lane
+constexpr int kParamRing = 4, kStaging = 2, kSlots = 4; // slots: keys, values, keys, values
 constexpr float kGrowth = 8.f;                          // in powers of two
 constexpr float kWeightBits = 7.f;
 
@@ -47,7 +50,7 @@ template <int DP> struct ManyShape {
     static constexpr int kQueryBytes = kRows * DP * 2;   // of one tile: panels of 64 elements
     static constexpr int kSlotBytes = kKeys * DP * 2;
     static constexpr int kStagingBytes = kKeys * DP;
-    static constexpr size_t kSmem = 2 * size_t(kQueryBytes) + kSlots * size_t(kSlotBytes) + kStaging * size_t(kStagingBytes) + 1024;
+    static constexpr size_t kTiles = 2 * size_t(kQueryBytes) + kSlots * size_t(kSlotBytes) + kStaging * size_t(kStagingBytes);
     // tensor-memory columns of the two tiles
     static constexpr __device__ uint32_t scores(int which) { return uint32_t(128 * which); }
     static constexpr __device__ uint32_t result(int which) { return uint32_t(256 + DP * which); }
@@ -66,6 +69,13 @@ struct ManyBarriers {
     uint64_t queries, params[kParamRing], stagingFull[kStaging], stagingEmpty[kStaging], full[kSlots], empty[kSlots];
     uint64_t scores[2], weights[2], result[2];
     uint32_t tmemBase;
+};
+
+// What lies behind the tiles in shared memory.
+struct ManyState {
+    ManyBarriers bars;
+    TileParams params[kParamRing];
+    float exchange[2][kRows][2]; // between the two lanes of a row
 };
 
 // kind::f16: f32 results, f16 operands, M = 128
@@ -107,20 +117,38 @@ __device__ __forceinline__ void tmemStore16(uint32_t taddr, const uint32_t (&r)[
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
+// Barrier of two warps that tells whether the predicate holds for any of their lanes.
+__device__ __forceinline__ uint32_t pairVote(int barrier, bool predicate) {
+    uint32_t any;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbar.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(any)
+                 : "r"(barrier), "r"(predicate ? 1u : 0u)
+                 : "memory");
+    return any;
+}
 __device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int DP, bool HALF, bool CAP>
-__global__ void __launch_bounds__(kThreads14, 1)
+__global__ void __launch_bounds__(kManyThreads, 1)
 pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p,
                          const FastDiv heads, const int levels) {
     using Shape = ManyShape<DP>;
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
-    extern __shared__ uint8_t rawSmem[];
+    extern __shared__ __align__(1024) uint8_t rawSmem[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rawSmem) + 1023) & ~uintptr_t(1023));
     uint8_t *queries = smem, *slots = smem + 2 * Shape::kQueryBytes, *staging = slots + kSlots * Shape::kSlotBytes;
-    __shared__ ManyBarriers bars;
-    __shared__ TileParams params[kParamRing];
+    ManyState &state = *reinterpret_cast<ManyState *>(smem + Shape::kTiles);
+    ManyBarriers &bars = state.bars;
+    TileParams(&params)[kParamRing] = state.params;
+    float(&exchange)[2][kRows][2] = state.exchange;
     const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
+    // There is no room to spare for rounding the address up; without static shared memory it is a multiple of 1024 already.
+    if (smem != rawSmem) {
+        if (threadIdx.x == 0) {
+            atomicCAS(&g_tcgen05Error, 0, 89);
+        }
+        return;
+    }
     dependencySync();
 
     // blocks: the tiles that see the most keys first
@@ -136,7 +164,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         return;
     }
     const int rows = min(2 * kRows, allRows - firstRow), old = q.length - q.fresh;
-    const int firstToken = firstRow / p.group, lastToken = (firstRow + rows - 1) / p.group;
+    const int firstToken = int(fastDiv(uint32_t(firstRow), p.groupDiv)), lastToken = int(fastDiv(uint32_t(firstRow + rows - 1), p.groupDiv));
     const int keyLo = (p.window > 0 ? max(0, old + firstToken - p.window + 1) : 0) / kGroup * kGroup;
     const int keyHi = p.causal ? old + lastToken + 1 : q.length;
     const int tiles = (keyHi - keyLo + kKeys - 1) / kKeys;
@@ -157,7 +185,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         }
         for (int i = 0; i < 2; ++i) {
             mbarInit(&bars.scores[i], 1u);
-            mbarInit(&bars.weights[i], 4u);
+            mbarInit(&bars.weights[i], uint32_t(kTileWarps));
             mbarInit(&bars.result[i], 1u);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -194,7 +222,8 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         for (int tile = 0; tile < tiles && ok; ++tile) {
             const int nextNextSlot = slotOf(tile + 2);
             const float nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
-            // parameters of the tile: the ring is longer than the softmax can be behind (see kSlots and kStaging)
+            // Parameters of the tile.  Here the converters are done with the values of tile - 2, for which those of tile - 4 had
+            // been used up: the softmax is past that tile, whose place this is.
             TileParams &to = params[tile % kParamRing];
             const float magnitude = fabsf(valueScale);
             int exponent = magnitude > 0.f && magnitude < INFINITY ? int(__float_as_uint(powerAbove(magnitude)) >> 23) - 127 : -126;
@@ -296,34 +325,33 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         }
     } else if (warp >= kSoftmaxWarps) {
         // ---------------- integers -> f16 ----------------
-        constexpr int kLanes = DP / 16, kRowsAtOnce = kConvertWarps * 32 / kLanes; // lanes of a key
-        const int thread = int(threadIdx.x) - kSoftmaxWarps * 32, part = thread % kLanes, row0 = thread / kLanes;
+        // A lane takes 16 bytes of a row: bytes 16 (lane % 4) on of a panel of 64, the panels a half of the warp each.  Eight
+        // neighbouring lanes write four chunks of two rows, which the swizzle keeps in different banks.
+        constexpr int kPanels = DP / 64, kRowsAtOnce = kConvertWarps * 8 / kPanels;
+        const int own = warp - kSoftmaxWarps, panel = kPanels == 2 ? lane >> 4 : 0, part = lane & 3;
+        const int row0 = own * (8 / kPanels) + (kPanels == 2 ? (lane >> 2) & 3 : lane >> 2); // its low three bits are those of all its rows
+        static_assert(kRowsAtOnce % 8 == 0, "rows of a lane share their swizzle");
+        const uint32_t fromLane = smemAddr(staging) + uint32_t(row0 * DP + panel * 64 + part * 16);
+        const uint32_t toLane = smemAddr(slots) + uint32_t(panel * (kKeys * 128) + row0 * 128);
+        const uint32_t low = toLane + uint32_t(((2 * part) ^ (row0 & 7)) << 4), high = toLane + uint32_t(((2 * part + 1) ^ (row0 & 7)) << 4);
         for (uint32_t unit = 0; unit < uint32_t(2 * tiles); ++unit) {
             const uint32_t buffer = unit % kStaging, slot = unit % kSlots;
             if (!mbarWaitWarp(&bars.stagingFull[buffer], (unit / kStaging) & 1u, 96) ||
                 !mbarWaitWarp(&bars.empty[slot], ((unit / kSlots) & 1u) ^ 1u, 97)) {
                 break;
             }
-            const uint32_t from = smemAddr(staging) + buffer * uint32_t(Shape::kStagingBytes);
-            // element chunk `part` (16 of them) fills chunks 2 part and 2 part + 1 of 8 elements; the upper half of the lanes
-            // takes its two in the other order, so that panels of the same banks are not written at once
-            const uint32_t to = smemAddr(slots) + slot * uint32_t(Shape::kSlotBytes) + uint32_t(part / 4) * (kKeys * 128u);
-            const int swap = part >> 2;
-#pragma unroll 4
-            for (int row = row0; row < kKeys; row += kRowsAtOnce) {
-                const uint4 v = ldsVector(from + uint32_t(row * DP + part * 16));
+            const uint32_t from = fromLane + buffer * uint32_t(Shape::kStagingBytes), to = slot * uint32_t(Shape::kSlotBytes);
+#pragma unroll 8
+            for (int step = 0; step < kKeys / kRowsAtOnce; ++step) {
+                const uint4 v = ldsVector(from + uint32_t(step * kRowsAtOnce * DP));
                 uint4 a, b;
                 bytesToHalves(v.x, a.x, a.y);
                 bytesToHalves(v.y, a.z, a.w);
                 bytesToHalves(v.z, b.x, b.y);
                 bytesToHalves(v.w, b.z, b.w);
-                const int chunk = 2 * (part & 3);
-                const uint32_t line = to + uint32_t(row * 128), at0 = line + uint32_t((chunk ^ (row & 7)) << 4),
-                               at1 = line + uint32_t(((chunk + 1) ^ (row & 7)) << 4);
-                const uint4 x = swap ? b : a, y = swap ? a : b;
-                const uint32_t atX = swap ? at1 : at0, atY = swap ? at0 : at1;
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(atX), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(atY), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w) : "memory");
+                const uint32_t line = to + uint32_t(step * kRowsAtOnce * 128);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(low + line), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w) : "memory");
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(high + line), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w) : "memory");
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -334,10 +362,12 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         }
         __syncwarp();
     } else {
-        // ---------------- softmax: a lane a row ----------------
-        const int which = warp >> 2, quarter = warp & 3, tileRow = quarter * 32 + lane, row = firstRow + which * kRows + tileRow;
+        // ---------------- softmax: a lane half a row ----------------
+        const int which = warp / kTileWarps, half = (warp >> 2) & 1, quarter = warp & 3, tileRow = quarter * 32 + lane,
+                  row = firstRow + which * kRows + tileRow;
+        const int pairBarrier = 1 + which * 4 + quarter; // of the two warps that share 32 rows
         const bool live = which * kRows + tileRow < rows;
-        const int token = live ? row / p.group : lastToken, queryHead = head * p.group + (live ? row - token * p.group : 0);
+        const int token = live ? int(fastDiv(uint32_t(row), p.groupDiv)) : lastToken, queryHead = head * p.group + (live ? row - token * p.group : 0);
         float rowScale;
         {
             const T *from = reinterpret_cast<const T *>(p.queries + int64_t(q.first + token) * p.queryStride[0] + queryHead * p.queryStride[1]);
@@ -360,8 +390,8 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             rowScale = unit * fabsf(p.scale) * (CAP ? 1.f : kLog2e);
             const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u; // keeps the order of scores that of the products
             const uint32_t line = smemAddr(queries) + uint32_t(which * Shape::kQueryBytes + tileRow * 128);
-#pragma unroll 2
-            for (int d = 0; d < DP; d += 16) {
+#pragma unroll 1
+            for (int d = half * (DP / 2); d < (half + 1) * (DP / 2); d += 16) {
                 uint32_t w[8];
                 loadQuerySixteen(from, d, length, p.wideQueries != 0, w);
 #pragma unroll
@@ -391,10 +421,12 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const int rowHi = !live ? 0 : p.causal ? position + 1 : q.length, rowLo = p.window > 0 ? max(0, position - p.window + 1) : 0;
         // keys that every row of this tile sees
         const int tileFirst = firstRow + which * kRows, tileLast = min(tileFirst + kRows, firstRow + rows) - 1;
-        const int openHi = tileFirst > tileLast ? 0x7fffffff : p.causal ? old + tileFirst / p.group + 1 : q.length;
-        const int openLo = p.window > 0 && tileFirst <= tileLast ? max(0, old + tileLast / p.group - p.window + 1) : 0;
-        const uint32_t scoresAt = tmem + Shape::scores(which) + (uint32_t(quarter * 32) << 16),
-                       resultAt = tmem + Shape::result(which) + (uint32_t(quarter * 32) << 16);
+        const int openHi = tileFirst > tileLast ? 0x7fffffff : p.causal ? old + int(fastDiv(uint32_t(tileFirst), p.groupDiv)) + 1 : q.length;
+        const int openLo = p.window > 0 && tileFirst <= tileLast ? max(0, old + int(fastDiv(uint32_t(tileLast), p.groupDiv)) - p.window + 1) : 0;
+        const uint32_t laneBase = tmem + (uint32_t(quarter * 32) << 16);
+        const uint32_t scoresAt = laneBase + Shape::scores(which) + uint32_t(half * (kKeys / 2)),
+                       weightsAt = laneBase + Shape::scores(which) + uint32_t(half * (kKeys / 4)),
+                       resultAt = laneBase + Shape::result(which) + uint32_t(half * (DP / 2));
 
         float most = -INFINITY, sum = 0.f;
         int reference = -126;
@@ -406,110 +438,114 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         for (int tile = 0; tile < tiles && ok; ++tile) {
             ok = mbarWaitWarp(&bars.params[tile % kParamRing], uint32_t(tile / kParamRing) & 1u, 98) &&
                  mbarWaitWarp(&bars.scores[which], uint32_t(tile) & 1u, 99);
+            ok = pairVote(pairBarrier, !ok) == 0u; // a wait that ran out ends it for both warps of the rows
             if (!ok) {
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const TileParams &tp = params[tile % kParamRing];
-            const int key0 = keyLo + tile * kKeys;
-            const bool masked = key0 + kKeys > openHi || key0 < openLo || tp.there != (1u << kGroups) - 1u;
-            uint32_t weights[kKeys / 2];
-            bool again = tile == 0 || masked || tp.reference != reference;
-            float added = 0.f;
-            if (!again) {
-                bool grows = false;
-                const float base = most == -INFINITY ? 0.f : most;
-#pragma unroll
-                for (int g = 0; g < kGroups; g += 2) {
-                    uint32_t s0[16], s1[16];
-                    tmemLoad16(scoresAt + uint32_t(g * 16), s0);
-                    tmemLoad16(scoresAt + uint32_t(g * 16 + 16), s1);
-                    tmemWait16(s0);
-                    tmemWait16(s1);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const float factor = rowScale * tp.keyScale[g + h], shift = tp.shift[g + h] - base;
-                        float top = -INFINITY, part = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const uint32_t a = h == 0 ? s0[j] : s1[j], b = h == 0 ? s0[j + 1] : s1[j + 1];
-                            float w0, w1;
-                            if (CAP) {
-                                const float x = scoreOf(a, factor), y = scoreOf(b, factor);
-                                top = fmaxf(top, fmaxf(x, y));
-                                w0 = exp2Fast(x + shift), w1 = exp2Fast(y + shift);
-                            } else {
-                                top = fmaxf(top, fmaxf(__uint_as_float(a), __uint_as_float(b)));
-                                w0 = exp2Fast(fmaf(__uint_as_float(a), factor, shift)), w1 = exp2Fast(fmaf(__uint_as_float(b), factor, shift));
-                            }
-                            part += w0 + w1;
-                            weights[(g + h) * 8 + j / 2] = packTwo(w0, w1, __half());
-                        }
-                        added = fmaf(part, tp.perWeight[g + h], added);
-                        // (a row that has seen nothing yet takes the long way, too)
-                        grows = grows || (CAP ? top : top * factor) > most + kGrowth;
-                    }
-                }
-                again = __any_sync(0xffffffffu, grows) != 0;
-            }
-            if (__any_sync(0xffffffffu, again)) {
-                // the maximum first, then sums and result in its units
-                const auto seen = [&](int key, int g) { return ((tp.there >> g) & 1u) != 0u && key < rowHi && key >= rowLo; };
-                float top = most;
+            const int key0 = keyLo + tile * kKeys + half * (kKeys / 2);
+            const bool masked = keyLo + (tile + 1) * kKeys > openHi || keyLo + tile * kKeys < openLo || tp.there != (1u << kGroups) - 1u;
+            // keys of group g that this row sees, a bit each
+            const auto seen = [&](int g) {
+                const int first = key0 + g * kGroup, hi = max(0, min(kGroup, rowHi - first)), lo = max(0, min(kGroup, rowLo - first));
+                return ((tp.there >> (half * kHalfGroups + g)) & 1u) != 0u ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
+            };
+            uint32_t weights[kKeys / 4];
+            bool maximumFirst = tile == 0 || tp.reference != reference;
+            float added;
+            while (true) {
+                if (maximumFirst) {
+                    float top = -INFINITY;
 #pragma unroll 1
-                for (int g = 0; g < kGroups; ++g) {
-                    uint32_t s[16];
-                    tmemLoad16(scoresAt + uint32_t(g * 16), s);
-                    tmemWait16(s);
-                    const float factor = rowScale * tp.keyScale[g];
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        top = !masked || seen(key0 + g * 16 + j, g) ? fmaxf(top, scoreOf(s[j], factor)) : top;
-                    }
-                }
-                const float keep = top == -INFINITY ? 1.f : exp2Fast(most - top);
-                const float factorO = keep * exp2f(float(reference - tp.reference));
-                sum *= keep;
-                if (tile > 0 && __any_sync(0xffffffffu, factorO != 1.f)) {
-#pragma unroll 1
-                    for (int d = 0; d < DP; d += 16) {
-                        uint32_t o[16];
-                        tmemLoad16(resultAt + uint32_t(d), o);
-                        tmemWait16(o);
+                    for (int g = 0; g < kHalfGroups; ++g) {
+                        uint32_t s[16];
+                        tmemLoad16(scoresAt + uint32_t(g * 16), s);
+                        tmemWait16(s);
+                        const float factor = rowScale * tp.keyScale[half * kHalfGroups + g];
+                        const uint32_t bits = masked ? seen(g) : 0xffffu;
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            o[j] = __float_as_uint(__uint_as_float(o[j]) * factorO);
+                            top = ((bits >> j) & 1u) != 0u ? fmaxf(top, scoreOf(s[j], factor)) : top;
                         }
-                        tmemStore16(resultAt + uint32_t(d), o);
                     }
-                    tmemStoreWait();
+                    exchange[which][tileRow][half] = top;
+                    asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
+                    top = fmaxf(fmaxf(top, exchange[which][tileRow][half ^ 1]), most);
+                    // sums and result in units of the new maximum and reference
+                    const float keep = top == -INFINITY ? 1.f : exp2Fast(most - top);
+                    const float factorO = keep * exp2f(float(reference - tp.reference));
+                    sum *= keep;
+                    if (tile > 0 && __any_sync(0xffffffffu, factorO != 1.f)) {
+#pragma unroll 1
+                        for (int d = 0; d < DP / 2; d += 16) {
+                            uint32_t o[16];
+                            tmemLoad16(resultAt + uint32_t(d), o);
+                            tmemWait16(o);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                o[j] = __float_as_uint(__uint_as_float(o[j]) * factorO);
+                            }
+                            tmemStore16(resultAt + uint32_t(d), o);
+                        }
+                        tmemStoreWait();
+                    }
+                    most = top, reference = tp.reference;
                 }
-                most = top, reference = tp.reference;
+                bool grows = false;
                 const float base = most == -INFINITY ? 0.f : most;
                 added = 0.f;
 #pragma unroll
-                for (int g = 0; g < kGroups; ++g) {
+                for (int g = 0; g < kHalfGroups; ++g) {
                     uint32_t s[16];
                     tmemLoad16(scoresAt + uint32_t(g * 16), s);
+                    const float factor = rowScale * tp.keyScale[half * kHalfGroups + g], shift = tp.shift[half * kHalfGroups + g] - base;
+                    const uint32_t bits = masked ? seen(g) : 0xffffu;
                     tmemWait16(s);
-                    const float factor = rowScale * tp.keyScale[g], shift = tp.shift[g] - base;
-                    float part = 0.f;
+                    float top = -INFINITY, part = 0.f;
+                    if (!__all_sync(0xffffffffu, bits == 0xffffu)) {
+                        // what the mask hides stays out, whatever its page's scales are
 #pragma unroll
-                    for (int j = 0; j < 16; j += 2) {
-                        float w0 = exp2Fast(scoreOf(s[j], factor) + shift), w1 = exp2Fast(scoreOf(s[j + 1], factor) + shift);
-                        if (masked) { // what the mask hides stays out, whatever its page's scales are
-                            w0 = seen(key0 + g * 16 + j, g) ? w0 : 0.f;
-                            w1 = seen(key0 + g * 16 + j + 1, g) ? w1 : 0.f;
+                        for (int j = 0; j < 16; j += 2) {
+                            const float x = scoreOf(s[j], factor), y = scoreOf(s[j + 1], factor);
+                            const bool one = ((bits >> j) & 1u) != 0u, two = ((bits >> (j + 1)) & 1u) != 0u;
+                            const float w0 = one ? exp2Fast(x + shift) : 0.f, w1 = two ? exp2Fast(y + shift) : 0.f;
+                            top = one ? fmaxf(top, x) : top, top = two ? fmaxf(top, y) : top;
+                            part += w0 + w1;
+                            weights[g * 8 + j / 2] = packTwo(w0, w1, __half());
                         }
-                        part += w0 + w1;
-                        weights[g * 8 + j / 2] = packTwo(w0, w1, __half());
+                        grows = grows || top > most + kGrowth;
+                        added = part == 0.f ? added : fmaf(part, tp.perWeight[half * kHalfGroups + g], added);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; j += 2) {
+                            float w0, w1;
+                            if (CAP) {
+                                const float x = scoreOf(s[j], factor), y = scoreOf(s[j + 1], factor);
+                                top = fmaxf(top, fmaxf(x, y));
+                                w0 = exp2Fast(x + shift), w1 = exp2Fast(y + shift);
+                            } else {
+                                top = fmaxf(top, fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
+                                w0 = exp2Fast(fmaf(__uint_as_float(s[j]), factor, shift)), w1 = exp2Fast(fmaf(__uint_as_float(s[j + 1]), factor, shift));
+                            }
+                            part += w0 + w1;
+                            weights[g * 8 + j / 2] = packTwo(w0, w1, __half());
+                        }
+                        grows = grows || (CAP ? top : top * factor) > most + kGrowth;
+                        added = fmaf(part, tp.perWeight[half * kHalfGroups + g], added);
                     }
-                    added = part == 0.f ? added : fmaf(part, tp.perWeight[g], added);
                 }
+                // Both warps of the rows have read their scores, and agree whether a maximum has to be taken up.
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                const uint32_t again = pairVote(pairBarrier, grows && !maximumFirst);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (again == 0u) {
+                    break;
+                }
+                maximumFirst = true;
             }
             sum += added;
-            tmemStore32(scoresAt, weights);
-            tmemStore32(scoresAt + 32u, weights + 32);
+            tmemStore32(weightsAt, weights);
             tmemStoreWait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -518,12 +554,17 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             }
         }
         // ---- the rows, by way of the queries' memory, which no product reads any more ----
-        if (ok && mbarWaitWarp(&bars.result[which], 0u, 90)) {
+        ok = mbarWaitWarp(&bars.result[which], 0u, 90) && ok;
+        exchange[which][tileRow][half] = sum;
+        asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
+        sum += exchange[which][tileRow][half ^ 1];
+        if (ok) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const float f = sum == 0.f ? 0.f : exp2f(float(reference) - kWeightBits) / sum;
-            uint8_t *mine = queries + which * Shape::kQueryBytes + quarter * (32 * DP * 2);
+            uint8_t *mine = queries + which * Shape::kQueryBytes + (quarter * 2 + half) * (32 * DP);
+            constexpr int kChunks = DP / 16, kLinesAtOnce = 32 / kChunks; // 16-byte chunks of half a row
 #pragma unroll 1
-            for (int d = 0; d < DP; d += 16) {
+            for (int d = 0; d < DP / 2; d += 16) {
                 uint32_t o[16];
                 tmemLoad16(resultAt + uint32_t(d), o);
                 tmemWait16(o);
@@ -533,24 +574,21 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                     const float x = sum == 0.f ? 0.f : __uint_as_float(o[2 * j]) * f, y = sum == 0.f ? 0.f : __uint_as_float(o[2 * j + 1]) * f;
                     w[j] = packTwo(x, y, T());
                 }
-                // 16-byte chunks of a row, each lane's turned by its number
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int chunk = d / 8 + half;
-                    *reinterpret_cast<uint4 *>(mine + lane * (DP * 2) + ((chunk ^ (lane & 7)) << 4)) = {w[4 * half], w[4 * half + 1],
-                                                                                                       w[4 * half + 2], w[4 * half + 3]};
+                for (int h = 0; h < 2; ++h) { // each lane's chunks turned by its number
+                    *reinterpret_cast<uint4 *>(mine + lane * DP + (((d / 8 + h) ^ (lane & (kChunks - 1))) << 4)) = {w[4 * h], w[4 * h + 1],
+                                                                                                                w[4 * h + 2], w[4 * h + 3]};
                 }
             }
             __syncwarp();
-            constexpr int kChunks = DP / 8, kLinesAtOnce = 32 / kChunks; // lanes of a row
-            const int chunk = lane % kChunks;
+            const int chunk = lane % kChunks, element = half * (DP / 2) + chunk * 8;
 #pragma unroll 1
             for (int r = lane / kChunks; r < 32; r += kLinesAtOnce) {
                 const int outRow = firstRow + which * kRows + quarter * 32 + r;
-                if (which * kRows + quarter * 32 + r < rows && chunk * 8 < p.cache.headDim) {
-                    const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * (DP * 2) + ((chunk ^ (r & 7)) << 4));
-                    const int outToken = outRow / p.group, outHead = head * p.group + outRow - outToken * p.group;
-                    char *to = p.out + int64_t(q.first + outToken) * p.outStride[0] + outHead * p.outStride[1] + chunk * 16;
+                if (which * kRows + quarter * 32 + r < rows && element < p.cache.headDim) {
+                    const uint4 v = *reinterpret_cast<const uint4 *>(mine + r * DP + ((chunk ^ (r & (kChunks - 1))) << 4));
+                    const int outToken = int(fastDiv(uint32_t(outRow), p.groupDiv)), outHead = head * p.group + outRow - outToken * p.group;
+                    char *to = p.out + int64_t(q.first + outToken) * p.outStride[0] + outHead * p.outStride[1] + element * 2;
                     if (p.wideOut) {
                         *reinterpret_cast<uint4 *>(to) = v;
                     } else {
@@ -574,20 +612,21 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
 
 template <int DP, bool HALF, bool CAP> int launchMany(const AttendParams &p, cudaStream_t s) {
     using Shape = ManyShape<DP>;
-    static_assert(Shape::kSmem + sizeof(ManyBarriers) + kParamRing * sizeof(TileParams) <= 232448, "shared memory per block");
+    constexpr size_t smemBytes = Shape::kTiles + sizeof(ManyState);
+    static_assert(smemBytes <= 232448, "shared memory per block");
     CUtensorMap k, v;
     if (!makeCacheMap(&k, p.cache.keys, p.cache, DP, kGroup, false) || !makeCacheMap(&v, p.cache.values, p.cache, DP, kGroup, false)) {
         return MLEL_ERROR_DEVICE;
     }
     const auto kernel = pagedAttentionManyKernel<DP, HALF, CAP>;
-    if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), Shape::kSmem)) {
+    if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), smemBytes)) {
         return MLEL_ERROR_DEVICE;
     }
     const int64_t levels = (int64_t(p.batch.maxNew) * p.group + 2 * kRows - 1) / (2 * kRows), blocks = levels * p.cache.heads * p.batch.sequences;
     if (blocks > 0x7fffffff) {
         refuse("mlel_cuda_paged_attention", "too many tokens and sequences for one call");
     }
-    return launchStatus("mlel_cuda_paged_attention", launchOverlapped(kernel, dim3(unsigned(blocks)), kThreads14, Shape::kSmem, s, k, v, p,
+    return launchStatus("mlel_cuda_paged_attention", launchOverlapped(kernel, dim3(unsigned(blocks)), kManyThreads, smemBytes, s, k, v, p,
                                                                       makeFastDiv(p.cache.heads), int(levels)));
 }
 
