@@ -4,14 +4,16 @@
 //
 // A block takes 256 rows of one sequence and cache head (a row is one token's query head; the heads that share a cache head are
 // neighbouring rows) as two tiles of 128, and walks the keys they see in tiles of 128:
-//   one warp       copies: 16 keys or values at a time (pages hold a multiple of 16), integers into staging buffers
-//   two warps      integers -> f16 (exact), in the 128-byte swizzled layout that both products read: keys are rows of a
-//                  K-major operand, values rows of an MN-major one, the same bytes either way
-//   one warp       products: S = Q K^T into tensor memory, O += P V with P read from tensor memory
-//   two x eight    softmax, a lane half a row: S out of tensor memory, weights as f16 back over it
+//   four warps     integers -> f16 (exact), in the 128-byte swizzled layout that both products read: keys are rows of a
+//                  K-major operand, values rows of an MN-major one, the same bytes either way; the first of them issues the
+//                  copies, 16 keys or values at a time (pages hold a multiple of 16), integers into staging buffers
+//   two x eight    softmax, a lane half a row: S out of tensor memory, weights as f16 back over it; the first of each
+//                  eight issues its tile's products (S = Q K^T into tensor memory, O += P V with P read from there) in the
+//                  time it would wait for them
 // The tiles take turns: while one's products run the other's softmax does.  Tensor memory is full (two times S and O), so a tile's
 // next scores wait for its weights to be used up; what counts is how long a tile's softmax takes, hence two warps to a
-// scheduler for it (with one, whose lanes had a row each: 5200 cycles per 128 keys, of which 2700 the softmax).
+// scheduler for it (with one, whose lanes had a row each: 5200 cycles per 128 keys, of which 2700 the softmax), and no warp
+// beyond twenty, which leaves a lane 96 registers.
 //
 // What bounds it: per 256 x 128 scores the products take 2048 cycles at 128 elements a head, and 32768 exponentials the
 // same at 16 a cycle; everything else (a multiply-add, half a maximum, half a sum, half a conversion per score, and the
@@ -40,9 +42,9 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 128, kKeys = 128, kGroup = 16, kGroups = kKeys / kGroup;
-constexpr int kSoftmaxWarps = 16, kConvertWarps = 2, kCopyWarp = 18, kProductWarp = 19, kManyThreads = 20 * 32;
+constexpr int kSoftmaxWarps = 16, kConvertWarps = 4, kManyThreads = (kSoftmaxWarps + kConvertWarps) * 32;
 constexpr int kTileWarps = kSoftmaxWarps / 2, kHalfGroups = kGroups / 2; // warps of a tile; groups of a lane
-constexpr int kParamRing = 4, kStaging = 2, kSlots = 4; // slots: keys, values, keys, values
+constexpr int kParamRing = 4, kStaging = 4, kSlots = 3; // of 128 keys or values: integers on their way, and f16
 constexpr float kGrowth = 8.f;                          // in powers of two
 constexpr float kWeightBits = 7.f;
 
@@ -117,6 +119,27 @@ __device__ __forceinline__ void tmemStore16(uint32_t taddr, const uint32_t (&r)[
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
+// Two 32-bit floats at a time.
+__device__ __forceinline__ float2 fmaTwo(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 addTwo(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float maxThree(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // Barrier of two warps that tells whether the predicate holds for any of their lanes.
 __device__ __forceinline__ uint32_t pairVote(int barrier, bool predicate) {
     uint32_t any;
@@ -169,9 +192,10 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     const int keyHi = p.causal ? old + lastToken + 1 : q.length;
     const int tiles = (keyHi - keyLo + kKeys - 1) / kKeys;
     const int32_t *table = p.batch.table + index * p.batch.tableStride;
+    const int active = rows > kRows ? 2 : 1; // tiles with rows
 
     if (threadIdx.x == 0) {
-        mbarInit(&bars.queries, kSoftmaxWarps);
+        mbarInit(&bars.queries, uint32_t(active * kTileWarps));
         for (int i = 0; i < kParamRing; ++i) {
             mbarInit(&bars.params[i], 1u);
         }
@@ -181,7 +205,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         }
         for (int i = 0; i < kSlots; ++i) {
             mbarInit(&bars.full[i], kConvertWarps);
-            mbarInit(&bars.empty[i], 1u);
+            mbarInit(&bars.empty[i], uint32_t(active)); // the tiles' products
         }
         for (int i = 0; i < 2; ++i) {
             mbarInit(&bars.scores[i], 1u);
@@ -190,7 +214,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kProductWarp) {
+    if (warp == kSoftmaxWarps) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smemAddr(&bars.tmemBase)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -199,132 +223,73 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = bars.tmemBase;
 
-    if (warp == kCopyWarp) {
-        // ---------------- copies, and what the softmax needs to know of their pages ----------------
+    if (warp >= kSoftmaxWarps) {
+        // ---------------- integers -> f16; the first warp: copies, and what the softmax needs to know of their pages ----------------
         const int groups = (keyHi - keyLo + kGroup - 1) / kGroup;
         const auto slotOf = [&](int tile) { // lane 0 .. 7: the page of a group of the tile; -1: there is none
             const int n = tile * kGroups + lane;
-            int slot = -1;
-            if (lane < kGroups && n < groups) {
-                slot = table[fastDiv(uint32_t(keyLo + n * kGroup), p.pageDiv)];
-                if (uint32_t(slot) >= uint32_t(p.cache.pages)) {
+            return lane < kGroups && n < groups ? table[fastDiv(uint32_t(keyLo + n * kGroup), p.pageDiv)] : -1;
+        };
+        const auto checked = [&](int tile, int slot) { // a tile later, when the entry has arrived
+            if (uint32_t(slot) >= uint32_t(p.cache.pages)) {
+                if (lane < kGroups && tile * kGroups + lane < groups) {
                     atomicCAS(&g_pagedError, 0, kBadPage);
-                    slot = -1;
                 }
+                return -1;
             }
             return slot;
         };
         const auto scaleOf = [&](const float *scales, int slot) { return slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : 0.f; };
-        int slot = slotOf(0), nextSlot = slotOf(1), reference = -126;
-        float keyScale = scaleOf(p.cache.keyScales, slot), valueScale = scaleOf(p.cache.valueScales, slot);
+        int slot = -1, nextSlot = -1, nextNextSlot = -1, reference = -126;
+        float keyScale = 0.f, valueScale = 0.f, nextKeyScale = 0.f, nextValueScale = 0.f;
         bool ok = true;
-        uint32_t unit = 0; // keys and values of the tiles in turn
-        for (int tile = 0; tile < tiles && ok; ++tile) {
-            const int nextNextSlot = slotOf(tile + 2);
-            const float nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
-            // Parameters of the tile.  Here the converters are done with the values of tile - 2, for which those of tile - 4 had
-            // been used up: the softmax is past that tile, whose place this is.
-            TileParams &to = params[tile % kParamRing];
-            const float magnitude = fabsf(valueScale);
-            int exponent = magnitude > 0.f && magnitude < INFINITY ? int(__float_as_uint(powerAbove(magnitude)) >> 23) - 127 : -126;
-            exponent = __reduce_max_sync(0xffffffffu, exponent);
-            reference = max(reference, exponent);
-            if (lane < kGroups) {
-                // (a scale that is not finite gives a shift and weights that are not)
-                const float shift = magnitude < 1.f * INFINITY ? fmaxf(log2f(magnitude) - float(reference), -60.f) + kWeightBits
-                                                               : magnitude - magnitude;
-                to.keyScale[lane] = keyScale, to.shift[lane] = valueScale < 0.f ? __int_as_float(0x7fc00000) : shift;
-                to.perWeight[lane] = exp2f(-shift);
-            }
-            const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
-            if (lane == 0) {
-                to.reference = reference, to.there = there;
-            }
-            __syncwarp();
-            if (lane == 0) {
-                mbarArrive(&bars.params[tile % kParamRing]);
-            }
-            const int n = tile * kGroups + lane, key = keyLo + n * kGroup;
-            const int row = (max(slot, 0) * p.cache.heads + head) * p.cache.page + key - int(fastDiv(uint32_t(key), p.pageDiv)) * p.cache.page;
-            const int count = min(kGroups, groups - tile * kGroups);
-#pragma unroll
-            for (int side = 0; side < 2; ++side, ++unit) {
-                const uint32_t buffer = unit % kStaging;
-                ok = ok && mbarWaitWarp(&bars.stagingEmpty[buffer], ((unit / kStaging) & 1u) ^ 1u, 91);
-                if (!ok) {
-                    break;
+        const auto copyUnit = [&](int unit) { // keys (unit 2 t) and values (2 t + 1) of the tiles in turn, into a free staging buffer
+            const int tile = unit >> 1, side = unit & 1;
+            if (side == 0) {
+                slot = nextSlot, keyScale = nextKeyScale, valueScale = nextValueScale, nextSlot = checked(tile + 1, nextNextSlot);
+                nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
+                nextNextSlot = slotOf(tile + 2);
+                // Parameters of the tile.  Here the converters are done with the keys of tile - 2, for which the values of tile - 4
+                // had been used up by both tiles: the softmax is past tile - 4, whose place this is.
+                TileParams &to = params[tile % kParamRing];
+                const float magnitude = fabsf(valueScale);
+                int exponent = magnitude > 0.f && magnitude < INFINITY ? int(__float_as_uint(powerAbove(magnitude)) >> 23) - 127 : -126;
+                exponent = __reduce_max_sync(0xffffffffu, exponent);
+                reference = max(reference, exponent);
+                if (lane < kGroups) {
+                    // (a scale that is not finite gives a shift and weights that are not)
+                    const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), -60.f) + kWeightBits : magnitude - magnitude;
+                    to.keyScale[lane] = keyScale, to.shift[lane] = shift, to.perWeight[lane] = exp2f(-shift);
                 }
+                const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
                 if (lane == 0) {
-                    mbarArriveExpectTx(&bars.stagingFull[buffer], uint32_t(count * kGroup * DP));
+                    to.reference = reference, to.there = there;
                 }
                 __syncwarp();
-                if (lane < count) {
-                    tmaLoad3d(side == 0 ? &mapK : &mapV, staging + buffer * Shape::kStagingBytes + lane * kGroup * DP, &bars.stagingFull[buffer],
-                              0, row, 0);
+                if (lane == 0) {
+                    mbarArrive(&bars.params[tile % kParamRing]);
                 }
             }
-            slot = nextSlot, keyScale = nextKeyScale, valueScale = nextValueScale;
-            nextSlot = nextNextSlot;
-        }
-        __syncwarp();
-    } else if (warp == kProductWarp) {
-        // ---------------- products (the whole warp: see ummaBlockPeek) ----------------
-        constexpr uint32_t kScoreDesc = instrF16(kKeys, false), kResultDesc = instrF16(DP, true);
-        constexpr uint32_t kPanel = kRows * 128; // bytes: 64 elements of 128 rows
-        const uint32_t queryAddr = smemAddr(queries), slotAddr = smemAddr(slots);
-        bool failed = !mbarWait(&bars.queries, 0u, 92);
-        const auto scoreProduct = [&](int tile, int which) {
-            const uint32_t slot = uint32_t(2 * tile) % kSlots;
-            if (which == 0) {
-                failed = failed || !mbarWait(&bars.full[slot], (uint32_t(2 * tile) / kSlots) & 1u, 93);
+            const int buffer = unit % kStaging, key = keyLo + (tile * kGroups + lane) * kGroup;
+            const int row = (max(slot, 0) * p.cache.heads + head) * p.cache.page + key - int(fastDiv(uint32_t(key), p.pageDiv)) * p.cache.page;
+            const int count = min(kGroups, groups - tile * kGroups);
+            if (lane == 0) {
+                mbarArriveExpectTx(&bars.stagingFull[buffer], uint32_t(count * kGroup * DP));
             }
             __syncwarp();
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t at = uint32_t(k / 4) * kPanel + uint32_t(k % 4) * 32u;
-                mmaShared(tmem + Shape::scores(which), descWords(smemDesc(queryAddr + uint32_t(which * Shape::kQueryBytes) + at, 16, 1024)),
-                          descWords(smemDesc(slotAddr + slot * uint32_t(Shape::kSlotBytes) + at, 16, 1024)), kScoreDesc, k != 0 ? 1u : 0u);
-            }
-            ummaCommit(&bars.scores[which]);
-            if (which == 1) {
-                ummaCommit(&bars.empty[slot]);
+            if (lane < count) {
+                tmaLoad3d(side == 0 ? &mapK : &mapV, staging + buffer * Shape::kStagingBytes + lane * kGroup * DP, &bars.stagingFull[buffer], 0,
+                          row, 0);
             }
         };
-        const auto resultProduct = [&](int tile, int which) {
-            const uint32_t unit = uint32_t(2 * tile + 1), slot = unit % kSlots;
-            if (which == 0) {
-                failed = failed || !mbarWait(&bars.full[slot], (unit / kSlots) & 1u, 94);
-            }
-            failed = failed || !mbarWait(&bars.weights[which], uint32_t(tile) & 1u, 95);
-            __syncwarp();
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k) {
-                mmaTensor(tmem + Shape::result(which), tmem + Shape::scores(which) + uint32_t(k * 8),
-                          descWords(smemDesc(slotAddr + slot * uint32_t(Shape::kSlotBytes) + uint32_t(k) * 2048u, kPanel, 1024)), kResultDesc,
-                          tile != 0 || k != 0 ? 1u : 0u);
-            }
-            if (tile == tiles - 1) {
-                ummaCommit(&bars.result[which]);
-            }
-            if (which == 1) {
-                ummaCommit(&bars.empty[slot]);
-            }
-        };
-        scoreProduct(0, 0);
-        scoreProduct(0, 1);
-        for (int tile = 0; tile < tiles; ++tile) {
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                resultProduct(tile, which);
-                if (tile + 1 < tiles) {
-                    scoreProduct(tile + 1, which);
-                }
+        if (warp == kSoftmaxWarps) {
+            nextNextSlot = slotOf(1);
+            nextSlot = checked(0, slotOf(0));
+            nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
+            for (int unit = 0; unit < min(kStaging, 2 * tiles); ++unit) {
+                copyUnit(unit);
             }
         }
-    } else if (warp >= kSoftmaxWarps) {
-        // ---------------- integers -> f16 ----------------
         // A lane takes 16 bytes of a row: bytes 16 (lane % 4) on of a panel of 64, the panels a half of the warp each.  Eight
         // neighbouring lanes write four chunks of two rows, which the swizzle keeps in different banks.
         constexpr int kPanels = DP / 64, kRowsAtOnce = kConvertWarps * 8 / kPanels;
@@ -335,12 +300,13 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const uint32_t toLane = smemAddr(slots) + uint32_t(panel * (kKeys * 128) + row0 * 128);
         const uint32_t low = toLane + uint32_t(((2 * part) ^ (row0 & 7)) << 4), high = toLane + uint32_t(((2 * part + 1) ^ (row0 & 7)) << 4);
         for (uint32_t unit = 0; unit < uint32_t(2 * tiles); ++unit) {
-            const uint32_t buffer = unit % kStaging, slot = unit % kSlots;
-            if (!mbarWaitWarp(&bars.stagingFull[buffer], (unit / kStaging) & 1u, 96) ||
-                !mbarWaitWarp(&bars.empty[slot], ((unit / kSlots) & 1u) ^ 1u, 97)) {
+            const uint32_t buffer = unit % kStaging, place = unit % kSlots;
+            ok = ok && mbarWaitWarp(&bars.stagingFull[buffer], (unit / kStaging) & 1u, 96) &&
+                 mbarWaitWarp(&bars.empty[place], ((unit / kSlots) & 1u) ^ 1u, 97);
+            if (!ok) {
                 break;
             }
-            const uint32_t from = fromLane + buffer * uint32_t(Shape::kStagingBytes), to = slot * uint32_t(Shape::kSlotBytes);
+            const uint32_t from = fromLane + buffer * uint32_t(Shape::kStagingBytes), to = place * uint32_t(Shape::kSlotBytes);
 #pragma unroll 8
             for (int step = 0; step < kKeys / kRowsAtOnce; ++step) {
                 const uint4 v = ldsVector(from + uint32_t(step * kRowsAtOnce * DP));
@@ -356,12 +322,18 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                mbarArrive(&bars.full[slot]);
+                mbarArrive(&bars.full[place]);
                 mbarArrive(&bars.stagingEmpty[buffer]);
+            }
+            if (warp == kSoftmaxWarps && int(unit) + kStaging < 2 * tiles) { // the buffer is free when all four have read it
+                ok = mbarWaitWarp(&bars.stagingEmpty[buffer], (unit / kStaging) & 1u, 91);
+                if (ok) {
+                    copyUnit(int(unit) + kStaging);
+                }
             }
         }
         __syncwarp();
-    } else {
+    } else if (warp < active * kTileWarps) {
         // ---------------- softmax: a lane half a row ----------------
         const int which = warp / kTileWarps, half = (warp >> 2) & 1, quarter = warp & 3, tileRow = quarter * 32 + lane,
                   row = firstRow + which * kRows + tileRow;
@@ -421,16 +393,54 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const int rowHi = !live ? 0 : p.causal ? position + 1 : q.length, rowLo = p.window > 0 ? max(0, position - p.window + 1) : 0;
         // keys that every row of this tile sees
         const int tileFirst = firstRow + which * kRows, tileLast = min(tileFirst + kRows, firstRow + rows) - 1;
-        const int openHi = tileFirst > tileLast ? 0x7fffffff : p.causal ? old + int(fastDiv(uint32_t(tileFirst), p.groupDiv)) + 1 : q.length;
-        const int openLo = p.window > 0 && tileFirst <= tileLast ? max(0, old + int(fastDiv(uint32_t(tileLast), p.groupDiv)) - p.window + 1) : 0;
+        const int openHi = p.causal ? old + int(fastDiv(uint32_t(tileFirst), p.groupDiv)) + 1 : q.length;
+        const int openLo = p.window > 0 ? max(0, old + int(fastDiv(uint32_t(tileLast), p.groupDiv)) - p.window + 1) : 0;
         const uint32_t laneBase = tmem + (uint32_t(quarter * 32) << 16);
         const uint32_t scoresAt = laneBase + Shape::scores(which) + uint32_t(half * (kKeys / 2)),
-                       weightsAt = laneBase + Shape::scores(which) + uint32_t(half * (kKeys / 4)),
+                       weightsAt = scoresAt,
                        resultAt = laneBase + Shape::result(which) + uint32_t(half * (DP / 2));
+
+        // ---- products of this tile, issued by its first warp as a whole (see ummaBlockPeek) ----
+        constexpr uint32_t kScoreDesc = instrF16(kKeys, false), kResultDesc = instrF16(DP, true);
+        constexpr uint32_t kPanel = kRows * 128; // bytes: 64 elements of 128 rows
+        const bool issues = warp % kTileWarps == 0;
+        const uint32_t queryAddr = smemAddr(queries) + uint32_t(which * Shape::kQueryBytes), slotAddr = smemAddr(slots);
+        bool ok = true;
+        const auto scoreProduct = [&](int tile) {
+            const uint32_t place = uint32_t(2 * tile) % kSlots;
+            ok = ok && mbarWaitWarp(&bars.full[place], (uint32_t(2 * tile) / kSlots) & 1u, 93);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                const uint32_t at = uint32_t(k / 4) * kPanel + uint32_t(k % 4) * 32u;
+                mmaShared(tmem + Shape::scores(which), descWords(smemDesc(queryAddr + at, 16, 1024)),
+                          descWords(smemDesc(slotAddr + place * uint32_t(Shape::kSlotBytes) + at, 16, 1024)), kScoreDesc, k != 0 ? 1u : 0u);
+            }
+            ummaCommit(&bars.scores[which]);
+            ummaCommit(&bars.empty[place]);
+        };
+        const auto resultProduct = [&](int tile) {
+            const uint32_t unit = uint32_t(2 * tile + 1), place = unit % kSlots;
+            ok = ok && mbarWaitWarp(&bars.full[place], (unit / kSlots) & 1u, 94) && mbarWaitWarp(&bars.weights[which], uint32_t(tile) & 1u, 95);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k) { // the weights of 16 keys lie in eight columns, of either half of the keys in its own
+                mmaTensor(tmem + Shape::result(which), tmem + Shape::scores(which) + uint32_t((k / kHalfGroups) * (kKeys / 2) + (k % kHalfGroups) * 8),
+                          descWords(smemDesc(slotAddr + place * uint32_t(Shape::kSlotBytes) + uint32_t(k) * 2048u, kPanel, 1024)), kResultDesc,
+                          tile != 0 || k != 0 ? 1u : 0u);
+            }
+            if (tile == tiles - 1) {
+                ummaCommit(&bars.result[which]);
+            }
+            ummaCommit(&bars.empty[place]);
+        };
+        if (issues) {
+            ok = mbarWaitWarp(&bars.queries, 0u, 92);
+            scoreProduct(0);
+        }
 
         float most = -INFINITY, sum = 0.f;
         int reference = -126;
-        bool ok = true;
         const auto scoreOf = [&](uint32_t s, float factor) { // in powers of two
             const float x = __uint_as_float(s) * factor;
             return CAP ? softCapped(x, p.softcap) * kLog2e : x;
@@ -495,13 +505,17 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 bool grows = false;
                 const float base = most == -INFINITY ? 0.f : most;
                 added = 0.f;
+                uint32_t buffered[2][16]; // the next group's scores come while one's are weighed
+                tmemLoad16(scoresAt, buffered[0]);
 #pragma unroll
                 for (int g = 0; g < kHalfGroups; ++g) {
-                    uint32_t s[16];
-                    tmemLoad16(scoresAt + uint32_t(g * 16), s);
+                    uint32_t(&s)[16] = buffered[g & 1];
                     const float factor = rowScale * tp.keyScale[half * kHalfGroups + g], shift = tp.shift[half * kHalfGroups + g] - base;
                     const uint32_t bits = masked ? seen(g) : 0xffffu;
                     tmemWait16(s);
+                    if (g + 1 < kHalfGroups) {
+                        tmemLoad16(scoresAt + uint32_t(g * 16 + 16), buffered[(g + 1) & 1]);
+                    }
                     float top = -INFINITY, part = 0.f;
                     if (!__all_sync(0xffffffffu, bits == 0xffffu)) {
                         // what the mask hides stays out, whatever its page's scales are
@@ -517,20 +531,21 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                         grows = grows || top > most + kGrowth;
                         added = part == 0.f ? added : fmaf(part, tp.perWeight[half * kHalfGroups + g], added);
                     } else {
+                        const float2 factors = {factor, factor}, shifts = {shift, shift};
+                        float2 parts = {0.f, 0.f};
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
-                            float w0, w1;
+                            float2 x = {__uint_as_float(s[j]), __uint_as_float(s[j + 1])};
                             if (CAP) {
-                                const float x = scoreOf(s[j], factor), y = scoreOf(s[j + 1], factor);
-                                top = fmaxf(top, fmaxf(x, y));
-                                w0 = exp2Fast(x + shift), w1 = exp2Fast(y + shift);
-                            } else {
-                                top = fmaxf(top, fmaxf(__uint_as_float(s[j]), __uint_as_float(s[j + 1])));
-                                w0 = exp2Fast(fmaf(__uint_as_float(s[j]), factor, shift)), w1 = exp2Fast(fmaf(__uint_as_float(s[j + 1]), factor, shift));
+                                x.x = scoreOf(s[j], factor), x.y = scoreOf(s[j + 1], factor);
                             }
-                            part += w0 + w1;
-                            weights[g * 8 + j / 2] = packTwo(w0, w1, __half());
+                            top = maxThree(top, x.x, x.y);
+                            x = CAP ? addTwo(x, shifts) : fmaTwo(x, factors, shifts);
+                            const float2 w = {exp2Fast(x.x), exp2Fast(x.y)};
+                            parts = addTwo(parts, w);
+                            weights[g * 8 + j / 2] = packTwo(w.x, w.y, __half());
                         }
+                        part = parts.x + parts.y;
                         grows = grows || (CAP ? top : top * factor) > most + kGrowth;
                         added = fmaf(part, tp.perWeight[half * kHalfGroups + g], added);
                     }
@@ -551,6 +566,12 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             __syncwarp();
             if (lane == 0) {
                 mbarArrive(&bars.weights[which]);
+            }
+            if (issues) {
+                resultProduct(tile);
+                if (tile + 1 < tiles) {
+                    scoreProduct(tile + 1);
+                }
             }
         }
         // ---- the rows, by way of the queries' memory, which no product reads any more ----
@@ -604,7 +625,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == kProductWarp) {
+    if (warp == kSoftmaxWarps) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
