@@ -4,16 +4,14 @@
 //
 // A block takes 256 rows of one sequence and cache head (a row is one token's query head; the heads that share a cache head are
 // neighbouring rows) as two tiles of 128, and walks the keys they see in tiles of 128:
+//   one warp       copies, integers into staging buffers: a page at a time, or the part of it that falls into a tile
 //   four warps     integers -> f16 (exact), in the 128-byte swizzled layout that both products read: keys are rows of a
-//                  K-major operand, values rows of an MN-major one, the same bytes either way; the first of them issues the
-//                  copies, 16 keys or values at a time (pages hold a multiple of 16), integers into staging buffers
-//   two x eight    softmax, a lane half a row: S out of tensor memory, weights as f16 back over it; the first of each
-//                  eight issues its tile's products (S = Q K^T into tensor memory, O += P V with P read from there) in the
-//                  time it would wait for them
+//                  K-major operand, values rows of an MN-major one, the same bytes either way
+//   one warp       products: S = Q K^T into tensor memory, O += P V with P read from tensor memory
+//   two x eight    softmax, a lane half a row: S out of tensor memory, weights as f16 back over it
 // The tiles take turns: while one's products run the other's softmax does.  Tensor memory is full (two times S and O), so a tile's
 // next scores wait for its weights to be used up; what counts is how long a tile's softmax takes, hence two warps to a
-// scheduler for it (with one, whose lanes had a row each: 5200 cycles per 128 keys, of which 2700 the softmax), and no warp
-// beyond twenty, which leaves a lane 96 registers.
+// scheduler for it (with one, whose lanes had a row each: 5200 cycles per 128 keys, of which 2700 the softmax).
 //
 // What bounds it: per 256 x 128 scores the products take 2048 cycles at 128 elements a head, and 32768 exponentials the
 // same at 16 a cycle; everything else (a multiply-add, half a maximum, half a sum, half a conversion per score, and the
@@ -42,7 +40,7 @@ namespace {
 using namespace tc;
 
 constexpr int kRows = 128, kKeys = 128, kGroup = 16, kGroups = kKeys / kGroup;
-constexpr int kSoftmaxWarps = 16, kConvertWarps = 4, kManyThreads = (kSoftmaxWarps + kConvertWarps) * 32;
+constexpr int kSoftmaxWarps = 16, kConvertWarps = 4, kCopyWarp = 20, kProductWarp = 21, kManyThreads = 22 * 32;
 constexpr int kTileWarps = kSoftmaxWarps / 2, kHalfGroups = kGroups / 2; // warps of a tile; groups of a lane
 constexpr int kParamRing = 4, kStaging = 4, kSlots = 3; // of 128 keys or values: integers on their way, and f16
 constexpr float kGrowth = 8.f;                          // in powers of two
@@ -84,22 +82,39 @@ struct ManyState {
 constexpr uint32_t instrF16(int n, bool bMnMajor) {
     return (1u << 4) | (uint32_t(bMnMajor) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 }
-__device__ __forceinline__ void mmaShared(uint32_t d, DescWords a, DescWords b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, l;\n\t.reg .b64 a, b;\n\t"
+// Four products of 16 elements of k each in one statement (see ummaBlock): both operands in shared memory, K-major, 32 bytes of
+// a swizzled row apart ...
+__device__ __forceinline__ void mmaSharedFour(uint32_t d, DescWords a, DescWords b, uint32_t idesc, uint32_t accumulateFirst) {
+    asm volatile("{\n\t.reg .pred l, p;\n\t.reg .b32 x, y;\n\t.reg .b64 a, b;\n\t"
                  "elect.sync _|l, 0xffffffff;\n\t"
                  "setp.ne.b32 p, %6, 0;\n\t"
                  "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t"
+                 "setp.eq.b32 p, %5, %5;\n\t"
+                 "add.u32 x, %1, 2;\n\tadd.u32 y, %3, 2;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t"
+                 "add.u32 x, %1, 4;\n\tadd.u32 y, %3, 4;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t"
+                 "add.u32 x, %1, 6;\n\tadd.u32 y, %3, 6;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
                  "@l tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d),
-                 "r"(a.low), "r"(a.high), "r"(b.low), "r"(b.high), "r"(idesc), "r"(accumulate)
+                 "r"(a.low), "r"(a.high), "r"(b.low), "r"(b.high), "r"(idesc), "r"(accumulateFirst)
                  : "memory");
 }
-__device__ __forceinline__ void mmaTensor(uint32_t d, uint32_t a, DescWords b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p, l;\n\t.reg .b64 b;\n\t"
+// ... and the first one in tensor memory, eight columns apart, the second MN-major in shared memory, 16 rows of 128 bytes apart.
+__device__ __forceinline__ void mmaTensorFour(uint32_t d, uint32_t a, DescWords b, uint32_t idesc, uint32_t accumulateFirst) {
+    asm volatile("{\n\t.reg .pred l, p;\n\t.reg .b32 x, y;\n\t.reg .b64 b;\n\t"
                  "elect.sync _|l, 0xffffffff;\n\t"
                  "setp.ne.b32 p, %5, 0;\n\t"
                  "mov.b64 b, {%2, %3};\n\t"
-                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
-                 "r"(a), "r"(b.low), "r"(b.high), "r"(idesc), "r"(accumulate)
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t"
+                 "setp.eq.b32 p, %4, %4;\n\t"
+                 "add.u32 x, %1, 8;\n\tadd.u32 y, %2, 128;\n\tmov.b64 b, {y, %3};\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %4, p;\n\t"
+                 "add.u32 x, %1, 16;\n\tadd.u32 y, %2, 256;\n\tmov.b64 b, {y, %3};\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %4, p;\n\t"
+                 "add.u32 x, %1, 24;\n\tadd.u32 y, %2, 384;\n\tmov.b64 b, {y, %3};\n\t"
+                 "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [x], b, %4, p;\n\t}" ::"r"(d),
+                 "r"(a), "r"(b.low), "r"(b.high), "r"(idesc), "r"(accumulateFirst)
                  : "memory");
 }
 __device__ __forceinline__ void tmemStore32(uint32_t taddr, const uint32_t *r) {
@@ -154,7 +169,7 @@ __device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st
 template <int DP, bool HALF, bool CAP>
 __global__ void __launch_bounds__(kManyThreads, 1)
 pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p,
-                         const FastDiv heads, const int levels) {
+                         const FastDiv heads, const int levels, const int boxRows) {
     using Shape = ManyShape<DP>;
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     extern __shared__ __align__(1024) uint8_t rawSmem[];
@@ -188,7 +203,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     }
     const int rows = min(2 * kRows, allRows - firstRow), old = q.length - q.fresh;
     const int firstToken = int(fastDiv(uint32_t(firstRow), p.groupDiv)), lastToken = int(fastDiv(uint32_t(firstRow + rows - 1), p.groupDiv));
-    const int keyLo = (p.window > 0 ? max(0, old + firstToken - p.window + 1) : 0) / kGroup * kGroup;
+    const int keyLo = (p.window > 0 ? max(0, old + firstToken - p.window + 1) : 0) / boxRows * boxRows;
     const int keyHi = p.causal ? old + lastToken + 1 : q.length;
     const int tiles = (keyHi - keyLo + kKeys - 1) / kKeys;
     const int32_t *table = p.batch.table + index * p.batch.tableStride;
@@ -205,7 +220,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         }
         for (int i = 0; i < kSlots; ++i) {
             mbarInit(&bars.full[i], kConvertWarps);
-            mbarInit(&bars.empty[i], uint32_t(active)); // the tiles' products
+            mbarInit(&bars.empty[i], 1u);
         }
         for (int i = 0; i < 2; ++i) {
             mbarInit(&bars.scores[i], 1u);
@@ -214,7 +229,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == kSoftmaxWarps) {
+    if (warp == kProductWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smemAddr(&bars.tmemBase)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -223,9 +238,9 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = bars.tmemBase;
 
-    if (warp >= kSoftmaxWarps) {
-        // ---------------- integers -> f16; the first warp: copies, and what the softmax needs to know of their pages ----------------
-        const int groups = (keyHi - keyLo + kGroup - 1) / kGroup;
+    if (warp == kCopyWarp) {
+        // ---------------- copies, and what the softmax needs to know of their pages ----------------
+        const int groups = (keyHi - keyLo + kGroup - 1) / kGroup, groupsOfBox = boxRows / kGroup;
         const auto slotOf = [&](int tile) { // lane 0 .. 7: the page of a group of the tile; -1: there is none
             const int n = tile * kGroups + lane;
             return lane < kGroups && n < groups ? table[fastDiv(uint32_t(keyLo + n * kGroup), p.pageDiv)] : -1;
@@ -240,56 +255,119 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             return slot;
         };
         const auto scaleOf = [&](const float *scales, int slot) { return slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : 0.f; };
-        int slot = -1, nextSlot = -1, nextNextSlot = -1, reference = -126;
-        float keyScale = 0.f, valueScale = 0.f, nextKeyScale = 0.f, nextValueScale = 0.f;
+        int nextNextSlot = slotOf(1), nextSlot = checked(0, slotOf(0)), reference = -126;
+        float nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
+        uint32_t unit = 0; // keys and values of the tiles in turn
         bool ok = true;
-        const auto copyUnit = [&](int unit) { // keys (unit 2 t) and values (2 t + 1) of the tiles in turn, into a free staging buffer
-            const int tile = unit >> 1, side = unit & 1;
-            if (side == 0) {
-                slot = nextSlot, keyScale = nextKeyScale, valueScale = nextValueScale, nextSlot = checked(tile + 1, nextNextSlot);
-                nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
-                nextNextSlot = slotOf(tile + 2);
-                // Parameters of the tile.  Here the converters are done with the keys of tile - 2, for which the values of tile - 4
-                // had been used up by both tiles: the softmax is past tile - 4, whose place this is.
-                TileParams &to = params[tile % kParamRing];
-                const float magnitude = fabsf(valueScale);
-                int exponent = magnitude > 0.f && magnitude < INFINITY ? int(__float_as_uint(powerAbove(magnitude)) >> 23) - 127 : -126;
-                exponent = __reduce_max_sync(0xffffffffu, exponent);
-                reference = max(reference, exponent);
-                if (lane < kGroups) {
-                    // (a scale that is not finite gives a shift and weights that are not)
-                    const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), -60.f) + kWeightBits : magnitude - magnitude;
-                    to.keyScale[lane] = keyScale, to.shift[lane] = shift, to.perWeight[lane] = exp2f(-shift);
+        for (int tile = 0; tile < tiles && ok; ++tile) {
+            const int slot = nextSlot, afterSlot = nextNextSlot;
+            const float keyScale = nextKeyScale, valueScale = nextValueScale;
+            nextNextSlot = slotOf(tile + 2);
+            // the copies first: what they need has long been here
+            const int key = keyLo + (tile * kGroups + lane) * kGroup, count = min(kGroups, groups - tile * kGroups);
+            const int row = (max(slot, 0) * p.cache.heads + head) * p.cache.page + key - int(fastDiv(uint32_t(key), p.pageDiv)) * p.cache.page;
+            const int boxes = (count + groupsOfBox - 1) / groupsOfBox; // the last one may reach behind the sequence, not behind its page
+#pragma unroll 1
+            for (int side = 0; side < 2; ++side, ++unit) {
+                const uint32_t buffer = unit % kStaging;
+                ok = ok && mbarWaitWarp(&bars.stagingEmpty[buffer], ((unit / kStaging) & 1u) ^ 1u, 91);
+                if (!ok) {
+                    break;
                 }
-                const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
                 if (lane == 0) {
-                    to.reference = reference, to.there = there;
+                    mbarArriveExpectTx(&bars.stagingFull[buffer], uint32_t(boxes * boxRows * DP));
                 }
                 __syncwarp();
-                if (lane == 0) {
-                    mbarArrive(&bars.params[tile % kParamRing]);
+                if (lane < kGroups && lane % groupsOfBox == 0 && lane < count) {
+                    tmaLoad3d(side == 0 ? &mapK : &mapV, staging + buffer * Shape::kStagingBytes + lane * kGroup * DP, &bars.stagingFull[buffer],
+                              0, row, 0);
+                }
+                if (side == 0) {
+                    // Parameters of the tile.  Here the converters are done with the keys of tile - 2, for which the values of
+                    // tile - 4 had been used up by both tiles: the softmax is past tile - 4, whose place this is.
+                    TileParams &to = params[tile % kParamRing];
+                    const float magnitude = fabsf(valueScale);
+                    int exponent = magnitude > 0.f && magnitude < INFINITY ? int(__float_as_uint(powerAbove(magnitude)) >> 23) - 127 : -126;
+                    exponent = __reduce_max_sync(0xffffffffu, exponent);
+                    reference = max(reference, exponent);
+                    if (lane < kGroups) {
+                        // (a scale that is not finite gives a shift and weights that are not)
+                        const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), -60.f) + kWeightBits : magnitude - magnitude;
+                        to.keyScale[lane] = keyScale, to.shift[lane] = shift, to.perWeight[lane] = exp2f(-shift);
+                    }
+                    const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
+                    if (lane == 0) {
+                        to.reference = reference, to.there = there;
+                    }
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbarArrive(&bars.params[tile % kParamRing]);
+                    }
                 }
             }
-            const int buffer = unit % kStaging, key = keyLo + (tile * kGroups + lane) * kGroup;
-            const int row = (max(slot, 0) * p.cache.heads + head) * p.cache.page + key - int(fastDiv(uint32_t(key), p.pageDiv)) * p.cache.page;
-            const int count = min(kGroups, groups - tile * kGroups);
-            if (lane == 0) {
-                mbarArriveExpectTx(&bars.stagingFull[buffer], uint32_t(count * kGroup * DP));
+            nextSlot = checked(tile + 1, afterSlot);
+            nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
+        }
+        __syncwarp();
+    } else if (warp == kProductWarp) {
+        // ---------------- products (the whole warp: see ummaBlockPeek) ----------------
+        constexpr uint32_t kScoreDesc = instrF16(kKeys, false), kResultDesc = instrF16(DP, true);
+        constexpr uint32_t kPanel = kRows * 128, kPlace = uint32_t(Shape::kSlotBytes) >> 4; // bytes of 64 elements of 128 rows; units of 16 bytes
+        const DescWords queryDesc = descWords(smemDesc(smemAddr(queries), 16, 1024)), keyDesc = descWords(smemDesc(smemAddr(slots), 16, 1024)),
+                        valueDesc = descWords(smemDesc(smemAddr(slots), kPanel, 1024));
+        bool failed = !mbarWait(&bars.queries, 0u, 92);
+        const auto scoreProduct = [&](int tile, int which) {
+            const uint32_t unit = uint32_t(2 * tile), place = unit % kSlots;
+            if (which == 0) {
+                failed = failed || !mbarWait(&bars.full[place], (unit / kSlots) & 1u, 93);
             }
             __syncwarp();
-            if (lane < count) {
-                tmaLoad3d(side == 0 ? &mapK : &mapV, staging + buffer * Shape::kStagingBytes + lane * kGroup * DP, &bars.stagingFull[buffer], 0,
-                          row, 0);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int panel = 0; panel < DP / 64; ++panel) {
+                mmaSharedFour(tmem + Shape::scores(which),
+                              {queryDesc.low + uint32_t(which * (Shape::kQueryBytes >> 4)) + uint32_t(panel) * (kPanel >> 4), queryDesc.high},
+                              {keyDesc.low + place * kPlace + uint32_t(panel) * (kPanel >> 4), keyDesc.high}, kScoreDesc, uint32_t(panel));
+            }
+            ummaCommit(&bars.scores[which]);
+            if (which == active - 1) {
+                ummaCommit(&bars.empty[place]);
             }
         };
-        if (warp == kSoftmaxWarps) {
-            nextNextSlot = slotOf(1);
-            nextSlot = checked(0, slotOf(0));
-            nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
-            for (int unit = 0; unit < min(kStaging, 2 * tiles); ++unit) {
-                copyUnit(unit);
+        const auto resultProduct = [&](int tile, int which) {
+            const uint32_t unit = uint32_t(2 * tile + 1), place = unit % kSlots;
+            if (which == 0) {
+                failed = failed || !mbarWait(&bars.full[place], (unit / kSlots) & 1u, 94);
+            }
+            failed = failed || !mbarWait(&bars.weights[which], uint32_t(tile) & 1u, 95);
+            __syncwarp();
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+            for (int h = 0; h < 2; ++h) { // the weights of 16 keys lie in eight columns, of either half of the keys in its own
+                static_assert(kHalfGroups == 4, "four products for half a tile's keys");
+                mmaTensorFour(tmem + Shape::result(which), tmem + Shape::scores(which) + uint32_t(h * (kKeys / 2)),
+                              {valueDesc.low + place * kPlace + uint32_t(h) * 512u, valueDesc.high}, kResultDesc, tile != 0 || h != 0 ? 1u : 0u);
+            }
+            if (tile == tiles - 1) {
+                ummaCommit(&bars.result[which]);
+            }
+            if (which == active - 1) {
+                ummaCommit(&bars.empty[place]);
+            }
+        };
+        for (int which = 0; which < active; ++which) {
+            scoreProduct(0, which);
+        }
+        for (int tile = 0; tile < tiles; ++tile) {
+            for (int which = 0; which < active; ++which) {
+                resultProduct(tile, which);
+                if (tile + 1 < tiles) {
+                    scoreProduct(tile + 1, which);
+                }
             }
         }
+    } else if (warp >= kSoftmaxWarps) {
+        // ---------------- integers -> f16 ----------------
         // A lane takes 16 bytes of a row: bytes 16 (lane % 4) on of a panel of 64, the panels a half of the warp each.  Eight
         // neighbouring lanes write four chunks of two rows, which the swizzle keeps in different banks.
         constexpr int kPanels = DP / 64, kRowsAtOnce = kConvertWarps * 8 / kPanels;
@@ -301,9 +379,8 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const uint32_t low = toLane + uint32_t(((2 * part) ^ (row0 & 7)) << 4), high = toLane + uint32_t(((2 * part + 1) ^ (row0 & 7)) << 4);
         for (uint32_t unit = 0; unit < uint32_t(2 * tiles); ++unit) {
             const uint32_t buffer = unit % kStaging, place = unit % kSlots;
-            ok = ok && mbarWaitWarp(&bars.stagingFull[buffer], (unit / kStaging) & 1u, 96) &&
-                 mbarWaitWarp(&bars.empty[place], ((unit / kSlots) & 1u) ^ 1u, 97);
-            if (!ok) {
+            if (!mbarWaitWarp(&bars.stagingFull[buffer], (unit / kStaging) & 1u, 96) ||
+                !mbarWaitWarp(&bars.empty[place], ((unit / kSlots) & 1u) ^ 1u, 97)) {
                 break;
             }
             const uint32_t from = fromLane + buffer * uint32_t(Shape::kStagingBytes), to = place * uint32_t(Shape::kSlotBytes);
@@ -325,12 +402,6 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 mbarArrive(&bars.full[place]);
                 mbarArrive(&bars.stagingEmpty[buffer]);
             }
-            if (warp == kSoftmaxWarps && int(unit) + kStaging < 2 * tiles) { // the buffer is free when all four have read it
-                ok = mbarWaitWarp(&bars.stagingEmpty[buffer], (unit / kStaging) & 1u, 91);
-                if (ok) {
-                    copyUnit(int(unit) + kStaging);
-                }
-            }
         }
         __syncwarp();
     } else if (warp < active * kTileWarps) {
@@ -343,45 +414,60 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         float rowScale;
         {
             const T *from = reinterpret_cast<const T *>(p.queries + int64_t(q.first + token) * p.queryStride[0] + queryHead * p.queryStride[1]);
+            constexpr int kVectors = DP / 32; // 16 elements each, of half a row: all on their way at once
+            uint32_t w[kVectors][8];
             const int length = live ? p.cache.headDim : 0;
-            float most = 0.f, inverse = 1.f, unit = 1.f;
+            if (p.wideQueries) {
+#pragma unroll
+                for (int v = 0; v < kVectors; ++v) {
+                    const int d = half * (DP / 2) + 16 * v;
+                    const uint4 zero = {0u, 0u, 0u, 0u}, *at = reinterpret_cast<const uint4 *>(from + d);
+                    const uint4 x = d < length ? at[0] : zero, y = d < length ? at[1] : zero;
+                    w[v][0] = x.x, w[v][1] = x.y, w[v][2] = x.z, w[v][3] = x.w, w[v][4] = y.x, w[v][5] = y.y, w[v][6] = y.z, w[v][7] = y.w;
+                }
+            } else {
+#pragma unroll
+                for (int v = 0; v < kVectors; ++v) {
+                    loadQuerySixteen(from, half * (DP / 2) + 16 * v, length, false, w[v]);
+                }
+            }
+            float unit = 1.f;
             if (!HALF) {
-#pragma unroll 1
-                for (int d = 0; d < length; d += 16) {
-                    uint32_t w[8];
-                    loadQuerySixteen(from, d, length, p.wideQueries != 0, w);
+                float most = 0.f;
+#pragma unroll
+                for (int v = 0; v < kVectors; ++v) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float2 f = unpackTwo(w[j], T());
+                        const float2 f = unpackTwo(w[v][j], T());
                         most = maxBits(most, maxBits(f.x, f.y));
                     }
                 }
-                unit = halfUnit(most);
-                inverse = 1.f / unit;
+                exchange[which][tileRow][half] = most;
+                asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
+                unit = halfUnit(maxBits(most, exchange[which][tileRow][half ^ 1]));
+                const float inverse = 1.f / unit;
+#pragma unroll
+                for (int v = 0; v < kVectors; ++v) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float2 f = unpackTwo(w[v][j], T());
+                        w[v][j] = packTwo(f.x * inverse, f.y * inverse, __half());
+                    }
+                }
             }
             rowScale = unit * fabsf(p.scale) * (CAP ? 1.f : kLog2e);
             const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u; // keeps the order of scores that of the products
             const uint32_t line = smemAddr(queries) + uint32_t(which * Shape::kQueryBytes + tileRow * 128);
-#pragma unroll 1
-            for (int d = half * (DP / 2); d < (half + 1) * (DP / 2); d += 16) {
-                uint32_t w[8];
-                loadQuerySixteen(from, d, length, p.wideQueries != 0, w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if (!HALF) {
-                        const float2 f = unpackTwo(w[j], T());
-                        w[j] = packTwo(f.x * inverse, f.y * inverse, __half());
-                    }
-                    w[j] ^= sign;
-                }
+            for (int v = 0; v < kVectors; ++v) {
+                const int d = half * (DP / 2) + 16 * v, chunk = (d % 64) / 8;
                 const uint32_t panel = line + uint32_t(d / 64) * (kRows * 128u);
-                const int chunk = (d % 64) / 8;
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(panel + uint32_t((chunk ^ (tileRow & 7)) << 4)), "r"(w[0]),
-                             "r"(w[1]), "r"(w[2]), "r"(w[3])
-                             : "memory");
-                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(panel + uint32_t(((chunk + 1) ^ (tileRow & 7)) << 4)), "r"(w[4]),
-                             "r"(w[5]), "r"(w[6]), "r"(w[7])
-                             : "memory");
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(panel + uint32_t(((chunk + h) ^ (tileRow & 7)) << 4)),
+                                 "r"(w[v][4 * h] ^ sign), "r"(w[v][4 * h + 1] ^ sign), "r"(w[v][4 * h + 2] ^ sign), "r"(w[v][4 * h + 3] ^ sign)
+                                 : "memory");
+                }
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
@@ -400,45 +486,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                        weightsAt = scoresAt,
                        resultAt = laneBase + Shape::result(which) + uint32_t(half * (DP / 2));
 
-        // ---- products of this tile, issued by its first warp as a whole (see ummaBlockPeek) ----
-        constexpr uint32_t kScoreDesc = instrF16(kKeys, false), kResultDesc = instrF16(DP, true);
-        constexpr uint32_t kPanel = kRows * 128; // bytes: 64 elements of 128 rows
-        const bool issues = warp % kTileWarps == 0;
-        const uint32_t queryAddr = smemAddr(queries) + uint32_t(which * Shape::kQueryBytes), slotAddr = smemAddr(slots);
         bool ok = true;
-        const auto scoreProduct = [&](int tile) {
-            const uint32_t place = uint32_t(2 * tile) % kSlots;
-            ok = ok && mbarWaitWarp(&bars.full[place], (uint32_t(2 * tile) / kSlots) & 1u, 93);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t at = uint32_t(k / 4) * kPanel + uint32_t(k % 4) * 32u;
-                mmaShared(tmem + Shape::scores(which), descWords(smemDesc(queryAddr + at, 16, 1024)),
-                          descWords(smemDesc(slotAddr + place * uint32_t(Shape::kSlotBytes) + at, 16, 1024)), kScoreDesc, k != 0 ? 1u : 0u);
-            }
-            ummaCommit(&bars.scores[which]);
-            ummaCommit(&bars.empty[place]);
-        };
-        const auto resultProduct = [&](int tile) {
-            const uint32_t unit = uint32_t(2 * tile + 1), place = unit % kSlots;
-            ok = ok && mbarWaitWarp(&bars.full[place], (unit / kSlots) & 1u, 94) && mbarWaitWarp(&bars.weights[which], uint32_t(tile) & 1u, 95);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k) { // the weights of 16 keys lie in eight columns, of either half of the keys in its own
-                mmaTensor(tmem + Shape::result(which), tmem + Shape::scores(which) + uint32_t((k / kHalfGroups) * (kKeys / 2) + (k % kHalfGroups) * 8),
-                          descWords(smemDesc(slotAddr + place * uint32_t(Shape::kSlotBytes) + uint32_t(k) * 2048u, kPanel, 1024)), kResultDesc,
-                          tile != 0 || k != 0 ? 1u : 0u);
-            }
-            if (tile == tiles - 1) {
-                ummaCommit(&bars.result[which]);
-            }
-            ummaCommit(&bars.empty[place]);
-        };
-        if (issues) {
-            ok = mbarWaitWarp(&bars.queries, 0u, 92);
-            scoreProduct(0);
-        }
-
         float most = -INFINITY, sum = 0.f;
         int reference = -126;
         const auto scoreOf = [&](uint32_t s, float factor) { // in powers of two
@@ -505,17 +553,13 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 bool grows = false;
                 const float base = most == -INFINITY ? 0.f : most;
                 added = 0.f;
-                uint32_t buffered[2][16]; // the next group's scores come while one's are weighed
-                tmemLoad16(scoresAt, buffered[0]);
 #pragma unroll
                 for (int g = 0; g < kHalfGroups; ++g) {
-                    uint32_t(&s)[16] = buffered[g & 1];
+                    uint32_t s[16];
+                    tmemLoad16(scoresAt + uint32_t(g * 16), s);
                     const float factor = rowScale * tp.keyScale[half * kHalfGroups + g], shift = tp.shift[half * kHalfGroups + g] - base;
                     const uint32_t bits = masked ? seen(g) : 0xffffu;
                     tmemWait16(s);
-                    if (g + 1 < kHalfGroups) {
-                        tmemLoad16(scoresAt + uint32_t(g * 16 + 16), buffered[(g + 1) & 1]);
-                    }
                     float top = -INFINITY, part = 0.f;
                     if (!__all_sync(0xffffffffu, bits == 0xffffu)) {
                         // what the mask hides stays out, whatever its page's scales are
@@ -566,12 +610,6 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             __syncwarp();
             if (lane == 0) {
                 mbarArrive(&bars.weights[which]);
-            }
-            if (issues) {
-                resultProduct(tile);
-                if (tile + 1 < tiles) {
-                    scoreProduct(tile + 1);
-                }
             }
         }
         // ---- the rows, by way of the queries' memory, which no product reads any more ----
@@ -625,7 +663,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == kSoftmaxWarps) {
+    if (warp == kProductWarp) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
     }
@@ -635,8 +673,13 @@ template <int DP, bool HALF, bool CAP> int launchMany(const AttendParams &p, cud
     using Shape = ManyShape<DP>;
     constexpr size_t smemBytes = Shape::kTiles + sizeof(ManyState);
     static_assert(smemBytes <= 232448, "shared memory per block");
+    // rows of a copy: the largest power of two of them, up to a tile, that pages are made of
+    int boxRows = kKeys;
+    while (p.cache.page % boxRows != 0) {
+        boxRows /= 2;
+    }
     CUtensorMap k, v;
-    if (!makeCacheMap(&k, p.cache.keys, p.cache, DP, kGroup, false) || !makeCacheMap(&v, p.cache.values, p.cache, DP, kGroup, false)) {
+    if (!makeCacheMap(&k, p.cache.keys, p.cache, DP, boxRows, false) || !makeCacheMap(&v, p.cache.values, p.cache, DP, boxRows, false)) {
         return MLEL_ERROR_DEVICE;
     }
     const auto kernel = pagedAttentionManyKernel<DP, HALF, CAP>;
@@ -648,7 +691,7 @@ template <int DP, bool HALF, bool CAP> int launchMany(const AttendParams &p, cud
         refuse("mlel_cuda_paged_attention", "too many tokens and sequences for one call");
     }
     return launchStatus("mlel_cuda_paged_attention", launchOverlapped(kernel, dim3(unsigned(blocks)), kManyThreads, smemBytes, s, k, v, p,
-                                                                      makeFastDiv(p.cache.heads), int(levels)));
+                                                                      makeFastDiv(p.cache.heads), int(levels), boxRows));
 }
 
 template <int DP> int launchManyType(const AttendParams &p, cudaStream_t s) {
