@@ -410,64 +410,74 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                   row = firstRow + which * kRows + tileRow;
         const int pairBarrier = 1 + which * 4 + quarter; // of the two warps that share 32 rows
         const bool live = which * kRows + tileRow < rows;
-        const int token = live ? int(fastDiv(uint32_t(row), p.groupDiv)) : lastToken, queryHead = head * p.group + (live ? row - token * p.group : 0);
+        const int token = live ? int(fastDiv(uint32_t(row), p.groupDiv)) : lastToken;
         float rowScale;
         {
-            const T *from = reinterpret_cast<const T *>(p.queries + int64_t(q.first + token) * p.queryStride[0] + queryHead * p.queryStride[1]);
-            constexpr int kVectors = DP / 32; // 16 elements each, of half a row: all on their way at once
-            uint32_t w[kVectors][8];
-            const int length = live ? p.cache.headDim : 0;
-            if (p.wideQueries) {
+            // The warp's half of its 32 rows, as runs of DP bytes: kLanes lanes a row, kRowsAtOnce rows at a time, all on their way at once.
+            constexpr int kLanes = DP / 16, kRowsAtOnce = 32 / kLanes, kSteps = 32 / kRowsAtOnce;
+            const int chunk = lane % kLanes, element = half * (DP / 2) + chunk * 8;
+            uint4 words[kSteps];
 #pragma unroll
-                for (int v = 0; v < kVectors; ++v) {
-                    const int d = half * (DP / 2) + 16 * v;
-                    const uint4 zero = {0u, 0u, 0u, 0u}, *at = reinterpret_cast<const uint4 *>(from + d);
-                    const uint4 x = d < length ? at[0] : zero, y = d < length ? at[1] : zero;
-                    w[v][0] = x.x, w[v][1] = x.y, w[v][2] = x.z, w[v][3] = x.w, w[v][4] = y.x, w[v][5] = y.y, w[v][6] = y.z, w[v][7] = y.w;
-                }
-            } else {
-#pragma unroll
-                for (int v = 0; v < kVectors; ++v) {
-                    loadQuerySixteen(from, half * (DP / 2) + 16 * v, length, false, w[v]);
+            for (int step = 0; step < kSteps; ++step) {
+                const int r = quarter * 32 + step * kRowsAtOnce + lane / kLanes, global = firstRow + which * kRows + r;
+                words[step] = {0u, 0u, 0u, 0u};
+                if (which * kRows + r < rows && element < p.cache.headDim) {
+                    const int itsToken = int(fastDiv(uint32_t(global), p.groupDiv));
+                    const char *from = p.queries + int64_t(q.first + itsToken) * p.queryStride[0] +
+                                       (head * p.group + global - itsToken * p.group) * p.queryStride[1] + element * 2;
+                    if (p.wideQueries) {
+                        words[step] = *reinterpret_cast<const uint4 *>(from);
+                    } else {
+                        const uint16_t *e = reinterpret_cast<const uint16_t *>(from);
+                        words[step] = {uint32_t(e[0]) | uint32_t(e[1]) << 16, uint32_t(e[2]) | uint32_t(e[3]) << 16,
+                                       uint32_t(e[4]) | uint32_t(e[5]) << 16, uint32_t(e[6]) | uint32_t(e[7]) << 16};
+                    }
                 }
             }
             float unit = 1.f;
             if (!HALF) {
-                float most = 0.f;
 #pragma unroll
-                for (int v = 0; v < kVectors; ++v) {
+                for (int step = 0; step < kSteps; ++step) {
+                    float x[8], most = 0.f;
+                    unpackEight(words[step], x, T());
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float2 f = unpackTwo(w[v][j], T());
-                        most = maxBits(most, maxBits(f.x, f.y));
+                        most = maxBits(most, x[j]);
+                    }
+#pragma unroll
+                    for (int other = 1; other < kLanes; other <<= 1) {
+                        most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, other));
+                    }
+                    if (chunk == 0) {
+                        exchange[which][quarter * 32 + step * kRowsAtOnce + lane / kLanes][half] = most;
                     }
                 }
-                exchange[which][tileRow][half] = most;
                 asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
-                unit = halfUnit(maxBits(most, exchange[which][tileRow][half ^ 1]));
-                const float inverse = 1.f / unit;
+                unit = halfUnit(maxBits(exchange[which][tileRow][0], exchange[which][tileRow][1]));
 #pragma unroll
-                for (int v = 0; v < kVectors; ++v) {
+                for (int step = 0; step < kSteps; ++step) {
+                    const int r = quarter * 32 + step * kRowsAtOnce + lane / kLanes;
+                    const float inverse = 1.f / halfUnit(maxBits(exchange[which][r][0], exchange[which][r][1])); // powers of two
+                    float x[8];
+                    unpackEight(words[step], x, T());
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const float2 f = unpackTwo(w[v][j], T());
-                        w[v][j] = packTwo(f.x * inverse, f.y * inverse, __half());
+                        x[j] *= inverse;
                     }
+                    words[step] = packEight(x, __half());
                 }
+                asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory"); // `exchange` is used again
             }
             rowScale = unit * fabsf(p.scale) * (CAP ? 1.f : kLog2e);
             const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u; // keeps the order of scores that of the products
-            const uint32_t line = smemAddr(queries) + uint32_t(which * Shape::kQueryBytes + tileRow * 128);
 #pragma unroll
-            for (int v = 0; v < kVectors; ++v) {
-                const int d = half * (DP / 2) + 16 * v, chunk = (d % 64) / 8;
-                const uint32_t panel = line + uint32_t(d / 64) * (kRows * 128u);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(panel + uint32_t(((chunk + h) ^ (tileRow & 7)) << 4)),
-                                 "r"(w[v][4 * h] ^ sign), "r"(w[v][4 * h + 1] ^ sign), "r"(w[v][4 * h + 2] ^ sign), "r"(w[v][4 * h + 3] ^ sign)
-                                 : "memory");
-                }
+            for (int step = 0; step < kSteps; ++step) {
+                const int r = quarter * 32 + step * kRowsAtOnce + lane / kLanes;
+                const uint32_t to = smemAddr(queries) + uint32_t(which * Shape::kQueryBytes + (element / 64) * (kRows * 128) + r * 128) +
+                                    uint32_t((((element % 64) / 8) ^ (r & 7)) << 4);
+                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(words[step].x ^ sign), "r"(words[step].y ^ sign),
+                             "r"(words[step].z ^ sign), "r"(words[step].w ^ sign)
+                             : "memory");
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
