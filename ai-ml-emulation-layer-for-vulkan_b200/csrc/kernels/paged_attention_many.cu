@@ -39,28 +39,33 @@ namespace {
 
 using namespace tc;
 
-constexpr int kRows = 128, kKeys = 128, kGroup = 16, kGroups = kKeys / kGroup;
-constexpr int kSoftmaxWarps = 16, kConvertWarps = 4, kCopyWarp = 20, kProductWarp = 21, kManyThreads = 22 * 32;
-constexpr int kTileWarps = kSoftmaxWarps / 2, kHalfGroups = kGroups / 2; // warps of a tile; groups of a lane
-constexpr int kParamRing = 4, kStaging = 4, kSlots = 3; // of 128 keys or values: integers on their way, and f16
+constexpr int kRows = 128, kGroup = 16, kMostGroups = 8;
+constexpr int kConvertWarps = 4;
+constexpr int kParamRing = 4, kStaging = 4, kSlots = 3; // of a tile's keys or values: integers on their way, and f16
 constexpr float kGrowth = 8.f;                          // in powers of two
 constexpr float kWeightBits = 7.f;
 
+// Heads of 256 elements: one tile of rows (its result alone has 256 columns of tensor memory), and 64 keys at a time, whose f16 form is
+// as large as that of 128 keys of 128 elements.
 template <int DP> struct ManyShape {
-    static constexpr int kQueryBytes = kRows * DP * 2;   // of one tile: panels of 64 elements
+    static constexpr int kTilesOfRows = DP > 128 ? 1 : 2, kKeys = DP > 128 ? 64 : 128, kGroups = kKeys / kGroup, kHalfGroups = kGroups / 2;
+    static constexpr int kTileWarps = 8, kSoftmaxWarps = kTilesOfRows * kTileWarps; // two for 32 rows
+    static constexpr int kCopyWarp = kSoftmaxWarps + kConvertWarps, kProductWarp = kCopyWarp + 1, kThreads = (kProductWarp + 1) * 32;
+    static constexpr int kPanels = DP / 64;
+    static constexpr int kQueryBytes = kRows * DP * 2; // of one tile: panels of 64 elements
     static constexpr int kSlotBytes = kKeys * DP * 2;
     static constexpr int kStagingBytes = kKeys * DP;
-    static constexpr size_t kTiles = 2 * size_t(kQueryBytes) + kSlots * size_t(kSlotBytes) + kStaging * size_t(kStagingBytes);
-    // tensor-memory columns of the two tiles
+    static constexpr size_t kTiles = kTilesOfRows * size_t(kQueryBytes) + kSlots * size_t(kSlotBytes) + kStaging * size_t(kStagingBytes);
+    // tensor-memory columns of the tiles
     static constexpr __device__ uint32_t scores(int which) { return uint32_t(128 * which); }
     static constexpr __device__ uint32_t result(int which) { return uint32_t(256 + DP * which); }
 };
 
 // What the softmax needs to know of a tile of keys.
 struct TileParams {
-    float keyScale[kGroups]; // 0 where there is nothing
-    float shift[kGroups];    // log2(value scale) - reference + kWeightBits
-    float perWeight[kGroups]; // 2^-shift
+    float keyScale[kMostGroups];  // 0 where there is nothing
+    float shift[kMostGroups];     // log2(value scale) - reference + kWeightBits
+    float perWeight[kMostGroups]; // 2^-shift
     int reference;           // a power of two
     uint32_t there;          // groups that exist
 };
@@ -134,6 +139,13 @@ __device__ __forceinline__ void tmemStore16(uint32_t taddr, const uint32_t (&r)[
                  "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
+template <int N> __device__ __forceinline__ void tmemStoreWeights(uint32_t taddr, const uint32_t (&r)[N]) {
+    if constexpr (N == 32) {
+        tmemStore32(taddr, r);
+    } else {
+        tmemStore16(taddr, r);
+    }
+}
 // Two 32-bit floats at a time.
 __device__ __forceinline__ float2 fmaTwo(float2 a, float2 b, float2 c) {
     float2 d;
@@ -167,14 +179,17 @@ __device__ __forceinline__ uint32_t pairVote(int barrier, bool predicate) {
 __device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 template <int DP, bool HALF, bool CAP>
-__global__ void __launch_bounds__(kManyThreads, 1)
+__global__ void __launch_bounds__(ManyShape<DP>::kThreads, 1)
 pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p,
                          const FastDiv heads, const int levels, const int boxRows) {
     using Shape = ManyShape<DP>;
+    constexpr int kKeys = Shape::kKeys, kGroups = Shape::kGroups, kHalfGroups = Shape::kHalfGroups, kTileWarps = Shape::kTileWarps,
+                  kSoftmaxWarps = Shape::kSoftmaxWarps, kCopyWarp = Shape::kCopyWarp, kProductWarp = Shape::kProductWarp,
+                  kBlockRows = Shape::kTilesOfRows * kRows;
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     extern __shared__ __align__(1024) uint8_t rawSmem[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rawSmem) + 1023) & ~uintptr_t(1023));
-    uint8_t *queries = smem, *slots = smem + 2 * Shape::kQueryBytes, *staging = slots + kSlots * Shape::kSlotBytes;
+    uint8_t *queries = smem, *slots = smem + Shape::kTilesOfRows * Shape::kQueryBytes, *staging = slots + kSlots * Shape::kSlotBytes;
     ManyState &state = *reinterpret_cast<ManyState *>(smem + Shape::kTiles);
     ManyBarriers &bars = state.bars;
     TileParams(&params)[kParamRing] = state.params;
@@ -197,11 +212,11 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     if (!q.sound && level == 0 && head == 0 && threadIdx.x == 0) {
         atomicCAS(&g_pagedError, 0, kBadSequence);
     }
-    const int allRows = q.sound ? q.fresh * p.group : 0, firstRow = (levels - 1 - level) * 2 * kRows;
+    const int allRows = q.sound ? q.fresh * p.group : 0, firstRow = (levels - 1 - level) * kBlockRows;
     if (firstRow >= allRows) {
         return;
     }
-    const int rows = min(2 * kRows, allRows - firstRow), old = q.length - q.fresh;
+    const int rows = min(kBlockRows, allRows - firstRow), old = q.length - q.fresh;
     const int firstToken = int(fastDiv(uint32_t(firstRow), p.groupDiv)), lastToken = int(fastDiv(uint32_t(firstRow + rows - 1), p.groupDiv));
     const int keyLo = (p.window > 0 ? max(0, old + firstToken - p.window + 1) : 0) / boxRows * boxRows;
     const int keyHi = p.causal ? old + lastToken + 1 : q.length;
@@ -312,7 +327,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     } else if (warp == kProductWarp) {
         // ---------------- products (the whole warp: see ummaBlockPeek) ----------------
         constexpr uint32_t kScoreDesc = instrF16(kKeys, false), kResultDesc = instrF16(DP, true);
-        constexpr uint32_t kPanel = kRows * 128, kPlace = uint32_t(Shape::kSlotBytes) >> 4; // bytes of 64 elements of 128 rows; units of 16 bytes
+        constexpr uint32_t kQueryPanel = kRows * 128, kPanel = kKeys * 128, kPlace = uint32_t(Shape::kSlotBytes) >> 4; // bytes of 64 elements; units of 16
         const DescWords queryDesc = descWords(smemDesc(smemAddr(queries), 16, 1024)), keyDesc = descWords(smemDesc(smemAddr(slots), 16, 1024)),
                         valueDesc = descWords(smemDesc(smemAddr(slots), kPanel, 1024));
         bool failed = !mbarWait(&bars.queries, 0u, 92);
@@ -324,10 +339,10 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-            for (int panel = 0; panel < DP / 64; ++panel) {
+            for (int panel = 0; panel < Shape::kPanels; ++panel) {
                 mmaSharedFour(tmem + Shape::scores(which),
-                              {queryDesc.low + uint32_t(which * (Shape::kQueryBytes >> 4)) + uint32_t(panel) * (kPanel >> 4), queryDesc.high},
-                              {keyDesc.low + place * kPlace + uint32_t(panel) * (kPanel >> 4), keyDesc.high}, kScoreDesc, uint32_t(panel));
+                              {queryDesc.low + uint32_t(which * (Shape::kQueryBytes >> 4)) + uint32_t(panel) * (kQueryPanel >> 4), queryDesc.high},
+                              {keyDesc.low + place * kPlace + uint32_t(panel) * (kPanel >> 4), keyDesc.high}, kScoreDesc, panel != 0 ? 1u : 0u);
             }
             ummaCommit(&bars.scores[which]);
             if (which == active - 1) {
@@ -343,10 +358,9 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
-            for (int h = 0; h < 2; ++h) { // the weights of 16 keys lie in eight columns, of either half of the keys in its own
-                static_assert(kHalfGroups == 4, "four products for half a tile's keys");
-                mmaTensorFour(tmem + Shape::result(which), tmem + Shape::scores(which) + uint32_t(h * (kKeys / 2)),
-                              {valueDesc.low + place * kPlace + uint32_t(h) * 512u, valueDesc.high}, kResultDesc, tile != 0 || h != 0 ? 1u : 0u);
+            for (int k = 0; k < kGroups; k += 4) { // the weights of 16 keys lie in eight columns
+                mmaTensorFour(tmem + Shape::result(which), tmem + Shape::scores(which) + uint32_t(k * 8),
+                              {valueDesc.low + place * kPlace + uint32_t(k) * 128u, valueDesc.high}, kResultDesc, tile != 0 || k != 0 ? 1u : 0u);
             }
             if (tile == tiles - 1) {
                 ummaCommit(&bars.result[which]);
@@ -368,11 +382,11 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         }
     } else if (warp >= kSoftmaxWarps) {
         // ---------------- integers -> f16 ----------------
-        // A lane takes 16 bytes of a row: bytes 16 (lane % 4) on of a panel of 64, the panels a half of the warp each.  Eight
-        // neighbouring lanes write four chunks of two rows, which the swizzle keeps in different banks.
-        constexpr int kPanels = DP / 64, kRowsAtOnce = kConvertWarps * 8 / kPanels;
-        const int own = warp - kSoftmaxWarps, panel = kPanels == 2 ? lane >> 4 : 0, part = lane & 3;
-        const int row0 = own * (8 / kPanels) + (kPanels == 2 ? (lane >> 2) & 3 : lane >> 2); // its low three bits are those of all its rows
+        // A lane takes 16 bytes of a row: bytes 16 (lane % 4) on of a panel of 64.  Eight neighbouring lanes write four chunks of two
+        // rows, which the swizzle keeps in different banks.
+        constexpr int kPanels = Shape::kPanels, kRowsOfWarp = 8 / kPanels, kRowsAtOnce = kConvertWarps * kRowsOfWarp;
+        const int own = warp - kSoftmaxWarps, panel = (lane >> 2) / kRowsOfWarp, part = lane & 3;
+        const int row0 = own * kRowsOfWarp + (lane >> 2) % kRowsOfWarp; // its low three bits are those of all its rows
         static_assert(kRowsAtOnce % 8 == 0, "rows of a lane share their swizzle");
         const uint32_t fromLane = smemAddr(staging) + uint32_t(row0 * DP + panel * 64 + part * 16);
         const uint32_t toLane = smemAddr(slots) + uint32_t(panel * (kKeys * 128) + row0 * 128);
@@ -493,7 +507,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const int openLo = p.window > 0 ? max(0, old + int(fastDiv(uint32_t(tileLast), p.groupDiv)) - p.window + 1) : 0;
         const uint32_t laneBase = tmem + (uint32_t(quarter * 32) << 16);
         const uint32_t scoresAt = laneBase + Shape::scores(which) + uint32_t(half * (kKeys / 2)),
-                       weightsAt = scoresAt,
+                       weightsAt = laneBase + Shape::scores(which) + uint32_t(half * (kKeys / 4)),
                        resultAt = laneBase + Shape::result(which) + uint32_t(half * (DP / 2));
 
         bool ok = true;
@@ -614,7 +628,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 maximumFirst = true;
             }
             sum += added;
-            tmemStore32(weightsAt, weights);
+            tmemStoreWeights<kKeys / 4>(weightsAt, weights);
             tmemStoreWait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -684,7 +698,7 @@ template <int DP, bool HALF, bool CAP> int launchMany(const AttendParams &p, cud
     constexpr size_t smemBytes = Shape::kTiles + sizeof(ManyState);
     static_assert(smemBytes <= 232448, "shared memory per block");
     // rows of a copy: the largest power of two of them, up to a tile, that pages are made of
-    int boxRows = kKeys;
+    int boxRows = Shape::kKeys;
     while (p.cache.page % boxRows != 0) {
         boxRows /= 2;
     }
@@ -696,11 +710,11 @@ template <int DP, bool HALF, bool CAP> int launchMany(const AttendParams &p, cud
     if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), smemBytes)) {
         return MLEL_ERROR_DEVICE;
     }
-    const int64_t levels = (int64_t(p.batch.maxNew) * p.group + 2 * kRows - 1) / (2 * kRows), blocks = levels * p.cache.heads * p.batch.sequences;
+    const int64_t levels = (int64_t(p.batch.maxNew) * p.group + Shape::kTilesOfRows * kRows - 1) / (Shape::kTilesOfRows * kRows), blocks = levels * p.cache.heads * p.batch.sequences;
     if (blocks > 0x7fffffff) {
         refuse("mlel_cuda_paged_attention", "too many tokens and sequences for one call");
     }
-    return launchStatus("mlel_cuda_paged_attention", launchOverlapped(kernel, dim3(unsigned(blocks)), kManyThreads, smemBytes, s, k, v, p,
+    return launchStatus("mlel_cuda_paged_attention", launchOverlapped(kernel, dim3(unsigned(blocks)), Shape::kThreads, smemBytes, s, k, v, p,
                                                                       makeFastDiv(p.cache.heads), int(levels), boxRows));
 }
 
@@ -714,10 +728,10 @@ template <int DP> int launchManyType(const AttendParams &p, cudaStream_t s) {
 } // namespace
 
 bool pagedAttentionManyApplies(const AttendParams &p) {
-    return p.cache.headDim <= 128 && int64_t(p.batch.maxNew) * p.group > 64;
+    return int64_t(p.batch.maxNew) * p.group > 64;
 }
 int pagedAttentionMany(const AttendParams &p, cudaStream_t s) {
-    return p.cache.headDim <= 64 ? launchManyType<64>(p, s) : launchManyType<128>(p, s);
+    return p.cache.headDim <= 64 ? launchManyType<64>(p, s) : p.cache.headDim <= 128 ? launchManyType<128>(p, s) : launchManyType<256>(p, s);
 }
 
 int takePagedErrorMany() { return takePagedError(); }
