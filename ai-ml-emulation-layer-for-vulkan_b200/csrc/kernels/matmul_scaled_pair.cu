@@ -20,6 +20,7 @@
 #include "matmul_scaled.hpp"
 #include "serving.hpp"
 #include "serving_device.cuh"
+#include "serving_wait.cuh"
 #include "tcgen05_common.cuh"
 #include "tcgen05_pair.cuh"
 
@@ -121,7 +122,7 @@ matmulScaledPair(const __grid_constant__ CUtensorMap mapA, const __grid_constant
                           n0 = column * BN + int(rank) * (BN / 2);
                 for (int kb = 0; kb < numKb; ++kb) {
                     if (ready == 0) {
-                        ok = mbarWait(&bars.empty[s], phase ^ 1u, 81);
+                        ok = mbarPoll(&bars.empty[s], phase ^ 1u, 81);
                         if (!ok) {
                             break;
                         }
@@ -145,13 +146,13 @@ matmulScaledPair(const __grid_constant__ CUtensorMap mapA, const __grid_constant
             bool failed = false;
             for (int t = first; t < tiles; t += pairs, ++count) {
                 const uint32_t buf = count & 1u;
-                failed = failed || !mbarWait(&bars.accEmpty[buf], ((count >> 1) & 1u) ^ 1u, 82);
+                failed = failed || !mbarPoll(&bars.accEmpty[buf], ((count >> 1) & 1u) ^ 1u, 82);
                 __syncwarp();
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 int left = p.K;
                 for (int kb = 0; kb < numKb; ++kb) {
                     if (ready == 0) {
-                        failed = failed || !mbarWait(&bars.full[s], phase, 83);
+                        failed = failed || !mbarPoll(&bars.full[s], phase, 83);
                     }
                     __syncwarp();
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -178,7 +179,7 @@ matmulScaledPair(const __grid_constant__ CUtensorMap mapA, const __grid_constant
             const int column = int(fastDiv(uint32_t(t), tilesM));
             const int row0 = (t - column * int(tilesM.d)) * 256 + int(rank) * 128 + quarter * 32, n0 = column * BN + half * (BN / 2);
             const float rowScale = row0 + lane < p.M ? p.aScales[row0 + lane] : 0.f;
-            if (!mbarWaitWarp(&bars.accFull[buf], (count >> 1) & 1u, 84)) {
+            if (!mbarPollWarp(&bars.accFull[buf], (count >> 1) & 1u, 84)) {
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");

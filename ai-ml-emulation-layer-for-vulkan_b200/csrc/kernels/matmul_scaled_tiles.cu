@@ -4,9 +4,10 @@
 //
 // and for few tokens the sum over k split over the CTAs of a cluster, which add up their 32-bit integers through distributed
 // shared memory (whole numbers: the order does not matter).  With few tokens the weights' bytes bound the product: splitting puts
-// every SM to reading them, and two or three CTAs an SM (96 to 108 KB each) keep one reading while another starts or ends.
-// A lane of the epilogue has one channel, its scale and its bias; a warp stores 32 neighbouring channels of a token,
-// which takes any alignment of the output.
+// every SM to reading them, and two or three CTAs an SM (60 to 96 KB each) keep one reading while another starts or ends.
+// A lane of the epilogue puts its channel's sums into shared memory, token by token; then a warp takes a token at a time, four
+// neighbouring channels a lane, from every CTA of the cluster, which takes any alignment of the output.  (One channel a lane and
+// a 32-bit read per token and CTA: 256 x 4096 x 4096 36 us with its quantisation.)
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -17,6 +18,7 @@
 #include "matmul_scaled.hpp"
 #include "serving.hpp"
 #include "serving_device.cuh"
+#include "serving_wait.cuh"
 #include "tcgen05_common.cuh"
 #include "tcgen05_pair.cuh"
 
@@ -30,17 +32,24 @@ constexpr int kRoles = 2;      // warps in front of the epilogue's four: copies,
 
 template <int TN> struct TileShape {
     static constexpr int kStageBytes = (kChannels + TN) * BK;
-    static constexpr int kStages = TN == 16 ? 6 : TN == 32 ? 5 : TN == 64 ? 4 : 3;
+    static constexpr int kStages = TN == 16 ? 4 : 3;
     static constexpr size_t kSmem = size_t(kStages) * kStageBytes + 1024;
     static constexpr uint32_t kTmemCols = TN < 32 ? 32 : TN;
     static_assert(kStages * kStageBytes >= TN * kChannels * 4, "the partial sums fit the stages");
 };
 
-__device__ __forceinline__ int loadShared(uint32_t clusterAddr) {
-    int v;
-    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(clusterAddr) : "memory");
+// Barrier among the epilogue's four warps (named barrier 1).
+__device__ __forceinline__ void epilogueBarrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ int4 loadShared(uint32_t clusterAddr) {
+    int4 v;
+    asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(clusterAddr) : "memory");
     return v;
 }
+// Four neighbouring values of the output.
+__device__ __forceinline__ uint4 packFour(const float4 &y, float) {
+    return {__float_as_uint(y.x), __float_as_uint(y.y), __float_as_uint(y.z), __float_as_uint(y.w)};
+}
+template <class T> __device__ __forceinline__ uint2 packFour(const float4 &y, T) { return {packTwo(y.x, y.y, T()), packTwo(y.z, y.w, T())}; }
 
 template <int TN, class T>
 __global__ void __launch_bounds__((kRoles + 4) * 32)
@@ -51,6 +60,7 @@ matmulScaledTiles(const __grid_constant__ CUtensorMap mapW, const __grid_constan
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rawSmem) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t full[NST], empty[NST], accFull;
     __shared__ uint32_t tmemSlot;
+    __shared__ float tokenScales[TN];
     const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
     const int rank = split > 1 ? int(clusterCtaRank()) : 0;
     const int c0 = int(blockIdx.x) / split * kChannels, m0 = int(blockIdx.y) * TN;
@@ -80,7 +90,7 @@ matmulScaledTiles(const __grid_constant__ CUtensorMap mapW, const __grid_constan
             int s = 0;
             uint32_t phase = 0;
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbarWait(&empty[s], phase ^ 1u, 71)) {
+                if (!mbarPoll(&empty[s], phase ^ 1u, 71)) {
                     break;
                 }
                 uint8_t *to = smem + s * Shape::kStageBytes;
@@ -100,7 +110,7 @@ matmulScaledTiles(const __grid_constant__ CUtensorMap mapW, const __grid_constan
         int left = p.K - kb0 * BK;
         for (int kb = kb0; kb < kb1; ++kb) {
             if (ready == 0) {
-                failed = failed || !mbarWait(&full[s], phase, 72);
+                failed = failed || !mbarPoll(&full[s], phase, 72);
             }
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -113,52 +123,66 @@ matmulScaledTiles(const __grid_constant__ CUtensorMap mapW, const __grid_constan
         }
         ummaCommit(&accFull);
     } else {
-        const int quarter = warp & 3, channel = c0 + quarter * 32 + lane;
-        const bool live = channel < p.N;
-        const float scale = live ? p.bScales[channel] : 0.f, bias = live && p.biases != nullptr ? p.biases[channel] : 0.f;
-        const bool done = mbarWaitWarp(&accFull, 0u, 73);
+        for (int m = int(threadIdx.x) - kRoles * 32; m < TN; m += 128) {
+            tokenScales[m] = m0 + m < p.M ? p.aScales[m0 + m] : 0.f;
+        }
+        const int quarter = warp & 3;
+        const bool done = mbarPollWarp(&accFull, 0u, 73);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        int *part = reinterpret_cast<int *>(smem);
-        char *out = p.out + int64_t(channel) * int64_t(sizeof(T));
-#pragma unroll 1
+        int *part = reinterpret_cast<int *>(smem) + quarter * 32 + lane;
+#pragma unroll 2
         for (int col = 0; col < TN && done; col += 16) {
             uint32_t r[16];
             tmemLoad16(tmem + (uint32_t(quarter * 32) << 16) + uint32_t(col), r);
             tmemWait16(r);
-            if (split > 1) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    part[(col + j) * kChannels + quarter * 32 + lane] = int(r[j]);
+            for (int j = 0; j < 16; ++j) {
+                part[(col + j) * kChannels] = int(r[j]);
+            }
+        }
+        epilogueBarrier();
+    }
+    __syncwarp();
+    if (split > 1) {
+        clusterSync();
+    }
+    if (warp >= kRoles) { // tokens rank, rank + split, ... of the tile, a warp each in turn
+        const int channel = c0 + 4 * lane;
+        const float4 scale = fourOf(p.bScales, channel, p.N);
+        const float4 bias = p.biases != nullptr ? fourOf(p.biases, channel, p.N) : float4{};
+        const bool wide = channel + 4 <= p.N && (reinterpret_cast<uintptr_t>(p.out) | uintptr_t(p.outStride)) % (4 * sizeof(T)) == 0;
+        const uint32_t at = smemAddr(smem) + uint32_t(lane) * 16u;
+#pragma unroll 4
+        for (int m = rank + split * (warp - kRoles); m < TN; m += split * 4) {
+            if (m0 + m < p.M) {
+                int4 sum = {0, 0, 0, 0};
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    if (r < split) {
+                        const uint32_t from = at + uint32_t(m * kChannels * 4);
+                        const int4 v = loadShared(split > 1 ? mapToCta(from, uint32_t(r)) : from);
+                        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+                    }
                 }
-            } else {
+                const float token = tokenScales[m];
+                const float4 y = {float(sum.x) * token * scale.x + bias.x, float(sum.y) * token * scale.y + bias.y,
+                                  float(sum.z) * token * scale.z + bias.z, float(sum.w) * token * scale.w + bias.w};
+                T *out = reinterpret_cast<T *>(p.out + int64_t(m0 + m) * p.outStride) + channel;
+                if (wide) {
+                    *reinterpret_cast<decltype(packFour(y, T())) *>(out) = packFour(y, T());
+                } else {
+                    const float v[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int m = m0 + col + j;
-                    if (m < p.M && live) {
-                        *reinterpret_cast<T *>(out + int64_t(m) * p.outStride) = fromFloat<T>(float(int(r[j])) * p.aScales[m] * scale + bias);
+                    for (int j = 0; j < 4; ++j) {
+                        if (channel + j < p.N) {
+                            out[j] = fromFloat<T>(v[j]);
+                        }
                     }
                 }
             }
         }
     }
-    if (split > 1) { // every CTA adds up the tokens rank, rank + split, ...
-        __syncwarp();
-        clusterSync();
-        if (warp >= kRoles) {
-            const int quarter = warp & 3, channel = c0 + quarter * 32 + lane;
-            if (channel < p.N) {
-                const float scale = p.bScales[channel], bias = p.biases != nullptr ? p.biases[channel] : 0.f;
-                const uint32_t at = smemAddr(smem) + uint32_t(quarter * 32 + lane) * 4u;
-                for (int m = rank; m < TN && m0 + m < p.M; m += split) {
-                    int sum = 0;
-                    for (int r = 0; r < split; ++r) {
-                        sum += loadShared(mapToCta(at + uint32_t(m * kChannels * 4), uint32_t(r)));
-                    }
-                    *reinterpret_cast<T *>(p.out + int64_t(m0 + m) * p.outStride + int64_t(channel) * int64_t(sizeof(T))) =
-                        fromFloat<T>(float(sum) * p.aScales[m0 + m] * scale + bias);
-                }
-            }
-        }
+    if (split > 1) {
         __syncwarp();
         clusterSync(); // nobody leaves while its sums are being read
     }
@@ -213,10 +237,16 @@ int matmulScaledOnTiles(const ScaledProblem &p, int32_t dtype, cudaStream_t s) {
     const int width = p.M <= 16 ? 16 : p.M <= 32 ? 32 : p.M <= 64 ? 64 : 128;
     const int64_t tiles = int64_t((p.N + kChannels - 1) / kChannels) * ((p.M + width - 1) / width);
     const int allKb = (p.K + BK - 1) / BK;
-    // the sum is split while that gives CTAs that the SMs have room for, and leaves each four K blocks
+    // What a tile's sum is split into: as the SM with the most CTAs sees it, each CTA costs its K blocks and as much as three more
+    // for its start and end.  (56 x 8192 x 10240, 80 tiles of 64 K blocks: 28 us in 2 parts, see the table of the cases for 5.)
+    const int64_t sms = smCount(), resident = (width == 128 ? 2 : 3) * sms;
     int split = 1;
-    while (split < 8 && tiles * split * 2 <= int64_t(smCount()) * 2 && allKb >= split * 8) {
-        split *= 2;
+    int64_t best = 0;
+    for (int parts = 1; parts <= 8 && (parts == 1 || (parts * 4 <= allKb && tiles * parts <= resident)); ++parts) {
+        const int64_t cost = (tiles * parts + sms - 1) / sms * ((allKb + parts - 1) / parts + 3);
+        if (parts == 1 || cost < best) {
+            split = parts, best = cost;
+        }
     }
     switch (width) {
     case 16:

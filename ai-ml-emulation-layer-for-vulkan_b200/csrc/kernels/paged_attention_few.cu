@@ -43,6 +43,7 @@
 #include "paged_attention_device.cuh"
 #include "paged_attention_map.hpp"
 #include "serving_device.cuh"
+#include "serving_wait.cuh"
 #include "tcgen05_common.cuh"
 #include "tcgen05_pair.cuh"
 
@@ -354,7 +355,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                 nextSlots = slotOf(2 * n + 32 + lane);
             }
             if (n < issued) {
-                broken = !mbarWaitWarp(&full[warp][stage], phase, 61) || broken;
+                broken = !mbarPollWarp(&full[warp][stage], phase, 61) || broken;
             }
 #pragma unroll 1
             for (int h0 = 0; h0 < kStageGroups && !broken; h0 += AT) {

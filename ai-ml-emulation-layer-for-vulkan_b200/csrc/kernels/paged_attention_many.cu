@@ -32,6 +32,7 @@
 #include "paged_attention_device.cuh"
 #include "paged_attention_map.hpp"
 #include "serving_device.cuh"
+#include "serving_wait.cuh"
 #include "tcgen05_common.cuh"
 
 namespace mlel {
@@ -285,7 +286,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
 #pragma unroll 1
             for (int side = 0; side < 2; ++side, ++unit) {
                 const uint32_t buffer = unit % kStaging;
-                ok = ok && mbarWaitWarp(&bars.stagingEmpty[buffer], ((unit / kStaging) & 1u) ^ 1u, 91);
+                ok = ok && mbarPollWarp(&bars.stagingEmpty[buffer], ((unit / kStaging) & 1u) ^ 1u, 91);
                 if (!ok) {
                     break;
                 }
@@ -330,11 +331,11 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         constexpr uint32_t kQueryPanel = kRows * 128, kPanel = kKeys * 128, kPlace = uint32_t(Shape::kSlotBytes) >> 4; // bytes of 64 elements; units of 16
         const DescWords queryDesc = descWords(smemDesc(smemAddr(queries), 16, 1024)), keyDesc = descWords(smemDesc(smemAddr(slots), 16, 1024)),
                         valueDesc = descWords(smemDesc(smemAddr(slots), kPanel, 1024));
-        bool failed = !mbarWait(&bars.queries, 0u, 92);
+        bool failed = !mbarPoll(&bars.queries, 0u, 92);
         const auto scoreProduct = [&](int tile, int which) {
             const uint32_t unit = uint32_t(2 * tile), place = unit % kSlots;
             if (which == 0) {
-                failed = failed || !mbarWait(&bars.full[place], (unit / kSlots) & 1u, 93);
+                failed = failed || !mbarPoll(&bars.full[place], (unit / kSlots) & 1u, 93);
             }
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -352,9 +353,9 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const auto resultProduct = [&](int tile, int which) {
             const uint32_t unit = uint32_t(2 * tile + 1), place = unit % kSlots;
             if (which == 0) {
-                failed = failed || !mbarWait(&bars.full[place], (unit / kSlots) & 1u, 94);
+                failed = failed || !mbarPoll(&bars.full[place], (unit / kSlots) & 1u, 94);
             }
-            failed = failed || !mbarWait(&bars.weights[which], uint32_t(tile) & 1u, 95);
+            failed = failed || !mbarPoll(&bars.weights[which], uint32_t(tile) & 1u, 95);
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
@@ -393,8 +394,8 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const uint32_t low = toLane + uint32_t(((2 * part) ^ (row0 & 7)) << 4), high = toLane + uint32_t(((2 * part + 1) ^ (row0 & 7)) << 4);
         for (uint32_t unit = 0; unit < uint32_t(2 * tiles); ++unit) {
             const uint32_t buffer = unit % kStaging, place = unit % kSlots;
-            if (!mbarWaitWarp(&bars.stagingFull[buffer], (unit / kStaging) & 1u, 96) ||
-                !mbarWaitWarp(&bars.empty[place], ((unit / kSlots) & 1u) ^ 1u, 97)) {
+            if (!mbarPollWarp(&bars.stagingFull[buffer], (unit / kStaging) & 1u, 96) ||
+                !mbarPollWarp(&bars.empty[place], ((unit / kSlots) & 1u) ^ 1u, 97)) {
                 break;
             }
             const uint32_t from = fromLane + buffer * uint32_t(Shape::kStagingBytes), to = place * uint32_t(Shape::kSlotBytes);
@@ -518,8 +519,8 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             return CAP ? softCapped(x, p.softcap) * kLog2e : x;
         };
         for (int tile = 0; tile < tiles && ok; ++tile) {
-            ok = mbarWaitWarp(&bars.params[tile % kParamRing], uint32_t(tile / kParamRing) & 1u, 98) &&
-                 mbarWaitWarp(&bars.scores[which], uint32_t(tile) & 1u, 99);
+            ok = mbarPollWarp(&bars.params[tile % kParamRing], uint32_t(tile / kParamRing) & 1u, 98) &&
+                 mbarPollWarp(&bars.scores[which], uint32_t(tile) & 1u, 99);
             ok = pairVote(pairBarrier, !ok) == 0u; // a wait that ran out ends it for both warps of the rows
             if (!ok) {
                 break;
@@ -637,7 +638,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             }
         }
         // ---- the rows, by way of the queries' memory, which no product reads any more ----
-        ok = mbarWaitWarp(&bars.result[which], 0u, 90) && ok;
+        ok = mbarPollWarp(&bars.result[which], 0u, 90) && ok;
         exchange[which][tileRow][half] = sum;
         asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
         sum += exchange[which][tileRow][half ^ 1];

@@ -2,7 +2,8 @@
 // the even one, decided as exact arithmetic would (see roundedQuotient).
 //
 // What bounds it: memory.  A row is read once: its 16-byte vectors stay in registers between the maximum and the
-// rounding, four to a thread, and as many threads share a row as that takes (32 to 1024; longer rows are read again).
+// rounding, four to a thread, as they lie in memory (16-bit magnitudes are compared two at a time), and as many threads share a
+// row as that takes (32 to 1024; longer rows are read again).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -25,14 +26,84 @@ struct QuantizeParams {
     int32_t rows, length;
 };
 
-// The eight elements from `first` on; those behind the end of the row are zeros.
-template <class T, bool WIDE> __device__ __forceinline__ void loadEight(const T *row, int first, int length, float (&x)[8]) {
-    if (WIDE && first + 8 <= length) {
-        loadWide(row + first, x);
-    } else {
+// Eight elements as they lie in memory, and their largest magnitude as the bits of a float.
+template <class T> struct Eight {
+    uint4 w;
+    __device__ void clear() { w = {0u, 0u, 0u, 0u}; }
+    __device__ void load(const T *from) { w = *reinterpret_cast<const uint4 *>(from); }
+    __device__ void set(int j, T x) { reinterpret_cast<T *>(&w)[j] = x; }
+    __device__ void values(float (&x)[8]) const { unpackEight(w, x, T()); }
+    __device__ uint32_t most() const { // (magnitudes of 16 bits are ordered like their bits, as those of floats are)
+        const uint32_t m = maxHalves(maxHalves(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), maxHalves(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+        const uint32_t top = max(m & 0xffffu, m >> 16);
+        const float2 f = unpackTwo(top, T());
+        return __float_as_uint(f.x);
+    }
+};
+template <> struct Eight<float> {
+    float v[8];
+    __device__ void clear() {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            x[j] = first + j < length ? toFloat(row[first + j]) : 0.f;
+            v[j] = 0.f;
+        }
+    }
+    __device__ void load(const float *from) { loadWide(from, v); }
+    __device__ void set(int j, float x) { v[j] = x; }
+    __device__ void values(float (&x)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[j] = v[j];
+        }
+    }
+    __device__ uint32_t most() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+        }
+        return m;
+    }
+};
+
+// Where thread `at` of a team finds the elements of its vector v: eight neighbours from (v TEAM + at) 8 on, or, for rows at any
+// address, every TEAM-th from v 8 TEAM + at on, so that neighbouring threads read neighbouring elements.
+template <class T, int TEAM, bool WIDE> __device__ __forceinline__ void loadEight(const T *row, int v, int at, int length, Eight<T> &x) {
+    if (WIDE) {
+        const int first = (v * TEAM + at) * 8;
+        if (first + 8 <= length) {
+            x.load(row + first);
+        } else {
+            x.clear();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (first + j < length) {
+                    x.set(j, row[first + j]);
+                }
+            }
+        }
+    } else {
+        x.clear();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = (v * 8 + j) * TEAM + at;
+            if (i < length) {
+                x.set(j, row[i]);
+            }
+        }
+    }
+}
+template <int TEAM, bool WIDE> __device__ __forceinline__ void storeEight(int8_t *out, int v, int at, int length, uint2 packed) {
+    const int first = (v * TEAM + at) * 8;
+    if (WIDE && first + 8 <= length) {
+        *reinterpret_cast<uint2 *>(out + first) = packed;
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int i = WIDE ? first + j : (v * 8 + j) * TEAM + at;
+        if (i < length) {
+            out[i] = int8_t((j < 4 ? packed.x >> (8 * j) : packed.y >> (8 * (j - 4))) & 0xffu);
         }
     }
 }
@@ -46,24 +117,21 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) quantizeRowsKernel(co
     const int64_t rowIndex = int64_t(blockIdx.x) * kTeams + team;
     const bool live = rowIndex < p.rows;
     const T *row = reinterpret_cast<const T *>(p.in + (live ? rowIndex : 0) * p.inStride);
-    const int length = live ? p.length : 0;
-    float x[kHeld][8];
+    const int length = live ? p.length : 0, vectors = (length + 8 * TEAM - 1) / (8 * TEAM);
+    Eight<T> x[kHeld];
     uint32_t most = 0; // magnitudes as bits: an infinity is above every number and a NaN above that
 #pragma unroll
     for (int v = 0; v < kHeld; ++v) {
-        loadEight<T, WIDE>(row, (v * TEAM + at) * 8, length, x[v]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            most = max(most, __float_as_uint(x[v][j]) & 0x7fffffffu);
-        }
+        loadEight<T, TEAM, WIDE>(row, v, at, length, x[v]);
     }
-    for (int first = (kHeld * TEAM + at) * 8; first < length; first += TEAM * 8) {
-        float y[8];
-        loadEight<T, WIDE>(row, first, length, y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            most = max(most, __float_as_uint(y[j]) & 0x7fffffffu);
-        }
+    for (int v = 0; v < kHeld; ++v) {
+        most = max(most, x[v].most());
+    }
+    for (int v = kHeld; v < vectors; ++v) {
+        Eight<T> y;
+        loadEight<T, TEAM, WIDE>(row, v, at, length, y);
+        most = max(most, y.most());
     }
     most = __reduce_max_sync(0xffffffffu, most);
     if (TEAM > 32) {
@@ -86,30 +154,17 @@ __global__ void __launch_bounds__(TEAM < 256 ? 256 : TEAM) quantizeRowsKernel(co
         p.scales[rowIndex] = scale.value;
     }
     int8_t *out = p.out + rowIndex * p.outStride;
-    const auto store = [&](int first, const float (&y)[8]) {
-        if (first >= length) {
-            return;
-        }
-        const uint2 packed = quantizeEight(y, scale);
-        if (WIDE && first + 8 <= length) {
-            *reinterpret_cast<uint2 *>(out + first) = packed;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (first + j < length) {
-                    out[first + j] = int8_t((j < 4 ? packed.x >> (8 * j) : packed.y >> (8 * (j - 4))) & 0xffu);
-                }
-            }
-        }
-    };
+    float y[8];
 #pragma unroll
     for (int v = 0; v < kHeld; ++v) {
-        store((v * TEAM + at) * 8, x[v]);
+        x[v].values(y);
+        storeEight<TEAM, WIDE>(out, v, at, length, quantizeEight(y, scale));
     }
-    for (int first = (kHeld * TEAM + at) * 8; first < length; first += TEAM * 8) {
-        float y[8];
-        loadEight<T, WIDE>(row, first, length, y);
-        store(first, y);
+    for (int v = kHeld; v < vectors; ++v) {
+        Eight<T> z;
+        loadEight<T, TEAM, WIDE>(row, v, at, length, z);
+        z.values(y);
+        storeEight<TEAM, WIDE>(out, v, at, length, quantizeEight(y, scale));
     }
 }
 
