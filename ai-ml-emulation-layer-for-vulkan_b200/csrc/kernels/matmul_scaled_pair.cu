@@ -322,12 +322,16 @@ bool matmulScaledOnPairs(const ScaledProblem &p, int32_t dtype, cudaStream_t s, 
     if (!aligned(p.out, 16) || p.outStride % 16 != 0) {
         return false;
     }
-    const int64_t pairs = smCount() / 2, rows = (int64_t(p.M) + 255) / 256;
+    // Tiles of 256 or 128 channels, whichever ends sooner: rounds over the pairs, each K block 512 cycles or, bound by the bytes that
+    // arrive, some 300, an epilogue as much as two of them.
+    const int64_t pairs = smCount() / 2, rows = (int64_t(p.M) + 255) / 256, numKb = (p.K + BK - 1) / BK;
     const int64_t wide = rows * ((p.N + 255) / 256), narrow = rows * ((p.N + 127) / 128);
-    if (p.M <= 128 || narrow < pairs || wide > 0x7fffffff / 2) {
+    // Under a third of the pairs at work, or with rows for one CTA of each only, the tiles of single CTAs and parts of the sum are quicker.
+    if (p.M <= 128 || 3 * narrow < pairs || narrow > 0x7fffffff / 2) {
         return false;
     }
-    *rc = wide >= pairs ? launchPairType<256>(p, dtype, s) : launchPairType<128>(p, dtype, s);
+    const int64_t wideCost = (wide + pairs - 1) / pairs * (numKb + 2) * 512, narrowCost = (narrow + pairs - 1) / pairs * (numKb + 2) * 300;
+    *rc = wideCost <= narrowCost ? launchPairType<256>(p, dtype, s) : launchPairType<128>(p, dtype, s);
     return true;
 }
 

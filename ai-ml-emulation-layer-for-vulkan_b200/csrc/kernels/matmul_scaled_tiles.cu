@@ -4,7 +4,8 @@
 //
 // and for few tokens the sum over k split over the CTAs of a cluster, which add up their 32-bit integers through distributed
 // shared memory (whole numbers: the order does not matter).  With few tokens the weights' bytes bound the product: splitting puts
-// every SM to reading them, and two or three CTAs an SM (60 to 96 KB each) keep one reading while another starts or ends.
+// every SM to reading them.  What an SM reads at a time decides how fast that is: its CTAs, one to three, share some 200 KB of
+// stages (96 KB to a lone CTA of 512 x 4096 x 4096: 24 us, a K block every 1100 cycles).
 // A lane of the epilogue puts its channel's sums into shared memory, token by token; then a warp takes a token at a time, four
 // neighbouring channels a lane, from every CTA of the cluster, which takes any alignment of the output.  (One channel a lane and
 // a 32-bit read per token and CTA: 256 x 4096 x 4096 36 us with its quantisation.)
@@ -30,12 +31,12 @@ using namespace tc;
 constexpr int kChannels = 128; // of a tile
 constexpr int kRoles = 2;      // warps in front of the epilogue's four: copies, products
 
+constexpr int kMostStages = 8;
+
 template <int TN> struct TileShape {
     static constexpr int kStageBytes = (kChannels + TN) * BK;
-    static constexpr int kStages = TN == 16 ? 4 : 3;
-    static constexpr size_t kSmem = size_t(kStages) * kStageBytes + 1024;
+    static constexpr int kLeastStages = (TN * kChannels * 4 + kStageBytes - 1) / kStageBytes; // hold the partial sums at the end
     static constexpr uint32_t kTmemCols = TN < 32 ? 32 : TN;
-    static_assert(kStages * kStageBytes >= TN * kChannels * 4, "the partial sums fit the stages");
 };
 
 // Barrier among the epilogue's four warps (named barrier 1).
@@ -53,12 +54,12 @@ template <class T> __device__ __forceinline__ uint2 packFour(const float4 &y, T)
 
 template <int TN, class T>
 __global__ void __launch_bounds__((kRoles + 4) * 32)
-matmulScaledTiles(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const ScaledProblem p, const int split) {
+matmulScaledTiles(const __grid_constant__ CUtensorMap mapW, const __grid_constant__ CUtensorMap mapX, const ScaledProblem p, const int split,
+                  const int stages) {
     using Shape = TileShape<TN>;
-    constexpr int NST = Shape::kStages;
     extern __shared__ uint8_t rawSmem[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rawSmem) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t full[NST], empty[NST], accFull;
+    __shared__ uint64_t full[kMostStages], empty[kMostStages], accFull;
     __shared__ uint32_t tmemSlot;
     __shared__ float tokenScales[TN];
     const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
@@ -66,7 +67,7 @@ matmulScaledTiles(const __grid_constant__ CUtensorMap mapW, const __grid_constan
     const int c0 = int(blockIdx.x) / split * kChannels, m0 = int(blockIdx.y) * TN;
     const int allKb = (p.K + BK - 1) / BK, kb0 = int(int64_t(allKb) * rank / split), kb1 = int(int64_t(allKb) * (rank + 1) / split);
     if (threadIdx.x == 0) {
-        for (int s = 0; s < NST; ++s) {
+        for (int s = 0; s < stages; ++s) {
             mbarInit(&full[s], 1u);
             mbarInit(&empty[s], 1u);
         }
@@ -97,7 +98,7 @@ matmulScaledTiles(const __grid_constant__ CUtensorMap mapW, const __grid_constan
                 mbarArriveExpectTx(&full[s], uint32_t(Shape::kStageBytes));
                 tmaLoad3d(&mapW, to, &full[s], kb * BK, c0, 0);
                 tmaLoad3d(&mapX, to + kChannels * BK, &full[s], kb * BK, m0, 0);
-                s = s + 1 == NST ? 0 : s + 1;
+                s = s + 1 == stages ? 0 : s + 1;
                 phase ^= s == 0 ? 1u : 0u;
             }
         }
@@ -114,7 +115,7 @@ matmulScaledTiles(const __grid_constant__ CUtensorMap mapW, const __grid_constan
             }
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t next = s + 1 == uint32_t(NST) ? 0u : s + 1, nextPhase = next == 0 ? phase ^ 1u : phase;
+            const uint32_t next = s + 1 == uint32_t(stages) ? 0u : s + 1, nextPhase = next == 0 ? phase ^ 1u : phase;
             const uint32_t step = s * uint32_t(Shape::kStageBytes >> 4);
             ready = ummaBlockPeek(tmem, {w0.low + step, w0.high}, UMMA_K >> 4, {x0.low + step, x0.high}, UMMA_K >> 4, idesc,
                                   kb != kb0 ? 1u : 0u, ummaCountFor(left), &empty[s], &full[next], nextPhase);
@@ -202,13 +203,19 @@ template <int TN, class T> int launchTiles(const ScaledProblem &p, int split, cu
         return MLEL_ERROR_DEVICE;
     }
     const auto kernel = matmulScaledTiles<TN, T>;
-    if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), Shape::kSmem)) {
+    // CTAs that an SM gets, and the stages that each has room for
+    const int64_t ctas = int64_t((p.N + kChannels - 1) / kChannels) * split * ((p.M + TN - 1) / TN);
+    const int perSm = ctas <= smCount() ? 1 : ctas <= 2 * int64_t(smCount()) || TN == 128 ? 2 : 3;
+    const int ownKb = ((p.K + BK - 1) / BK + split - 1) / split;
+    const int stages = std::max(Shape::kLeastStages, std::min({kMostStages, 200 * 1024 / perSm / Shape::kStageBytes, std::max(2, ownKb)}));
+    const size_t smemBytes = size_t(stages) * Shape::kStageBytes + 1024;
+    if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), size_t(std::min(kMostStages, 200 * 1024 / Shape::kStageBytes)) * Shape::kStageBytes + 1024)) {
         return MLEL_ERROR_DEVICE;
     }
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned((p.N + kChannels - 1) / kChannels * split), unsigned((p.M + TN - 1) / TN));
     cfg.blockDim = dim3((kRoles + 4) * 32);
-    cfg.dynamicSmemBytes = Shape::kSmem;
+    cfg.dynamicSmemBytes = smemBytes;
     cfg.stream = s;
     cudaLaunchAttribute attrs[2]{};
     int count = 0;
@@ -222,7 +229,7 @@ template <int TN, class T> int launchTiles(const ScaledProblem &p, int split, cu
     }
     cfg.attrs = attrs;
     cfg.numAttrs = unsigned(count);
-    return launchStatus("mlel_cuda_matmul_scaled", cudaLaunchKernelEx(&cfg, kernel, w, x, p, split));
+    return launchStatus("mlel_cuda_matmul_scaled", cudaLaunchKernelEx(&cfg, kernel, w, x, p, split, stages));
 }
 
 template <int TN> int launchTilesType(const ScaledProblem &p, int32_t dtype, int split, cudaStream_t s) {
