@@ -3,7 +3,7 @@
 //   o = sum_j softmax(s)_j v_j,  s_j = scale * q . k_j (capped or not), over the tokens that the masks leave
 //
 // What bounds it: the bytes of the cache, and close behind them the instructions that turn them into operands.  Every key and
-// value is read once per tile of 8, 16 or 32 rows (a row is one token's query head; the heads that share a cache head are rows of
+// value is read once per tile of 8 or 16 rows (a row is one token's query head; the heads that share a cache head are rows of
 // one tile).  At 6.5 TB/s an SM gets some 23 bytes a cycle, 16 keys and values of 128 elements every 180 cycles.
 //
 // Work.  All tiles' keys, in steps of 128, form one line that is cut into as many equal pieces as there are blocks, whatever the
@@ -760,10 +760,7 @@ template <int DP> int launchFewRows(const AttendParams &p, const FewPlan &plan, 
     if (plan.rows == 8) {
         return p.halves ? launchFew<DP, 1, true>(p, plan, s) : launchFew<DP, 1, false>(p, plan, s);
     }
-    if (DP == 256 || plan.rows == 16) {
-        return p.halves ? launchFew<DP, 2, true>(p, plan, s) : launchFew<DP, 2, false>(p, plan, s);
-    }
-    return p.halves ? launchFew<(DP < 256 ? DP : 128), 4, true>(p, plan, s) : launchFew<(DP < 256 ? DP : 128), 4, false>(p, plan, s);
+    return p.halves ? launchFew<DP, 2, true>(p, plan, s) : launchFew<DP, 2, false>(p, plan, s);
 }
 
 } // namespace
@@ -772,7 +769,7 @@ FewPlan pagedAttentionFewPlan(const AttendParams &p) {
     FewPlan plan{};
     const int dp = paddedHead(p.cache.headDim);
     const int64_t rows = int64_t(p.batch.maxNew) * p.group;
-    plan.rows = rows <= 8 ? 8 : rows <= 16 || dp == 256 ? 16 : 32;
+    plan.rows = rows <= 8 ? 8 : kFewRows;
     // the most tiles and steps that the batch can have
     const int64_t steps = (int64_t(p.batch.maxLength) + kGroup * kStepGroups - 1) / (kGroup * kStepGroups);
     const int64_t tiles = (rows + plan.rows - 1) / plan.rows * p.cache.heads * p.batch.sequences, work = steps * tiles;

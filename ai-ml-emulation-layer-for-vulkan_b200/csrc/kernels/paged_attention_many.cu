@@ -34,6 +34,7 @@
 #include "serving_device.cuh"
 #include "serving_wait.cuh"
 #include "tcgen05_common.cuh"
+#include "tcgen05_pair.cuh"
 
 namespace mlel {
 namespace {
@@ -182,11 +183,14 @@ __device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st
 template <int DP, bool HALF, bool CAP>
 __global__ void __launch_bounds__(ManyShape<DP>::kThreads, 1)
 pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p,
-                         const FastDiv heads, const int levels, const int boxRows) {
+                         const FastDiv heads, const int levels, const int boxRows, const int split) {
     using Shape = ManyShape<DP>;
     constexpr int kKeys = Shape::kKeys, kGroups = Shape::kGroups, kHalfGroups = Shape::kHalfGroups, kTileWarps = Shape::kTileWarps,
                   kSoftmaxWarps = Shape::kSoftmaxWarps, kCopyWarp = Shape::kCopyWarp, kProductWarp = Shape::kProductWarp,
                   kBlockRows = Shape::kTilesOfRows * kRows;
+    constexpr int kPitch = DP + 4; // floats between the rows of a part
+    static_assert(size_t(kBlockRows) * kPitch * 4 <= Shape::kTilesOfRows * size_t(Shape::kQueryBytes) + kSlots * size_t(Shape::kSlotBytes),
+                  "the parts of the rows fit the queries' and keys' memory");
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     extern __shared__ __align__(1024) uint8_t rawSmem[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rawSmem) + 1023) & ~uintptr_t(1023));
@@ -206,11 +210,12 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     dependencySync();
 
     // blocks: the tiles that see the most keys first
-    const uint32_t overHeads = fastDiv(blockIdx.x, heads);
-    const int head = int(blockIdx.x - overHeads * heads.d), level = int(overHeads / uint32_t(p.batch.sequences)),
+    const uint32_t item = split > 1 ? blockIdx.x / uint32_t(split) : blockIdx.x, overHeads = fastDiv(item, heads);
+    const int head = int(item - overHeads * heads.d), level = int(overHeads / uint32_t(p.batch.sequences)),
               index = int(overHeads - uint32_t(level) * uint32_t(p.batch.sequences));
     const Sequence q = sequenceOf(p.batch, index);
-    if (!q.sound && level == 0 && head == 0 && threadIdx.x == 0) {
+    const int rank = split > 1 ? int(clusterCtaRank()) : 0;
+    if (!q.sound && level == 0 && head == 0 && rank == 0 && threadIdx.x == 0) {
         atomicCAS(&g_pagedError, 0, kBadSequence);
     }
     const int allRows = q.sound ? q.fresh * p.group : 0, firstRow = (levels - 1 - level) * kBlockRows;
@@ -219,9 +224,11 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     }
     const int rows = min(kBlockRows, allRows - firstRow), old = q.length - q.fresh;
     const int firstToken = int(fastDiv(uint32_t(firstRow), p.groupDiv)), lastToken = int(fastDiv(uint32_t(firstRow + rows - 1), p.groupDiv));
-    const int keyLo = (p.window > 0 ? max(0, old + firstToken - p.window + 1) : 0) / boxRows * boxRows;
-    const int keyHi = p.causal ? old + lastToken + 1 : q.length;
-    const int tiles = (keyHi - keyLo + kKeys - 1) / kKeys;
+    // the keys that any row sees, and of those this block's part: whole tiles
+    const int allLo = (p.window > 0 ? max(0, old + firstToken - p.window + 1) : 0) / boxRows * boxRows;
+    const int allHi = p.causal ? old + lastToken + 1 : q.length, allTiles = (allHi - allLo + kKeys - 1) / kKeys;
+    const int firstTile = split > 1 ? int(int64_t(allTiles) * rank / split) : 0, endTile = split > 1 ? int(int64_t(allTiles) * (rank + 1) / split) : allTiles;
+    const int keyLo = allLo + firstTile * kKeys, keyHi = min(allHi, allLo + endTile * kKeys), tiles = endTile - firstTile;
     const int32_t *table = p.batch.table + index * p.batch.tableStride;
     const int active = rows > kRows ? 2 : 1; // tiles with rows
 
@@ -370,7 +377,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 ummaCommit(&bars.empty[place]);
             }
         };
-        for (int which = 0; which < active; ++which) {
+        for (int which = 0; which < active && tiles > 0; ++which) {
             scoreProduct(0, which);
         }
         for (int tile = 0; tile < tiles; ++tile) {
@@ -637,13 +644,33 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 mbarArrive(&bars.weights[which]);
             }
         }
-        // ---- the rows, by way of the queries' memory, which no product reads any more ----
-        ok = mbarPollWarp(&bars.result[which], 0u, 90) && ok;
+        ok = (tiles == 0 || mbarPollWarp(&bars.result[which], 0u, 90)) && ok;
         exchange[which][tileRow][half] = sum;
         asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
         sum += exchange[which][tileRow][half ^ 1];
-        if (ok) {
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (split > 1) {
+            // ---- parts of the rows, over the queries and keys, which no product of either tile reads any more ----
+            asm volatile("bar.sync 9, %0;" ::"r"(active * kTileWarps * 32) : "memory");
+            float *part = reinterpret_cast<float *>(smem) + (which * kRows + tileRow) * kPitch;
+            const float unit = exp2f(float(reference) - kWeightBits);
+#pragma unroll 1
+            for (int d = 0; d < DP / 2; d += 16) {
+                uint32_t o[16] = {};
+                if (tiles > 0) {
+                    tmemLoad16(resultAt + uint32_t(d), o);
+                    tmemWait16(o);
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    *reinterpret_cast<float4 *>(part + half * (DP / 2) + d + j) = {__uint_as_float(o[j]) * unit, __uint_as_float(o[j + 1]) * unit,
+                                                                                   __uint_as_float(o[j + 2]) * unit, __uint_as_float(o[j + 3]) * unit};
+                }
+            }
+            if (half == 0) {
+                part[DP] = most, part[DP + 1] = sum;
+            }
+        } else if (ok) { // ---- the rows, by way of the queries' memory, which no product reads any more ----
             const float f = sum == 0.f ? 0.f : exp2f(float(reference) - kWeightBits) / sum;
             uint8_t *mine = queries + which * Shape::kQueryBytes + (quarter * 2 + half) * (32 * DP);
             constexpr int kChunks = DP / 16, kLinesAtOnce = 32 / kChunks; // 16-byte chunks of half a row
@@ -686,6 +713,27 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             }
         }
     }
+    if (split > 1) { // the cluster's parts as one, four elements of a row a thread
+        __syncwarp();
+        clusterSync();
+        const uint32_t from = smemAddr(smem);
+        for (int i = int(threadIdx.x) + rank * Shape::kThreads; i < rows * (DP / 4); i += split * Shape::kThreads) {
+            const int r = i / (DP / 4), d = (i - r * (DP / 4)) * 4;
+            float top = -INFINITY, weights = 0.f;
+            float4 y = {};
+            for (int other = 0; other < split; ++other) { // one pass with a running maximum, as over keys
+                const float4 stats = loadCluster(mapToCta(from + uint32_t((r * kPitch + DP) * 4), uint32_t(other)));
+                const float4 a = loadCluster(mapToCta(from + uint32_t((r * kPitch + d) * 4), uint32_t(other)));
+                const float now = fmaxf(top, stats.x);
+                const float keep = now == -INFINITY ? 1.f : exp2Fast(top - now), factor = now == -INFINITY ? 1.f : exp2Fast(stats.x - now);
+                top = now, weights = weights * keep + stats.y * factor;
+                y.x = y.x * keep + a.x * factor, y.y = y.y * keep + a.y * factor, y.z = y.z * keep + a.z * factor, y.w = y.w * keep + a.w * factor;
+            }
+            writeOut<T>(p, q.first, firstRow + r, head, d, y, weights);
+        }
+        __syncwarp();
+        clusterSync(); // nobody leaves while its parts are being read
+    }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == kProductWarp) {
@@ -711,12 +759,37 @@ template <int DP, bool HALF, bool CAP> int launchMany(const AttendParams &p, cud
     if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), smemBytes)) {
         return MLEL_ERROR_DEVICE;
     }
-    const int64_t levels = (int64_t(p.batch.maxNew) * p.group + Shape::kTilesOfRows * kRows - 1) / (Shape::kTilesOfRows * kRows), blocks = levels * p.cache.heads * p.batch.sequences;
+    const int64_t levels = (int64_t(p.batch.maxNew) * p.group + Shape::kTilesOfRows * kRows - 1) / (Shape::kTilesOfRows * kRows);
+    const int64_t blocks = levels * p.cache.heads * p.batch.sequences;
     if (blocks > 0x7fffffff) {
         refuse("mlel_cuda_paged_attention", "too many tokens and sequences for one call");
     }
-    return launchStatus("mlel_cuda_paged_attention", launchOverlapped(kernel, dim3(unsigned(blocks)), Shape::kThreads, smemBytes, s, k, v, p,
-                                                                      makeFastDiv(p.cache.heads), int(levels), boxRows));
+    // Few blocks with many keys each share them in clusters (one sequence, 128 new tokens of 16000, 16 blocks: 323 us, in parts of
+    // eight 117), as long as a part keeps four tiles or so of the longest sequence.
+    const int64_t keys = p.window > 0 ? std::min<int64_t>(p.batch.maxLength, int64_t(p.window) + p.batch.maxNew) : p.batch.maxLength;
+    int split = 1;
+    while (split < 8 && blocks * split * 2 <= smCount() && keys >= int64_t(split) * 2 * 4 * Shape::kKeys) {
+        split *= 2;
+    }
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(blocks * split));
+    cfg.blockDim = dim3(Shape::kThreads);
+    cfg.dynamicSmemBytes = smemBytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attrs[2]{};
+    int count = 0;
+    if (dependentLaunches()) {
+        attrs[count].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[count++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (split > 1) {
+        attrs[count].id = cudaLaunchAttributeClusterDimension;
+        attrs[count].val.clusterDim.x = unsigned(split), attrs[count].val.clusterDim.y = 1, attrs[count++].val.clusterDim.z = 1;
+    }
+    cfg.attrs = attrs;
+    cfg.numAttrs = unsigned(count);
+    return launchStatus("mlel_cuda_paged_attention",
+                        cudaLaunchKernelEx(&cfg, kernel, k, v, p, makeFastDiv(p.cache.heads), int(levels), boxRows, split));
 }
 
 template <int DP> int launchManyType(const AttendParams &p, cudaStream_t s) {
@@ -728,9 +801,10 @@ template <int DP> int launchManyType(const AttendParams &p, cudaStream_t s) {
 
 } // namespace
 
-bool pagedAttentionManyApplies(const AttendParams &p) {
-    return int64_t(p.batch.maxNew) * p.group > 64;
-}
+// More rows per cache head than one tile of the kernel for few of them has.  (That kernel with tiles of 32 rows, 16 sequences of up to
+// 4000 tokens, 8 heads of 128 elements: 20 rows 83 us and here 75, 32 rows 88 and 76, 64 rows 120 and 76; one of 16000, 32 rows: 45
+// and 45.)
+bool pagedAttentionManyApplies(const AttendParams &p) { return int64_t(p.batch.maxNew) * p.group > kFewRows; }
 int pagedAttentionMany(const AttendParams &p, cudaStream_t s) {
     return p.cache.headDim <= 64 ? launchManyType<64>(p, s) : p.cache.headDim <= 128 ? launchManyType<128>(p, s) : launchManyType<256>(p, s);
 }

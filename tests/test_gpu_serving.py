@@ -389,6 +389,15 @@ def test_attention_long(serving, fresh, length, heads, group, d, page):
     check_attention(serving, p, *query(p, heads * group, torch.bfloat16), torch.bfloat16)
 
 
+@pytest.mark.parametrize("how", [{}, {"window": 700}, {"softcap": 5.0}, {"causal": False}], ids=str)
+@pytest.mark.parametrize("sequences, heads, group, d, page", [([(70, 5000)], 1, 1, 128, 64), ([(40, 3000), (33, 40), (0, 9), (1, 2500)], 1, 2, 64, 16),
+                                                              ([(300, 2600)], 2, 1, 96, 48), ([(20, 4100)], 1, 4, 256, 32)])
+def test_attention_chunks_of_long_sequences(serving, sequences, heads, group, d, page, how):
+    """Few tiles of rows over many keys, which blocks share, some sequences with fewer keys than there are shares."""
+    p = Paged(serving, d + page, sequences, heads, page, d, behind=1)
+    check_attention(serving, p, *query(p, heads * group, torch.float16), torch.float16, **how)
+
+
 @pytest.mark.parametrize("sequences", [[(1, 300)], [(100, 300)]], ids=["one", "chunk"])
 def test_attention_one_key_has_all(serving, sequences):
     """A score that drowns all others: the answer is that token's value; and thousands of others share what is left."""
