@@ -749,7 +749,7 @@ template <int DP, int NQ, bool HALF> int launchFew(const AttendParams &p, const 
     cfg.numAttrs = unsigned(count);
     cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, k, v, p, plan.split);
     if (err == cudaSuccess && plan.workspace > 0) {
-        const int64_t rows = int64_t(p.batch.maxNew) * p.group, tiles = (rows + 8 * NQ - 1) / (8 * NQ) * p.cache.heads;
+        const int64_t rows = std::max<int64_t>(1, int64_t(p.batch.maxNew) * p.group), tiles = (rows + 8 * NQ - 1) / (8 * NQ) * p.cache.heads;
         err = launchOverlapped(pagedAttentionFewJoin<DP, NQ, HALF>,
                                dim3(unsigned(tiles * p.batch.sequences), unsigned(std::min<int64_t>(rows, 8 * NQ))), kWarps * 32, 0, s, p, plan.blocks);
     }
@@ -768,10 +768,10 @@ template <int DP> int launchFewRows(const AttendParams &p, const FewPlan &plan, 
 FewPlan pagedAttentionFewPlan(const AttendParams &p) {
     FewPlan plan{};
     const int dp = paddedHead(p.cache.headDim);
-    const int64_t rows = int64_t(p.batch.maxNew) * p.group;
+    const int64_t rows = std::max<int64_t>(1, int64_t(p.batch.maxNew) * p.group); // (without new tokens the sequences are looked at all the same)
     plan.rows = rows <= 8 ? 8 : kFewRows;
     // the most tiles and steps that the batch can have
-    const int64_t steps = (int64_t(p.batch.maxLength) + kGroup * kStepGroups - 1) / (kGroup * kStepGroups);
+    const int64_t steps = std::max<int64_t>(1, (int64_t(p.batch.maxLength) + kGroup * kStepGroups - 1) / (kGroup * kStepGroups));
     const int64_t tiles = (rows + plan.rows - 1) / plan.rows * p.cache.heads * p.batch.sequences, work = steps * tiles;
     if (work > 0x7fffffff) {
         refuse("mlel_cuda_paged_attention", "sequences, tokens and lengths give too much work for one call");

@@ -485,7 +485,7 @@ typedef struct mlel_paged_batch {
  * be the same tensor.  cosines and sines NULL: no rotation.
  * A page's scale is max |element| / 127 over what is in it.  Where new tokens join older ones in a page and have larger
  * elements, its older integers are rescaled once, to the nearest whole numbers.  A page whose first row is new starts afresh.
- * New tokens with an infinity or a NaN make the page's scale that, and with it all that reads the page NaN.
+ * New tokens with an infinity or a NaN make the page's scale that, and with it all that attends to the page no number either.
  * A page that receives tokens belongs to one sequence; pages that are only read may be shared. */
 int mlel_cuda_paged_append(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *keys,
                            const mlel_tensor *values, const mlel_tensor *cosines, const mlel_tensor *sines,

@@ -550,6 +550,80 @@ def test_capture_replay_and_other_streams(serving):
         assert torch.equal(layer(), replayed)
 
 
+def test_capture_with_a_workspace(serving):
+    """Two captured graphs of one long sequence each, whose parts lie in a workspace, replayed in turn and from two streams."""
+    jobs = []
+    for seed in (31, 32):
+        p = Paged(serving, seed, [(1, 20000), (1, 30)], 2, 64, 128)
+        q = query(p, 8, torch.bfloat16)[0]
+        want = p.cache.attend(q, p.batch)
+        graph = torch.cuda.CUDAGraph()
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            held = p.cache.attend(q, p.batch)
+        jobs.append((graph, stream, want, held, p, q))
+    assert any(v > 0 for v in jobs[0][4].batch._space.values()), "the case is meant to want a workspace"
+    for _ in range(3):
+        for graph, stream, *_ in jobs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, want, held, *_ in jobs:
+        assert torch.equal(want, held)
+
+
+def test_ordinary_launches_give_the_same(mlel, serving):
+    """Without programmatic dependent launches."""
+    lib = mlel.lib()
+    p = Paged(serving, 41, [(1, 900), (1, 20000)], 2, 16, 64, wild=False)
+    many = Paged(serving, 42, [(90, 400)], 2, 32, 128, wild=False)
+    x = randn(gen(1), 40, 512).bfloat16()
+    linear = serving.QuantizedLinear(torch.randint(-127, 128, (700, 512), generator=p.g, device="cuda", dtype=torch.int8), torch.ones(700, device="cuda"))
+    q, q2 = query(p, 4, torch.float16)[0], query(many, 4, torch.float16)[0]
+    got = []
+    try:
+        for value in (1, 0):
+            assert lib.mlel_set_tuning(b"dependent_launch", value) == 0
+            got.append((linear(x), p.cache.attend(q, p.batch), many.cache.attend(q2, many.batch)))
+    finally:
+        assert lib.mlel_set_tuning(b"dependent_launch", 1) == 0
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_nothing_to_do(serving):
+    """No tokens, no sequences, sequences without new tokens."""
+    linear = serving.QuantizedLinear(torch.zeros(5, 33, dtype=torch.int8, device="cuda"), torch.ones(5, device="cuda"))
+    assert linear(torch.zeros(0, 33, device="cuda")).shape == (0, 5)
+    q, s = serving.quantize_rows(torch.zeros(0, 7, device="cuda"))
+    assert q.shape == (0, 7) and s.shape == (0,)
+    for sequences in ([], [(0, 20), (0, 0)]):
+        p = Paged(serving, 1, sequences, 1, 16, 16, behind=2)
+        x, out = query(p, 2, torch.float16)
+        before = p.data.clone()
+        p.cache.attend(x, p.batch, out=out)
+        p.cache.append(x[:, :1].contiguous(), x[:, :1].contiguous(), None, None, p.batch)
+        assert (out == 77).all() and torch.equal(p.data, before)
+
+
+def test_page_table_of_a_larger_program(serving):
+    """Rows of the page table apart from one another, lengths far below their bound, as a program's own tables have them."""
+    p = Paged(serving, 51, [(1, 100), (3, 300), (1, 40)], 2, 16, 64)
+    q, out = query(p, 4, torch.float16)
+    check_attention(serving, p, q, out, torch.float16)
+    wide = torch.full((3, 1000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :p.batch.page_table.shape[1]] = p.batch.page_table
+    for bound in (1000 * 16, 600 * 16):
+        other = serving.PagedBatch(p.batch.starts, p.batch.lengths, wide[:, :bound // 16], 7, bound)
+        again = torch.full_like(out, 77.0)
+        p.cache.attend(q, other, out=again)
+        # another division of the keys: the same up to a rounding of the result
+        assert ((again.float() - out.float()).abs() <= 2.0 ** -10 * out.float().abs() + 2.0 ** -9 * out.float().abs().amax()).all()
+    wide_rows = serving.PagedBatch(p.batch.starts, p.batch.lengths, wide, 40, 16000)  # the kernel for many rows
+    p.cache.attend(q, wide_rows, out=again)
+    assert ((again.float() - out.float()).abs() <= 2.0 ** -10 * out.float().abs() + 2.0 ** -9 * out.float().abs().amax()).all()
+
+
 def test_two_streams_at_once(serving):
     """Calls that run beside one another share nothing: the same results as one after another."""
     jobs = []
