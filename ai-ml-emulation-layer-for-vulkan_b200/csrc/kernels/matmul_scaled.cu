@@ -124,8 +124,9 @@ ScaledProblem scaledProblemOf(const std::string &call, const mlel_tensor *a, con
     return p;
 }
 
+// Tensor maps describe rows on 16-byte boundaries that do not overlap; others go the way of any rows.
 int launchScaled(const std::string &call, const ScaledProblem &p, int32_t dtype, cudaStream_t s) {
-    if (aligned(p.a, 16) && p.aStride % 16 == 0 && aligned(p.b, 16) && p.bStride % 16 == 0) {
+    if (p.aStride >= p.K && p.bStride >= p.K && aligned(p.a, 16) && p.aStride % 16 == 0 && aligned(p.b, 16) && p.bStride % 16 == 0) {
         int rc = MLEL_SUCCESS;
         return matmulScaledOnPairs(p, dtype, s, &rc) ? rc : matmulScaledOnTiles(p, dtype, s);
     }

@@ -207,6 +207,9 @@ int quantizeRows(const mlel_tensor *input, const mlel_tensor *output, const mlel
     if (in.dims[1] == 0) {
         refuse(call, "rows without elements have no scale");
     }
+    if (in.dims[1] > (1 << 30)) {
+        refuse(call, "rows of more than 2^30 elements");
+    }
     wantCurrentDevice(call, "output", out.ptr);
     const QuantizeParams p{in.ptr, reinterpret_cast<int8_t *>(out.ptr), reinterpret_cast<float *>(sc.ptr), in.strides[0], out.strides[0],
                            int32_t(in.dims[0]), int32_t(in.dims[1])};

@@ -3,7 +3,7 @@ paged int8 cache (``PagedCache``, ``PagedBatch``) with its attention.
 
 Thin calls of the direct entry points in include/mlel_b200.h (``mlel_cuda_quantize_rows`` and the following), which say what
 each computes.  Work is enqueued on torch's current stream of the tensors' device; nothing waits.  Every call may be captured
-into a CUDA graph.  What the library refuses raises ``MlelError``.
+into a CUDA graph.  What the library refuses raises ``MlelError``.  They are for inference: results carry no gradients.
 
 A decode step's kernels take a few microseconds each, so the way to them is kept short: objects that a program keeps
 (weights, a cache, a batch) hold their descriptions ready, a call describes its own tensors and enters the library once.
@@ -118,10 +118,20 @@ def matmul_scaled(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_sc
     return out
 
 
-class QuantizedLinear:
+class _Described:
+    """What is described to the library once: an attribute that has been set is not set again (a new tensor is a new object)."""
+
+    def __setattr__(self, name, value):
+        if name in self.__dict__:
+            raise AttributeError(f"{name} is described to the library already: make a new {type(self).__name__}")
+        super().__setattr__(name, value)
+
+
+class QuantizedLinear(_Described):
     """A projection in 8 bits: ``linear(x)`` quantises the rows of ``x`` [..., K] and multiplies them with int8 ``weight`` [N, K],
     one f32 scale per output channel, optional f32 bias; the result has ``x``'s type.  The weights are laid out once: rows on
-    16-byte boundaries (copied only where they are not there already).  Their values may change between calls, their tensors not."""
+    16-byte boundaries, copied where they are not there already.  Calls use ``linear.weight``, ``scales`` and ``bias``, whose values may
+    change between them; the attributes themselves stay."""
 
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None):
         self.device = _device(weight, scales, bias)
@@ -151,10 +161,10 @@ class QuantizedLinear:
         return y if len(shape) == 2 else y.view(*shape[:-1], self.out_features)
 
 
-class PagedBatch:
+class PagedBatch(_Described):
     """The sequences of one call: new tokens of sequence b are rows ``starts[b]`` to ``starts[b + 1] - 1`` of the token axis and the last
     of its ``lengths[b]`` tokens; token t lies in page ``page_table[b, t // page]``.  All int32 on the device, read when the kernels
-    run; ``max_new`` and ``max_length`` are bounds that the host knows."""
+    run (a decode loop or a captured graph changes their values in place); ``max_new`` and ``max_length`` are bounds that the host knows."""
 
     def __init__(self, starts: torch.Tensor, lengths: torch.Tensor, page_table: torch.Tensor, max_new: int, max_length: int):
         self.device = _device(starts, lengths, page_table)
@@ -164,7 +174,7 @@ class PagedBatch:
         self._space = {}  # bytes of workspace by the sizes that decide them
 
 
-class PagedCache:
+class PagedCache(_Described):
     """Keys and values of a layer, int8 with a scale for each page and head.  ``data`` [2, pages, heads, page, head_dim] and
     ``scales`` f32 [2, pages, heads]: keys first, then values."""
 

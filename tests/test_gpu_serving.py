@@ -151,6 +151,16 @@ def test_matmul_scaled_strided(serving, m, n, k, a_off, b_off, out_off):
     assert (store[mask] == 77).all()
 
 
+@pytest.mark.parametrize("m, n", [(5, 200), (700, 900)])
+def test_matmul_scaled_rows_that_overlap(serving, m, n):
+    """Windows over one row of tokens, or of weights, 16 apart."""
+    g = gen(m)
+    line = torch.randint(-128, 128, (16 * 1000 + 96,), generator=g, device="cuda", dtype=torch.int8)
+    a, sa, b, sb, bias = product_operands(m, m, n, 96, True)
+    check_product(serving, (line.as_strided((m, 96), (16, 1)), sa, b, sb, bias), torch.float32)
+    check_product(serving, (a, sa, line.as_strided((n, 96), (16, 1)), sb, bias), torch.float32)
+
+
 def test_matmul_scaled_scales_that_are_not_finite(serving):
     a, sa, b, sb, _ = product_operands(5, 40, 150, 64, False)
     sa[3], sa[7], sb[100] = float("nan"), float("inf"), float("inf")
@@ -650,6 +660,22 @@ def test_operands_are_where_they_are_said_to_be(mlel, serving):
     rc = lib.mlel_cuda_quantize_rows(ctypes.byref(T(x.data_ptr(), mlel.F32, (4, 64))), ctypes.byref(T(x.data_ptr(), mlel.I8, (4, 64))),
                                      ctypes.byref(T(x.data_ptr(), mlel.F32, (4,))), None)
     assert rc == -13 and b"current device" in ctypes.c_char_p(lib.mlel_last_error()).value
+
+
+def test_what_is_described_stays(serving):
+    """Objects hold descriptions of their tensors: values change in place, the tensors do not."""
+    i32 = dict(dtype=torch.int32, device="cuda")
+    batch = serving.PagedBatch(torch.tensor([0, 1], **i32), torch.tensor([1], **i32), torch.tensor([[0]], **i32), 1, 16)
+    cache = serving.PagedCache.empty(2, 1, 16, 64)
+    linear = serving.QuantizedLinear(torch.ones(16, 32, dtype=torch.int8, device="cuda"), torch.ones(16, device="cuda"))
+    for thing, name in ((batch, "lengths"), (batch, "max_new"), (cache, "data"), (linear, "weight"), (linear, "bias")):
+        with pytest.raises(AttributeError, match="make a new"):
+            setattr(thing, name, getattr(thing, name))
+    x = torch.ones(2, 32, device="cuda")
+    before = linear(x)
+    linear.scales.mul_(2.0)
+    linear.weight.neg_()
+    assert torch.equal(linear(x), -2 * before)
 
 
 def test_offsets_beyond_32_bits(serving):

@@ -47,6 +47,7 @@ QUANTIZE = dict(x=(F16, (3, 40)), q=(I8, (3, 40)), s=(F32, (3,)))
     (dict(x=(77, (3, 40))), "type", -13),
     (dict(q=(I8, (3, 40), 0x10000, (39, 1))), "overlap", -13),
     (dict(x=None), "missing", -13),
+    (dict(x=(F16, (1, 2 ** 30 + 1)), q=(I8, (1, 2 ** 30 + 1)), s=(F32, (1,))), "more than", -13),
     (dict(), *OK_BUT_NO_DEVICE[::-1]),
 ])
 def test_quantize_rows_refuses(calls, change, word, status):
