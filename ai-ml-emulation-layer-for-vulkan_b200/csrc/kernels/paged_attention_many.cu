@@ -43,7 +43,7 @@ using namespace tc;
 
 constexpr int kRows = 128, kGroup = 16, kMostGroups = 8;
 constexpr int kConvertWarps = 4;
-constexpr int kParamRing = 4, kStaging = 4, kSlots = 3; // of a tile's keys or values: integers on their way, and f16
+constexpr int kParamRing = 5, kStaging = 4, kSlots = 3; // of a tile's keys or values: integers on their way, and f16
 constexpr float kGrowth = 8.f;                          // in powers of two
 constexpr float kWeightBits = 7.f;
 
@@ -74,7 +74,7 @@ struct TileParams {
 
 struct ManyBarriers {
     uint64_t queries, params[kParamRing], stagingFull[kStaging], stagingEmpty[kStaging], full[kSlots], empty[kSlots];
-    uint64_t scores[2], weights[2], result[2];
+    uint64_t scores[2], weights[2], result[2], added;
     uint32_t tmemBase;
 };
 
@@ -231,6 +231,10 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     const int keyLo = allLo + firstTile * kKeys, keyHi = min(allHi, allLo + endTile * kKeys), tiles = endTile - firstTile;
     const int32_t *table = p.batch.table + index * p.batch.tableStride;
     const int active = rows > kRows ? 2 : 1; // tiles with rows
+    // One tile alone has both places for scores in turn: the next ones are formed before the softmax wants them.  Keys then come
+    // before the values of the tile in front of them.  (Three sequences of 300 new tokens, 16 heads of 256 elements over 8, window 1024,
+    // capped: 61 us with one place, so 51; 16 sequences of 4000 tokens, 32 rows a head of 128: 76 and 64.)
+    const bool ahead = active == 1;
 
     if (threadIdx.x == 0) {
         mbarInit(&bars.queries, uint32_t(active * kTileWarps));
@@ -250,6 +254,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             mbarInit(&bars.weights[i], uint32_t(kTileWarps));
             mbarInit(&bars.result[i], 1u);
         }
+        mbarInit(&bars.added, 1u);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kProductWarp) {
@@ -281,6 +286,22 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         int nextNextSlot = slotOf(1), nextSlot = checked(0, slotOf(0)), reference = -126;
         float nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
         uint32_t unit = 0; // keys and values of the tiles in turn
+        const auto copy = [&](const CUtensorMap &map, int row, int count) {
+            const uint32_t buffer = unit % kStaging;
+            if (!mbarPollWarp(&bars.stagingEmpty[buffer], ((unit / kStaging) & 1u) ^ 1u, 91)) {
+                return false;
+            }
+            if (lane == 0) { // the last box may reach behind the sequence, not behind its page
+                mbarArriveExpectTx(&bars.stagingFull[buffer], uint32_t((count + groupsOfBox - 1) / groupsOfBox * boxRows * DP));
+            }
+            __syncwarp();
+            if (lane < kGroups && lane % groupsOfBox == 0 && lane < count) {
+                tmaLoad3d(&map, staging + buffer * Shape::kStagingBytes + lane * kGroup * DP, &bars.stagingFull[buffer], 0, row, 0);
+            }
+            ++unit;
+            return true;
+        };
+        int lastRow = 0, lastCount = 0;
         bool ok = true;
         for (int tile = 0; tile < tiles && ok; ++tile) {
             const int slot = nextSlot, afterSlot = nextNextSlot;
@@ -289,47 +310,44 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             // the copies first: what they need has long been here
             const int key = keyLo + (tile * kGroups + lane) * kGroup, count = min(kGroups, groups - tile * kGroups);
             const int row = (max(slot, 0) * p.cache.heads + head) * p.cache.page + key - int(fastDiv(uint32_t(key), p.pageDiv)) * p.cache.page;
-            const int boxes = (count + groupsOfBox - 1) / groupsOfBox; // the last one may reach behind the sequence, not behind its page
-#pragma unroll 1
-            for (int side = 0; side < 2; ++side, ++unit) {
-                const uint32_t buffer = unit % kStaging;
-                ok = ok && mbarPollWarp(&bars.stagingEmpty[buffer], ((unit / kStaging) & 1u) ^ 1u, 91);
-                if (!ok) {
-                    break;
+            ok = copy(mapK, row, count);
+            if (!ok) {
+                break;
+            }
+            {
+                // Parameters of the tile.  Here the converters are done with the keys of tile - 2, for which the values of tile - 4
+                // (tile - 5, where keys come before values) had been used up by both tiles: the softmax is past tile - 5,
+                // whose place this is.
+                TileParams &to = params[tile % kParamRing];
+                const float magnitude = fabsf(valueScale);
+                int exponent = magnitude > 0.f && magnitude < INFINITY ? int(__float_as_uint(powerAbove(magnitude)) >> 23) - 127 : -126;
+                exponent = __reduce_max_sync(0xffffffffu, exponent);
+                reference = max(reference, exponent);
+                if (lane < kGroups) {
+                    // (a scale that is not finite gives a shift and weights that are not)
+                    const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), -60.f) + kWeightBits : magnitude - magnitude;
+                    to.keyScale[lane] = keyScale, to.shift[lane] = shift, to.perWeight[lane] = exp2f(-shift);
                 }
+                const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
                 if (lane == 0) {
-                    mbarArriveExpectTx(&bars.stagingFull[buffer], uint32_t(boxes * boxRows * DP));
+                    to.reference = reference, to.there = there;
                 }
                 __syncwarp();
-                if (lane < kGroups && lane % groupsOfBox == 0 && lane < count) {
-                    tmaLoad3d(side == 0 ? &mapK : &mapV, staging + buffer * Shape::kStagingBytes + lane * kGroup * DP, &bars.stagingFull[buffer],
-                              0, row, 0);
-                }
-                if (side == 0) {
-                    // Parameters of the tile.  Here the converters are done with the keys of tile - 2, for which the values of
-                    // tile - 4 had been used up by both tiles: the softmax is past tile - 4, whose place this is.
-                    TileParams &to = params[tile % kParamRing];
-                    const float magnitude = fabsf(valueScale);
-                    int exponent = magnitude > 0.f && magnitude < INFINITY ? int(__float_as_uint(powerAbove(magnitude)) >> 23) - 127 : -126;
-                    exponent = __reduce_max_sync(0xffffffffu, exponent);
-                    reference = max(reference, exponent);
-                    if (lane < kGroups) {
-                        // (a scale that is not finite gives a shift and weights that are not)
-                        const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), -60.f) + kWeightBits : magnitude - magnitude;
-                        to.keyScale[lane] = keyScale, to.shift[lane] = shift, to.perWeight[lane] = exp2f(-shift);
-                    }
-                    const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
-                    if (lane == 0) {
-                        to.reference = reference, to.there = there;
-                    }
-                    __syncwarp();
-                    if (lane == 0) {
-                        mbarArrive(&bars.params[tile % kParamRing]);
-                    }
+                if (lane == 0) {
+                    mbarArrive(&bars.params[tile % kParamRing]);
                 }
             }
+            if (!ahead) {
+                ok = copy(mapV, row, count);
+            } else if (tile > 0) {
+                ok = copy(mapV, lastRow, kGroups);
+            }
+            lastRow = row, lastCount = count;
             nextSlot = checked(tile + 1, afterSlot);
             nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
+        }
+        if (ahead && ok && tiles > 0) {
+            copy(mapV, lastRow, lastCount);
         }
         __syncwarp();
     } else if (warp == kProductWarp) {
@@ -340,7 +358,8 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                         valueDesc = descWords(smemDesc(smemAddr(slots), kPanel, 1024));
         bool failed = !mbarPoll(&bars.queries, 0u, 92);
         const auto scoreProduct = [&](int tile, int which) {
-            const uint32_t unit = uint32_t(2 * tile), place = unit % kSlots;
+            const uint32_t unit = ahead ? uint32_t(max(0, 2 * tile - 1)) : uint32_t(2 * tile), place = unit % kSlots;
+            const int buffer = ahead ? tile & 1 : which;
             if (which == 0) {
                 failed = failed || !mbarPoll(&bars.full[place], (unit / kSlots) & 1u, 93);
             }
@@ -348,27 +367,31 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
             for (int panel = 0; panel < Shape::kPanels; ++panel) {
-                mmaSharedFour(tmem + Shape::scores(which),
+                mmaSharedFour(tmem + Shape::scores(buffer),
                               {queryDesc.low + uint32_t(which * (Shape::kQueryBytes >> 4)) + uint32_t(panel) * (kQueryPanel >> 4), queryDesc.high},
                               {keyDesc.low + place * kPlace + uint32_t(panel) * (kPanel >> 4), keyDesc.high}, kScoreDesc, panel != 0 ? 1u : 0u);
             }
-            ummaCommit(&bars.scores[which]);
+            ummaCommit(&bars.scores[buffer]);
             if (which == active - 1) {
                 ummaCommit(&bars.empty[place]);
             }
         };
         const auto resultProduct = [&](int tile, int which) {
-            const uint32_t unit = uint32_t(2 * tile + 1), place = unit % kSlots;
+            const uint32_t unit = uint32_t(ahead ? min(2 * tile + 2, 2 * tiles - 1) : 2 * tile + 1), place = unit % kSlots;
+            const int buffer = ahead ? tile & 1 : which;
             if (which == 0) {
                 failed = failed || !mbarPoll(&bars.full[place], (unit / kSlots) & 1u, 94);
             }
-            failed = failed || !mbarPoll(&bars.weights[which], uint32_t(tile) & 1u, 95);
+            failed = failed || !mbarPoll(&bars.weights[buffer], uint32_t(ahead ? tile >> 1 : tile) & 1u, 95);
             __syncwarp();
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
             for (int k = 0; k < kGroups; k += 4) { // the weights of 16 keys lie in eight columns
-                mmaTensorFour(tmem + Shape::result(which), tmem + Shape::scores(which) + uint32_t(k * 8),
+                mmaTensorFour(tmem + Shape::result(which), tmem + Shape::scores(buffer) + uint32_t(k * 8),
                               {valueDesc.low + place * kPlace + uint32_t(k) * 128u, valueDesc.high}, kResultDesc, tile != 0 || k != 0 ? 1u : 0u);
+            }
+            if (ahead) {
+                ummaCommit(&bars.added);
             }
             if (tile == tiles - 1) {
                 ummaCommit(&bars.result[which]);
@@ -381,9 +404,12 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             scoreProduct(0, which);
         }
         for (int tile = 0; tile < tiles; ++tile) {
+            if (ahead && tile + 1 < tiles) {
+                scoreProduct(tile + 1, 0);
+            }
             for (int which = 0; which < active; ++which) {
                 resultProduct(tile, which);
-                if (tile + 1 < tiles) {
+                if (!ahead && tile + 1 < tiles) {
                     scoreProduct(tile + 1, which);
                 }
             }
@@ -514,11 +540,9 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const int openHi = p.causal ? old + int(fastDiv(uint32_t(tileFirst), p.groupDiv)) + 1 : q.length;
         const int openLo = p.window > 0 ? max(0, old + int(fastDiv(uint32_t(tileLast), p.groupDiv)) - p.window + 1) : 0;
         const uint32_t laneBase = tmem + (uint32_t(quarter * 32) << 16);
-        const uint32_t scoresAt = laneBase + Shape::scores(which) + uint32_t(half * (kKeys / 2)),
-                       weightsAt = laneBase + Shape::scores(which) + uint32_t(half * (kKeys / 4)),
-                       resultAt = laneBase + Shape::result(which) + uint32_t(half * (DP / 2));
+        const uint32_t resultAt = laneBase + Shape::result(which) + uint32_t(half * (DP / 2));
 
-        bool ok = true;
+        bool ok = true, late = false;
         float most = -INFINITY, sum = 0.f;
         int reference = -126;
         const auto scoreOf = [&](uint32_t s, float factor) { // in powers of two
@@ -526,9 +550,12 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             return CAP ? softCapped(x, p.softcap) * kLog2e : x;
         };
         for (int tile = 0; tile < tiles && ok; ++tile) {
+            const int buffer = ahead ? tile & 1 : which;
+            const uint32_t scoresAt = laneBase + Shape::scores(buffer) + uint32_t(half * (kKeys / 2)),
+                           weightsAt = laneBase + Shape::scores(buffer) + uint32_t(half * (kKeys / 4));
             ok = mbarPollWarp(&bars.params[tile % kParamRing], uint32_t(tile / kParamRing) & 1u, 98) &&
-                 mbarPollWarp(&bars.scores[which], uint32_t(tile) & 1u, 99);
-            ok = pairVote(pairBarrier, !ok) == 0u; // a wait that ran out ends it for both warps of the rows
+                 mbarPollWarp(&bars.scores[buffer], uint32_t(ahead ? tile >> 1 : tile) & 1u, 99);
+            ok = pairVote(pairBarrier, !ok || late) == 0u; // a wait that ran out ends it for both warps of the rows
             if (!ok) {
                 break;
             }
@@ -540,6 +567,13 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             const auto seen = [&](int g) {
                 const int first = key0 + g * kGroup, hi = max(0, min(kGroup, rowHi - first)), lo = max(0, min(kGroup, rowLo - first));
                 return ((tp.there >> (half * kHalfGroups + g)) & 1u) != 0u ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
+            };
+            bool pending = ahead && tile > 0; // whether the products of the tile before may still be adding to the result
+            const auto addedBefore = [&] {
+                if (pending) {
+                    late = !mbarPollWarp(&bars.added, uint32_t(tile - 1) & 1u, 88) || late;
+                    pending = false;
+                }
             };
             uint32_t weights[kKeys / 4];
             bool maximumFirst = tile == 0 || tp.reference != reference;
@@ -567,6 +601,8 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                     const float factorO = keep * exp2f(float(reference - tp.reference));
                     sum *= keep;
                     if (tile > 0 && __any_sync(0xffffffffu, factorO != 1.f)) {
+                        addedBefore();
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
                         for (int d = 0; d < DP / 2; d += 16) {
                             uint32_t o[16];
@@ -636,12 +672,13 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 maximumFirst = true;
             }
             sum += added;
+            addedBefore(); // (waited for at every tile: no phase is passed over)
             tmemStoreWeights<kKeys / 4>(weightsAt, weights);
             tmemStoreWait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                mbarArrive(&bars.weights[which]);
+                mbarArrive(&bars.weights[buffer]);
             }
         }
         ok = (tiles == 0 || mbarPollWarp(&bars.result[which], 0u, 90)) && ok;
