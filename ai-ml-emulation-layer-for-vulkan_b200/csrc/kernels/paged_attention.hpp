@@ -26,9 +26,7 @@ struct AttendParams {
 };
 
 // paged_attention_few.cu: few rows per cache head (single tokens, or a handful), keys split over the whole device
-constexpr int kFewRows = 16;
 struct FewPlan {
-    int rows;           // of a tile: 8 or 16
     int split;          // blocks of the cluster that shares a tile's keys; 0: all blocks share all keys
     int blocks;
     uint64_t workspace; // where parts of a tile may lie with blocks that are no cluster: a second kernel joins them

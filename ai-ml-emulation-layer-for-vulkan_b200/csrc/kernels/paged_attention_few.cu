@@ -3,8 +3,9 @@
 //   o = sum_j softmax(s)_j v_j,  s_j = scale * q . k_j (capped or not), over the tokens that the masks leave
 //
 // What bounds it: the bytes of the cache, and close behind them the instructions that turn them into operands.  Every key and
-// value is read once per tile of 8 or 16 rows (a row is one token's query head; the heads that share a cache head are rows of
-// one tile).  At 6.5 TB/s an SM gets some 23 bytes a cycle, 16 keys and values of 128 elements every 180 cycles.
+// value is read once per tile of 8 rows (a row is one token's query head; the heads that share a cache head are rows of
+// one tile), by the second and further tiles of a cache head out of L2.  (Tiles of 16 rows for 9 to 16, 16 sequences of up to 4000
+// tokens, 8 heads of 128 elements, 16 rows: 41 us, of 8 rows 33; 4 heads of 256, 12 rows: 71 and 39.)  At 6.5 TB/s an SM gets some 23 bytes a cycle, 16 keys and values of 128 elements every 180 cycles.
 //
 // Work.  All tiles' keys, in steps of 128, form one line that is cut into as many equal pieces as there are blocks, whatever the
 // lengths of the sequences: a block works through the ends of the tiles that its piece touches.  Tiles that lie in
@@ -18,8 +19,8 @@
 // the other warps before the end of a tile.
 //
 // Products on m16n8k16 in f16 with f32 sums, transposed: S^T = K Q^T and O^T = V^T P^T, so that 16 keys (16 elements of the
-// result) are the rows and 8 queries the columns: with at most 8 rows to a tile that is half the products and half the scores
-// per lane of the untransposed form, which pads to 16.  P^T changes from result to operand by a transposition of 8 x 8.
+// result) are the rows and 8 queries the columns: half the products and half the scores per lane of the untransposed form, which
+// pads to 16.  P^T changes from result to operand by a transposition of 8 x 8.
 // Which element of a head is which k of the first product is free as long as both operands agree, so a lane takes 16
 // consecutive bytes of a key; which key is which row is free as long as weights and values agree, so a lane's keys are t,
 // t + 4, t + 8, t + 12 and its values 16 consecutive bytes of each.  All these reads are free of bank conflicts.
@@ -52,7 +53,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4, kTileRows = 8;
 constexpr int kGroup = 16; // keys that share a page and a scale for certain
 constexpr int kStageGroups = 2;
 constexpr int kStepGroups = kWarps * kStageGroups;
@@ -74,7 +75,7 @@ struct FewWork {
     Sequence q;
     int firstGroup, groups, steps, tiles, work;
 };
-template <int ROWS> __device__ __forceinline__ FewWork fewWorkOf(const AttendParams &p, int index) {
+__device__ __forceinline__ FewWork fewWorkOf(const AttendParams &p, int index) {
     FewWork w{};
     w.q = sequenceOf(p.batch, index);
     if (w.q.sound && w.q.fresh > 0) {
@@ -82,7 +83,7 @@ template <int ROWS> __device__ __forceinline__ FewWork fewWorkOf(const AttendPar
         w.firstGroup = lo / kGroup;
         w.groups = (w.q.length + kGroup - 1) / kGroup - w.firstGroup;
         w.steps = (w.groups + kStepGroups - 1) / kStepGroups;
-        w.tiles = (w.q.fresh * p.group + ROWS - 1) / ROWS * p.cache.heads;
+        w.tiles = (w.q.fresh * p.group + kTileRows - 1) / kTileRows * p.cache.heads;
         w.work = w.steps * w.tiles; // (the plan has seen to it that the whole line has fewer than 2^31 steps)
     }
     return w;
@@ -106,14 +107,14 @@ struct FewScan {
 };
 
 // All threads: how many steps the batch has, and the sequence that this block's piece starts in.
-template <int ROWS> __device__ void locate(const AttendParams &p, FewScan &scan, int piece, int pieces, bool report) {
+__device__ void locate(const AttendParams &p, FewScan &scan, int piece, int pieces, bool report) {
     const int B = p.batch.sequences, each = (B + kWarps * 32 - 1) / (kWarps * 32);
     const int lo = min(B, int(threadIdx.x) * each), hi = min(B, lo + each);
     const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
     int own = 0;
     FewWork w{};
     for (int b = lo; b < hi; ++b) {
-        w = fewWorkOf<ROWS>(p, b);
+        w = fewWorkOf(p, b);
         own += w.work;
         if (report && !w.q.sound) {
             atomicCAS(&g_pagedError, 0, kBadSequence);
@@ -141,7 +142,7 @@ template <int ROWS> __device__ void locate(const AttendParams &p, FewScan &scan,
         int b = lo;
         if (each > 1) {
             for (;; ++b) {
-                w = fewWorkOf<ROWS>(p, b);
+                w = fewWorkOf(p, b);
                 if (at < before + w.work) {
                     break;
                 }
@@ -157,23 +158,23 @@ template <int ROWS> __device__ void locate(const AttendParams &p, FewScan &scan,
 }
 
 // One row of a partial result: maximum, sum, then DP elements.
-template <int DP> __device__ __forceinline__ float *partialRow(const AttendParams &p, int piece, int which, int row, int rows) {
-    return p.partials + ((int64_t(piece) * 2 + which) * rows + row) * (DP + 4);
+template <int DP> __device__ __forceinline__ float *partialRow(const AttendParams &p, int piece, int which, int row) {
+    return p.partials + ((int64_t(piece) * 2 + which) * kTileRows + row) * (DP + 4);
 }
 
-template <int DP, int NQ, bool HALF>
-__global__ void __launch_bounds__(kWarps * 32, NQ * DP <= 128 ? 3 : 2)
+template <int DP, bool HALF>
+__global__ void __launch_bounds__(kWarps * 32, DP <= 128 ? 3 : 2)
 pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p,
                         const int split) { // blocks of the cluster that shares a tile; 0: pieces of the line
     using Shape = FewShape<DP>;
-    constexpr int ROWS = 8 * NQ, SEGS = DP / 64, MT = DP / 16, STAGES = Shape::kStages;
-    constexpr int AT = NQ * DP <= 128 ? 2 : 1; // groups taken at once: as many as the registers hold
+    constexpr int SEGS = DP / 64, MT = DP / 16, STAGES = Shape::kStages;
+    constexpr int AT = DP <= 128 ? 2 : 1; // groups taken at once: as many as the registers hold
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     extern __shared__ uint8_t rawSmem[];
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rawSmem) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t full[kWarps][STAGES];
     __shared__ FewScan scan;
-    __shared__ float joinMax[kWarps][ROWS], joinSum[kWarps][ROWS];
+    __shared__ float joinMax[kWarps][kTileRows], joinSum[kWarps][kTileRows];
     const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5, g = lane >> 2, t = lane & 3;
     if (threadIdx.x == 0) {
         for (int w = 0; w < kWarps; ++w) {
@@ -190,7 +191,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         rank = int(clusterCtaRank());
         const int cluster = int(blockIdx.x) / split, perSequence = int(gridDim.x) / (split * p.batch.sequences);
         index = cluster / perSequence;
-        w = fewWorkOf<ROWS>(p, index);
+        w = fewWorkOf(p, index);
         const int tile = cluster - index * perSequence;
         if (!w.q.sound && tile == 0 && rank == 0 && threadIdx.x == 0) {
             atomicCAS(&g_pagedError, 0, kBadSequence);
@@ -201,7 +202,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         begin = tile * w.steps + w.steps * rank / split, end = tile * w.steps + w.steps * (rank + 1) / split;
         __syncthreads();
     } else {
-        locate<ROWS>(p, scan, int(blockIdx.x), int(gridDim.x), blockIdx.x == 0); // (its barriers cover mbarInit too)
+        locate(p, scan, int(blockIdx.x), int(gridDim.x), blockIdx.x == 0); // (its barriers cover mbarInit too)
         const Pieces pieces(scan.total, int(gridDim.x));
         begin = pieces.start(int(blockIdx.x)), end = pieces.start(int(blockIdx.x) + 1);
         if (begin >= end) {
@@ -218,12 +219,12 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
     do { // (a block of a cluster whose part is empty still takes part in joining)
         while (split == 0 && at >= before + w.work) {
             before += w.work;
-            w = fewWorkOf<ROWS>(p, ++index); // (there is one: `at` lies on the line)
+            w = fewWorkOf(p, ++index); // (there is one: `at` lies on the line)
         }
         const int tileIndex = split > 0 ? int(blockIdx.x) / split % (int(gridDim.x) / (split * p.batch.sequences)) : (at - before) / w.steps;
         const int firstStep = at - before - tileIndex * w.steps, lastStep = min(w.steps, firstStep + (end - at));
-        const int head = tileIndex % p.cache.heads, firstRow = tileIndex / p.cache.heads * ROWS;
-        const int rows = min(ROWS, w.q.fresh * p.group - firstRow), old = w.q.length - w.q.fresh;
+        const int head = tileIndex % p.cache.heads, firstRow = tileIndex / p.cache.heads * kTileRows;
+        const int rows = min(kTileRows, w.q.fresh * p.group - firstRow), old = w.q.length - w.q.fresh;
         // this warp's stages: two groups each, every fourth pair of the piece
         const int firstGroup = w.firstGroup + firstStep * kStepGroups + warp * kStageGroups,
                   groupEnd = min(w.firstGroup + w.groups, w.firstGroup + lastStep * kStepGroups);
@@ -273,81 +274,74 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             writeStage = writeStage + 1 == STAGES ? 0 : writeStage + 1;
         };
 
-        // queries, the second operand of S^T: lane (g, t) holds row 8 nq + g, elements 64 seg + 16 t .. + 15
-        uint32_t qf[NQ][SEGS][4][2];
-        float rowScale[NQ][2], offset[NQ][2]; // of rows 8 nq + 2 t and + 1, whose scores the lane gets
-        int rowLo[NQ][2], rowHi[NQ][2];
+        // queries, the second operand of S^T: lane (g, t) holds row g, elements 64 seg + 16 t .. + 15
+        uint32_t qf[SEGS][4][2];
+        float rowScale[2], offset[2]; // of rows 2 t and 2 t + 1, whose scores the lane gets
+        int rowLo[2], rowHi[2];
+        const int row = firstRow + g;
+        const bool live = g < rows;
+        const int token = live ? int(fastDiv(uint32_t(row), p.groupDiv)) : 0, queryHead = head * p.group + (live ? row - token * p.group : 0);
+        const T *q = reinterpret_cast<const T *>(p.queries + int64_t(w.q.first + token) * p.queryStride[0] + queryHead * p.queryStride[1]);
+        uint32_t words[SEGS][8]; // two elements each, as they lie in memory
 #pragma unroll
-        for (int nq = 0; nq < NQ; ++nq) {
-            const int row = firstRow + 8 * nq + g;
-            const bool live = 8 * nq + g < rows;
-            const int token = live ? int(fastDiv(uint32_t(row), p.groupDiv)) : 0, queryHead = head * p.group + (live ? row - token * p.group : 0);
-            const T *q = reinterpret_cast<const T *>(p.queries + int64_t(w.q.first + token) * p.queryStride[0] + queryHead * p.queryStride[1]);
-            uint32_t words[SEGS][8]; // two elements each, as they lie in memory
-#pragma unroll
-            for (int seg = 0; seg < SEGS; ++seg) {
-                loadQuerySixteen(q, seg * 64 + t * 16, live ? p.cache.headDim : 0, p.wideQueries != 0, words[seg]);
-            }
-            if (nq == 0) { // the first copies go out while the queries are on their way
-                for (int n = 0; n < min(count, STAGES) && !broken; ++n) {
-                    fill();
-                }
-            }
-            float unit = 1.f, total = 0.f;
-            if (!HALF) {
-                float most = 0.f;
-#pragma unroll
-                for (int seg = 0; seg < SEGS; ++seg) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 f = unpackTwo(words[seg][j], T());
-                        most = maxBits(most, maxBits(f.x, f.y));
-                    }
-                }
-                most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, 1));
-                most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, 2));
-                unit = halfUnit(most);
-                const float inverse = 1.f / unit; // powers of two
-#pragma unroll
-                for (int seg = 0; seg < SEGS; ++seg) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float2 f = unpackTwo(words[seg][j], T());
-                        words[seg][j] = packTwo(f.x * inverse, f.y * inverse, __half());
-                    }
-                }
-            }
+        for (int seg = 0; seg < SEGS; ++seg) {
+            loadQuerySixteen(q, seg * 64 + t * 16, live ? p.cache.headDim : 0, p.wideQueries != 0, words[seg]);
+        }
+        // the first copies go out while the queries are on their way
+        for (int n = 0; n < min(count, STAGES) && !broken; ++n) {
+            fill();
+        }
+        float unit = 1.f, total = 0.f;
+        if (!HALF) {
+            float most = 0.f;
 #pragma unroll
             for (int seg = 0; seg < SEGS; ++seg) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    qf[nq][seg][u][0] = words[seg][2 * u], qf[nq][seg][u][1] = words[seg][2 * u + 1];
-                    const float2 a = unpackTwo(words[seg][2 * u], __half()), b = unpackTwo(words[seg][2 * u + 1], __half());
-                    total += (a.x + a.y) + (b.x + b.y);
+                for (int j = 0; j < 8; ++j) {
+                    const float2 f = unpackTwo(words[seg][j], T());
+                    most = maxBits(most, maxBits(f.x, f.y));
                 }
             }
-            total += __shfl_xor_sync(0xffffffffu, total, 1);
-            total += __shfl_xor_sync(0xffffffffu, total, 2);
-            const int position = old + token;
-            const int hi = !live ? 0 : p.causal ? position + 1 : w.q.length, lo = p.window > 0 ? max(0, position - p.window + 1) : 0;
+            most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, 1));
+            most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, 2));
+            unit = halfUnit(most);
+            const float inverse = 1.f / unit; // powers of two
 #pragma unroll
-            for (int x = 0; x < 2; ++x) { // from the lanes that hold rows 2 t and 2 t + 1
-                const int from = (2 * t + x) * 4;
-                rowScale[nq][x] = __shfl_sync(0xffffffffu, unit, from) * 16777216.f * p.scale * (p.softcap > 0.f ? 1.f : kLog2e);
-                offset[nq][x] = __shfl_sync(0xffffffffu, total, from) * (-128.f / 16777216.f);
-                rowLo[nq][x] = __shfl_sync(0xffffffffu, lo, from), rowHi[nq][x] = __shfl_sync(0xffffffffu, hi, from);
+            for (int seg = 0; seg < SEGS; ++seg) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float2 f = unpackTwo(words[seg][j], T());
+                    words[seg][j] = packTwo(f.x * inverse, f.y * inverse, __half());
+                }
             }
+        }
+#pragma unroll
+        for (int seg = 0; seg < SEGS; ++seg) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                qf[seg][u][0] = words[seg][2 * u], qf[seg][u][1] = words[seg][2 * u + 1];
+                const float2 a = unpackTwo(words[seg][2 * u], __half()), b = unpackTwo(words[seg][2 * u + 1], __half());
+                total += (a.x + a.y) + (b.x + b.y);
+            }
+        }
+        total += __shfl_xor_sync(0xffffffffu, total, 1);
+        total += __shfl_xor_sync(0xffffffffu, total, 2);
+        const int position = old + token;
+        const int hi = !live ? 0 : p.causal ? position + 1 : w.q.length, lo = p.window > 0 ? max(0, position - p.window + 1) : 0;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) { // from the lanes that hold rows 2 t and 2 t + 1
+            const int from = (2 * t + x) * 4;
+            rowScale[x] = __shfl_sync(0xffffffffu, unit, from) * 16777216.f * p.scale * (p.softcap > 0.f ? 1.f : kLog2e);
+            offset[x] = __shfl_sync(0xffffffffu, total, from) * (-128.f / 16777216.f);
+            rowLo[x] = __shfl_sync(0xffffffffu, lo, from), rowHi[x] = __shfl_sync(0xffffffffu, hi, from);
         }
         // keys below `openLo` or from `openHi` on are hidden from some row
         const int lastToken = int(fastDiv(uint32_t(firstRow + rows - 1), p.groupDiv)), firstToken = int(fastDiv(uint32_t(firstRow), p.groupDiv));
         const int openHi = p.causal ? old + firstToken + 1 : w.q.length, openLo = p.window > 0 ? max(0, old + lastToken - p.window + 1) : 0;
 
-        float o[NQ][MT][4] = {}, most[NQ][2], sum[NQ][2] = {};
+        float o[MT][4] = {}, most[2], sum[2] = {};
         float reference = 0.f, perReference = 1.f; // unit of `o`, a power of two, and kWeightScale over it
-#pragma unroll
-        for (int nq = 0; nq < NQ; ++nq) {
-            most[nq][0] = most[nq][1] = -INFINITY;
-        }
+        most[0] = most[1] = -INFINITY;
         for (int n = 0; n < count; ++n) {
             if (n > 0 && (n & 15) == 0) {
                 slots = nextSlots;
@@ -370,13 +364,10 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                 const int key0 = groupOf(2 * n + h0) * kGroup;
                 const uint32_t keys = smemAddr(own + stage * Shape::kStageBytes) + uint32_t(h0 * Shape::kGroupBytes),
                                values = keys + kStageGroups * Shape::kGroupBytes;
-                float s[AT][NQ][4]; // [group][..]: keys g and g + 8 in the lanes' order, rows 2 t and 2 t + 1
+                float s[AT][4]; // [group][..]: keys g and g + 8 in the lanes' order, rows 2 t and 2 t + 1
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
-#pragma unroll
-                    for (int nq = 0; nq < NQ; ++nq) {
-                        s[h][nq][0] = s[h][nq][2] = offset[nq][0], s[h][nq][1] = s[h][nq][3] = offset[nq][1];
-                    }
+                    s[h][0] = s[h][2] = offset[0], s[h][1] = s[h][3] = offset[1];
 #pragma unroll
                     for (int seg = 0; seg < SEGS; ++seg) {
                         const uint32_t group = keys + uint32_t(h * Shape::kGroupBytes);
@@ -388,10 +379,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                             uint32_t a[4];
                             bytesToSubnormals(low[u], a[0], a[2]);
                             bytesToSubnormals(high[u], a[1], a[3]);
-#pragma unroll
-                            for (int nq = 0; nq < NQ; ++nq) {
-                                mmaF16(s[h][nq], a, qf[nq][seg][u][0], qf[nq][seg][u][1]);
-                            }
+                            mmaF16(s[h], a, qf[seg][u][0], qf[seg][u][1]);
                         }
                     }
                 }
@@ -400,20 +388,17 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
 #pragma unroll
-                    for (int nq = 0; nq < NQ; ++nq) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float x = s[h][nq][e] * (rowScale[nq][e & 1] * keyScale[h]);
-                            if (p.softcap > 0.f) {
-                                x = softCapped(x, p.softcap) * kLog2e;
-                            }
-                            if (masked) { // row g (or g + 8) of the product is key (g >> 1) + 4 (g & 1) (+ 8) of the group
-                                const int key = key0 + h * kGroup + (g >> 1) + 4 * (g & 1) + 8 * (e >> 1);
-                                x = key < rowHi[nq][e & 1] && key >= rowLo[nq][e & 1] && keyScale[h] != -1.f ? x : -INFINITY;
-                            }
-                            s[h][nq][e] = x;
-                            grows = grows || x > most[nq][e & 1];
+                    for (int e = 0; e < 4; ++e) {
+                        float x = s[h][e] * (rowScale[e & 1] * keyScale[h]);
+                        if (p.softcap > 0.f) {
+                            x = softCapped(x, p.softcap) * kLog2e;
                         }
+                        if (masked) { // row g (or g + 8) of the product is key (g >> 1) + 4 (g & 1) (+ 8) of the group
+                            const int key = key0 + h * kGroup + (g >> 1) + 4 * (g & 1) + 8 * (e >> 1);
+                            x = key < rowHi[e & 1] && key >= rowLo[e & 1] && keyScale[h] != -1.f ? x : -INFINITY;
+                        }
+                        s[h][e] = x;
+                        grows = grows || x > most[e & 1];
                     }
                 }
                 // the values' unit; a scale that is not finite reaches the rows that see it through their weights
@@ -429,45 +414,39 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                     reference = unit;
                     perReference = unit > 0.f ? kWeightScale / unit : 1.f;
 #pragma unroll
-                    for (int nq = 0; nq < NQ; ++nq) {
+                    for (int x = 0; x < 2; ++x) {
+                        float top = most[x];
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            float top = most[nq][x];
+                        for (int h = 0; h < AT; ++h) {
+                            top = fmaxf(top, fmaxf(s[h][x], s[h][2 + x]));
+                        }
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                        const float keep = top == -INFINITY ? 1.f : exp2Fast(most[x] - top);
+                        most[x] = top;
+                        sum[x] *= keep;
+                        const float factor = keep * shrink;
 #pragma unroll
-                            for (int h = 0; h < AT; ++h) {
-                                top = fmaxf(top, fmaxf(s[h][nq][x], s[h][nq][2 + x]));
-                            }
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                            const float keep = top == -INFINITY ? 1.f : exp2Fast(most[nq][x] - top);
-                            most[nq][x] = top;
-                            sum[nq][x] *= keep;
-                            const float factor = keep * shrink;
-#pragma unroll
-                            for (int mt = 0; mt < MT; ++mt) {
-                                o[nq][mt][x] *= factor, o[nq][mt][2 + x] *= factor;
-                            }
+                        for (int mt = 0; mt < MT; ++mt) {
+                            o[mt][x] *= factor, o[mt][2 + x] *= factor;
                         }
                     }
                 }
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
                     const float weightUnit = valueScale[h] * perReference;
-                    uint32_t wf[NQ][2]; // P^T: rows 2 t and 2 t + 1 of the group's keys, rows 8 nq + g
+                    uint32_t wf[2]; // P^T: keys in pairs by t, row g
+                    const float shift0 = most[0] == -INFINITY ? 0.f : most[0], shift1 = most[1] == -INFINITY ? 0.f : most[1];
 #pragma unroll
-                    for (int nq = 0; nq < NQ; ++nq) {
-                        const float shift0 = most[nq][0] == -INFINITY ? 0.f : most[nq][0], shift1 = most[nq][1] == -INFINITY ? 0.f : most[nq][1];
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const float x0 = s[h][nq][2 * half], x1 = s[h][nq][2 * half + 1];
-                            const float p0 = exp2Fast(x0 - shift0), p1 = exp2Fast(x1 - shift1);
-                            sum[nq][0] += p0, sum[nq][1] += p1;
-                            // what the mask hides stays out, whatever its page's scale is
-                            const float w0 = masked && x0 == -INFINITY ? 0.f : p0 * weightUnit;
-                            const float w1 = masked && x1 == -INFINITY ? 0.f : p1 * weightUnit;
-                            wf[nq][half] = transposeHalves(packTwo(w0, w1, __half()));
-                        }
+                    for (int half = 0; half < 2; ++half) {
+                        const float x0 = s[h][2 * half], x1 = s[h][2 * half + 1];
+                        const float p0 = exp2Fast(x0 - shift0), p1 = exp2Fast(x1 - shift1);
+                        sum[0] += p0, sum[1] += p1;
+                        // what the mask hides stays out, whatever its page's scale is
+                        const float w0 = masked && x0 == -INFINITY ? 0.f : p0 * weightUnit;
+                        const float w1 = masked && x1 == -INFINITY ? 0.f : p1 * weightUnit;
+                        wf[half] = transposeHalves(packTwo(w0, w1, __half()));
                     }
                     constexpr int CHUNKS = DP < 128 ? 1 : DP / 128, WORDS = DP < 128 ? 2 : 4; // 16 (or, below 128, 8) bytes of a value row per lane each
                     const uint32_t group = values + uint32_t(h * Shape::kGroupBytes);
@@ -492,10 +471,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
 #pragma unroll
                             for (int d = 0; d < 2; ++d) {
                                 const uint32_t a[4] = {low[2 * d], low[2 * d + 1], high[2 * d], high[2 * d + 1]};
-#pragma unroll
-                                for (int nq = 0; nq < NQ; ++nq) {
-                                    mmaF16(o[nq][c * 8 + word * 2 + d], a, wf[nq][0], wf[nq][1]);
-                                }
+                                mmaF16(o[c * 8 + word * 2 + d], a, wf[0], wf[1]);
                             }
                         }
                     }
@@ -513,97 +489,84 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
 
         // ---- the four warps' results as one ----
 #pragma unroll
-        for (int nq = 0; nq < NQ; ++nq) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                sum[nq][x] += __shfl_xor_sync(0xffffffffu, sum[nq][x], 4);
-                sum[nq][x] += __shfl_xor_sync(0xffffffffu, sum[nq][x], 8);
-                sum[nq][x] += __shfl_xor_sync(0xffffffffu, sum[nq][x], 16);
-                if (g == 0) {
-                    joinMax[warp][8 * nq + 2 * t + x] = most[nq][x], joinSum[warp][8 * nq + 2 * t + x] = sum[nq][x];
-                }
+        for (int x = 0; x < 2; ++x) {
+            sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 4);
+            sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 8);
+            sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 16);
+            if (g == 0) {
+                joinMax[warp][2 * t + x] = most[x], joinSum[warp][2 * t + x] = sum[x];
             }
         }
         __syncthreads(); // every warp's copies have been read: the ring holds results from here on
-        constexpr int kPitch = Shape::kPitch, PASS = NQ < 2 ? 8 : 16; // rows joined at a time
-        float *results = reinterpret_cast<float *>(ring), *joined = results + kWarps * PASS * kPitch;
-        static_assert((kWarps * PASS + ROWS) * kPitch * 4 <= Shape::kRing, "the results fit the ring");
+        constexpr int kPitch = Shape::kPitch;
+        float *results = reinterpret_cast<float *>(ring), *joined = results + kWarps * kTileRows * kPitch;
+        static_assert((kWarps + 1) * kTileRows * kPitch * 4 <= Shape::kRing, "the results fit the ring");
         const bool whole = split <= 1 && firstStep == 0 && lastStep == w.steps;
 #pragma unroll
-        for (int pass = 0; pass < ROWS / PASS; ++pass) {
+        for (int x = 0; x < 2; ++x) {
+            const int itsRow = 2 * t + x;
+            if (itsRow < rows) {
+                float top = -INFINITY;
+                for (int v = 0; v < kWarps; ++v) {
+                    top = fmaxf(top, joinMax[v][itsRow]);
+                }
+                const float factor = (top == -INFINITY ? 1.f : exp2Fast(most[x] - top)) * (reference * (1.f / kWeightScale));
+                float *to = results + (warp * kTileRows + itsRow) * kPitch;
+                // tile mt holds elements 2 (mt % 8) and the next of the lane's 16 (or 8) of each chunk
 #pragma unroll
-            for (int sub8 = 0; sub8 < PASS / 8; ++sub8) {
-                const int nq = pass * (PASS / 8) + sub8;
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const int row = 8 * nq + 2 * t + x;
-                    if (row < rows) {
-                        float top = -INFINITY;
-                        for (int v = 0; v < kWarps; ++v) {
-                            top = fmaxf(top, joinMax[v][row]);
-                        }
-                        const float factor = (top == -INFINITY ? 1.f : exp2Fast(most[nq][x] - top)) * (reference * (1.f / kWeightScale));
-                        float *to = results + (warp * PASS + 8 * sub8 + 2 * t + x) * kPitch;
-                        // tile mt holds elements 2 (mt % 8) and the next of the lane's 16 (or 8) of each chunk
-#pragma unroll
-                        for (int mt = 0; mt < MT; mt += 2) {
-                            float4 four;
-                            four.x = o[nq][mt][x] * factor, four.y = o[nq][mt][2 + x] * factor;
-                            four.z = o[nq][mt + 1][x] * factor, four.w = o[nq][mt + 1][2 + x] * factor;
-                            const int element = DP < 128 ? g * 8 + 2 * mt : (mt >> 3) * 128 + ((g >> 1) + 4 * (g & 1)) * 16 + 2 * (mt & 7);
-                            *reinterpret_cast<float4 *>(to + element) = four;
-                        }
-                    }
+                for (int mt = 0; mt < MT; mt += 2) {
+                    float4 four;
+                    four.x = o[mt][x] * factor, four.y = o[mt][2 + x] * factor;
+                    four.z = o[mt + 1][x] * factor, four.w = o[mt + 1][2 + x] * factor;
+                    const int element = DP < 128 ? g * 8 + 2 * mt : (mt >> 3) * 128 + ((g >> 1) + 4 * (g & 1)) * 16 + 2 * (mt & 7);
+                    *reinterpret_cast<float4 *>(to + element) = four;
                 }
             }
-            __syncthreads();
-            const int live = min(PASS, rows - PASS * pass);
-            for (int i = int(threadIdx.x); i < live * (DP / 4); i += kWarps * 32) {
-                const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
-                float4 y = {};
-                float top = -INFINITY, weights = 0.f;
-#pragma unroll
-                for (int v = 0; v < kWarps; ++v) {
-                    top = fmaxf(top, joinMax[v][PASS * pass + row]);
-                    const float4 a = *reinterpret_cast<const float4 *>(results + (v * PASS + row) * kPitch + d);
-                    y.x += a.x, y.y += a.y, y.z += a.z, y.w += a.w;
-                }
-#pragma unroll
-                for (int v = 0; v < kWarps; ++v) {
-                    const float m = joinMax[v][PASS * pass + row];
-                    weights += joinSum[v][PASS * pass + row] * (top == -INFINITY ? 1.f : exp2Fast(m - top));
-                }
-                if (whole) {
-                    writeOut<T>(p, w.q.first, firstRow + PASS * pass + row, head, d, y, weights);
-                } else {
-                    float *to = split > 0 ? joined + (PASS * pass + row) * kPitch
-                                          : partialRow<DP>(p, blockIdx.x, at == begin ? 0 : 1, PASS * pass + row, ROWS);
-                    *reinterpret_cast<float4 *>(to + 4 + d - (split > 0 ? 4 : 0)) = y;
-                    if (d == 0) {
-                        to[split > 0 ? DP : 0] = top, to[split > 0 ? DP + 1 : 1] = weights;
-                    }
-                }
-            }
-            __syncthreads();
         }
+        __syncthreads();
+        for (int i = int(threadIdx.x); i < rows * (DP / 4); i += kWarps * 32) {
+            const int itsRow = i / (DP / 4), d = (i - itsRow * (DP / 4)) * 4;
+            float4 y = {};
+            float top = -INFINITY, weights = 0.f;
+#pragma unroll
+            for (int v = 0; v < kWarps; ++v) {
+                top = fmaxf(top, joinMax[v][itsRow]);
+                const float4 a = *reinterpret_cast<const float4 *>(results + (v * kTileRows + itsRow) * kPitch + d);
+                y.x += a.x, y.y += a.y, y.z += a.z, y.w += a.w;
+            }
+#pragma unroll
+            for (int v = 0; v < kWarps; ++v) {
+                weights += joinSum[v][itsRow] * (top == -INFINITY ? 1.f : exp2Fast(joinMax[v][itsRow] - top));
+            }
+            if (whole) {
+                writeOut<T>(p, w.q.first, firstRow + itsRow, head, d, y, weights);
+            } else {
+                float *to = split > 0 ? joined + itsRow * kPitch : partialRow<DP>(p, blockIdx.x, at == begin ? 0 : 1, itsRow);
+                *reinterpret_cast<float4 *>(to + 4 + d - (split > 0 ? 4 : 0)) = y;
+                if (d == 0) {
+                    to[split > 0 ? DP : 0] = top, to[split > 0 ? DP + 1 : 1] = weights;
+                }
+            }
+        }
+        __syncthreads();
         if (split > 1) { // the cluster's parts as one: elements in turn
             clusterSync();
             const uint32_t from = smemAddr(joined);
             for (int i = int(threadIdx.x) + rank * (kWarps * 32); i < rows * (DP / 4); i += split * (kWarps * 32)) {
-                const int row = i / (DP / 4), d = (i - row * (DP / 4)) * 4;
+                const int itsRow = i / (DP / 4), d = (i - itsRow * (DP / 4)) * 4;
                 float top = -INFINITY, weights = 0.f;
                 float4 y = {};
                 for (int r = 0; r < split; ++r) {
-                    top = fmaxf(top, loadCluster(mapToCta(from + uint32_t((row * kPitch + DP) * 4), uint32_t(r))).x);
+                    top = fmaxf(top, loadCluster(mapToCta(from + uint32_t((itsRow * kPitch + DP) * 4), uint32_t(r))).x);
                 }
                 for (int r = 0; r < split; ++r) {
-                    const float4 stats = loadCluster(mapToCta(from + uint32_t((row * kPitch + DP) * 4), uint32_t(r)));
-                    const float4 a = loadCluster(mapToCta(from + uint32_t((row * kPitch + d) * 4), uint32_t(r)));
+                    const float4 stats = loadCluster(mapToCta(from + uint32_t((itsRow * kPitch + DP) * 4), uint32_t(r)));
+                    const float4 a = loadCluster(mapToCta(from + uint32_t((itsRow * kPitch + d) * 4), uint32_t(r)));
                     const float factor = top == -INFINITY ? 1.f : exp2Fast(stats.x - top);
                     y.x += a.x * factor, y.y += a.y * factor, y.z += a.z * factor, y.w += a.w * factor;
                     weights += stats.y * factor;
                 }
-                writeOut<T>(p, w.q.first, firstRow + row, head, d, y, weights);
+                writeOut<T>(p, w.q.first, firstRow + itsRow, head, d, y, weights);
             }
             __syncwarp();
             clusterSync(); // nobody leaves while its part is being read
@@ -619,26 +582,26 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
 // results, pieces in turn over the warps, so that a row in hundreds of pieces (one long sequence) waits for a few reads only.
 constexpr int kMostPieces = 1024;
 
-template <int DP, int NQ, bool HALF>
+template <int DP, bool HALF>
 __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const AttendParams p, const int count) {
-    constexpr int ROWS = 8 * NQ, THREADS = kWarps * 32;
+    constexpr int THREADS = kWarps * 32;
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     __shared__ int parts[2][kWarps];
     __shared__ float factors[kMostPieces], stats[2][kWarps];
     __shared__ float4 sums[THREADS];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    // the tiles of all sequences in a row, those of a sequence without work included: ceil(max_new * group / ROWS) * heads each
+    // the tiles of all sequences in a row, those of a sequence without work included: ceil(max_new * group / kTileRows) * heads each
     const int perSequence = int(gridDim.x) / p.batch.sequences, lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5;
     const int index = int(blockIdx.x) / perSequence, tile = int(blockIdx.x) - index * perSequence;
     // the steps of all sequences, and of those in front of this one
     int all = 0, front = 0;
     for (int b = int(threadIdx.x); b < p.batch.sequences; b += THREADS) {
-        const int work = fewWorkOf<ROWS>(p, b).work;
+        const int work = fewWorkOf(p, b).work;
         all += work;
         front += b < index ? work : 0;
     }
-    const FewWork w = fewWorkOf<ROWS>(p, index);
-    const int row = int(blockIdx.y), head = tile % p.cache.heads, firstRow = tile / p.cache.heads * ROWS;
+    const FewWork w = fewWorkOf(p, index);
+    const int row = int(blockIdx.y), head = tile % p.cache.heads, firstRow = tile / p.cache.heads * kTileRows;
     if (tile >= w.tiles || row >= w.q.fresh * p.group - firstRow || w.steps < 2) { // (the whole block)
         return;
     }
@@ -658,7 +621,7 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
         return; // written by that piece
     }
     const int first = x0 == pieces.start(c0) ? 0 : 1; // where piece c0 left it: as its first tile, or as its last
-    const auto part = [&](int c) { return partialRow<DP>(p, c0 + c, c == 0 ? first : 0, row, ROWS); };
+    const auto part = [&](int c) { return partialRow<DP>(p, c0 + c, c == 0 ? first : 0, row); };
     float top = -INFINITY;
     for (int c = int(threadIdx.x); c < n; c += THREADS) {
         top = fmaxf(top, part(c)[0]);
@@ -718,7 +681,7 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
 
 int paddedHead(int headDim) { return headDim <= 64 ? 64 : headDim <= 128 ? 128 : 256; }
 
-template <int DP, int NQ, bool HALF> int launchFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
+template <int DP, bool HALF> int launchFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
     using Shape = FewShape<DP>;
     CUtensorMap k, v;
     if (!makeCacheMap(&k, p.cache.keys, p.cache, Shape::kPanel, kGroup, true) ||
@@ -726,7 +689,7 @@ template <int DP, int NQ, bool HALF> int launchFew(const AttendParams &p, const 
         return MLEL_ERROR_DEVICE;
     }
     constexpr size_t smemBytes = Shape::kRing + 1024;
-    const auto kernel = pagedAttentionFewKernel<DP, NQ, HALF>;
+    const auto kernel = pagedAttentionFewKernel<DP, HALF>;
     if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), smemBytes)) {
         return MLEL_ERROR_DEVICE;
     }
@@ -749,18 +712,11 @@ template <int DP, int NQ, bool HALF> int launchFew(const AttendParams &p, const 
     cfg.numAttrs = unsigned(count);
     cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, k, v, p, plan.split);
     if (err == cudaSuccess && plan.workspace > 0) {
-        const int64_t rows = std::max<int64_t>(1, int64_t(p.batch.maxNew) * p.group), tiles = (rows + 8 * NQ - 1) / (8 * NQ) * p.cache.heads;
-        err = launchOverlapped(pagedAttentionFewJoin<DP, NQ, HALF>,
-                               dim3(unsigned(tiles * p.batch.sequences), unsigned(std::min<int64_t>(rows, 8 * NQ))), kWarps * 32, 0, s, p, plan.blocks);
+        const int64_t rows = std::max<int64_t>(1, int64_t(p.batch.maxNew) * p.group), tiles = (rows + kTileRows - 1) / kTileRows * p.cache.heads;
+        err = launchOverlapped(pagedAttentionFewJoin<DP, HALF>,
+                               dim3(unsigned(tiles * p.batch.sequences), unsigned(std::min<int64_t>(rows, kTileRows))), kWarps * 32, 0, s, p, plan.blocks);
     }
     return launchStatus("mlel_cuda_paged_attention", err);
-}
-
-template <int DP> int launchFewRows(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
-    if (plan.rows == 8) {
-        return p.halves ? launchFew<DP, 1, true>(p, plan, s) : launchFew<DP, 1, false>(p, plan, s);
-    }
-    return p.halves ? launchFew<DP, 2, true>(p, plan, s) : launchFew<DP, 2, false>(p, plan, s);
 }
 
 } // namespace
@@ -769,14 +725,13 @@ FewPlan pagedAttentionFewPlan(const AttendParams &p) {
     FewPlan plan{};
     const int dp = paddedHead(p.cache.headDim);
     const int64_t rows = std::max<int64_t>(1, int64_t(p.batch.maxNew) * p.group); // (without new tokens the sequences are looked at all the same)
-    plan.rows = rows <= 8 ? 8 : kFewRows;
     // the most tiles and steps that the batch can have
     const int64_t steps = std::max<int64_t>(1, (int64_t(p.batch.maxLength) + kGroup * kStepGroups - 1) / (kGroup * kStepGroups));
-    const int64_t tiles = (rows + plan.rows - 1) / plan.rows * p.cache.heads * p.batch.sequences, work = steps * tiles;
+    const int64_t tiles = (rows + kTileRows - 1) / kTileRows * p.cache.heads * p.batch.sequences, work = steps * tiles;
     if (work > 0x7fffffff) {
         refuse("mlel_cuda_paged_attention", "sequences, tokens and lengths give too much work for one call");
     }
-    const int64_t resident = int64_t(dp * plan.rows <= 8 * 128 ? 3 : 2) * smCount();
+    const int64_t resident = int64_t(dp <= 128 ? 3 : 2) * smCount();
     int split = 1;
     while (split < 8 && split < steps && tiles * split * 2 <= resident) {
         split *= 2;
@@ -787,13 +742,16 @@ FewPlan pagedAttentionFewPlan(const AttendParams &p) {
         return plan;
     }
     plan.blocks = int(std::max<int64_t>(1, std::min<int64_t>({work, resident, kMostPieces})));
-    plan.workspace = steps > 1 && plan.blocks > 1 ? uint64_t(plan.blocks) * 2 * uint64_t(plan.rows) * uint64_t(dp + 4) * 4 : 0;
+    plan.workspace = steps > 1 && plan.blocks > 1 ? uint64_t(plan.blocks) * 2 * kTileRows * uint64_t(dp + 4) * 4 : 0;
     return plan;
 }
 
 int pagedAttentionFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s) {
     const int dp = paddedHead(p.cache.headDim);
-    return dp == 256 ? launchFewRows<256>(p, plan, s) : dp == 128 ? launchFewRows<128>(p, plan, s) : launchFewRows<64>(p, plan, s);
+    if (p.halves) {
+        return dp == 256 ? launchFew<256, true>(p, plan, s) : dp == 128 ? launchFew<128, true>(p, plan, s) : launchFew<64, true>(p, plan, s);
+    }
+    return dp == 256 ? launchFew<256, false>(p, plan, s) : dp == 128 ? launchFew<128, false>(p, plan, s) : launchFew<64, false>(p, plan, s);
 }
 
 int takePagedErrorFew() { return takePagedError(); }

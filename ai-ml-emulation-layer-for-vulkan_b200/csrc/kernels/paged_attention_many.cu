@@ -838,10 +838,10 @@ template <int DP> int launchManyType(const AttendParams &p, cudaStream_t s) {
 
 } // namespace
 
-// More rows per cache head than one tile of the kernel for few of them has.  (That kernel with tiles of 32 rows, 16 sequences of up to
-// 4000 tokens, 8 heads of 128 elements: 20 rows 83 us and here 75, 32 rows 88 and 76, 64 rows 120 and 76; one of 16000, 32 rows: 45
-// and 45.)
-bool pagedAttentionManyApplies(const AttendParams &p) { return int64_t(p.batch.maxNew) * p.group > kFewRows; }
+// More than 32 rows per cache head, or 16 of more than 128 elements.  (The kernel for few of them, whose tiles have 8 rows, and this
+// one: 16 sequences of up to 4000 tokens, 8 heads of 128 elements, 32 rows 56 and 64 us, 48 rows 77 and 64; 4 heads of 256, 12 rows 39
+// and 56, 24 rows 60 and 57.)
+bool pagedAttentionManyApplies(const AttendParams &p) { return int64_t(p.batch.maxNew) * p.group > (p.cache.headDim <= 128 ? 32 : 16); }
 int pagedAttentionMany(const AttendParams &p, cudaStream_t s) {
     return p.cache.headDim <= 64 ? launchManyType<64>(p, s) : p.cache.headDim <= 128 ? launchManyType<128>(p, s) : launchManyType<256>(p, s);
 }

@@ -374,7 +374,7 @@ CHUNKS = [(40, 40), (1, 70), (130, 200), (17, 400), (0, 3), (64, 64), (129, 129)
 
 
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
-@pytest.mark.parametrize("heads, group", [(2, 1), (2, 4), (1, 5), (1, 16), (1, 20), (2, 40)])
+@pytest.mark.parametrize("heads, group", [(2, 1), (2, 4), (1, 5), (1, 9), (1, 16), (1, 20), (2, 32), (2, 40)])
 @pytest.mark.parametrize("page, d", [(16, 64), (64, 128), (48, 80), (32, 256), (256, 16), (16, 96)])
 def test_attention_single_tokens(serving, dtype, heads, group, page, d):
     t = DTYPES[dtype]
