@@ -211,14 +211,23 @@ template <class T, bool WIDE> __device__ __forceinline__ void appendUnit(const A
         }
 #pragma unroll
         for (int h = 0; h < kHeldPairs; ++h) {
-            if (at + h * kSideThreads < fresh * vectors) {
-                VectorPair v;
-                int token;
-                float x[8], y[8];
-                heldPair(h, v, token, x, y, product);
+            const int i = at + h * kSideThreads;
+            if (i < fresh * vectors) {
+                if (rotates && vectorPair(p, i - int(fastDiv(uint32_t(i), p.vectors)) * vectors).turned) {
+                    VectorPair v;
+                    int token;
+                    float x[8], y[8];
+                    heldPair(h, v, token, x, y, product);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    magnitude = max(magnitude, max(__float_as_uint(x[j]) & 0x7fffffffu, __float_as_uint(y[j]) & 0x7fffffffu));
+                    for (int j = 0; j < 8; ++j) {
+                        magnitude = max(magnitude, max(__float_as_uint(x[j]) & 0x7fffffffu, __float_as_uint(y[j]) & 0x7fffffffu));
+                    }
+                } else { // magnitudes of 16 bits are ordered like their bits
+                    constexpr uint32_t kSigns = 0x7fff7fffu;
+                    const uint4 a = one[h], b = two[h];
+                    const uint32_t m = maxHalves(maxHalves(maxHalves(a.x & kSigns, a.y & kSigns), maxHalves(a.z & kSigns, a.w & kSigns)),
+                                                 maxHalves(maxHalves(b.x & kSigns, b.y & kSigns), maxHalves(b.z & kSigns, b.w & kSigns)));
+                    magnitude = max(magnitude, __float_as_uint(unpackTwo(max(m & 0xffffu, m >> 16), T()).x));
                 }
             }
         }
@@ -368,24 +377,37 @@ template <class T, bool WIDE> __device__ __forceinline__ void appendUnit(const A
                 float x[8], y[8];
                 uint32_t product = 0;
                 heldPair(h, v, token, x, y, product);
+                // (as quantizeEight: the nearest whole number by one fused multiply-add, how far the product lies from it by another)
                 constexpr float kMagic = 12582912.f;
-                uint32_t a[8], b[8], doubtful = 0;
+                uint32_t a[8], b[8];
+                float farthest = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float q0 = x[j] * inverse32, q1 = y[j] * inverse32, t0 = q0 + kMagic, t1 = q1 + kMagic;
-                    doubtful |= !(fabsf(q0 - (t0 - kMagic)) <= middle) ? 1u << j : 0u;
-                    doubtful |= !(fabsf(q1 - (t1 - kMagic)) <= middle) ? 256u << j : 0u;
-                    a[j] = some ? __float_as_uint(t0) : 0u, b[j] = some ? __float_as_uint(t1) : 0u;
+                    const float t0 = fmaf(x[j], inverse32, kMagic), t1 = fmaf(y[j], inverse32, kMagic);
+                    farthest = fmaxf(farthest, fmaxf(fabsf(fmaf(x[j], inverse32, kMagic - t0)), fabsf(fmaf(y[j], inverse32, kMagic - t1))));
+                    a[j] = __float_as_uint(t0), b[j] = __float_as_uint(t1);
                 }
                 if (rotates && v.turned) {
                     pairDown(p.interleaved != 0, a, b);
                 }
-                *reinterpret_cast<uint2 *>(to + token * D + v.one) = {lowBytes(a[0], a[1], a[2], a[3]), lowBytes(a[4], a[5], a[6], a[7])};
-                *reinterpret_cast<uint2 *>(to + token * D + v.two) = {lowBytes(b[0], b[1], b[2], b[3]), lowBytes(b[4], b[5], b[6], b[7])};
-                while (doubtful != 0u && some) {
-                    const int d = elementOf(v, __ffs(int(doubtful)) - 1);
-                    doubtful &= doubtful - 1u;
-                    to[token * D + d] = int8_t(roundedExactly(element(token, d), inverse, double(now), careful));
+                const uint2 low = {lowBytes(a[0], a[1], a[2], a[3]), lowBytes(a[4], a[5], a[6], a[7])},
+                            high = {lowBytes(b[0], b[1], b[2], b[3]), lowBytes(b[4], b[5], b[6], b[7])};
+                *reinterpret_cast<uint2 *>(to + token * D + v.one) = some ? low : uint2{0u, 0u};
+                *reinterpret_cast<uint2 *>(to + token * D + v.two) = some ? high : uint2{0u, 0u};
+                if (__builtin_expect(some && !(farthest <= middle), 0)) {
+                    uint32_t doubtful = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float t0 = fmaf(x[j], inverse32, kMagic), t1 = fmaf(y[j], inverse32, kMagic);
+                        doubtful |= !(fabsf(fmaf(x[j], inverse32, kMagic - t0)) <= middle) ? 1u << j : 0u;
+                        doubtful |= !(fabsf(fmaf(y[j], inverse32, kMagic - t1)) <= middle) ? 256u << j : 0u;
+                    }
+#pragma unroll 1
+                    while (doubtful != 0u) {
+                        const int d = elementOf(v, __ffs(int(doubtful)) - 1);
+                        doubtful &= doubtful - 1u;
+                        to[token * D + d] = int8_t(roundedExactly(element(token, d), inverse, double(now), careful));
+                    }
                 }
             }
         }
