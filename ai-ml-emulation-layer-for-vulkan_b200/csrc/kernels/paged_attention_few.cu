@@ -32,7 +32,8 @@
 //
 // bf16 queries become f16 after a row-wise power of two that puts the largest at 2^14; elements down to 2^-29 of that stay
 // exact.  Weights are rounded to f16: p * (v scale / reference) * 2^14, the reference a running power of two, so that
-// what is lost lies 2^-38 below the largest.  The result stays in registers in units of that reference; it is
+// what is lost lies 2^-38 below the largest.  The sum is over the weights as they are rounded, so that what rounding does to
+// the key that has most of a row cancels.  The result stays in registers in units of that reference; it is
 // rescaled only when a maximum or the reference grows, which one vote per 32 keys finds out.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -436,18 +437,24 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
                     const float weightUnit = valueScale[h] * perReference;
+                    const bool rounded = weightUnit >= 256.f && weightUnit < INFINITY; // no weight that matters is a subnormal number
+                    float2 part = {0.f, 0.f};
                     uint32_t wf[2]; // P^T: keys in pairs by t, row g
                     const float shift0 = most[0] == -INFINITY ? 0.f : most[0], shift1 = most[1] == -INFINITY ? 0.f : most[1];
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const float x0 = s[h][2 * half], x1 = s[h][2 * half + 1];
                         const float p0 = exp2Fast(x0 - shift0), p1 = exp2Fast(x1 - shift1);
-                        sum[0] += p0, sum[1] += p1;
                         // what the mask hides stays out, whatever its page's scale is
                         const float w0 = masked && x0 == -INFINITY ? 0.f : p0 * weightUnit;
                         const float w1 = masked && x1 == -INFINITY ? 0.f : p1 * weightUnit;
-                        wf[half] = transposeHalves(packTwo(w0, w1, __half()));
+                        const uint32_t two = packTwo(w0, w1, __half());
+                        wf[half] = transposeHalves(two);
+                        const float2 w = rounded ? unpackTwo(two, __half()) : float2{p0, p1};
+                        part.x += w.x, part.y += w.y;
                     }
+                    const float perUnit = rounded ? __fdividef(1.f, weightUnit) : 1.f;
+                    sum[0] = fmaf(part.x, perUnit, sum[0]), sum[1] = fmaf(part.y, perUnit, sum[1]);
                     constexpr int CHUNKS = DP < 128 ? 1 : DP / 128, WORDS = DP < 128 ? 2 : 4; // 16 (or, below 128, 8) bytes of a value row per lane each
                     const uint32_t group = values + uint32_t(h * Shape::kGroupBytes);
 #pragma unroll

@@ -116,8 +116,10 @@ def attend(data, scales, starts, lengths, table, q, scale, causal, window, softc
                 p /= p.sum()
                 o, most = p @ v[lo:hi], p @ np.abs(v[lo:hi])
                 out[first + i, h] = o
-                # weights: twice the scores' error (numerator and sum), f16's half step, the exponential's and the sums' roundings
-                error = most * (2 * off + 2.0 ** -11 + 2.0 ** -20 + (hi - lo) * 2.0 ** -23)
+                # weights: twice the scores' error (numerator and sum), twice f16's half step (the sum may be over the rounded weights:
+                # with w (1 + e) for w, |e| <= u, the result moves by |sum w e (v - o)| / sum w (1 + e) <= 2 u / (1 - u) sum w |v|), the
+                # exponential's and the sums' roundings
+                error = most * (2 * off + 2 * 2.0 ** -11 + 2.0 ** -20 + (hi - lo) * 2.0 ** -23)
                 # f16 has steps of 2^-24 at its lower end.  Weights are held as p * scale / r * 2^n, r at most twice the largest
                 # scale of the sequence's pages (rows of one call are weighed together, whatever the mask leaves to each), and n at least 7 (more would leave no room for a maximum that grows by up to 2^8 before it is
                 # taken up), so half a step is 2^-25 * 2^-7 * 2 * scale = 2^-31 * scale for each integer; sums of p are at least 1
