@@ -5,7 +5,8 @@
 // with the protocol of the pair in gemm_i8_pair.cu's head (barriers full, empty, accFull, accEmpty), persistent over the tiles, two
 // accumulators, so that the epilogue of a tile runs under the products of the next.
 //
-// What bounds it: the tensor pipe.  A K block of 128 takes a pair 512 cycles at BN = 256 and brings each CTA 32 KB.
+// What bounds it: the tensor pipe.  A K block of 128 takes a pair 512 cycles at BN = 256 and brings each CTA 32 KB.  8192 x 8192 x 8192:
+// 369 us, 2.98 POP/s.
 //
 // Epilogue: a lane has one token, its columns are neighbouring channels: integer to float, times the two scales, plus the bias, packed
 // and put into a 128-byte swizzled box of 32 rows of the warp's own, which a bulk tensor store takes to the output.  No

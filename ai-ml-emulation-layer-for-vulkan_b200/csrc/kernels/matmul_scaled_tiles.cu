@@ -245,7 +245,7 @@ int matmulScaledOnTiles(const ScaledProblem &p, int32_t dtype, cudaStream_t s) {
     const int64_t tiles = int64_t((p.N + kChannels - 1) / kChannels) * ((p.M + width - 1) / width);
     const int allKb = (p.K + BK - 1) / BK;
     // What a tile's sum is split into: as the SM with the most CTAs sees it, each CTA costs its K blocks and as much as three more
-    // for its start and end.  (56 x 8192 x 10240, 80 tiles of 64 K blocks: 28 us in 2 parts, see the table of the cases for 5.)
+    // for its start and end.  (56 x 8192 x 10240, 80 tiles of 64 K blocks: 28 us in 2 parts, 20 in 5.)
     const int64_t sms = smCount(), resident = (width == 128 ? 2 : 3) * sms;
     int split = 1;
     int64_t best = 0;

@@ -11,7 +11,8 @@
 // Integers are those of exact arithmetic.  A rotated key u c - w s in 32 bits is off by at most 2^-24 (|w s| + the result): the
 // largest magnitude is formed again in 64 bits from the elements within twice that of the largest found, and a quotient
 // that lies as near to the middle between two integers is decided in 64 bits.  (All of it in 64 bits, in two passes over the
-// tokens: 68 us for the keys and values of 6600 tokens with 8 heads of 128 elements, so 26.)  A unit of up to 512 vector
+// tokens: 87 us for 8270 tokens with 8 heads of keys and 32 of queries, 128 elements each, so 63: some 25 of them the queries', at
+// 5.4 TB/s.)  A unit of up to 512 vector
 // pairs stays in registers between the two; larger ones, and magnitudes beyond 32 bits, take two passes in 64 bits.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -555,7 +556,7 @@ template <class T, bool WIDE> cudaError_t launchAppend(const AppendParams &p, cu
     const bool wideUnits = WIDE && int64_t(p.batch.maxNew) * p.cache.headDim > kShortUnit;
     const auto kernel = wideUnits ? pagedAppendKernel<T, WIDE, WIDE> : pagedAppendKernel<T, false, WIDE>;
     // Up to eight blocks an SM one launch for both (64 tokens: 5.8 us; as two launches 8.0).  Above, the queries, which have most of
-    // the bytes, in a kernel whose registers let four times as many threads wait for memory (6600 tokens: 107 and 87 us).
+    // the bytes, in a kernel whose registers let four times as many threads wait for memory (8270 tokens, with units in 64 bits: 107 and 87 us).
     if (p.unitBlocks + tokens <= 8 * kNumSMs || tokens == 0) {
         return launchOverlapped(kernel, dim3(unsigned(p.unitBlocks) + tokens), 2 * kSideThreads, 0, s, p);
     }

@@ -15,15 +15,16 @@
 //
 // What bounds it: per 256 x 128 scores the products take 2048 cycles at 128 elements a head, and 32768 exponentials the
 // same at 16 a cycle; everything else (a multiply-add, half a maximum, half a sum, half a conversion per score, and the
-// keys' and values' conversion) shares the four schedulers with them.
+// keys' and values' conversion) shares the four schedulers with them: some 4500 cycles.  Four prompts of 6000 tokens, 32 heads of 128
+// elements over 8: 822 us, 773 TFLOP/s.
 //
 // Softmax in one pass where it can: scores are weighed with the maximum known from the tiles before, and only if one exceeds
 // it by more than 2^8, or at a row's first tile and where the values' reference grows, the maximum is taken first and sums
 // and result are rescaled.  The scale of 16 values is part of the exponent: w = 2^(s - m + log2(scale / r) + 7), r a
-// running power of two, and the sum over the weights of 16 keys is divided by it again.  For f16 results the
-// sum is over the weights as they are rounded, so that what rounding does to the key that has most of a row cancels (a fifth off the
-// error against 64 bits; bf16 has steps eight times as large, and four prompts of 6000 tokens would take 899 us for 822).  So a weight is at most 2^15, f16's steps
-// end 2^-31 below the largest, and values whose scale is below 2^-60 of r count as nothing.
+// running power of two, and the sum over the weights of 16 keys is divided by it again.  So a weight is at most 2^15, f16's steps
+// end 2^-31 below the largest, and values whose scale is below 2^-60 of r count as nothing.  For f16 results the sum is over the
+// weights as they are rounded, so that what rounding does to the key that has most of a row cancels (a seventh off the error
+// against 64 bits; bf16 has steps eight times as large, and four prompts of 6000 tokens would take 899 us for 822).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
