@@ -408,6 +408,15 @@ def test_attention_chunks_of_long_sequences(serving, sequences, heads, group, d,
     check_attention(serving, p, *query(p, heads * group, torch.float16), torch.float16, **how)
 
 
+@pytest.mark.parametrize("fresh, d, how", [(3, 64, {}), (7, 128, {"window": 900}), (3, 256, {"softcap": 5.0}), (4, 256, {})], ids=str)
+def test_attention_several_tiles_share_the_line(serving, fresh, d, how):
+    """Drafts of several tiles of eight rows, cut into pieces over the whole device and joined: many sequences, some long."""
+    lengths = [2000, 9, 1500, 40, 300, 17] + [(37 * i) % 120 + fresh for i in range(54)]
+    p = Paged(serving, fresh + d, [(min(fresh, 1 + i % fresh) if i % 5 else 0 if i % 2 else fresh, n) for i, n in enumerate(lengths)], 4, 16, d)
+    check_attention(serving, p, *query(p, 16, torch.float16), torch.float16, **how)
+    assert any(v > 0 for v in p.batch._space.values()), "the case is meant to want a workspace"
+
+
 @pytest.mark.parametrize("sequences", [[(1, 300)], [(100, 300)]], ids=["one", "chunk"])
 def test_attention_one_key_has_all(serving, sequences):
     """A score that drowns all others: the answer is that token's value; and thousands of others share what is left."""
