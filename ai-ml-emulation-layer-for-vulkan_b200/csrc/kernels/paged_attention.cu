@@ -22,6 +22,9 @@ AttendParams paramsOf(const std::string &call, const mlel_paged_cache *cache, co
     p.batch = batchOf(call, batch, p.cache, q.dims[0]);
     p.queries = q.ptr, p.queryStride[0] = q.strides[0], p.queryStride[1] = q.strides[1];
     p.queryHeads = int32_t(q.dims[1]), p.group = p.queryHeads / p.cache.heads;
+    if (int64_t(p.batch.maxNew) * p.group > 0x7fffffff - kMostRowsOfBlock) { // the kernels number a sequence's rows in 32 bits
+        refuse(call, "a sequence may have more than 2^31 rows of queries per cache head");
+    }
     p.halves = q.dtype == MLEL_F16;
     p.wideQueries = aligned(q.ptr, 16) && q.strides[0] % 16 == 0 && q.strides[1] % 16 == 0;
     p.pageDiv = makeFastDiv(p.cache.page), p.groupDiv = makeFastDiv(p.group);

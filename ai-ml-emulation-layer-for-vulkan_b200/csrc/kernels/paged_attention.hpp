@@ -10,6 +10,8 @@
 
 namespace mlel {
 
+constexpr int kMostRowsOfBlock = 256; // the rows of a sequence are handed out in blocks of at most so many
+
 struct AttendParams {
     PagedCache cache;
     PagedBatch batch;

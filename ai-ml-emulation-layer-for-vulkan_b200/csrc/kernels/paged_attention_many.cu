@@ -192,6 +192,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                   kSoftmaxWarps = Shape::kSoftmaxWarps, kCopyWarp = Shape::kCopyWarp, kProductWarp = Shape::kProductWarp,
                   kBlockRows = Shape::kTilesOfRows * kRows;
     constexpr int kPitch = DP + 4; // floats between the rows of a part
+    static_assert(kBlockRows <= kMostRowsOfBlock, "row numbers of the last block fit 32 bits");
     static_assert(size_t(kBlockRows) * kPitch * 4 <= Shape::kTilesOfRows * size_t(Shape::kQueryBytes) + kSlots * size_t(Shape::kSlotBytes),
                   "the parts of the rows fit the queries' and keys' memory");
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;

@@ -3,6 +3,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "../graph_pipeline.hpp"
@@ -114,7 +115,9 @@ inline PagedBatch batchOf(const std::string &call, const mlel_paged_batch *batch
     b.starts = reinterpret_cast<const int32_t *>(starts.ptr), b.lengths = reinterpret_cast<const int32_t *>(lengths.ptr);
     b.table = reinterpret_cast<const int32_t *>(table.ptr);
     b.tableStride = table.strides[0] / 4;
-    b.sequences = int32_t(lengths.dims[0]), b.maxNew = batch->max_new, b.maxLength = batch->max_length, b.tokens = int32_t(tokens);
+    // no sequence has more new tokens than the token axis: a loose bound costs nothing
+    b.sequences = int32_t(lengths.dims[0]), b.maxNew = int32_t(std::min<int64_t>(batch->max_new, tokens)), b.maxLength = batch->max_length;
+    b.tokens = int32_t(tokens);
     return b;
 }
 

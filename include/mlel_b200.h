@@ -465,8 +465,8 @@ typedef struct mlel_paged_cache {
  * axis; those of sequence b are rows starts[b] .. starts[b + 1] - 1 (none at all is allowed).  lengths[b] counts the
  * tokens of the sequence with the new ones, which are its last.  Token t of sequence b is row t % page of page
  * page_table[b][t / page]; entries past the last token are not read.  Rows of the token axis outside starts[0] ..
- * starts[sequences] are neither read nor written.  max_new and max_length bound the new tokens and the lengths of any
- * sequence of the call; closer bounds make better launches.
+ * starts[sequences] are neither read nor written.  max_new and max_length (at most 2^30) bound the new tokens and the lengths of
+ * any sequence of the call; closer bounds make better launches (max_new above the rows of the token axis counts as those).
  * starts, lengths and page_table are read on the device.  A sequence whose numbers contradict these bounds or the shapes is left
  * out as a whole (its rows are not written), a page outside the cache by itself (nothing is written there, and its tokens are not
  * attended to); mlel_paged_error() tells of both. */

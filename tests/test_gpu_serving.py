@@ -703,3 +703,29 @@ def test_offsets_beyond_32_bits(serving):
         y = cache.attend(q, batch)
         assert torch.equal(data[:, 0], data[:, -1]) and (data[:, 0, :, :fresh] != 0).any()
         assert torch.equal(y[:fresh], y[fresh:]) and y.abs().max() > 0
+
+
+@pytest.mark.parametrize("sequences, group", [([(3, 300), (1, 40), (2, 2)], 3), ([(60, 300), (1, 700), (33, 33)], 8)], ids=["few", "many"])
+@pytest.mark.parametrize("bound", [1 << 28, 1 << 30])
+def test_loose_bounds_on_new_tokens(serving, sequences, group, bound):
+    """Bounds far above the tokens there are, whose rows 32 bits would not count."""
+    p = Paged(serving, 61, sequences, 2, 256, 64, skip=1, behind=2)
+    wide = torch.full((3, bound // 256), -1, dtype=torch.int32, device="cuda")
+    wide[:, :p.batch.page_table.shape[1]] = p.batch.page_table
+    p.batch = serving.PagedBatch(p.batch.starts, p.batch.lengths, wide, bound, bound)
+    q, out = query(p, 2 * group, torch.float16)
+    check_attention(serving, p, q, out, torch.float16)
+    k, v = randn(p.g, p.tokens, 2, 64).half(), randn(p.g, p.tokens, 2, 64).half()
+    before = p.arrays()
+    p.cache.append(k, v, None, None, p.batch)
+    want, want_scales = ref.append(*before, ref.f64(k), ref.f64(v), None, None, False)
+    assert np.array_equal(p.scales.cpu().numpy(), want_scales, equal_nan=True) and np.array_equal(p.data.cpu().numpy(), want)
+
+
+def test_page_table_of_a_larger_program_with_many_rows(serving):
+    """The kernel for many rows over rows of a page table that are wider than needed, and lengths far below their bound."""
+    p = Paged(serving, 52, [(1, 100), (30, 300), (1, 40)], 2, 16, 64)
+    wide = torch.full((3, 1000), -1, dtype=torch.int32, device="cuda")
+    wide[:, :p.batch.page_table.shape[1]] = p.batch.page_table
+    p.batch = serving.PagedBatch(p.batch.starts, p.batch.lengths, wide, 40, 16000)
+    check_attention(serving, p, *query(p, 8, torch.float16), torch.float16)

@@ -165,6 +165,31 @@ def test_attention_refuses(calls, cache, change, word, status):
     assert refused(mlel, rc, word) == status
 
 
+def test_attention_refuses_rows_beyond_32_bits(calls):
+    """2^28 new tokens with eight query heads a cache head: more rows than a 32-bit number counts."""
+    mlel, lib = calls
+    c, b = paged(mlel, table=(I32, (3, 1 << 23)), max_new=1 << 28, max_length=1 << 28)
+    q = T(mlel, F16, (1 << 28, 16, 64))
+    rc = lib.mlel_cuda_paged_attention(*by(c, b, q, q), ctypes.c_float(0.125), 1, 0, ctypes.c_float(0.0), ctypes.c_void_p(0x10000),
+                                       ctypes.c_uint64(1 << 40), None)
+    assert refused(mlel, rc, "rows of queries") == -13
+    need = ctypes.c_uint64()
+    assert refused(mlel, lib.mlel_paged_attention_workspace(*by(c, b, q, need)), "rows of queries") == -13
+
+
+@pytest.mark.parametrize("loose", [31, 1 << 20, 1 << 28, 1 << 30])
+def test_loose_bounds_on_new_tokens_change_nothing(calls, loose):
+    """No sequence has more new tokens than the token axis: the launch is that of the close bound."""
+    mlel, lib = calls
+    needs = []
+    for bound in (3, loose):
+        c, b = paged(mlel, table=(I32, (3, 1 << 25)), max_new=bound, max_length=1 << 30)
+        need = ctypes.c_uint64()
+        assert lib.mlel_paged_attention_workspace(*by(c, b, T(mlel, F16, (3, 8, 64)), need)) == 0
+        needs.append(need.value)
+    assert needs[0] == needs[1] > 0
+
+
 def test_python_layer_refuses_host_tensors(mlel):
     import torch
     from mlel_b200 import serving
