@@ -36,7 +36,8 @@
 // exact.  Weights are rounded to f16: p * (v scale / reference) * 2^14, the reference a running power of two, so that
 // what is lost lies 2^-38 below the largest.  The sum is over the weights as they are rounded, so that what rounding does to
 // the key that has most of a row cancels.  The result stays in registers in units of that reference; it is
-// rescaled only when a maximum or the reference grows, which one vote per 32 keys finds out.
+// rescaled only when a maximum or the reference grows, which one vote per 32 keys finds out.  The reference does not go below
+// 2^-112: weights of values with smaller scales end 2^-151 above zero, which is below what a result of either type holds.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -61,6 +62,7 @@ constexpr int kGroup = 16; // keys that share a page and a scale for certain
 constexpr int kStageGroups = 2;
 constexpr int kStepGroups = kWarps * kStageGroups;
 constexpr float kWeightScale = 16384.f;
+constexpr float kLeastUnit = 0x1p-112f; // of the values' reference: kWeightScale over it is still a finite number
 constexpr int kClusterSteps = 3; // steps by which a cluster's blocks may outlast the line's
 
 template <int DP> struct FewShape {
@@ -412,7 +414,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                 }
                 const bool raise = magnitude > reference;
                 if (__any_sync(0xffffffffu, grows) || raise) {
-                    const float unit = raise ? powerAbove(magnitude) : reference;
+                    const float unit = raise ? fmaxf(powerAbove(magnitude), kLeastUnit) : reference;
                     const float shrink = raise ? (reference > 0.f ? reference / unit : 0.f) : 1.f;
                     reference = unit;
                     perReference = unit > 0.f ? kWeightScale / unit : 1.f;

@@ -729,3 +729,17 @@ def test_page_table_of_a_larger_program_with_many_rows(serving):
     wide[:, :p.batch.page_table.shape[1]] = p.batch.page_table
     p.batch = serving.PagedBatch(p.batch.starts, p.batch.lengths, wide, 40, 16000)
     check_attention(serving, p, *query(p, 8, torch.float16), torch.float16)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("mixed", [False, True], ids=["alone", "mixed"])
+@pytest.mark.parametrize("tiny", [1e-40, 1e-38, 1e-36, 4e-35])
+@pytest.mark.parametrize("sequences, group, d", [([(1, 200), (1, 1000), (1, 9)], 4, 128), ([(3, 700), (2, 40)], 2, 64), ([(1, 20000)], 8, 64),
+                                                 ([(130, 700), (1, 30)], 4, 128), ([(40, 300)], 2, 256), ([(70, 5000)], 1, 128)])
+def test_attention_with_the_smallest_value_scales(serving, sequences, group, d, tiny, mixed, dtype):
+    """Pages whose values are next to nothing, as the append leaves them: alone, and among ordinary ones."""
+    t = DTYPES[dtype]
+    p = Paged(serving, group + d, sequences, 1, 16, d, wild=False)
+    small = torch.rand(p.scales[1].shape, generator=p.g, device="cuda") < (0.6 if mixed else 2.0)
+    p.scales[1, small] = tiny
+    check_attention(serving, p, *query(p, group, t, 0.2), t)
