@@ -714,7 +714,8 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 part[DP] = most, part[DP + 1] = sum;
             }
         } else if (ok) { // ---- the rows, by way of the queries' memory, which no product reads any more ----
-            const float f = sum == 0.f ? 0.f : exp2f(float(reference) - kWeightBits) / sum;
+            // two factors, since their product may be too small for all its bits
+            const float f = sum == 0.f ? 0.f : 1.f / sum, unit = exp2f(float(reference) - kWeightBits);
             uint8_t *mine = queries + which * Shape::kQueryBytes + (quarter * 2 + half) * (32 * DP);
             constexpr int kChunks = DP / 16, kLinesAtOnce = 32 / kChunks; // 16-byte chunks of half a row
 #pragma unroll 1
@@ -725,7 +726,8 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 uint32_t w[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float x = sum == 0.f ? 0.f : __uint_as_float(o[2 * j]) * f, y = sum == 0.f ? 0.f : __uint_as_float(o[2 * j + 1]) * f;
+                    const float x = sum == 0.f ? 0.f : __uint_as_float(o[2 * j]) * f * unit,
+                                y = sum == 0.f ? 0.f : __uint_as_float(o[2 * j + 1]) * f * unit;
                     w[j] = packTwo(x, y, T());
                 }
 #pragma unroll

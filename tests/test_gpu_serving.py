@@ -743,3 +743,12 @@ def test_attention_with_the_smallest_value_scales(serving, sequences, group, d, 
     small = torch.rand(p.scales[1].shape, generator=p.g, device="cuda") < (0.6 if mixed else 2.0)
     p.scales[1, small] = tiny
     check_attention(serving, p, *query(p, group, t, 0.2), t)
+
+
+def test_attention_over_many_keys_with_the_smallest_value_scales(serving):
+    """Thousands of equal weights: their sum and the smallest scale together leave the normal numbers, the result does not."""
+    p = Paged(serving, 71, [(33, 4000)] * 10, 8, 16, 16, wild=False)
+    p.scales[1] = 1e-38
+    q, out = query(p, 8, torch.bfloat16, 0.0)
+    p.data[1] = p.data[1].abs() // 2 + 60
+    check_attention(serving, p, q, out, torch.bfloat16)
