@@ -33,11 +33,13 @@
 // result would have to be subtracted from sums that may be a thousand times smaller than it.
 //
 // bf16 queries become f16 after a row-wise power of two that puts the largest at 2^14; elements down to 2^-29 of that stay
-// exact.  Weights are rounded to f16: p * (v scale / reference) * 2^14, the reference a running power of two, so that
-// what is lost lies 2^-38 below the largest.  The sum is over the weights as they are rounded, so that what rounding does to
-// the key that has most of a row cancels.  The result stays in registers in units of that reference; it is
-// rescaled only when a maximum or the reference grows, which one vote per 32 keys finds out.  The reference does not go below
-// 2^-112: weights of values with smaller scales end 2^-151 above zero, which is below what a result of either type holds.
+// exact.  The scale of 16 values is part of the exponent: weights are rounded to f16 as 2^(s + log2(scale / r) - m + 14), r a running
+// power of two, m the row's largest s + log2(scale / r), so that what is lost lies 2^-38 below what counts most in the row's own sum:
+// values that a row does not see, or gives next to no weight, take no bits from the others, however large they are.  (r keeps the
+// numbers in range; values whose scale is below 2^-90 of it count as 2^-90 of it.)  The sum is over the weights as they are rounded,
+// so that what rounding does to the key that has most of a row cancels.  The result stays in registers in units of 2^(m + r); it is
+// rescaled only when a maximum or r grows, which one vote per 32 keys finds out.  r does not go below 2^-112, so that the factor of
+// the result is a normal number.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -61,8 +63,9 @@ constexpr int kWarps = 4, kTileRows = 8;
 constexpr int kGroup = 16; // keys that share a page and a scale for certain
 constexpr int kStageGroups = 2;
 constexpr int kStepGroups = kWarps * kStageGroups;
-constexpr float kWeightScale = 16384.f;
-constexpr float kLeastUnit = 0x1p-112f; // of the values' reference: kWeightScale over it is still a finite number
+constexpr float kWeightBits = 14.f;       // a row's largest weight is 2^14
+constexpr float kLeastReference = -112.f; // of the values, a power of two: over the largest weight still a normal number
+constexpr float kLeastBits = -90.f;       // of a value scale against the reference: sums of 2^-kLeastBits are still far from infinite
 constexpr int kClusterSteps = 3; // steps by which a cluster's blocks may outlast the line's
 
 template <int DP> struct FewShape {
@@ -253,7 +256,9 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         // a key scale of -1 stands for a group that is not there
         const auto scaleOf = [&](const float *scales, int slot) { return slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : -1.f; };
         int slots = slotOf(lane), nextSlots = slotOf(32 + lane);
-        float keyScales = scaleOf(p.cache.keyScales, slots), valueScales = scaleOf(p.cache.valueScales, slots);
+        // value scales as logarithms: -infinity for 0, NaN for what is not finite
+        const auto logOf = [&](float scale) { return scale < INFINITY ? log2f(scale) : NAN; };
+        float keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = logOf(scaleOf(p.cache.valueScales, slots));
         int issued = 0, writeStage = stage, issueSlots = slots;
         // lanes that issue a copy: keys or values, which of the two groups, which panel
         const int side = lane & 1, sub = (lane >> 1) & 1, panel = lane >> 2;
@@ -345,12 +350,12 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         const int openHi = p.causal ? old + firstToken + 1 : w.q.length, openLo = p.window > 0 ? max(0, old + lastToken - p.window + 1) : 0;
 
         float o[MT][4] = {}, most[2], sum[2] = {};
-        float reference = 0.f, perReference = 1.f; // unit of `o`, a power of two, and kWeightScale over it
+        float reference = kLeastReference; // of the values, as a power of two
         most[0] = most[1] = -INFINITY;
         for (int n = 0; n < count; ++n) {
             if (n > 0 && (n & 15) == 0) {
                 slots = nextSlots;
-                keyScales = scaleOf(p.cache.keyScales, slots), valueScales = scaleOf(p.cache.valueScales, slots);
+                keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = logOf(scaleOf(p.cache.valueScales, slots));
                 nextSlots = slotOf(2 * n + 32 + lane);
             }
             if (n < issued) {
@@ -358,12 +363,12 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             }
 #pragma unroll 1
             for (int h0 = 0; h0 < kStageGroups && !broken; h0 += AT) {
-                float keyScale[AT], valueScale[AT];
+                float keyScale[AT], valueLog[AT];
                 bool absent = false;
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
                     keyScale[h] = __shfl_sync(0xffffffffu, keyScales, (2 * n + h0 + h) & 31);
-                    valueScale[h] = __shfl_sync(0xffffffffu, valueScales, (2 * n + h0 + h) & 31);
+                    valueLog[h] = __shfl_sync(0xffffffffu, valueLogs, (2 * n + h0 + h) & 31);
                     absent = absent || keyScale[h] == -1.f;
                 }
                 const int key0 = groupOf(2 * n + h0) * kGroup;
@@ -389,15 +394,28 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                     }
                 }
                 const bool masked = key0 + AT * kGroup > openHi || key0 < openLo || absent;
-                bool grows = false;
+                // the values' reference, and their scales in units of it (a scale that is not finite reaches the rows that see it through
+                // their weights)
+                float loudest = valueLog[0], shift[AT];
+#pragma unroll
+                for (int h = 1; h < AT; ++h) {
+                    loudest = fmaxf(loudest, valueLog[h]);
+                }
+                const bool raise = loudest > reference;
+                const float before = reference;
+                reference = raise ? fminf(ceilf(loudest), 127.f) : reference;
+                bool grows = raise;
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
+                    shift[h] = valueLog[h] - reference;
+                    shift[h] = shift[h] < kLeastBits ? kLeastBits : shift[h];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float x = s[h][e] * (rowScale[e & 1] * keyScale[h]);
                         if (p.softcap > 0.f) {
                             x = softCapped(x, p.softcap) * kLog2e;
                         }
+                        x += shift[h];
                         if (masked) { // row g (or g + 8) of the product is key (g >> 1) + 4 (g & 1) (+ 8) of the group
                             const int key = key0 + h * kGroup + (g >> 1) + 4 * (g & 1) + 8 * (e >> 1);
                             x = key < rowHi[e & 1] && key >= rowLo[e & 1] && keyScale[h] != -1.f ? x : -INFINITY;
@@ -406,21 +424,11 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                         grows = grows || x > most[e & 1];
                     }
                 }
-                // the values' unit; a scale that is not finite reaches the rows that see it through their weights
-                float magnitude = 0.f;
-#pragma unroll
-                for (int h = 0; h < AT; ++h) {
-                    magnitude = fmaxf(magnitude, valueScale[h] < INFINITY ? valueScale[h] : 0.f);
-                }
-                const bool raise = magnitude > reference;
-                if (__any_sync(0xffffffffu, grows) || raise) {
-                    const float unit = raise ? fmaxf(powerAbove(magnitude), kLeastUnit) : reference;
-                    const float shrink = raise ? (reference > 0.f ? reference / unit : 0.f) : 1.f;
-                    reference = unit;
-                    perReference = unit > 0.f ? kWeightScale / unit : 1.f;
+                if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        float top = most[x];
+                        const float same = most[x] - (reference - before); // a reference that grows lowers the maximum
+                        float top = same;
 #pragma unroll
                         for (int h = 0; h < AT; ++h) {
                             top = fmaxf(top, fmaxf(s[h][x], s[h][2 + x]));
@@ -428,10 +436,10 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        const float keep = top == -INFINITY ? 1.f : exp2Fast(most[x] - top);
+                        // sums are in units of 2^most, results of 2^(most + reference)
+                        sum[x] *= top == -INFINITY ? 1.f : exp2Fast(fminf(most[x] - top, -kLeastBits));
+                        const float factor = top == -INFINITY ? 1.f : exp2Fast(same - top);
                         most[x] = top;
-                        sum[x] *= keep;
-                        const float factor = keep * shrink;
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             o[mt][x] *= factor, o[mt][2 + x] *= factor;
@@ -440,25 +448,22 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                 }
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
-                    const float weightUnit = valueScale[h] * perReference;
-                    const bool rounded = weightUnit >= 256.f && weightUnit < INFINITY; // no weight that matters is a subnormal number
+                    const bool rounded = shift[h] >= -6.f; // no weight that matters is a subnormal number
                     float2 part = {0.f, 0.f};
                     uint32_t wf[2]; // P^T: keys in pairs by t, row g
-                    const float shift0 = most[0] == -INFINITY ? 0.f : most[0], shift1 = most[1] == -INFINITY ? 0.f : most[1];
+                    const float base0 = most[0] == -INFINITY ? kWeightBits : kWeightBits - most[0],
+                                base1 = most[1] == -INFINITY ? kWeightBits : kWeightBits - most[1];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const float x0 = s[h][2 * half], x1 = s[h][2 * half + 1];
-                        const float p0 = exp2Fast(x0 - shift0), p1 = exp2Fast(x1 - shift1);
-                        // what the mask hides stays out, whatever its page's scale is
-                        const float w0 = masked && x0 == -INFINITY ? 0.f : p0 * weightUnit;
-                        const float w1 = masked && x1 == -INFINITY ? 0.f : p1 * weightUnit;
+                    for (int half = 0; half < 2; ++half) { // what the mask hides has a weight of 0
+                        const float w0 = exp2Fast(s[h][2 * half] + base0), w1 = exp2Fast(s[h][2 * half + 1] + base1);
                         const uint32_t two = packTwo(w0, w1, __half());
                         wf[half] = transposeHalves(two);
-                        const float2 w = rounded ? unpackTwo(two, __half()) : float2{p0, p1};
+                        const float2 w = rounded ? unpackTwo(two, __half()) : float2{w0, w1};
                         part.x += w.x, part.y += w.y;
                     }
-                    const float perUnit = rounded ? __fdividef(1.f, weightUnit) : 1.f;
-                    sum[0] = fmaf(part.x, perUnit, sum[0]), sum[1] = fmaf(part.y, perUnit, sum[1]);
+                    const float perWeight = exp2Fast(-kWeightBits - shift[h]);
+                    sum[0] = part.x == 0.f ? sum[0] : fmaf(part.x, perWeight, sum[0]);
+                    sum[1] = part.y == 0.f ? sum[1] : fmaf(part.y, perWeight, sum[1]);
                     constexpr int CHUNKS = DP < 128 ? 1 : DP / 128, WORDS = DP < 128 ? 2 : 4; // 16 (or, below 128, 8) bytes of a value row per lane each
                     const uint32_t group = values + uint32_t(h * Shape::kGroupBytes);
 #pragma unroll
@@ -521,7 +526,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                 for (int v = 0; v < kWarps; ++v) {
                     top = fmaxf(top, joinMax[v][itsRow]);
                 }
-                const float factor = (top == -INFINITY ? 1.f : exp2Fast(most[x] - top)) * (reference * (1.f / kWeightScale));
+                const float factor = (top == -INFINITY ? 1.f : exp2Fast(most[x] - top)) * exp2Fast(reference - kWeightBits);
                 float *to = results + (warp * kTileRows + itsRow) * kPitch;
                 // tile mt holds elements 2 (mt % 8) and the next of the lane's 16 (or 8) of each chunk
 #pragma unroll

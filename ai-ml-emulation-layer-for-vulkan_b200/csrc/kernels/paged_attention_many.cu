@@ -20,9 +20,11 @@
 //
 // Softmax in one pass where it can: scores are weighed with the maximum known from the tiles before, and only if one exceeds
 // it by more than 2^8, or at a row's first tile and where the values' reference grows, the maximum is taken first and sums
-// and result are rescaled.  The scale of 16 values is part of the exponent: w = 2^(s - m + log2(scale / r) + 7), r a
-// running power of two, and the sum over the weights of 16 keys is divided by it again.  So a weight is at most 2^15, f16's steps
-// end 2^-31 below the largest, and values whose scale is below 2^-60 of r count as nothing.  For f16 results the sum is over the
+// and result are rescaled.  The scale of 16 values is part of the exponent: w = 2^(s + log2(scale / r) - m + 7), r a running
+// power of two, m the row's largest s + log2(scale / r), and the sum over the weights of 16 keys is divided by scale / r again.  So a
+// weight is at most 2^15, and f16's steps end 2^-31 below what counts most in the row's own sum: values that a row does not see, or gives
+// next to no weight, take no bits from the others, however large they are.  (r keeps the numbers in range; values whose scale
+// is below 2^-90 of it count as 2^-90 of it.)  For f16 results the sum is over the
 // weights as they are rounded, so that what rounding does to the key that has most of a row cancels (a seventh off the error
 // against 64 bits; bf16 has steps eight times as large, and four prompts of 6000 tokens would take 899 us for 822).
 #include <cuda_bf16.h>
@@ -49,6 +51,7 @@ constexpr int kConvertWarps = 4;
 constexpr int kParamRing = 5, kStaging = 4, kSlots = 3; // of a tile's keys or values: integers on their way, and f16
 constexpr float kGrowth = 8.f;                          // in powers of two
 constexpr float kWeightBits = 7.f;
+constexpr float kLeastBits = -90.f; // of a value scale against the reference: sums of 2^-kLeastBits are still far from infinite
 
 // Heads of 256 elements: one tile of rows (its result alone has 256 columns of tensor memory), and 64 keys at a time, whose f16 form is
 // as large as that of 128 keys of 128 elements.
@@ -329,7 +332,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 reference = max(reference, exponent);
                 if (lane < kGroups) {
                     // (a scale that is not finite gives a shift and weights that are not)
-                    const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), -60.f) + kWeightBits : magnitude - magnitude;
+                    const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), kLeastBits) + kWeightBits : magnitude - magnitude;
                     to.keyScale[lane] = keyScale, to.shift[lane] = shift, to.perWeight[lane] = exp2f(-shift);
                 }
                 const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
@@ -592,19 +595,21 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                         tmemWait16(s);
                         const float factor = rowScale * tp.keyScale[half * kHalfGroups + g];
                         const uint32_t bits = masked ? seen(g) : 0xffffu;
+                        float topOfGroup = -INFINITY;
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            top = ((bits >> j) & 1u) != 0u ? fmaxf(top, scoreOf(s[j], factor)) : top;
+                            topOfGroup = ((bits >> j) & 1u) != 0u ? fmaxf(topOfGroup, scoreOf(s[j], factor)) : topOfGroup;
                         }
+                        top = fmaxf(top, topOfGroup + (tp.shift[half * kHalfGroups + g] - kWeightBits));
                     }
                     exchange[which][tileRow][half] = top;
                     asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
-                    top = fmaxf(fmaxf(top, exchange[which][tileRow][half ^ 1]), most);
-                    // sums and result in units of the new maximum and reference
-                    const float keep = top == -INFINITY ? 1.f : exp2Fast(most - top);
-                    const float factorO = keep * exp2f(float(reference - tp.reference));
-                    sum *= keep;
-                    if (tile > 0 && __any_sync(0xffffffffu, factorO != 1.f)) {
+                    // Sums are in units of 2^most, results of 2^(most + reference): a reference that grows lowers the maximum.
+                    const float same = most - float(tp.reference - reference);
+                    top = fmaxf(fmaxf(top, exchange[which][tileRow][half ^ 1]), same);
+                    const float keep = top == -INFINITY ? 1.f : exp2Fast(same - top);
+                    sum *= top == -INFINITY ? 1.f : exp2Fast(fminf(most - top, -kLeastBits));
+                    if (tile > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
                         addedBefore();
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
@@ -614,7 +619,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                             tmemWait16(o);
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
-                                o[j] = __float_as_uint(__uint_as_float(o[j]) * factorO);
+                                o[j] = __float_as_uint(__uint_as_float(o[j]) * keep);
                             }
                             tmemStore16(resultAt + uint32_t(d), o);
                         }
@@ -629,9 +634,10 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 for (int g = 0; g < kHalfGroups; ++g) {
                     uint32_t s[16];
                     tmemLoad16(scoresAt + uint32_t(g * 16), s);
-                    const float factor = rowScale * tp.keyScale[half * kHalfGroups + g], shift = tp.shift[half * kHalfGroups + g] - base;
+                    const float factor = rowScale * tp.keyScale[half * kHalfGroups + g], bitsOfScale = tp.shift[half * kHalfGroups + g],
+                                shift = bitsOfScale - base;
                     const uint32_t bits = masked ? seen(g) : 0xffffu;
-                    const bool rounded = HALF && tp.shift[half * kHalfGroups + g] >= 1.f; // no weight that matters is a subnormal number
+                    const bool rounded = HALF && bitsOfScale >= 1.f; // no weight that matters is a subnormal number
                     tmemWait16(s);
                     float top = -INFINITY, part = 0.f;
                     if ((HALF && !rounded) || !__all_sync(0xffffffffu, bits == 0xffffu)) {
@@ -646,7 +652,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                             const float2 w = unpackTwo(weights[g * 8 + j / 2], __half());
                             part += rounded ? w.x + w.y : w0 + w1;
                         }
-                        grows = grows || top > most + kGrowth;
+                        grows = grows || top + bitsOfScale > most + (kWeightBits + kGrowth);
                         added = part == 0.f ? added : fmaf(part, tp.perWeight[half * kHalfGroups + g], added);
                     } else {
                         const float2 factors = {factor, factor}, shifts = {shift, shift};
@@ -664,7 +670,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                             parts = addTwo(parts, HALF ? unpackTwo(weights[g * 8 + j / 2], __half()) : w);
                         }
                         part = parts.x + parts.y;
-                        grows = grows || (CAP ? top : top * factor) > most + kGrowth;
+                        grows = grows || (CAP ? top + bitsOfScale : fmaf(top, factor, bitsOfScale)) > most + (kWeightBits + kGrowth);
                         added = fmaf(part, tp.perWeight[half * kHalfGroups + g], added);
                     }
                 }

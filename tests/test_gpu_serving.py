@@ -752,3 +752,29 @@ def test_attention_over_many_keys_with_the_smallest_value_scales(serving):
     q, out = query(p, 8, torch.bfloat16, 0.0)
     p.data[1] = p.data[1].abs() // 2 + 60
     check_attention(serving, p, q, out, torch.bfloat16)
+
+
+@pytest.mark.parametrize("loud", [1e3, 1e8, 1e16, 1e24])
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("sequences, group, d, how", [([(4, 34), (3, 18)], 2, 64, {}), ([(8, 40), (6, 90)], 2, 128, {"window": 20}), ([(4, 19), (2, 33)], 4, 256, {}),
+                                                      ([(4, 20002), (1, 40)], 2, 64, {}), ([(100, 160), (40, 300)], 4, 128, {}), ([(90, 200)], 3, 64, {"window": 33}),
+                                                      ([(40, 70)], 2, 256, {"softcap": 9.0}), ([(70, 5000)], 1, 128, {})], ids=str)
+def test_attention_values_that_a_row_does_not_see(serving, sequences, group, d, how, dtype, loud):
+    """Pages whose values are far larger than all others, hidden from some rows: those rows are as exact as without them."""
+    t = DTYPES[dtype]
+    p = Paged(serving, 91 + d, sequences, 1, 16, d, wild=False)
+    q, out = query(p, group, t)
+    want, bound = ref.attend(*p.arrays(), ref.f64(q), d ** -0.5, True, how.get("window", 0), how.get("softcap", 0.0), t)
+    pages = [[0 if "window" in how else (length - 1) // 16] for length in p.lengths]  # behind a window, or in front of the causal mask
+    for b, of in enumerate(pages):
+        p.scales[1, [p.table[b][i] for i in of]] *= loud
+    got = ref.f64(p.cache.attend(q, p.batch, out=out, **how))
+    unseen = 0
+    for b, length in enumerate(p.lengths):
+        for i in range(p.starts[b], p.starts[b + 1]):
+            position = length - p.starts[b + 1] + i
+            lo = max(0, position - how["window"] + 1) if "window" in how else 0
+            if not any(page * 16 <= position and page * 16 + 16 > lo for page in pages[b]):
+                assert (np.abs(got[i] - want[i]) <= bound[i]).all(), (b, i, np.abs(got[i] - want[i]).max())
+                unseen += 1
+    assert unseen > 0
