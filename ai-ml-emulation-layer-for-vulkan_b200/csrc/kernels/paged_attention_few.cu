@@ -253,12 +253,14 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             }
             return slot;
         };
-        // a key scale of -1 stands for a group that is not there
-        const auto scaleOf = [&](const float *scales, int slot) { return slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : -1.f; };
+        // a key scale of -1 stands for a group that is not there; one that is not finite is no number, whatever it would be multiplied with
+        const auto scaleOf = [&](const float *scales, int slot) {
+            const float scale = slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : -1.f;
+            return scale < INFINITY ? scale : NAN;
+        };
         int slots = slotOf(lane), nextSlots = slotOf(32 + lane);
         // value scales as logarithms: -infinity for 0, NaN for what is not finite
-        const auto logOf = [&](float scale) { return scale < INFINITY ? log2f(scale) : NAN; };
-        float keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = logOf(scaleOf(p.cache.valueScales, slots));
+        float keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = log2f(scaleOf(p.cache.valueScales, slots));
         int issued = 0, writeStage = stage, issueSlots = slots;
         // lanes that issue a copy: keys or values, which of the two groups, which panel
         const int side = lane & 1, sub = (lane >> 1) & 1, panel = lane >> 2;
@@ -355,7 +357,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         for (int n = 0; n < count; ++n) {
             if (n > 0 && (n & 15) == 0) {
                 slots = nextSlots;
-                keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = logOf(scaleOf(p.cache.valueScales, slots));
+                keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = log2f(scaleOf(p.cache.valueScales, slots));
                 nextSlots = slotOf(2 * n + 32 + lane);
             }
             if (n < issued) {

@@ -289,7 +289,11 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             }
             return slot;
         };
-        const auto scaleOf = [&](const float *scales, int slot) { return slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : 0.f; };
+        // (a scale that is not finite is no number, whatever it would be multiplied with)
+        const auto scaleOf = [&](const float *scales, int slot) {
+            const float scale = slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : 0.f;
+            return scale < INFINITY ? scale : NAN;
+        };
         int nextNextSlot = slotOf(1), nextSlot = checked(0, slotOf(0)), reference = -126;
         float nextKeyScale = scaleOf(p.cache.keyScales, nextSlot), nextValueScale = scaleOf(p.cache.valueScales, nextSlot);
         uint32_t unit = 0; // keys and values of the tiles in turn
@@ -331,8 +335,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 exponent = __reduce_max_sync(0xffffffffu, exponent);
                 reference = max(reference, exponent);
                 if (lane < kGroups) {
-                    // (a scale that is not finite gives a shift and weights that are not)
-                    const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), kLeastBits) + kWeightBits : magnitude - magnitude;
+                    const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), kLeastBits) + kWeightBits : NAN;
                     to.keyScale[lane] = keyScale, to.shift[lane] = shift, to.perWeight[lane] = exp2f(-shift);
                 }
                 const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);

@@ -778,3 +778,27 @@ def test_attention_values_that_a_row_does_not_see(serving, sequences, group, d, 
                 assert (np.abs(got[i] - want[i]) <= bound[i]).all(), (b, i, np.abs(got[i] - want[i]).max())
                 unseen += 1
     assert unseen > 0
+
+
+@pytest.mark.parametrize("softcap", [0.0, 5.0])
+@pytest.mark.parametrize("sequences, group, d", [([(1, 40), (3, 24)], 2, 64), ([(1, 5000)], 1, 128), ([(40, 60), (70, 90)], 4, 128), ([(30, 40)], 1, 256),
+                                                 ([(50, 3000)], 1, 64)])
+@pytest.mark.parametrize("side", [0, 1], ids=["keys", "values"])
+def test_attention_with_an_infinite_scale(serving, sequences, group, d, side, softcap):
+    """What attends to a page whose scale is infinite is no number, whatever the page's integers are; the rest does not notice."""
+    p = Paged(serving, 81 + d, sequences, 1, 16, d, wild=False)
+    q, out = query(p, group, torch.float16)
+    p.data[side, :, :, ::2] = 0
+    if side == 0:
+        p.data[0] = torch.where(p.data[0] == 0, p.data[0], 1)  # and scores of one sign, below zero
+        q.copy_(-q.abs())
+    want, bound = ref.attend(*p.arrays(), ref.f64(q), d ** -0.5, True, 0, softcap, torch.float16)
+    for b, length in enumerate(p.lengths):  # the page of each sequence's last token
+        p.scales[side, p.table[b][(length - 1) // 16]] = float("inf")
+    got = ref.f64(p.cache.attend(q, p.batch, out=out, softcap=softcap))
+    for b, length in enumerate(p.lengths):
+        for i in range(p.starts[b], p.starts[b + 1]):
+            if length - p.starts[b + 1] + i >= (length - 1) // 16 * 16:
+                assert np.isnan(got[i]).all(), (b, i)
+            else:
+                assert (np.abs(got[i] - want[i]) <= bound[i]).all(), (b, i)
