@@ -23,6 +23,7 @@ BOOL, I8, I16, I32, I64, U8, U16, U32, F16, BF16, F32 = range(11)
 MAX_RANK = 6
 PIPELINE_NO_FUSION = 1
 INCOMPLETE = 5
+ERROR_DEVICE = -4
 PROPERTY_CREATION_LOG = 0
 PROPERTY_PROFILING = 0x7FFFFFFE
 

@@ -1077,13 +1077,18 @@ int mlel_paged_attention_workspace(const mlel_paged_cache *cache, const mlel_pag
 
 int mlel_paged_error(void) {
     int code = 0;
-    guarded([&] {
-        cudaDeviceSynchronize();
-        const int append = takePagedErrorAppend(), attention = takePagedErrorAttention();
-        code = append != 0 ? append : attention;
-        return MLEL_SUCCESS;
+    const int status = guarded([&] {
+        cudaError_t err = cudaDeviceSynchronize();
+        err = err != cudaSuccess ? err : takePagedErrorAppend(code);
+        err = err != cudaSuccess ? err : takePagedErrorAttention(code);
+        if (err != cudaSuccess) {
+            cudaGetLastError();
+            setLastError(std::string("mlel_paged_error: the record cannot be read: ") + cudaGetErrorString(err));
+            return int(MLEL_ERROR_DEVICE);
+        }
+        return int(MLEL_SUCCESS);
     });
-    return code;
+    return status != MLEL_SUCCESS ? status : code;
 }
 
 } // extern "C"

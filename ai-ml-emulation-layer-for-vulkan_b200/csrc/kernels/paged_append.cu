@@ -648,6 +648,6 @@ int pagedAppend(const mlel_paged_cache *cache, const mlel_paged_batch *batch, co
                                                           : launchAppend<__nv_bfloat16, false>(p, s));
 }
 
-int takePagedErrorAppend() { return takePagedError(); }
+cudaError_t takePagedErrorAppend(int &code) { return takePagedError(code); }
 
 } // namespace mlel

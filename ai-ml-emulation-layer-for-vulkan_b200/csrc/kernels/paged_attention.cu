@@ -71,9 +71,9 @@ int pagedAttention(const mlel_paged_cache *cache, const mlel_paged_batch *batch,
     return pagedAttentionFew(p, plan, s);
 }
 
-int takePagedErrorAttention() {
-    const int few = takePagedErrorFew(), many = takePagedErrorMany();
-    return few != 0 ? few : many;
+cudaError_t takePagedErrorAttention(int &code) {
+    const cudaError_t err = takePagedErrorFew(code);
+    return err != cudaSuccess ? err : takePagedErrorMany(code);
 }
 int servingErrorWord() {
     for (const auto word : {fewAttentionErrorWord, manyAttentionErrorWord, scaledTilesErrorWord, scaledPairErrorWord}) {

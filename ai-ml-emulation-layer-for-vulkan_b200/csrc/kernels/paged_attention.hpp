@@ -35,13 +35,13 @@ struct FewPlan {
 };
 FewPlan pagedAttentionFewPlan(const AttendParams &p);
 int pagedAttentionFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s);
-int takePagedErrorFew();
+cudaError_t takePagedErrorFew(int &code);
 int fewAttentionErrorWord();
 
 // paged_attention_many.cu: many rows per cache head (prompts)
 bool pagedAttentionManyApplies(const AttendParams &p);
 int pagedAttentionMany(const AttendParams &p, cudaStream_t s);
-int takePagedErrorMany();
+cudaError_t takePagedErrorMany(int &code);
 int manyAttentionErrorWord();
 
 } // namespace mlel

@@ -772,7 +772,7 @@ int pagedAttentionFew(const AttendParams &p, const FewPlan &plan, cudaStream_t s
     return dp == 256 ? launchFew<256, false>(p, plan, s) : dp == 128 ? launchFew<128, false>(p, plan, s) : launchFew<64, false>(p, plan, s);
 }
 
-int takePagedErrorFew() { return takePagedError(); }
+cudaError_t takePagedErrorFew(int &code) { return takePagedError(code); }
 int fewAttentionErrorWord() { return tc::readErrorWord(); }
 
 } // namespace mlel

@@ -863,7 +863,7 @@ int pagedAttentionMany(const AttendParams &p, cudaStream_t s) {
     return p.cache.headDim <= 64 ? launchManyType<64>(p, s) : p.cache.headDim <= 128 ? launchManyType<128>(p, s) : launchManyType<256>(p, s);
 }
 
-int takePagedErrorMany() { return takePagedError(); }
+cudaError_t takePagedErrorMany(int &code) { return takePagedError(code); }
 int manyAttentionErrorWord() { return tc::readErrorWord(); }
 
 } // namespace mlel

@@ -15,13 +15,15 @@ namespace mlel {
 static __device__ int g_pagedError = 0;
 enum : int { kBadSequence = 1, kBadPage = 2 };
 
-static inline int takePagedError() {
+static inline cudaError_t takePagedError(int &code) {
+    const int zero = 0;
     int v = 0;
-    if (cudaMemcpyFromSymbol(&v, g_pagedError, sizeof(int)) == cudaSuccess && v != 0) {
-        const int zero = 0;
-        cudaMemcpyToSymbol(g_pagedError, &zero, sizeof(int));
+    cudaError_t err = cudaMemcpyFromSymbol(&v, g_pagedError, sizeof(int));
+    if (err == cudaSuccess && v != 0) {
+        err = cudaMemcpyToSymbol(g_pagedError, &zero, sizeof(int));
+        code = code != 0 ? code : v;
     }
-    return v;
+    return err;
 }
 
 struct PagedCache {

@@ -26,9 +26,9 @@ int pagedAttention(const mlel_paged_cache *cache, const mlel_paged_batch *batch,
                    uint64_t workspaceBytes, cudaStream_t s);
 uint64_t pagedAttentionWorkspace(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries);
 
-// The word in which the kernels of the paged cache record what they left out; reading clears it.
-int takePagedErrorAppend();
-int takePagedErrorAttention();
+// The words in which the kernels of the paged cache record what they left out, read into `code` where that is still 0 and cleared.
+cudaError_t takePagedErrorAppend(int &code);
+cudaError_t takePagedErrorAttention(int &code);
 
 // An operand of a direct call with its strides filled in.
 struct Operand {

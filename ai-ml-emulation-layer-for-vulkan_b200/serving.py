@@ -15,7 +15,7 @@ import struct
 
 import torch
 
-from . import BF16, F16, F32, I8, I32, check, lib
+from . import BF16, ERROR_DEVICE, F16, F32, I8, I32, MlelError, check, lib
 from .runtime import _current_stream
 
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.int8: I8, torch.int32: I32}
@@ -229,6 +229,13 @@ class PagedCache(_Described):
 
 def paged_error(device: int | None = None) -> int:
     """0, or what the cache's kernels left out on the device since the last call: 1 a sequence whose numbers contradict the batch's
-    bounds, 2 a page outside the cache.  Waits for the device and clears the record."""
+    bounds, 2 a page outside the cache.  Waits for the device and clears the record.  Raises ``MlelError`` where the device cannot be
+    read, and where a kernel gave up on a wait (its results are not complete)."""
     with torch.cuda.device(torch.cuda.current_device() if device is None else device):
-        return lib().mlel_paged_error()
+        code = lib().mlel_paged_error()
+        if code < 0:
+            check(code)
+        wait = lib().mlel_device_error()
+    if wait != 0:
+        raise MlelError(ERROR_DEVICE, f"a kernel gave up on a wait that ran out (code {wait})")
+    return code

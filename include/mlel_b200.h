@@ -505,7 +505,8 @@ int mlel_cuda_paged_attention(const mlel_paged_cache *cache, const mlel_paged_ba
 int mlel_paged_attention_workspace(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries,
                                    uint64_t *bytes);
 /* What the kernels of the paged cache left out on the current device since the last call: 0 nothing, 1 a sequence whose starts or
- * lengths contradict the bounds or shapes, 2 a page outside the cache.  Synchronises the device and clears the record. */
+ * lengths contradict the bounds or shapes, 2 a page outside the cache; a negative mlel_status where the device or its record cannot
+ * be read.  Synchronises the device and clears the record.  (Waits that ran out are told of by mlel_device_error().) */
 int mlel_paged_error(void);
 
 #ifdef __cplusplus

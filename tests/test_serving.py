@@ -190,6 +190,34 @@ def test_loose_bounds_on_new_tokens_change_nothing(calls, loose):
     assert needs[0] == needs[1] > 0
 
 
+def test_a_record_that_cannot_be_read_is_no_clean_one(calls):
+    """Without a device, or with one in an error state, there is no telling what was left out."""
+    import torch
+    mlel, lib = calls
+    if torch.cuda.is_available():
+        pytest.skip("there is a device to read")
+    assert refused(mlel, lib.mlel_paged_error(), "cannot be read") == -4
+
+
+@pytest.mark.parametrize("code, wait, raised", [(0, 0, None), (2, 0, None), (-4, 0, "status -4"), (0, 61, "code 61"), (1, 88, "code 88")])
+def test_python_layer_raises_for_failed_devices_and_waits(mlel, monkeypatch, code, wait, raised):
+    import contextlib
+
+    import torch
+    from mlel_b200 import serving
+
+    class Fake:
+        mlel_paged_error = staticmethod(lambda: code)
+        mlel_device_error = staticmethod(lambda: wait)
+    monkeypatch.setattr(serving, "lib", Fake)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    if raised is None:
+        assert serving.paged_error(0) == code
+    else:
+        with pytest.raises(mlel.MlelError, match=raised):
+            serving.paged_error(0)
+
+
 def test_python_layer_refuses_host_tensors(mlel):
     import torch
     from mlel_b200 import serving
