@@ -134,6 +134,9 @@ class QuantizedLinear(_Described):
     change between them; the attributes themselves stay."""
 
     def __init__(self, weight: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None):
+        for name, t, dtype in (("weight", weight, torch.int8), ("scales", scales, torch.float32), ("bias", bias, torch.float32)):
+            if t is not None and t.dtype != dtype:  # (laying the rows out would convert them in silence)
+                raise TypeError(f"{name} has to be {dtype}, not {t.dtype}")
         self.device = _device(weight, scales, bias)
         n, k = weight.shape
         self._padded = (k + 15) // 16 * 16

@@ -218,6 +218,20 @@ def test_python_layer_raises_for_failed_devices_and_waits(mlel, monkeypatch, cod
             serving.paged_error(0)
 
 
+@pytest.mark.parametrize("k", [33, 48])
+@pytest.mark.parametrize("change, word", [(dict(weight="float32"), "weight has to be torch.int8"), (dict(weight="float16"), "weight has to be torch.int8"),
+                                          (dict(weight="uint8"), "weight has to be torch.int8"), (dict(scales="float16"), "scales has to be torch.float32"),
+                                          (dict(bias="bfloat16"), "bias has to be torch.float32")], ids=str)
+def test_weights_of_other_types_are_refused(mlel, change, word, k):
+    """Rows on 16-byte boundaries or not: nothing is converted in silence."""
+    import torch
+    from mlel_b200 import serving
+    types = {**dict(weight="int8", scales="float32", bias="float32"), **change}
+    operands = [torch.zeros(*shape, dtype=getattr(torch, types[name])) for name, shape in (("weight", (5, k)), ("scales", (5,)), ("bias", (5,)))]
+    with pytest.raises(TypeError, match=word):
+        serving.QuantizedLinear(*operands)
+
+
 def test_python_layer_refuses_host_tensors(mlel):
     import torch
     from mlel_b200 import serving
