@@ -1,7 +1,9 @@
 // Attention over a paged int8 cache with a scale for each page and head: the checks of a call, and which kernel takes it.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <limits>
 
 #include "matmul_scaled.hpp"
 #include "paged_attention.hpp"
@@ -55,7 +57,7 @@ int pagedAttention(const mlel_paged_cache *cache, const mlel_paged_batch *batch,
     }
     p.out = out.ptr, p.outStride[0] = out.strides[0], p.outStride[1] = out.strides[1];
     p.wideOut = aligned(out.ptr, 16) && out.strides[0] % 16 == 0 && out.strides[1] % 16 == 0;
-    p.scale = scale, p.softcap = softcap, p.causal = causal != 0, p.window = window;
+    p.scale = scale, p.softcap = softcap, p.perCap = std::min(1.f / softcap, std::numeric_limits<float>::max() / 4.f), p.causal = causal != 0, p.window = window;
     if (p.batch.tokens == 0 || p.batch.sequences == 0) {
         return MLEL_SUCCESS;
     }

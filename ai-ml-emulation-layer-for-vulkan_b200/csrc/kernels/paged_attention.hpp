@@ -18,7 +18,7 @@ struct AttendParams {
     const char *queries;
     char *out;
     int64_t queryStride[2], outStride[2]; // bytes: token, head
-    float scale, softcap;                 // softcap 0: none
+    float scale, softcap, perCap;         // softcap 0: none; perCap: 1 / softcap, and finite
     int32_t causal, window, queryHeads, group;
     int32_t halves;      // queries and output are f16 (else bf16)
     int32_t wideQueries; // every head of the queries starts on a 16-byte boundary; the same for the output

@@ -170,7 +170,7 @@ template <int DP> __device__ __forceinline__ float *partialRow(const AttendParam
     return p.partials + ((int64_t(piece) * 2 + which) * kTileRows + row) * (DP + 4);
 }
 
-template <int DP, bool HALF>
+template <int DP, bool HALF, bool LARGE_CAP> // (see softCapped)
 __global__ void __launch_bounds__(kWarps * 32, DP <= 128 ? 3 : 2)
 pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p,
                         const int split) { // blocks of the cluster that shares a tile; 0: pieces of the line
@@ -415,7 +415,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                     for (int e = 0; e < 4; ++e) {
                         float x = s[h][e] * (rowScale[e & 1] * keyScale[h]);
                         if (p.softcap > 0.f) {
-                            x = softCapped(x, p.softcap) * kLog2e;
+                            x = softCapped<LARGE_CAP>(x, p.softcap, p.perCap) * kLog2e;
                         }
                         x += shift[h];
                         if (masked) { // row g (or g + 8) of the product is key (g >> 1) + 4 (g & 1) (+ 8) of the group
@@ -707,7 +707,7 @@ template <int DP, bool HALF> int launchFew(const AttendParams &p, const FewPlan 
         return MLEL_ERROR_DEVICE;
     }
     constexpr size_t smemBytes = Shape::kRing + 1024;
-    const auto kernel = pagedAttentionFewKernel<DP, HALF>;
+    const auto kernel = p.softcap > kWideCap ? pagedAttentionFewKernel<DP, HALF, true> : pagedAttentionFewKernel<DP, HALF, false>;
     if (!allowDynamicSmem(reinterpret_cast<const void *>(kernel), smemBytes)) {
         return MLEL_ERROR_DEVICE;
     }

@@ -186,7 +186,9 @@ __device__ __forceinline__ uint32_t pairVote(int barrier, bool predicate) {
 }
 __device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <int DP, bool HALF, bool CAP>
+enum Cap : int { kNoCap, kCap, kLargeCap }; // see softCapped
+
+template <int DP, bool HALF, int CAP>
 __global__ void __launch_bounds__(ManyShape<DP>::kThreads, 1)
 pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_constant__ CUtensorMap mapV, const AttendParams p,
                          const FastDiv heads, const int levels, const int boxRows, const int split) {
@@ -526,7 +528,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 }
                 asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory"); // `exchange` is used again
             }
-            rowScale = unit * fabsf(p.scale) * (CAP ? 1.f : kLog2e);
+            rowScale = unit * fabsf(p.scale) * (CAP != kNoCap ? 1.f : kLog2e);
             const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u; // keeps the order of scores that of the products
 #pragma unroll
             for (int step = 0; step < kSteps; ++step) {
@@ -557,7 +559,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         int reference = -126;
         const auto scoreOf = [&](uint32_t s, float factor) { // in powers of two
             const float x = __uint_as_float(s) * factor;
-            return CAP ? softCapped(x, p.softcap) * kLog2e : x;
+            return CAP != kNoCap ? softCapped<CAP == kLargeCap>(x, p.softcap, p.perCap) * kLog2e : x;
         };
         for (int tile = 0; tile < tiles && ok; ++tile) {
             const int buffer = ahead ? tile & 1 : which;
@@ -663,17 +665,17 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
                             float2 x = {__uint_as_float(s[j]), __uint_as_float(s[j + 1])};
-                            if (CAP) {
+                            if (CAP != kNoCap) {
                                 x.x = scoreOf(s[j], factor), x.y = scoreOf(s[j + 1], factor);
                             }
                             top = maxThree(top, x.x, x.y);
-                            x = CAP ? addTwo(x, shifts) : fmaTwo(x, factors, shifts);
+                            x = CAP != kNoCap ? addTwo(x, shifts) : fmaTwo(x, factors, shifts);
                             const float2 w = {exp2Fast(x.x), exp2Fast(x.y)};
                             weights[g * 8 + j / 2] = packTwo(w.x, w.y, __half());
                             parts = addTwo(parts, HALF ? unpackTwo(weights[g * 8 + j / 2], __half()) : w);
                         }
                         part = parts.x + parts.y;
-                        grows = grows || (CAP ? top + bitsOfScale : fmaf(top, factor, bitsOfScale)) > most + (kWeightBits + kGrowth);
+                        grows = grows || (CAP != kNoCap ? top + bitsOfScale : fmaf(top, factor, bitsOfScale)) > most + (kWeightBits + kGrowth);
                         added = fmaf(part, tp.perWeight[half * kHalfGroups + g], added);
                     }
                 }
@@ -796,7 +798,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     }
 }
 
-template <int DP, bool HALF, bool CAP> int launchMany(const AttendParams &p, cudaStream_t s) {
+template <int DP, bool HALF, int CAP> int launchMany(const AttendParams &p, cudaStream_t s) {
     using Shape = ManyShape<DP>;
     constexpr size_t smemBytes = Shape::kTiles + sizeof(ManyState);
     static_assert(smemBytes <= 232448, "shared memory per block");
@@ -847,10 +849,13 @@ template <int DP, bool HALF, bool CAP> int launchMany(const AttendParams &p, cud
 }
 
 template <int DP> int launchManyType(const AttendParams &p, cudaStream_t s) {
-    if (p.softcap > 0.f) {
-        return p.halves ? launchMany<DP, true, true>(p, s) : launchMany<DP, false, true>(p, s);
+    if (p.softcap > kWideCap) {
+        return p.halves ? launchMany<DP, true, kLargeCap>(p, s) : launchMany<DP, false, kLargeCap>(p, s);
     }
-    return p.halves ? launchMany<DP, true, false>(p, s) : launchMany<DP, false, false>(p, s);
+    if (p.softcap > 0.f) {
+        return p.halves ? launchMany<DP, true, kCap>(p, s) : launchMany<DP, false, kCap>(p, s);
+    }
+    return p.halves ? launchMany<DP, true, kNoCap>(p, s) : launchMany<DP, false, kNoCap>(p, s);
 }
 
 } // namespace

@@ -802,3 +802,17 @@ def test_attention_with_an_infinite_scale(serving, sequences, group, d, side, so
                 assert np.isnan(got[i]).all(), (b, i)
             else:
                 assert (np.abs(got[i] - want[i]) <= bound[i]).all(), (b, i)
+
+
+@pytest.mark.parametrize("cap", [1e-42, 1e-20, 0.01, 1.0, 50.0, 300.0, 1e4, 1e6, 1e7, 1e20, 3e38])
+@pytest.mark.parametrize("sequences, group, d", [([(1, 200), (1, 40)], 4, 64), ([(3, 300)], 2, 128), ([(1, 50), (2, 90)], 3, 256), ([(1, 9000)], 2, 64),
+                                                 ([(130, 300), (20, 40)], 4, 128), ([(30, 100)], 2, 256), ([(60, 2500)], 1, 64)])
+def test_attention_with_caps_of_every_size(serving, sequences, group, d, cap):
+    """Capped scores are as exact as scores without a cap, from caps far below the scores to caps far above them."""
+    p = Paged(serving, 95 + d, sequences, 1, 16, d, wild=False)
+    q, out = query(p, group, torch.float16, 4.0)
+    got = ref.f64(p.cache.attend(q, p.batch, out=out, softcap=cap))
+    want, bound = ref.attend_capped(*p.arrays(), ref.f64(q), d ** -0.5, cap, torch.float16)
+    inside = ~np.isnan(want)
+    wrong = ~(np.abs(got - want) <= bound) & inside
+    assert not wrong.any(), (int(wrong.sum()), np.argwhere(wrong)[:4].tolist(), float(np.nanmax(np.where(inside, np.abs(got - want) / bound, 0))))
