@@ -129,8 +129,9 @@ def attend(data, scales, starts, lengths, table, q, scale, causal, window, softc
     return out, bound
 
 
-def attend_capped(data, scales, starts, lengths, table, q, scale, softcap, dtype):
-    """As ``attend`` with a causal mask, its bound for caps of any size: a capped score is off by 16 units of 2^-24 of itself.  (Just above
+def attend_capped(data, scales, starts, lengths, table, q, scale, softcap, dtype, missing=()):
+    """As ``attend`` with a causal mask; without the tokens of the pages (sequence, index in its table) that are ``missing``.  The bound is
+    for caps of any size, 0 for none: a capped score is off by 16 units of 2^-24 of itself.  (Just above
     a half of the cap it is cap (1 - q), q = 2 / (e^(2 z) + 1) = 0.54: e to 2^-22 and four roundings of its argument of 1, so the
     denominator to 5.9 + 1 units, the quotient to another 4; 10.9 * 0.54 / 0.46 + 1 = 13.7.  Below, a quotient of sums of positive terms: 9.)"""
     tokens, heads, d = q.shape
@@ -138,19 +139,24 @@ def attend_capped(data, scales, starts, lengths, table, q, scale, softcap, dtype
     out, bound = np.full(q.shape, np.nan), np.zeros(q.shape)
     for b, length in enumerate(lengths):
         first, fresh = starts[b], starts[b + 1] - starts[b]
-        at = np.arange(length)
+        at = np.array([j for j in range(length) if (b, j // page) not in missing], dtype=np.int64)
         slot, row = np.array(table[b], dtype=np.int64)[at // page], at % page
         for h in range(heads):
             of = scales[:, slot, h // group].astype(np.float64)[..., None]
             k, v = (data[side, slot, h // group, row].astype(np.float64) * of[side] for side in (0, 1))
             for i in range(fresh):
-                hi = length - fresh + i + 1
+                hi = int((at <= length - fresh + i).sum())
                 x = q[first + i, h]
+                if hi == 0:
+                    out[first + i, h] = 0
+                    continue
                 s = k[:hi] @ x * scale
                 off = ((d + 6) * 2.0 ** -24 * abs(scale) * ((np.abs(k[:hi]) + 256 * of[0, :hi]) @ np.abs(x))).max()
-                s = softcap * np.tanh(s / softcap)
+                if softcap > 0:
+                    s = softcap * np.tanh(s / softcap)
                 off += (16 + 4) * 2.0 ** -24 * np.abs(s).max()
-                off = min(off, 2 * softcap)  # both lie within the cap
+                if softcap > 0:
+                    off = min(off, 2 * softcap)  # both lie within the cap
                 p = np.exp(s - s.max())
                 p /= p.sum()
                 o, most = p @ v[:hi], p @ np.abs(v[:hi])

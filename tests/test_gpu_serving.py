@@ -816,3 +816,27 @@ def test_attention_with_caps_of_every_size(serving, sequences, group, d, cap):
     inside = ~np.isnan(want)
     wrong = ~(np.abs(got - want) <= bound) & inside
     assert not wrong.any(), (int(wrong.sum()), np.argwhere(wrong)[:4].tolist(), float(np.nanmax(np.where(inside, np.abs(got - want) / bound, 0))))
+
+
+@pytest.mark.parametrize("bad", [[0], [2], [0, 1, 2, 3], [11]], ids=str)
+@pytest.mark.parametrize("fresh, group, d", [(1, 2, 64), (3, 2, 128), (4, 4, 256), (30, 4, 64), (150, 2, 128), (40, 1, 256)])
+def test_tokens_of_a_page_outside_the_cache_are_not_attended_to(serving, fresh, group, d, bad):
+    """What is left of the sequence is attended to as if those tokens did not exist; a row that has nothing left gives zeros."""
+    p = Paged(serving, 97 + d, [(fresh, 170), (fresh, 190)], 2, 16, d, wild=False)
+    q, out = query(p, 2 * group, torch.float16)
+    for i, page in enumerate(bad):
+        p.batch.page_table[1, page] = (-1, p.data.shape[1], 1 << 30, -(1 << 31))[i]
+    got = ref.f64(p.cache.attend(q, p.batch, out=out))
+    assert serving.paged_error() == 2
+    want, bound = ref.attend_capped(*p.arrays(), ref.f64(q), d ** -0.5, 0.0, torch.float16, missing={(1, page) for page in bad})
+    assert (np.abs(got - want) <= bound).all()
+
+
+@pytest.mark.parametrize("fresh", [1, 5, 150])
+def test_rows_without_any_page_are_zeros(serving, fresh):
+    p = Paged(serving, 98, [(fresh, 160), (fresh, 150)], 2, 16, 64, wild=False)
+    q, out = query(p, 4, torch.float16)
+    p.batch.page_table[0] = -1
+    p.cache.attend(q, p.batch, out=out)
+    assert serving.paged_error() == 2
+    assert (out[:fresh] == 0).all() and (out[fresh:] != 0).any()
