@@ -211,7 +211,7 @@ class PagedCache(_Described):
     def attend(self, q: torch.Tensor, batch: PagedBatch, out: torch.Tensor | None = None, scale: float | None = None, causal: bool = True,
                window: int = 0, softcap: float = 0.0) -> torch.Tensor:
         """Attention of the new tokens' queries [tokens, query_heads, head_dim] over the cache, which holds the new tokens already.
-        ``scale`` defaults to head_dim ** -0.5; rows of no sequence are left as they are in ``out``, undefined in a new tensor."""
+        ``scale`` defaults to head_dim ** -0.5; a ``window`` of 0 is none, and one as long as the sequence hides nothing; rows of no sequence are left as they are in ``out``, undefined in a new tensor."""
         if _device(q, out) != self.device or batch.device != self.device:
             raise ValueError("tensors have to be on the cache's device")
         if out is None:
@@ -225,7 +225,7 @@ class PagedCache(_Described):
             need = batch._space[sizes] = value.value
         space = q.new_empty(need, dtype=torch.int8) if need else None
         _enter(self.device, _entries.mlel_cuda_paged_attention, self._packed, batch._packed, packed, _pack(out),
-               q.shape[-1] ** -0.5 if scale is None else scale, 1 if causal else 0, window, softcap,
+               q.shape[-1] ** -0.5 if scale is None else scale, 1 if causal else 0, max(-1, min(window, 0x7fffffff)), softcap,
                None if space is None else space.data_ptr(), need)
         return out
 

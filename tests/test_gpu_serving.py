@@ -840,3 +840,13 @@ def test_rows_without_any_page_are_zeros(serving, fresh):
     p.cache.attend(q, p.batch, out=out)
     assert serving.paged_error() == 2
     assert (out[:fresh] == 0).all() and (out[fresh:] != 0).any()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 63 - 1])
+def test_windows_beyond_32_bits_hide_nothing(serving, mlel, window):
+    p = Paged(serving, 99, [(1, 60), (3, 40)], 1, 16, 64, wild=False)
+    q, out = query(p, 2, torch.float16)
+    want = p.cache.attend(q, p.batch)
+    assert torch.equal(p.cache.attend(q, p.batch, window=window)[:4], want[:4])
+    with pytest.raises(mlel.MlelError, match="not negative"):
+        p.cache.attend(q, p.batch, window=-window)
