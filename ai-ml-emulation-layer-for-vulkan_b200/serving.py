@@ -92,7 +92,8 @@ def _enter(index: int, entry, *arguments) -> None:
 
 def quantize_rows(x: torch.Tensor, out: torch.Tensor | None = None, scales: torch.Tensor | None = None):
     """``(q, scales)``: the rows of ``x`` [..., K] (f32, f16 or bf16) in 8 bits with an f32 scale for each: ``scales = max|x| / 127``,
-    ``q = round(x / scales)``.  ``out`` and ``scales`` are written where they are given ([M, K] int8 and [M], for M rows in all)."""
+    ``q = round(x / scales)``.  ``out`` and ``scales`` are written where they are given ([M, K] int8 and [M], for M rows in all).  A new
+    ``q`` is packed: where K is no multiple of 16 and a product follows, give an ``out`` whose rows lie on 16-byte boundaries."""
     index = _device(x, out, scales)
     shape = x.shape
     if len(shape) < 1:
@@ -109,7 +110,9 @@ def quantize_rows(x: torch.Tensor, out: torch.Tensor | None = None, scales: torc
 def matmul_scaled(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor, bias: torch.Tensor | None = None,
                   out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``(a @ b.T) * a_scales[:, None] * b_scales + bias`` for int8 ``a`` [M, K] (tokens) and ``b`` [N, K] (weights, a row per
-    output channel), scales and bias in f32: the sums are exact, the result is rounded once to ``dtype`` (or ``out``'s type)."""
+    output channel), scales and bias in f32: the sums are exact, the result is rounded once to ``dtype`` (or ``out``'s type).  Tensor
+    cores want the rows of both on 16-byte boundaries, as ``QuantizedLinear`` lays them out; packed rows of a K that is no multiple of
+    16 go a far slower way."""
     index = _device(a, a_scales, b, b_scales, bias, out)
     if out is None:
         out = a.new_empty((a.shape[0], b.shape[0]), dtype=dtype)

@@ -442,9 +442,10 @@ int mlel_cuda_quantize_rows(const mlel_tensor *input, const mlel_tensor *output,
 
 /* Product in 8-bit integers with a scale for each token and channel:
  *   output[m][n] = (sum_k a[m][k] * b[n][k]) * a_scales[m] * b_scales[n] + biases[n]
- * The sum is exact (K at most 131071); the rest is computed in f32 and rounded once to the output's type.  a [M, K] int8 (tokens),
- * b [N, K] int8 (weights, a row per output channel), a_scales [M], b_scales [N], biases [N] or NULL, all packed f32; output
- * [M, N] f32, f16 or bf16.  Rows of a and b that start on 16-byte boundaries go the fast way. */
+ * The sum is exact (K at most 131071); the rest is computed in f32 and rounded once to the output's type.  a [M, K] int8 (tokens, at
+ * most 4194240), b [N, K] int8 (weights, a row per output channel), a_scales [M], b_scales [N], biases [N] or NULL, all packed f32;
+ * output [M, N] f32, f16 or bf16.  Rows of a and b that start on 16-byte boundaries go to the tensor cores, others (packed rows of a K
+ * that is no multiple of 16 among them) the far slower way of any address. */
 int mlel_cuda_matmul_scaled(const mlel_tensor *a, const mlel_tensor *a_scales, const mlel_tensor *b, const mlel_tensor *b_scales,
                             const mlel_tensor *biases, const mlel_tensor *output, void *cuda_stream);
 
@@ -484,7 +485,8 @@ typedef struct mlel_paged_batch {
  * queries, rotated_queries [tokens, query_heads, head_dim] of the keys' type, both NULL where there is nothing to rotate; they may
  * be the same tensor.  cosines and sines NULL: no rotation.
  * A page's scale is max |element| / 127 over what is in it.  Where new tokens join older ones in a page and have larger
- * elements, its older integers are rescaled once, to the nearest whole numbers.  A page whose first row is new starts afresh.
+ * elements, its older integers are rescaled once, to the nearest whole numbers (under a scale of 0 they are zeros, as this call writes
+ * them, and stay as they are).  A page whose first row is new starts afresh.
  * New tokens with an infinity or a NaN make the page's scale that, and with it all that attends to the page no number either.
  * A page that receives tokens belongs to one sequence; pages that are only read may be shared. */
 int mlel_cuda_paged_append(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *keys,
@@ -496,7 +498,9 @@ int mlel_cuda_paged_append(const mlel_paged_cache *cache, const mlel_paged_batch
  * over the tokens j of the query's own sequence: all of them, or with `causal` those up to the query's own position p; with
  * window > 0 only j > p - window.  queries, output [tokens, query_heads, head_dim], both f16 or both bf16; query_heads a multiple of
  * the cache's heads, query head h reads cache head h / (query_heads / heads).  The products run in f16 with f32 sums; the softmax
- * is in f32.  `workspace`: mlel_paged_attention_workspace() bytes of device memory on a 16-byte boundary that nothing else uses
+ * is in f32, its weights rounded to f16 (bf16 results of many rows divide by the sum of the weights before that rounding, all others
+ * by the sum after it).  Tokens that the masks hide from a query change nothing of its result beyond such roundings, whatever they are;
+ * a scale that is not finite, seen, makes it NaN.  `workspace`: mlel_paged_attention_workspace() bytes of device memory on a 16-byte boundary that nothing else uses
  * until the call's work is done (its contents do not matter before or after). */
 int mlel_cuda_paged_attention(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries,
                               const mlel_tensor *output, float scale, int causal, int32_t window, float softcap, void *workspace,
