@@ -129,16 +129,30 @@ __device__ __forceinline__ void loadQuerySixteen(const T *q, int first, int leng
     }
 }
 
-// Four elements of one row of the answer: y / sum, or zeros for a row that nothing was added to.
+// What turns units of 2^from into units of 2^to, both maxima of one row and from <= to.
+__device__ __forceinline__ float unitsOf(float from, float to) { return from == to ? 1.f : exp2Fast(from - to); }
+// Logarithm of a value scale: that of the smallest number for 0, NaN for what is not finite.
+__device__ __forceinline__ float logOfScale(float scale) {
+    const float y = log2f(scale);
+    return y < -150.f ? -150.f : y;
+}
+// The exponent of a weight of 14 bits in excess of its score's, by the logarithm of its value's scale and its row's two maxima.
+__device__ __forceinline__ float weightShift(float valueLog, float loudest, float most) {
+    const float own = valueLog - loudest, least = -60.f - most;
+    return (own < least ? least : own) + 14.f; // (a NaN stays one)
+}
+
+// Four elements of one row of the answer: y / sum * 2^exponent, or zeros for a row that nothing was added to.
 template <class T>
-__device__ __forceinline__ void writeOut(const AttendParams &p, int firstToken, int row, int head, int d, float4 y, float sum) {
+__device__ __forceinline__ void writeOut(const AttendParams &p, int firstToken, int row, int head, int d, float4 y, float sum, float exponent) {
     if (d >= p.cache.headDim) {
         return;
     }
     const int token = row / p.group, queryHead = head * p.group + row - token * p.group;
     T *to = reinterpret_cast<T *>(p.out + int64_t(firstToken + token) * p.outStride[0] + queryHead * p.outStride[1]) + d;
-    const float f = sum == 0.f ? 0.f : 1.f / sum;
-    const uint2 packed = {packTwo(y.x * f, y.y * f, T()), packTwo(y.z * f, y.w * f, T())};
+    // (in two halves: the power of two may be outside the normal numbers where the result is not)
+    const float unit = sum == 0.f ? 0.f : exp2Fast(0.5f * exponent), f = sum == 0.f ? 0.f : unit / sum;
+    const uint2 packed = {packTwo(y.x * f * unit, y.y * f * unit, T()), packTwo(y.z * f * unit, y.w * f * unit, T())};
     if (p.wideOut) {
         *reinterpret_cast<uint2 *>(to) = packed;
     } else {

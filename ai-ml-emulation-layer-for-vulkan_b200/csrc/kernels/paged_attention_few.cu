@@ -33,13 +33,12 @@
 // result would have to be subtracted from sums that may be a thousand times smaller than it.
 //
 // bf16 queries become f16 after a row-wise power of two that puts the largest at 2^14; elements down to 2^-29 of that stay
-// exact.  The scale of 16 values is part of the exponent: weights are rounded to f16 as 2^(s + log2(scale / r) - m + 14), r a running
-// power of two, m the row's largest s + log2(scale / r), so that what is lost lies 2^-38 below what counts most in the row's own sum:
-// values that a row does not see, or gives next to no weight, take no bits from the others, however large they are.  (r keeps the
-// numbers in range; values whose scale is below 2^-90 of it count as 2^-90 of it.)  The sum is over the weights as they are rounded,
-// so that what rounding does to the key that has most of a row cancels.  The result stays in registers in units of 2^(m + r); it is
-// rescaled only when a maximum or r grows, which one vote per 32 keys finds out.  r does not go below 2^-112, so that the factor of
-// the result is a normal number.
+// exact.  A row keeps two maxima: m of its scores x, in whose units the sum of the softmax is, and e of x + log2(value scale), in
+// whose units the result is.  The scale of 16 values is part of the exponent: weights are rounded to f16 as 2^(x + log2(scale) - e + 14), so
+// that what is lost lies 2^-38 below what counts most in the row's own result: values that a row does not see, or gives next to no
+// weight, take no bits from the others, however large they are.  (A scale below 2^-60 of e's counts as 2^-60 of it, so that its
+// weights reach the sum.)  The sum is over the weights as they are rounded, so that what rounding does to the key that has most of
+// a row cancels.  The result stays in registers; it is rescaled only when a maximum grows, which one vote per 32 keys finds out.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -63,9 +62,8 @@ constexpr int kWarps = 4, kTileRows = 8;
 constexpr int kGroup = 16; // keys that share a page and a scale for certain
 constexpr int kStageGroups = 2;
 constexpr int kStepGroups = kWarps * kStageGroups;
-constexpr float kWeightBits = 14.f;       // a row's largest weight is 2^14
-constexpr float kLeastReference = -112.f; // of the values, a power of two: over the largest weight still a normal number
-constexpr float kLeastBits = -90.f;       // of a value scale against the reference: sums of 2^-kLeastBits are still far from infinite
+constexpr float kWeightBits = 14.f; // a row's largest weight is 2^14
+constexpr float kSlack = 30.f;      // by which scores may exceed m, in powers of two, before it is taken up: it only is the sum's unit
 constexpr int kClusterSteps = 3; // steps by which a cluster's blocks may outlast the line's
 
 template <int DP> struct FewShape {
@@ -165,7 +163,7 @@ __device__ void locate(const AttendParams &p, FewScan &scan, int piece, int piec
     __syncthreads();
 }
 
-// One row of a partial result: maximum, sum, then DP elements.
+// One row of a partial result: e, sum, m and nothing, then DP elements.
 template <int DP> __device__ __forceinline__ float *partialRow(const AttendParams &p, int piece, int which, int row) {
     return p.partials + ((int64_t(piece) * 2 + which) * kTileRows + row) * (DP + 4);
 }
@@ -182,7 +180,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
     uint8_t *ring = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(rawSmem) + 1023) & ~uintptr_t(1023));
     __shared__ uint64_t full[kWarps][STAGES];
     __shared__ FewScan scan;
-    __shared__ float joinMax[kWarps][kTileRows], joinSum[kWarps][kTileRows];
+    __shared__ float joinMost[kWarps][kTileRows], joinLoudest[kWarps][kTileRows], joinSum[kWarps][kTileRows];
     const int lane = int(threadIdx.x) & 31, warp = int(threadIdx.x) >> 5, g = lane >> 2, t = lane & 3;
     if (threadIdx.x == 0) {
         for (int w = 0; w < kWarps; ++w) {
@@ -259,8 +257,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             return scale < INFINITY ? scale : NAN;
         };
         int slots = slotOf(lane), nextSlots = slotOf(32 + lane);
-        // value scales as logarithms: -infinity for 0, NaN for what is not finite
-        float keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = log2f(scaleOf(p.cache.valueScales, slots));
+        float keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = logOfScale(scaleOf(p.cache.valueScales, slots));
         int issued = 0, writeStage = stage, issueSlots = slots;
         // lanes that issue a copy: keys or values, which of the two groups, which panel
         const int side = lane & 1, sub = (lane >> 1) & 1, panel = lane >> 2;
@@ -351,13 +348,12 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         const int lastToken = int(fastDiv(uint32_t(firstRow + rows - 1), p.groupDiv)), firstToken = int(fastDiv(uint32_t(firstRow), p.groupDiv));
         const int openHi = p.causal ? old + firstToken + 1 : w.q.length, openLo = p.window > 0 ? max(0, old + lastToken - p.window + 1) : 0;
 
-        float o[MT][4] = {}, most[2], sum[2] = {};
-        float reference = kLeastReference; // of the values, as a power of two
-        most[0] = most[1] = -INFINITY;
+        float o[MT][4] = {}, most[2], loudest[2], sum[2] = {}; // m and e of two rows
+        most[0] = most[1] = loudest[0] = loudest[1] = -INFINITY;
         for (int n = 0; n < count; ++n) {
             if (n > 0 && (n & 15) == 0) {
                 slots = nextSlots;
-                keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = log2f(scaleOf(p.cache.valueScales, slots));
+                keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = logOfScale(scaleOf(p.cache.valueScales, slots));
                 nextSlots = slotOf(2 * n + 32 + lane);
             }
             if (n < issued) {
@@ -396,52 +392,42 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                     }
                 }
                 const bool masked = key0 + AT * kGroup > openHi || key0 < openLo || absent;
-                // the values' reference, and their scales in units of it (a scale that is not finite reaches the rows that see it through
-                // their weights)
-                float loudest = valueLog[0], shift[AT];
-#pragma unroll
-                for (int h = 1; h < AT; ++h) {
-                    loudest = fmaxf(loudest, valueLog[h]);
-                }
-                const bool raise = loudest > reference;
-                const float before = reference;
-                reference = raise ? fminf(ceilf(loudest), 127.f) : reference;
-                bool grows = raise;
+                bool grows = false;
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
-                    shift[h] = valueLog[h] - reference;
-                    shift[h] = shift[h] < kLeastBits ? kLeastBits : shift[h];
+                    // what a score may be before one of the maxima grows (a scale that is no number limits nothing)
+                    const float limit[2] = {fminf(loudest[0] - valueLog[h], most[0] + kSlack), fminf(loudest[1] - valueLog[h], most[1] + kSlack)};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         float x = s[h][e] * (rowScale[e & 1] * keyScale[h]);
                         if (p.softcap > 0.f) {
                             x = softCapped<LARGE_CAP>(x, p.softcap, p.perCap) * kLog2e;
                         }
-                        x += shift[h];
                         if (masked) { // row g (or g + 8) of the product is key (g >> 1) + 4 (g & 1) (+ 8) of the group
                             const int key = key0 + h * kGroup + (g >> 1) + 4 * (g & 1) + 8 * (e >> 1);
                             x = key < rowHi[e & 1] && key >= rowLo[e & 1] && keyScale[h] != -1.f ? x : -INFINITY;
                         }
                         s[h][e] = x;
-                        grows = grows || x > most[e & 1];
+                        grows = grows || x > limit[e & 1];
                     }
                 }
                 if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const float same = most[x] - (reference - before); // a reference that grows lowers the maximum
-                        float top = same;
+                        float top = most[x], loud = loudest[x];
 #pragma unroll
-                        for (int h = 0; h < AT; ++h) {
-                            top = fmaxf(top, fmaxf(s[h][x], s[h][2 + x]));
+                        for (int h = 0; h < AT; ++h) { // (a maximum passes over what is no number)
+                            const float score = fmaxf(s[h][x], s[h][2 + x]);
+                            top = fmaxf(top, score), loud = fmaxf(loud, score + valueLog[h]);
                         }
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                        // sums are in units of 2^most, results of 2^(most + reference)
-                        sum[x] *= top == -INFINITY ? 1.f : exp2Fast(fminf(most[x] - top, -kLeastBits));
-                        const float factor = top == -INFINITY ? 1.f : exp2Fast(same - top);
-                        most[x] = top;
+#pragma unroll
+                        for (int step = 4; step < 32; step <<= 1) {
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+                            loud = fmaxf(loud, __shfl_xor_sync(0xffffffffu, loud, step));
+                        }
+                        sum[x] *= unitsOf(most[x], top);
+                        const float factor = unitsOf(loudest[x], loud);
+                        most[x] = top, loudest[x] = loud;
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
                             o[mt][x] *= factor, o[mt][2 + x] *= factor;
@@ -450,22 +436,29 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                 }
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
-                    const bool rounded = shift[h] >= -6.f; // no weight that matters is a subnormal number
-                    float2 part = {0.f, 0.f};
                     uint32_t wf[2]; // P^T: keys in pairs by t, row g
-                    const float base0 = most[0] == -INFINITY ? kWeightBits : kWeightBits - most[0],
-                                base1 = most[1] == -INFINITY ? kWeightBits : kWeightBits - most[1];
+                    float shift[2], part[2] = {0.f, 0.f};
+                    bool rounded[2];
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) { // what the mask hides has a weight of 0
-                        const float w0 = exp2Fast(s[h][2 * half] + base0), w1 = exp2Fast(s[h][2 * half + 1] + base1);
+                    for (int x = 0; x < 2; ++x) {
+                        const float base = most[x] == -INFINITY ? 0.f : most[x];
+                        shift[x] = weightShift(valueLog[h], loudest[x], base);
+                        rounded[x] = shift[x] + base >= 8.f; // no weight that matters is a subnormal number
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) { // what the mask hides stays out, whatever its page's scale is
+                        const float x0 = s[h][2 * half], x1 = s[h][2 * half + 1];
+                        const float w0 = masked && x0 == -INFINITY ? 0.f : exp2Fast(x0 + shift[0]);
+                        const float w1 = masked && x1 == -INFINITY ? 0.f : exp2Fast(x1 + shift[1]);
                         const uint32_t two = packTwo(w0, w1, __half());
                         wf[half] = transposeHalves(two);
-                        const float2 w = rounded ? unpackTwo(two, __half()) : float2{w0, w1};
-                        part.x += w.x, part.y += w.y;
+                        const float2 w = unpackTwo(two, __half());
+                        part[0] += rounded[0] ? w.x : w0, part[1] += rounded[1] ? w.y : w1;
                     }
-                    const float perWeight = exp2Fast(-kWeightBits - shift[h]);
-                    sum[0] = part.x == 0.f ? sum[0] : fmaf(part.x, perWeight, sum[0]);
-                    sum[1] = part.y == 0.f ? sum[1] : fmaf(part.y, perWeight, sum[1]);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        sum[x] = part[x] == 0.f ? sum[x] : fmaf(part[x], exp2Fast(-shift[x] - most[x]), sum[x]);
+                    }
                     constexpr int CHUNKS = DP < 128 ? 1 : DP / 128, WORDS = DP < 128 ? 2 : 4; // 16 (or, below 128, 8) bytes of a value row per lane each
                     const uint32_t group = values + uint32_t(h * Shape::kGroupBytes);
 #pragma unroll
@@ -512,7 +505,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 8);
             sum[x] += __shfl_xor_sync(0xffffffffu, sum[x], 16);
             if (g == 0) {
-                joinMax[warp][2 * t + x] = most[x], joinSum[warp][2 * t + x] = sum[x];
+                joinMost[warp][2 * t + x] = most[x], joinLoudest[warp][2 * t + x] = loudest[x], joinSum[warp][2 * t + x] = sum[x];
             }
         }
         __syncthreads(); // every warp's copies have been read: the ring holds results from here on
@@ -524,11 +517,11 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         for (int x = 0; x < 2; ++x) {
             const int itsRow = 2 * t + x;
             if (itsRow < rows) {
-                float top = -INFINITY;
+                float loud = -INFINITY;
                 for (int v = 0; v < kWarps; ++v) {
-                    top = fmaxf(top, joinMax[v][itsRow]);
+                    loud = fmaxf(loud, joinLoudest[v][itsRow]);
                 }
-                const float factor = (top == -INFINITY ? 1.f : exp2Fast(most[x] - top)) * exp2Fast(reference - kWeightBits);
+                const float factor = unitsOf(loudest[x], loud);
                 float *to = results + (warp * kTileRows + itsRow) * kPitch;
                 // tile mt holds elements 2 (mt % 8) and the next of the lane's 16 (or 8) of each chunk
 #pragma unroll
@@ -545,24 +538,24 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         for (int i = int(threadIdx.x); i < rows * (DP / 4); i += kWarps * 32) {
             const int itsRow = i / (DP / 4), d = (i - itsRow * (DP / 4)) * 4;
             float4 y = {};
-            float top = -INFINITY, weights = 0.f;
+            float top = -INFINITY, loud = -INFINITY, weights = 0.f;
 #pragma unroll
             for (int v = 0; v < kWarps; ++v) {
-                top = fmaxf(top, joinMax[v][itsRow]);
+                top = fmaxf(top, joinMost[v][itsRow]), loud = fmaxf(loud, joinLoudest[v][itsRow]);
                 const float4 a = *reinterpret_cast<const float4 *>(results + (v * kTileRows + itsRow) * kPitch + d);
                 y.x += a.x, y.y += a.y, y.z += a.z, y.w += a.w;
             }
 #pragma unroll
             for (int v = 0; v < kWarps; ++v) {
-                weights += joinSum[v][itsRow] * (top == -INFINITY ? 1.f : exp2Fast(joinMax[v][itsRow] - top));
+                weights += joinSum[v][itsRow] * unitsOf(joinMost[v][itsRow], top);
             }
             if (whole) {
-                writeOut<T>(p, w.q.first, firstRow + itsRow, head, d, y, weights);
+                writeOut<T>(p, w.q.first, firstRow + itsRow, head, d, y, weights, loud - top - kWeightBits);
             } else {
                 float *to = split > 0 ? joined + itsRow * kPitch : partialRow<DP>(p, blockIdx.x, at == begin ? 0 : 1, itsRow);
                 *reinterpret_cast<float4 *>(to + 4 + d - (split > 0 ? 4 : 0)) = y;
                 if (d == 0) {
-                    to[split > 0 ? DP : 0] = top, to[split > 0 ? DP + 1 : 1] = weights;
+                    *reinterpret_cast<float4 *>(to + (split > 0 ? DP : 0)) = {loud, weights, top, 0.f};
                 }
             }
         }
@@ -572,19 +565,20 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             const uint32_t from = smemAddr(joined);
             for (int i = int(threadIdx.x) + rank * (kWarps * 32); i < rows * (DP / 4); i += split * (kWarps * 32)) {
                 const int itsRow = i / (DP / 4), d = (i - itsRow * (DP / 4)) * 4;
-                float top = -INFINITY, weights = 0.f;
+                float top = -INFINITY, loud = -INFINITY, weights = 0.f;
                 float4 y = {};
                 for (int r = 0; r < split; ++r) {
-                    top = fmaxf(top, loadCluster(mapToCta(from + uint32_t((itsRow * kPitch + DP) * 4), uint32_t(r))).x);
+                    const float4 stats = loadCluster(mapToCta(from + uint32_t((itsRow * kPitch + DP) * 4), uint32_t(r)));
+                    loud = fmaxf(loud, stats.x), top = fmaxf(top, stats.z);
                 }
                 for (int r = 0; r < split; ++r) {
                     const float4 stats = loadCluster(mapToCta(from + uint32_t((itsRow * kPitch + DP) * 4), uint32_t(r)));
                     const float4 a = loadCluster(mapToCta(from + uint32_t((itsRow * kPitch + d) * 4), uint32_t(r)));
-                    const float factor = top == -INFINITY ? 1.f : exp2Fast(stats.x - top);
+                    const float factor = unitsOf(stats.x, loud);
                     y.x += a.x * factor, y.y += a.y * factor, y.z += a.z * factor, y.w += a.w * factor;
-                    weights += stats.y * factor;
+                    weights += stats.y * unitsOf(stats.z, top);
                 }
-                writeOut<T>(p, w.q.first, firstRow + itsRow, head, d, y, weights);
+                writeOut<T>(p, w.q.first, firstRow + itsRow, head, d, y, weights, loud - top - kWeightBits);
             }
             __syncwarp();
             clusterSync(); // nobody leaves while its part is being read
@@ -605,7 +599,7 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
     constexpr int THREADS = kWarps * 32;
     using T = typename std::conditional<HALF, __half, __nv_bfloat16>::type;
     __shared__ int parts[2][kWarps];
-    __shared__ float factors[kMostPieces], stats[2][kWarps];
+    __shared__ float factors[kMostPieces], stats[3][kWarps];
     __shared__ float4 sums[THREADS];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // the tiles of all sequences in a row, those of a sequence without work included: ceil(max_new * group / kTileRows) * heads each
@@ -640,28 +634,29 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
     }
     const int first = x0 == pieces.start(c0) ? 0 : 1; // where piece c0 left it: as its first tile, or as its last
     const auto part = [&](int c) { return partialRow<DP>(p, c0 + c, c == 0 ? first : 0, row); };
-    float top = -INFINITY;
+    float top = -INFINITY, loud = -INFINITY;
     for (int c = int(threadIdx.x); c < n; c += THREADS) {
-        top = fmaxf(top, part(c)[0]);
+        const float4 s = *reinterpret_cast<const float4 *>(part(c));
+        loud = fmaxf(loud, s.x), top = fmaxf(top, s.z);
     }
 #pragma unroll
     for (int step = 16; step > 0; step >>= 1) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+        loud = fmaxf(loud, __shfl_xor_sync(0xffffffffu, loud, step));
     }
     if (lane == 0) {
-        stats[0][warp] = top;
+        stats[0][warp] = top, stats[2][warp] = loud;
     }
     __syncthreads();
 #pragma unroll
     for (int v = 0; v < kWarps; ++v) {
-        top = fmaxf(top, stats[0][v]);
+        top = fmaxf(top, stats[0][v]), loud = fmaxf(loud, stats[2][v]);
     }
     float weights = 0.f;
     for (int c = int(threadIdx.x); c < n; c += THREADS) {
-        const float2 s = *reinterpret_cast<const float2 *>(part(c));
-        const float factor = top == -INFINITY ? 1.f : exp2Fast(s.x - top);
-        factors[c] = factor;
-        weights += s.y * factor;
+        const float4 s = *reinterpret_cast<const float4 *>(part(c));
+        factors[c] = unitsOf(s.x, loud);
+        weights += s.y * unitsOf(s.z, top);
     }
 #pragma unroll
     for (int step = 16; step > 0; step >>= 1) {
@@ -693,7 +688,7 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
             const float4 a = sums[v * kLanes + int(threadIdx.x)];
             y.x += a.x, y.y += a.y, y.z += a.z, y.w += a.w;
         }
-        writeOut<T>(p, w.q.first, firstRow + row, head, d, y, weights);
+        writeOut<T>(p, w.q.first, firstRow + row, head, d, y, weights, loud - top - kWeightBits);
     }
 }
 

@@ -16,17 +16,23 @@
 // What bounds it: per 256 x 128 scores the products take 2048 cycles at 128 elements a head, and 32768 exponentials the
 // same at 16 a cycle; everything else (a multiply-add, half a maximum, half a sum, half a conversion per score, and the
 // keys' and values' conversion) shares the four schedulers with them: some 4500 cycles.  Four prompts of 6000 tokens, 32 heads of 128
-// elements over 8: 819 us, 775 TFLOP/s.
+// elements over 8: 790 us, 803 TFLOP/s.
 //
 // Softmax in one pass where it can: scores are weighed with the maximum known from the tiles before, and only if one exceeds
 // it by more than 2^8, or at a row's first tile and where the values' reference grows, the maximum is taken first and sums
-// and result are rescaled.  The scale of 16 values is part of the exponent: w = 2^(s + log2(scale / r) - m + 7), r a running
-// power of two, m the row's largest s + log2(scale / r), and the sum over the weights of 16 keys is divided by scale / r again.  So a
-// weight is at most 2^15, and f16's steps end 2^-31 below what counts most in the row's own sum: values that a row does not see, or gives
-// next to no weight, take no bits from the others, however large they are.  (r keeps the numbers in range; values whose scale
-// is below 2^-90 of it count as 2^-90 of it.)  For f16 results the sum is over the
-// weights as they are rounded, so that what rounding does to the key that has most of a row cancels (a seventh off the error
-// against 64 bits; bf16 has steps eight times as large, and four prompts of 6000 tokens would take 899 us for 822).
+// and result are rescaled.  A row keeps two maxima: m of its scores x, in whose units the sum of the softmax is, and e of
+// x + log2(value scale), in whose units the result is.  The scale of 16 values is part of the exponent: w = 2^(x + log2(scale) - e + 7),
+// so a weight is at most 2^15, and f16's steps end 2^-31 below what counts most in the row's own result: values that a row does not see,
+// or gives next to no weight, take no bits from the others, however large they are.  (e is kept against r, a running power of two
+// above the scales, so that log2(scale / r) and its power belong to a tile and not to a row.)
+// The sum is over the weights as they are rounded, so that what rounding does to the key that has most of a row cancels (a seventh off
+// the error against 64 bits).
+// Tiles that a mask cuts, or with scales far below r, go a second way, which asks for each key and forms by the row what the first way
+// takes from the tile.  The two are apart, rather than a group at a time, and the second takes eight scores at a time, so that the weights
+// of 64 keys and all else fit 80 registers: what does not comes back from L2, shared memory having all of the L1 cache (the same
+// with both ways in one loop: 860 us).  The queries' loads are issued one after another before any is used: the compiler
+// would save registers and wait for each in turn (3.6 us a block).
+
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -51,7 +57,8 @@ constexpr int kConvertWarps = 4;
 constexpr int kParamRing = 5, kStaging = 4, kSlots = 3; // of a tile's keys or values: integers on their way, and f16
 constexpr float kGrowth = 8.f;                          // in powers of two
 constexpr float kWeightBits = 7.f;
-constexpr float kLeastBits = -90.f; // of a value scale against the reference: sums of 2^-kLeastBits are still far from infinite
+constexpr float kEvenBits = -6.f;   // of a value scale against the reference: no weight that matters is a subnormal number
+constexpr float kSlack = 60.f;      // by which scores may exceed m where the scales do not bound it: it only is the sum's unit
 
 // Heads of 256 elements: one tile of rows (its result alone has 256 columns of tensor memory), and 64 keys at a time, whose f16 form is
 // as large as that of 128 keys of 128 elements.
@@ -76,6 +83,7 @@ struct TileParams {
     float perWeight[kMostGroups]; // 2^-shift
     int reference;           // a power of two
     uint32_t there;          // groups that exist
+    uint32_t uneven;         // those whose value scale is too far below the reference for a sum of rounded weights
 };
 
 struct ManyBarriers {
@@ -184,6 +192,37 @@ __device__ __forceinline__ uint32_t pairVote(int barrier, bool predicate) {
                  : "memory");
     return any;
 }
+__device__ __forceinline__ void tmemLoad8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmemWait8(uint32_t (&r)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+                 :
+                 : "memory");
+}
+// 1 / unit for a power of two from 2^-126 to 2^126.
+__device__ __forceinline__ float inverseOfPower(float unit) { return __uint_as_float(0x7f000000u - __float_as_uint(unit)); }
+// 16 bytes from a 16-byte boundary where `there`, zeros elsewhere.  (In order with one another: a row of these is on its way at once,
+// where the compiler would rather save registers and wait for each in turn.)
+__device__ __forceinline__ uint4 loadIf(const char *from, bool there) {
+    uint4 v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.u32 %0, 0;\n\tmov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+                 "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+                 : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+                 : "l"(from), "r"(there ? 1u : 0u)
+                 : "memory");
+    return v;
+}
+// exp2Fast, not to be moved ahead of others (whose results would wait in registers).
+__device__ __forceinline__ float exp2InOrder(float x) {
+    float y;
+    asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 __device__ __forceinline__ void tmemStoreWait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 enum Cap : int { kNoCap, kCap, kLargeCap }; // see softCapped
@@ -208,7 +247,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     ManyBarriers &bars = state.bars;
     TileParams(&params)[kParamRing] = state.params;
     float(&exchange)[2][kRows][2] = state.exchange;
-    const int warp = int(threadIdx.x) >> 5, lane = int(threadIdx.x) & 31;
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) >> 5, 0), lane = int(threadIdx.x) & 31;
     // There is no room to spare for rounding the address up; without static shared memory it is a multiple of 1024 already.
     if (smem != rawSmem) {
         if (threadIdx.x == 0) {
@@ -336,13 +375,14 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 int exponent = magnitude > 0.f && magnitude < INFINITY ? int(__float_as_uint(powerAbove(magnitude)) >> 23) - 127 : -126;
                 exponent = __reduce_max_sync(0xffffffffu, exponent);
                 reference = max(reference, exponent);
+                const float bits = logOfScale(valueScale) - float(reference); // (no number for a scale that is not finite)
                 if (lane < kGroups) {
-                    const float shift = magnitude < INFINITY ? fmaxf(log2f(magnitude) - float(reference), kLeastBits) + kWeightBits : NAN;
-                    to.keyScale[lane] = keyScale, to.shift[lane] = shift, to.perWeight[lane] = exp2f(-shift);
+                    to.keyScale[lane] = keyScale, to.shift[lane] = bits + kWeightBits, to.perWeight[lane] = exp2f(-kWeightBits - bits);
                 }
                 const uint32_t there = __ballot_sync(0xffffffffu, slot >= 0);
+                const uint32_t uneven = __ballot_sync(0xffffffffu, slot >= 0 && !(bits >= kEvenBits));
                 if (lane == 0) {
-                    to.reference = reference, to.there = there;
+                    to.reference = reference, to.there = there, to.uneven = uneven;
                 }
                 __syncwarp();
                 if (lane == 0) {
@@ -476,19 +516,26 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             // The warp's half of its 32 rows, as runs of DP bytes: kLanes lanes a row, kRowsAtOnce rows at a time, all on their way at once.
             constexpr int kLanes = DP / 16, kRowsAtOnce = 32 / kLanes, kSteps = 32 / kRowsAtOnce;
             const int chunk = lane % kLanes, element = half * (DP / 2) + chunk * 8;
+            const auto queryOf = [&](int r) { // where the lane's eight elements of a row of the tile lie
+                const int global = firstRow + which * kRows + r, itsToken = int(fastDiv(uint32_t(global), p.groupDiv));
+                return p.queries + int64_t(q.first + itsToken) * p.queryStride[0] + (head * p.group + global - itsToken * p.group) * p.queryStride[1] +
+                       element * 2;
+            };
             uint4 words[kSteps];
+            if (p.wideQueries) {
 #pragma unroll
-            for (int step = 0; step < kSteps; ++step) {
-                const int r = quarter * 32 + step * kRowsAtOnce + lane / kLanes, global = firstRow + which * kRows + r;
-                words[step] = {0u, 0u, 0u, 0u};
-                if (which * kRows + r < rows && element < p.cache.headDim) {
-                    const int itsToken = int(fastDiv(uint32_t(global), p.groupDiv));
-                    const char *from = p.queries + int64_t(q.first + itsToken) * p.queryStride[0] +
-                                       (head * p.group + global - itsToken * p.group) * p.queryStride[1] + element * 2;
-                    if (p.wideQueries) {
-                        words[step] = *reinterpret_cast<const uint4 *>(from);
-                    } else {
-                        const uint16_t *e = reinterpret_cast<const uint16_t *>(from);
+                for (int step = 0; step < kSteps; ++step) {
+                    const int r = quarter * 32 + step * kRowsAtOnce + lane / kLanes;
+                    const bool there = which * kRows + r < rows && element < p.cache.headDim;
+                    words[step] = loadIf(queryOf(there ? r : 0), there);
+                }
+            } else {
+#pragma unroll
+                for (int step = 0; step < kSteps; ++step) {
+                    const int r = quarter * 32 + step * kRowsAtOnce + lane / kLanes;
+                    words[step] = {0u, 0u, 0u, 0u};
+                    if (which * kRows + r < rows && element < p.cache.headDim) {
+                        const uint16_t *e = reinterpret_cast<const uint16_t *>(queryOf(r));
                         words[step] = {uint32_t(e[0]) | uint32_t(e[1]) << 16, uint32_t(e[2]) | uint32_t(e[3]) << 16,
                                        uint32_t(e[4]) | uint32_t(e[5]) << 16, uint32_t(e[6]) | uint32_t(e[7]) << 16};
                     }
@@ -497,19 +544,15 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             float unit = 1.f;
             if (!HALF) {
 #pragma unroll
-                for (int step = 0; step < kSteps; ++step) {
-                    float x[8], most = 0.f;
-                    unpackEight(words[step], x, T());
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        most = maxBits(most, x[j]);
-                    }
+                for (int step = 0; step < kSteps; ++step) { // magnitudes of 16 bits are ordered like their bits
+                    constexpr uint32_t kSigns = 0x7fff7fffu;
+                    uint32_t m = maxHalves(maxHalves(words[step].x & kSigns, words[step].y & kSigns), maxHalves(words[step].z & kSigns, words[step].w & kSigns));
 #pragma unroll
                     for (int other = 1; other < kLanes; other <<= 1) {
-                        most = maxBits(most, __shfl_xor_sync(0xffffffffu, most, other));
+                        m = maxHalves(m, __shfl_xor_sync(0xffffffffu, m, other));
                     }
                     if (chunk == 0) {
-                        exchange[which][quarter * 32 + step * kRowsAtOnce + lane / kLanes][half] = most;
+                        exchange[which][quarter * 32 + step * kRowsAtOnce + lane / kLanes][half] = __uint_as_float(max(m & 0xffffu, m >> 16) << 16);
                     }
                 }
                 asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
@@ -517,7 +560,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
 #pragma unroll
                 for (int step = 0; step < kSteps; ++step) {
                     const int r = quarter * 32 + step * kRowsAtOnce + lane / kLanes;
-                    const float inverse = 1.f / halfUnit(maxBits(exchange[which][r][0], exchange[which][r][1])); // powers of two
+                    const float inverse = inverseOfPower(halfUnit(maxBits(exchange[which][r][0], exchange[which][r][1])));
                     float x[8];
                     unpackEight(words[step], x, T());
 #pragma unroll
@@ -545,8 +588,17 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 mbarArrive(&bars.queries);
             }
         }
-        const int position = old + token;
-        const int rowHi = !live ? 0 : p.causal ? position + 1 : q.length, rowLo = p.window > 0 ? max(0, position - p.window + 1) : 0;
+        // The keys that the lane's row sees, and its place among the rows: formed where they are wanted, from a lane number that is read
+        // again, so that they are not held in registers meanwhile.
+        const auto rowAgain = [&] {
+            int own;
+            asm volatile("mov.u32 %0, %%laneid;" : "=r"(own));
+            return quarter * 32 + own;
+        };
+        const auto limits = [&](int &lo, int &hi) {
+            const int own = which * kRows + rowAgain(), position = old + int(fastDiv(uint32_t(firstRow + min(own, rows - 1)), p.groupDiv));
+            hi = own >= rows ? 0 : p.causal ? position + 1 : q.length, lo = p.window > 0 ? max(0, position - p.window + 1) : 0;
+        };
         // keys that every row of this tile sees
         const int tileFirst = firstRow + which * kRows, tileLast = min(tileFirst + kRows, firstRow + rows) - 1;
         const int openHi = p.causal ? old + int(fastDiv(uint32_t(tileFirst), p.groupDiv)) + 1 : q.length;
@@ -555,7 +607,9 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const uint32_t resultAt = laneBase + Shape::result(which) + uint32_t(half * (DP / 2));
 
         bool ok = true, late = false;
-        float most = -INFINITY, sum = 0.f;
+        // e against the reference, and m (of this lane's half of the keys; at least e); the sums since e was last taken up, in units of
+        // 2^loudest, and all others, in units of 2^most
+        float loudest = -INFINITY, most = -INFINITY, sum = 0.f, others = 0.f;
         int reference = -126;
         const auto scoreOf = [&](uint32_t s, float factor) { // in powers of two
             const float x = __uint_as_float(s) * factor;
@@ -576,7 +630,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             const int key0 = keyLo + tile * kKeys + half * (kKeys / 2);
             const bool masked = keyLo + (tile + 1) * kKeys > openHi || keyLo + tile * kKeys < openLo || tp.there != (1u << kGroups) - 1u;
             // keys of group g that this row sees, a bit each
-            const auto seen = [&](int g) {
+            const auto seen = [&](int g, int rowLo, int rowHi) {
                 const int first = key0 + g * kGroup, hi = max(0, min(kGroup, rowHi - first)), lo = max(0, min(kGroup, rowLo - first));
                 return ((tp.there >> (half * kHalfGroups + g)) & 1u) != 0u ? ((1u << hi) - 1u) & ~((1u << lo) - 1u) : 0u;
             };
@@ -589,31 +643,39 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             };
             uint32_t weights[kKeys / 4];
             bool maximumFirst = tile == 0 || tp.reference != reference;
-            float added;
+            float added, apart; // to the sum: in units of 2^loudest, and of 2^most
             while (true) {
                 if (maximumFirst) {
-                    float top = -INFINITY;
+                    float top = -INFINITY, topScore = -INFINITY;
+                    int rowLo, rowHi;
+                    limits(rowLo, rowHi);
 #pragma unroll 1
                     for (int g = 0; g < kHalfGroups; ++g) {
+                        const uint32_t bits = masked ? seen(g, rowLo, rowHi) : 0xffffu;
+                        if (!__any_sync(0xffffffffu, bits != 0u)) { // as most groups of a causal mask's last tile
+                            continue;
+                        }
                         uint32_t s[16];
                         tmemLoad16(scoresAt + uint32_t(g * 16), s);
                         tmemWait16(s);
                         const float factor = rowScale * tp.keyScale[half * kHalfGroups + g];
-                        const uint32_t bits = masked ? seen(g) : 0xffffu;
                         float topOfGroup = -INFINITY;
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
                             topOfGroup = ((bits >> j) & 1u) != 0u ? fmaxf(topOfGroup, scoreOf(s[j], factor)) : topOfGroup;
                         }
-                        top = fmaxf(top, topOfGroup + (tp.shift[half * kHalfGroups + g] - kWeightBits));
+                        top = fmaxf(top, topOfGroup + (tp.shift[half * kHalfGroups + g] - kWeightBits)), topScore = fmaxf(topScore, topOfGroup);
                     }
-                    exchange[which][tileRow][half] = top;
+                    const int own = rowAgain();
+                    exchange[which][own][half] = top;
                     asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
-                    // Sums are in units of 2^most, results of 2^(most + reference): a reference that grows lowers the maximum.
-                    const float same = most - float(tp.reference - reference);
-                    top = fmaxf(fmaxf(top, exchange[which][tileRow][half ^ 1]), same);
-                    const float keep = top == -INFINITY ? 1.f : exp2Fast(same - top);
-                    sum *= top == -INFINITY ? 1.f : exp2Fast(fminf(most - top, -kLeastBits));
+                    // results are in units of 2^(loudest + reference): a reference that grows lowers the maximum
+                    const float same = loudest - float(tp.reference - reference);
+                    top = fmaxf(fmaxf(top, exchange[which][own][half ^ 1]), same);
+                    const float keep = unitsOf(same, top);
+                    topScore = fmaxf(fmaxf(topScore, top), most);
+                    others = others * unitsOf(most, topScore) + sum * unitsOf(loudest, topScore);
+                    most = topScore, sum = 0.f;
                     if (tile > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
                         addedBefore();
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -630,38 +692,22 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                         }
                         tmemStoreWait();
                     }
-                    most = top, reference = tp.reference;
+                    loudest = top, reference = tp.reference;
                 }
                 bool grows = false;
-                const float base = most == -INFINITY ? 0.f : most;
-                added = 0.f;
+                const float base = loudest == -INFINITY ? 0.f : loudest;
+                added = apart = 0.f;
+                if (!masked && tp.uneven == 0u) {
 #pragma unroll
-                for (int g = 0; g < kHalfGroups; ++g) {
-                    uint32_t s[16];
-                    tmemLoad16(scoresAt + uint32_t(g * 16), s);
-                    const float factor = rowScale * tp.keyScale[half * kHalfGroups + g], bitsOfScale = tp.shift[half * kHalfGroups + g],
-                                shift = bitsOfScale - base;
-                    const uint32_t bits = masked ? seen(g) : 0xffffu;
-                    const bool rounded = HALF && bitsOfScale >= 1.f; // no weight that matters is a subnormal number
-                    tmemWait16(s);
-                    float top = -INFINITY, part = 0.f;
-                    if ((HALF && !rounded) || !__all_sync(0xffffffffu, bits == 0xffffu)) {
-                        // what the mask hides stays out, whatever its page's scales are
-#pragma unroll
-                        for (int j = 0; j < 16; j += 2) {
-                            const float x = scoreOf(s[j], factor), y = scoreOf(s[j + 1], factor);
-                            const bool one = ((bits >> j) & 1u) != 0u, two = ((bits >> (j + 1)) & 1u) != 0u;
-                            const float w0 = one ? exp2Fast(x + shift) : 0.f, w1 = two ? exp2Fast(y + shift) : 0.f;
-                            top = one ? fmaxf(top, x) : top, top = two ? fmaxf(top, y) : top;
-                            weights[g * 8 + j / 2] = packTwo(w0, w1, __half());
-                            const float2 w = unpackTwo(weights[g * 8 + j / 2], __half());
-                            part += rounded ? w.x + w.y : w0 + w1;
-                        }
-                        grows = grows || top + bitsOfScale > most + (kWeightBits + kGrowth);
-                        added = part == 0.f ? added : fmaf(part, tp.perWeight[half * kHalfGroups + g], added);
-                    } else {
+                    for (int g = 0; g < kHalfGroups; ++g) {
+                        uint32_t s[16];
+                        tmemLoad16(scoresAt + uint32_t(g * 16), s);
+                        const float factor = rowScale * tp.keyScale[half * kHalfGroups + g], bitsOfScale = tp.shift[half * kHalfGroups + g],
+                                    shift = bitsOfScale - base;
                         const float2 factors = {factor, factor}, shifts = {shift, shift};
                         float2 parts = {0.f, 0.f};
+                        float top = -INFINITY;
+                        tmemWait16(s);
 #pragma unroll
                         for (int j = 0; j < 16; j += 2) {
                             float2 x = {__uint_as_float(s[j]), __uint_as_float(s[j + 1])};
@@ -672,11 +718,39 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                             x = CAP != kNoCap ? addTwo(x, shifts) : fmaTwo(x, factors, shifts);
                             const float2 w = {exp2Fast(x.x), exp2Fast(x.y)};
                             weights[g * 8 + j / 2] = packTwo(w.x, w.y, __half());
-                            parts = addTwo(parts, HALF ? unpackTwo(weights[g * 8 + j / 2], __half()) : w);
+                            parts = addTwo(parts, unpackTwo(weights[g * 8 + j / 2], __half()));
                         }
-                        part = parts.x + parts.y;
-                        grows = grows || (CAP != kNoCap ? top + bitsOfScale : fmaf(top, factor, bitsOfScale)) > most + (kWeightBits + kGrowth);
-                        added = fmaf(part, tp.perWeight[half * kHalfGroups + g], added);
+                        grows = grows || (CAP != kNoCap ? top + bitsOfScale : fmaf(top, factor, bitsOfScale)) > loudest + (kWeightBits + kGrowth);
+                        added = fmaf(parts.x + parts.y, tp.perWeight[half * kHalfGroups + g], added);
+                    }
+                } else {
+                    // What the mask hides stays out, whatever its page's scales are.  Scales count as 2^-60 of e's at least, so that their
+                    // weights reach the sum.
+                    const float least = kWeightBits - 60.f - (most - base);
+                    int rowLo, rowHi;
+                    limits(rowLo, rowHi);
+#pragma unroll
+                    for (int g = 0; g < 2 * kHalfGroups; ++g) { // halves of the groups: eight scores leave room for the rest
+                        uint32_t s[8];
+                        tmemLoad8(scoresAt + uint32_t(g * 8), s);
+                        const float factor = rowScale * tp.keyScale[half * kHalfGroups + g / 2], bitsOfScale = tp.shift[half * kHalfGroups + g / 2];
+                        const float shift = (bitsOfScale < least ? least : bitsOfScale) - base; // (a NaN stays one)
+                        const uint32_t bits = masked ? seen(g / 2, rowLo, rowHi) >> (g % 2 * 8) : 0xffu;
+                        const bool rounded = shift + most >= 1.f;
+                        float top = -INFINITY, part = 0.f;
+                        tmemWait8(s);
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) {
+                            const float x = scoreOf(s[j], factor), y = scoreOf(s[j + 1], factor);
+                            const bool one = ((bits >> j) & 1u) != 0u, two = ((bits >> (j + 1)) & 1u) != 0u;
+                            const float e0 = exp2InOrder(x + shift), e1 = exp2InOrder(y + shift), w0 = one ? e0 : 0.f, w1 = two ? e1 : 0.f;
+                            top = one ? fmaxf(top, x) : top, top = two ? fmaxf(top, y) : top;
+                            weights[g * 4 + j / 2] = packTwo(w0, w1, __half());
+                            const float2 w = unpackTwo(weights[g * 4 + j / 2], __half());
+                            part += rounded ? w.x + w.y : w0 + w1;
+                        }
+                        grows = grows || top + bitsOfScale > loudest + (kWeightBits + kGrowth) || top > most + kSlack;
+                        apart = part == 0.f ? apart : fmaf(part, exp2Fast(-shift - most), apart);
                     }
                 }
                 // Both warps of the rows have read their scores, and agree whether a maximum has to be taken up.
@@ -688,7 +762,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 }
                 maximumFirst = true;
             }
-            sum += added;
+            sum += added, others += apart;
             addedBefore(); // (waited for at every tile: no phase is passed over)
             tmemStoreWeights<kKeys / 4>(weightsAt, weights);
             tmemStoreWait();
@@ -699,15 +773,21 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
             }
         }
         ok = (tiles == 0 || mbarPollWarp(&bars.result[which], 0u, 90)) && ok;
+        // the two halves' sums in units of the larger m
+        exchange[which][tileRow][half] = most;
+        asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
+        const float mostOfBoth = fmaxf(most, exchange[which][tileRow][half ^ 1]);
+        sum = others * unitsOf(most, mostOfBoth) + sum * unitsOf(loudest, mostOfBoth), most = mostOfBoth;
+        asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
         exchange[which][tileRow][half] = sum;
         asm volatile("bar.sync %0, 64;" ::"r"(pairBarrier) : "memory");
         sum += exchange[which][tileRow][half ^ 1];
+        const float exponent = loudest + float(reference) - kWeightBits; // of the results' units
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (split > 1) {
             // ---- parts of the rows, over the queries and keys, which no product of either tile reads any more ----
             asm volatile("bar.sync 9, %0;" ::"r"(active * kTileWarps * 32) : "memory");
             float *part = reinterpret_cast<float *>(smem) + (which * kRows + tileRow) * kPitch;
-            const float unit = exp2f(float(reference) - kWeightBits);
 #pragma unroll 1
             for (int d = 0; d < DP / 2; d += 16) {
                 uint32_t o[16] = {};
@@ -717,16 +797,16 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                 }
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
-                    *reinterpret_cast<float4 *>(part + half * (DP / 2) + d + j) = {__uint_as_float(o[j]) * unit, __uint_as_float(o[j + 1]) * unit,
-                                                                                   __uint_as_float(o[j + 2]) * unit, __uint_as_float(o[j + 3]) * unit};
+                    *reinterpret_cast<float4 *>(part + half * (DP / 2) + d + j) = {__uint_as_float(o[j]), __uint_as_float(o[j + 1]),
+                                                                                   __uint_as_float(o[j + 2]), __uint_as_float(o[j + 3])};
                 }
             }
             if (half == 0) {
-                part[DP] = most, part[DP + 1] = sum;
+                *reinterpret_cast<float4 *>(part + DP) = {exponent, sum, most, 0.f};
             }
         } else if (ok) { // ---- the rows, by way of the queries' memory, which no product reads any more ----
-            // two factors, since their product may be too small for all its bits
-            const float f = sum == 0.f ? 0.f : 1.f / sum, unit = exp2f(float(reference) - kWeightBits);
+            // (in two halves: the power of two may be outside the normal numbers where the result is not)
+            const float unit = exp2Fast(0.5f * (exponent - most)), f = unit / sum;
             uint8_t *mine = queries + which * Shape::kQueryBytes + (quarter * 2 + half) * (32 * DP);
             constexpr int kChunks = DP / 16, kLinesAtOnce = 32 / kChunks; // 16-byte chunks of half a row
 #pragma unroll 1
@@ -775,17 +855,18 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
         const uint32_t from = smemAddr(smem);
         for (int i = int(threadIdx.x) + rank * Shape::kThreads; i < rows * (DP / 4); i += split * Shape::kThreads) {
             const int r = i / (DP / 4), d = (i - r * (DP / 4)) * 4;
-            float top = -INFINITY, weights = 0.f;
+            float top = -INFINITY, loud = -INFINITY, weights = 0.f;
             float4 y = {};
-            for (int other = 0; other < split; ++other) { // one pass with a running maximum, as over keys
+            for (int other = 0; other < split; ++other) { // one pass with running maxima, as over keys
                 const float4 stats = loadCluster(mapToCta(from + uint32_t((r * kPitch + DP) * 4), uint32_t(other)));
                 const float4 a = loadCluster(mapToCta(from + uint32_t((r * kPitch + d) * 4), uint32_t(other)));
-                const float now = fmaxf(top, stats.x);
-                const float keep = now == -INFINITY ? 1.f : exp2Fast(top - now), factor = now == -INFINITY ? 1.f : exp2Fast(stats.x - now);
-                top = now, weights = weights * keep + stats.y * factor;
+                const float nowTop = fmaxf(top, stats.z), nowLoud = fmaxf(loud, stats.x);
+                weights = weights * unitsOf(top, nowTop) + stats.y * unitsOf(stats.z, nowTop);
+                const float keep = unitsOf(loud, nowLoud), factor = unitsOf(stats.x, nowLoud);
                 y.x = y.x * keep + a.x * factor, y.y = y.y * keep + a.y * factor, y.z = y.z * keep + a.z * factor, y.w = y.w * keep + a.w * factor;
+                top = nowTop, loud = nowLoud;
             }
-            writeOut<T>(p, q.first, firstRow + r, head, d, y, weights);
+            writeOut<T>(p, q.first, firstRow + r, head, d, y, weights, loud - top);
         }
         __syncwarp();
         clusterSync(); // nobody leaves while its parts are being read

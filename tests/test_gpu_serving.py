@@ -850,3 +850,38 @@ def test_windows_beyond_32_bits_hide_nothing(serving, mlel, window):
     assert torch.equal(p.cache.attend(q, p.batch, window=window)[:4], want[:4])
     with pytest.raises(mlel.MlelError, match="not negative"):
         p.cache.attend(q, p.batch, window=-window)
+
+
+@pytest.mark.parametrize("mode", ["ordinary", "tiny", "zero"])
+@pytest.mark.parametrize("sequences, group, d, how", [([(4, 34), (3, 18)], 2, 64, {}), ([(8, 40), (6, 90)], 2, 128, {"window": 20}), ([(4, 19), (2, 33)], 4, 256, {}),
+                                                      ([(4, 20002), (1, 40)], 2, 64, {}), ([(100, 160), (40, 300)], 4, 128, {}), ([(90, 200)], 3, 64, {"window": 33}),
+                                                      ([(40, 70)], 2, 256, {"softcap": 9.0}), ([(70, 5000)], 1, 128, {}), ([(33, 600)] * 4, 1, 64, {"window": 150})], ids=str)
+def test_attention_over_the_whole_range_of_value_scales(serving, sequences, group, d, how, mode):
+    """One page of each sequence as large as bf16 allows, the others ordinary, next to nothing in part, or zeros in part: rows that do not
+    see the large page are as exact as without it, and rows that do are its values."""
+    t = torch.bfloat16
+    p = Paged(serving, 101 + d, sequences, 1, 16, d, wild=False)
+    q, out = query(p, group, t)
+    small = torch.rand(p.scales[1].shape, generator=p.g, device="cuda") < (0.0 if mode == "ordinary" else 0.5)
+    if mode != "ordinary":
+        p.scales[1, small] = 1e-38 if mode == "tiny" else 0.0
+    if mode == "zero":
+        p.data[1, small[:, 0]] = 0
+    windowed = lambda b: 0 if "window" in how else (p.lengths[b] - 1) // 16
+    args = d ** -0.5, True, how.get("window", 0), how.get("softcap", 0.0), t
+    without, bound_without = ref.attend(*p.arrays(), ref.f64(q), *args)
+    for b in range(len(sequences)):
+        p.scales[1, p.table[b][windowed(b)]] = 3e38 / 127 / 4
+    got = ref.f64(p.cache.attend(q, p.batch, out=out, **how))
+    want, bound = ref.attend(*p.arrays(), ref.f64(q), *args)
+    unseen = 0
+    for b, length in enumerate(p.lengths):
+        for i in range(p.starts[b], p.starts[b + 1]):
+            position = length - p.starts[b + 1] + i
+            lo = max(0, position - how["window"] + 1) if "window" in how else 0
+            if windowed(b) * 16 <= position and windowed(b) * 16 + 16 > lo:
+                assert (np.abs(got[i] - want[i]) <= bound[i]).all(), (b, i)
+            else:
+                assert (np.abs(got[i] - without[i]) <= bound_without[i]).all(), (b, i, np.abs(got[i] - without[i]).max())
+                unseen += 1
+    assert unseen > 0
