@@ -5,9 +5,9 @@
 // What bounds it: the bytes of the cache, and close behind them the instructions that turn them into operands.  Every key and
 // value is read once per tile of 8 rows (a row is one token's query head; the heads that share a cache head are rows of
 // one tile), by the second and further tiles of a cache head out of L2.  (Tiles of 16 rows for 9 to 16, 16 sequences of up to 4000
-// tokens, 8 heads of 128 elements, 16 rows: 41 us, of 8 rows 32; 4 heads of 256, 12 rows: 71 and 39.)  At 6.5 TB/s an SM gets some
+// tokens, 8 heads of 128 elements, 16 rows: 41 us, of 8 rows 33; 4 heads of 256, 12 rows: 71 and 39.)  At 6.5 TB/s an SM gets some
 // 23 bytes a cycle, 16 keys and values of 128 elements every 180 cycles.  32 sequences of up to 16000 tokens, 8 heads of 128: 106 us,
-// 5.8 TB/s; 8 of up to 700: 9.1 us.
+// 5.8 TB/s; 8 of up to 700: 9.2 us.
 //
 // Work.  All tiles' keys, in steps of 128, form one line that is cut into as many equal pieces as there are blocks, whatever the
 // lengths of the sequences: a block works through the ends of the tiles that its piece touches.  Tiles that lie in

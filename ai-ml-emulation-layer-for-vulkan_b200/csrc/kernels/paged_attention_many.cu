@@ -16,7 +16,7 @@
 // What bounds it: per 256 x 128 scores the products take 2048 cycles at 128 elements a head, and 32768 exponentials the
 // same at 16 a cycle; everything else (a multiply-add, half a maximum, half a sum, half a conversion per score, and the
 // keys' and values' conversion) shares the four schedulers with them: some 4500 cycles.  Four prompts of 6000 tokens, 32 heads of 128
-// elements over 8: 790 us, 803 TFLOP/s.
+// elements over 8: 799 us, 795 TFLOP/s.
 //
 // Softmax in one pass where it can: scores are weighed with the maximum known from the tiles before, and only if one exceeds
 // it by more than 2^8, or at a row's first tile and where the values' reference grows, the maximum is taken first and sums
@@ -281,7 +281,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     const int active = rows > kRows ? 2 : 1; // tiles with rows
     // One tile alone has both places for scores in turn: the next ones are formed before the softmax wants them.  Keys then come
     // before the values of the tile in front of them.  (Three sequences of 300 new tokens, 16 heads of 256 elements over 8, window 1024,
-    // capped: 61 us with one place, so 51, 54 with the sums that f16 results get and 55 with maxima that include the values' scales; 16 sequences of 4000 tokens, 32 rows a head of 128: 76 and 64.)
+    // capped: 61 us with one place, so 51, 53 with the sums over rounded weights; 16 sequences of 4000 tokens, 32 rows a head of 128: 76 and 64.)
     const bool ahead = active == 1;
 
     if (threadIdx.x == 0) {
