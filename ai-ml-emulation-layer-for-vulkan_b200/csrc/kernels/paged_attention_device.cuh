@@ -136,12 +136,6 @@ __device__ __forceinline__ float logOfScale(float scale) {
     const float y = log2f(scale);
     return y < -150.f ? -150.f : y;
 }
-// The exponent of a weight of 14 bits in excess of its score's, by the logarithm of its value's scale and its row's two maxima.
-__device__ __forceinline__ float weightShift(float valueLog, float loudest, float most) {
-    const float own = valueLog - loudest, least = -60.f - most;
-    return (own < least ? least : own) + 14.f; // (a NaN stays one)
-}
-
 // Four elements of one row of the answer: y / sum * 2^exponent, or zeros for a row that nothing was added to.
 template <class T>
 __device__ __forceinline__ void writeOut(const AttendParams &p, int firstToken, int row, int head, int d, float4 y, float sum, float exponent) {

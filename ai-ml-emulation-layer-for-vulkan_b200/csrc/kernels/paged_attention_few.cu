@@ -63,6 +63,7 @@ constexpr int kGroup = 16; // keys that share a page and a scale for certain
 constexpr int kStageGroups = 2;
 constexpr int kStepGroups = kWarps * kStageGroups;
 constexpr float kWeightBits = 14.f; // a row's largest weight is 2^14
+constexpr float kNothing = -3e38f;  // both maxima of a row that has seen no key: differences with it are numbers
 constexpr float kSlack = 30.f;      // by which scores may exceed m, in powers of two, before it is taken up: it only is the sum's unit
 constexpr int kClusterSteps = 3; // steps by which a cluster's blocks may outlast the line's
 
@@ -251,13 +252,17 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             }
             return slot;
         };
-        // a key scale of -1 stands for a group that is not there; one that is not finite is no number, whatever it would be multiplied with
-        const auto scaleOf = [&](const float *scales, int slot) {
-            const float scale = slot >= 0 ? scales[int64_t(slot) * p.cache.heads + head] : -1.f;
-            return scale < INFINITY ? scale : NAN;
+        // A key scale of -1 stands for a group that is not there; no number, whatever it would be multiplied with, for one whose scales are
+        // not both finite.
+        const auto scalesOf = [&](int slot, float &key, float &valueLog) {
+            const int64_t at = int64_t(max(slot, 0)) * p.cache.heads + head;
+            const float value = slot >= 0 ? p.cache.valueScales[at] : 0.f;
+            key = slot < 0 ? -1.f : p.cache.keyScales[at];
+            key = key < INFINITY && value < INFINITY ? key : NAN, valueLog = logOfScale(value);
         };
         int slots = slotOf(lane), nextSlots = slotOf(32 + lane);
-        float keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = logOfScale(scaleOf(p.cache.valueScales, slots));
+        float keyScales, valueLogs;
+        scalesOf(slots, keyScales, valueLogs);
         int issued = 0, writeStage = stage, issueSlots = slots;
         // lanes that issue a copy: keys or values, which of the two groups, which panel
         const int side = lane & 1, sub = (lane >> 1) & 1, panel = lane >> 2;
@@ -349,11 +354,11 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         const int openHi = p.causal ? old + firstToken + 1 : w.q.length, openLo = p.window > 0 ? max(0, old + lastToken - p.window + 1) : 0;
 
         float o[MT][4] = {}, most[2], loudest[2], sum[2] = {}; // m and e of two rows
-        most[0] = most[1] = loudest[0] = loudest[1] = -INFINITY;
+        most[0] = most[1] = loudest[0] = loudest[1] = kNothing;
         for (int n = 0; n < count; ++n) {
             if (n > 0 && (n & 15) == 0) {
                 slots = nextSlots;
-                keyScales = scaleOf(p.cache.keyScales, slots), valueLogs = logOfScale(scaleOf(p.cache.valueScales, slots));
+                scalesOf(slots, keyScales, valueLogs);
                 nextSlots = slotOf(2 * n + 32 + lane);
             }
             if (n < issued) {
@@ -395,7 +400,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                 bool grows = false;
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
-                    // what a score may be before one of the maxima grows (a scale that is no number limits nothing)
+                    // what a score may be before one of the maxima grows
                     const float limit[2] = {fminf(loudest[0] - valueLog[h], most[0] + kSlack), fminf(loudest[1] - valueLog[h], most[1] + kSlack)};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
@@ -437,13 +442,13 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
 #pragma unroll
                 for (int h = 0; h < AT; ++h) {
                     uint32_t wf[2]; // P^T: keys in pairs by t, row g
-                    float shift[2], part[2] = {0.f, 0.f};
+                    // what weights have in excess of their scores, and of their scores against m
+                    float shift[2], excess[2], part[2] = {0.f, 0.f};
                     bool rounded[2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const float base = most[x] == -INFINITY ? 0.f : most[x];
-                        shift[x] = weightShift(valueLog[h], loudest[x], base);
-                        rounded[x] = shift[x] + base >= 8.f; // no weight that matters is a subnormal number
+                        shift[x] = fmaxf(kWeightBits - (loudest[x] - valueLog[h]), kWeightBits - 60.f - most[x]);
+                        excess[x] = shift[x] + most[x], rounded[x] = excess[x] >= 8.f; // no weight that matters is a subnormal number
                     }
 #pragma unroll
                     for (int half = 0; half < 2; ++half) { // what the mask hides stays out, whatever its page's scale is
@@ -457,7 +462,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
                     }
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        sum[x] = part[x] == 0.f ? sum[x] : fmaf(part[x], exp2Fast(-shift[x] - most[x]), sum[x]);
+                        sum[x] = fmaf(part[x], exp2Fast(-excess[x]), sum[x]);
                     }
                     constexpr int CHUNKS = DP < 128 ? 1 : DP / 128, WORDS = DP < 128 ? 2 : 4; // 16 (or, below 128, 8) bytes of a value row per lane each
                     const uint32_t group = values + uint32_t(h * Shape::kGroupBytes);
@@ -517,7 +522,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         for (int x = 0; x < 2; ++x) {
             const int itsRow = 2 * t + x;
             if (itsRow < rows) {
-                float loud = -INFINITY;
+                float loud = kNothing;
                 for (int v = 0; v < kWarps; ++v) {
                     loud = fmaxf(loud, joinLoudest[v][itsRow]);
                 }
@@ -538,7 +543,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
         for (int i = int(threadIdx.x); i < rows * (DP / 4); i += kWarps * 32) {
             const int itsRow = i / (DP / 4), d = (i - itsRow * (DP / 4)) * 4;
             float4 y = {};
-            float top = -INFINITY, loud = -INFINITY, weights = 0.f;
+            float top = kNothing, loud = kNothing, weights = 0.f;
 #pragma unroll
             for (int v = 0; v < kWarps; ++v) {
                 top = fmaxf(top, joinMost[v][itsRow]), loud = fmaxf(loud, joinLoudest[v][itsRow]);
@@ -565,7 +570,7 @@ pagedAttentionFewKernel(const __grid_constant__ CUtensorMap mapK, const __grid_c
             const uint32_t from = smemAddr(joined);
             for (int i = int(threadIdx.x) + rank * (kWarps * 32); i < rows * (DP / 4); i += split * (kWarps * 32)) {
                 const int itsRow = i / (DP / 4), d = (i - itsRow * (DP / 4)) * 4;
-                float top = -INFINITY, loud = -INFINITY, weights = 0.f;
+                float top = kNothing, loud = kNothing, weights = 0.f;
                 float4 y = {};
                 for (int r = 0; r < split; ++r) {
                     const float4 stats = loadCluster(mapToCta(from + uint32_t((itsRow * kPitch + DP) * 4), uint32_t(r)));
@@ -634,7 +639,7 @@ __global__ void __launch_bounds__(kWarps * 32) pagedAttentionFewJoin(const Atten
     }
     const int first = x0 == pieces.start(c0) ? 0 : 1; // where piece c0 left it: as its first tile, or as its last
     const auto part = [&](int c) { return partialRow<DP>(p, c0 + c, c == 0 ? first : 0, row); };
-    float top = -INFINITY, loud = -INFINITY;
+    float top = kNothing, loud = kNothing;
     for (int c = int(threadIdx.x); c < n; c += THREADS) {
         const float4 s = *reinterpret_cast<const float4 *>(part(c));
         loud = fmaxf(loud, s.x), top = fmaxf(top, s.z);

@@ -499,8 +499,8 @@ int mlel_cuda_paged_append(const mlel_paged_cache *cache, const mlel_paged_batch
  * window > 0 only j > p - window.  queries, output [tokens, query_heads, head_dim], both f16 or both bf16; query_heads a multiple of
  * the cache's heads, query head h reads cache head h / (query_heads / heads).  The products run in f16 with f32 sums; the softmax
  * is in f32, its weights rounded to f16.  Tokens that the masks hide from a query change nothing of its result beyond such roundings,
- * whatever they are; a scale that is not finite, seen, makes it NaN.  `workspace`: mlel_paged_attention_workspace() bytes of device memory on a 16-byte boundary that nothing else uses
- * until the call's work is done (its contents do not matter before or after). */
+ * whatever they are; a scale that is not finite, seen, makes it NaN.  `workspace`: mlel_paged_attention_workspace() bytes of device
+ * memory on a 16-byte boundary that nothing else uses until the call's work is done (its contents do not matter before or after). */
 int mlel_cuda_paged_attention(const mlel_paged_cache *cache, const mlel_paged_batch *batch, const mlel_tensor *queries,
                               const mlel_tensor *output, float scale, int causal, int32_t window, float softcap, void *workspace,
                               uint64_t workspace_bytes, void *cuda_stream);
