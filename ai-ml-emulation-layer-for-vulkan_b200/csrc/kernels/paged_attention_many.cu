@@ -16,7 +16,7 @@
 // What bounds it: per 256 x 128 scores the products take 2048 cycles at 128 elements a head, and 32768 exponentials the
 // same at 16 a cycle; everything else (a multiply-add, half a maximum, half a sum, half a conversion per score, and the
 // keys' and values' conversion) shares the four schedulers with them: some 4500 cycles.  Four prompts of 6000 tokens, 32 heads of 128
-// elements over 8: 799 us, 795 TFLOP/s.
+// elements over 8: 818 us, 777 TFLOP/s.
 //
 // Softmax in one pass where it can: scores are weighed with the maximum known from the tiles before, and only if one exceeds
 // it by more than 2^8, or at a row's first tile and where the values' reference grows, the maximum is taken first and sums
@@ -27,10 +27,11 @@
 // above the scales, so that log2(scale / r) and its power belong to a tile and not to a row.)
 // The sum is over the weights as they are rounded, so that what rounding does to the key that has most of a row cancels (a seventh off
 // the error against 64 bits).
-// Tiles that a mask cuts, or with scales far below r, go a second way, which asks for each key and forms by the row what the first way
-// takes from the tile.  The two are apart, rather than a group at a time, and the second takes eight scores at a time, so that the weights
-// of 64 keys and all else fit 80 registers: what does not comes back from L2, shared memory having all of the L1 cache (the same
-// with both ways in one loop: 860 us).  The queries' loads are issued one after another before any is used: the compiler
+// Tiles that a mask cuts, or with scales far below r, go a second way, which asks for each key, passes over groups that no row sees and
+// forms by the row what the first way takes from the tile.  The two are apart, rather than a group at a time, so that the weights of 64
+// keys and all else fit 80 registers: what does not comes back from L2, shared memory having all of the L1 cache (both ways in one
+// loop: 860 us).  (With eight scores at a time instead of sixteen in the second way these prompts take 800 us, but 2000 new tokens with a
+// window of 100, all of whose tiles are cut, 70 for 64.)  The queries' loads are issued one after another before any is used: the compiler
 // would save registers and wait for each in turn (3.6 us a block).
 
 #include <cuda_bf16.h>
@@ -192,18 +193,6 @@ __device__ __forceinline__ uint32_t pairVote(int barrier, bool predicate) {
                  : "memory");
     return any;
 }
-__device__ __forceinline__ void tmemLoad8(uint32_t taddr, uint32_t (&r)[8]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmemWait8(uint32_t (&r)[8]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
-                 :
-                 : "memory");
-}
 // 1 / unit for a power of two from 2^-126 to 2^126.
 __device__ __forceinline__ float inverseOfPower(float unit) { return __uint_as_float(0x7f000000u - __float_as_uint(unit)); }
 // 16 bytes from a 16-byte boundary where `there`, zeros elsewhere.  (In order with one another: a row of these is on its way at once,
@@ -281,7 +270,7 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
     const int active = rows > kRows ? 2 : 1; // tiles with rows
     // One tile alone has both places for scores in turn: the next ones are formed before the softmax wants them.  Keys then come
     // before the values of the tile in front of them.  (Three sequences of 300 new tokens, 16 heads of 256 elements over 8, window 1024,
-    // capped: 61 us with one place, so 51, 53 with the sums over rounded weights; 16 sequences of 4000 tokens, 32 rows a head of 128: 76 and 64.)
+    // capped: 61 us with one place, so 51; 16 sequences of 4000 tokens, 32 rows a head of 128: 76 and 64.)
     const bool ahead = active == 1;
 
     if (threadIdx.x == 0) {
@@ -652,9 +641,6 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
 #pragma unroll 1
                     for (int g = 0; g < kHalfGroups; ++g) {
                         const uint32_t bits = masked ? seen(g, rowLo, rowHi) : 0xffffu;
-                        if (!__any_sync(0xffffffffu, bits != 0u)) { // as most groups of a causal mask's last tile
-                            continue;
-                        }
                         uint32_t s[16];
                         tmemLoad16(scoresAt + uint32_t(g * 16), s);
                         tmemWait16(s);
@@ -730,23 +716,30 @@ pagedAttentionManyKernel(const __grid_constant__ CUtensorMap mapK, const __grid_
                     int rowLo, rowHi;
                     limits(rowLo, rowHi);
 #pragma unroll
-                    for (int g = 0; g < 2 * kHalfGroups; ++g) { // halves of the groups: eight scores leave room for the rest
-                        uint32_t s[8];
-                        tmemLoad8(scoresAt + uint32_t(g * 8), s);
-                        const float factor = rowScale * tp.keyScale[half * kHalfGroups + g / 2], bitsOfScale = tp.shift[half * kHalfGroups + g / 2];
+                    for (int g = 0; g < kHalfGroups; ++g) {
+                        const uint32_t bits = masked ? seen(g, rowLo, rowHi) : 0xffffu;
+                        if (!__any_sync(0xffffffffu, bits != 0u)) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) {
+                                weights[8 * g + j] = 0u;
+                            }
+                            continue;
+                        }
+                        uint32_t s[16];
+                        tmemLoad16(scoresAt + uint32_t(g * 16), s);
+                        const float factor = rowScale * tp.keyScale[half * kHalfGroups + g], bitsOfScale = tp.shift[half * kHalfGroups + g];
                         const float shift = (bitsOfScale < least ? least : bitsOfScale) - base; // (a NaN stays one)
-                        const uint32_t bits = masked ? seen(g / 2, rowLo, rowHi) >> (g % 2 * 8) : 0xffu;
                         const bool rounded = shift + most >= 1.f;
                         float top = -INFINITY, part = 0.f;
-                        tmemWait8(s);
+                        tmemWait16(s);
 #pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
+                        for (int j = 0; j < 16; j += 2) {
                             const float x = scoreOf(s[j], factor), y = scoreOf(s[j + 1], factor);
                             const bool one = ((bits >> j) & 1u) != 0u, two = ((bits >> (j + 1)) & 1u) != 0u;
                             const float e0 = exp2InOrder(x + shift), e1 = exp2InOrder(y + shift), w0 = one ? e0 : 0.f, w1 = two ? e1 : 0.f;
                             top = one ? fmaxf(top, x) : top, top = two ? fmaxf(top, y) : top;
-                            weights[g * 4 + j / 2] = packTwo(w0, w1, __half());
-                            const float2 w = unpackTwo(weights[g * 4 + j / 2], __half());
+                            weights[g * 8 + j / 2] = packTwo(w0, w1, __half());
+                            const float2 w = unpackTwo(weights[g * 8 + j / 2], __half());
                             part += rounded ? w.x + w.y : w0 + w1;
                         }
                         grows = grows || top + bitsOfScale > loudest + (kWeightBits + kGrowth) || top > most + kSlack;
